@@ -95,7 +95,8 @@ nva_status nva_ctx_sync(nva_ctx *ctx);
 const char *nva_last_error(nva_ctx *ctx);
 const char *nva_status_string(nva_status status);
 /* Per-kernel timing with HIP events on the context's stream (off by default).  Kernel names:
- * "rope_store", "store", "decode", "merge", "prefill", "gather", "linear", "rms_norm";
+ * "rope_store", "store", "decode", "merge", "prefill", "gather", "linear", "rms_norm", and of
+ * shared prefixes and cross attention "span" (few columns) and "span_tiles" (many);
  * "attention" spans the attention kernels of one call (decode and prefill kernels that
  * overlap count once).  "prefill_split" and "prefill_fp32" are the part of "prefill" that each of
  * its two tile kernels took, "linear_tiles" the part of "linear" of its 128 x 128-tile kernel.
@@ -230,6 +231,39 @@ nva_status nva_step_prepare_prefill(nva_ctx *ctx, const nva_seq *seqs, int num_s
 nva_status nva_step_prepare_decode(nva_ctx *ctx, const nva_seq *seqs, int num_seqs,
                                    int block_size);
 
+/* Shared prefixes.  A run of num_seqs sequences of the step, first_seq and those after it, whose
+ * first num_tokens tokens lie in the same pages (the engine's prefix-hash reuse,
+ * engine/BlockManager.java:147-201, gives sequences with equal prompts equal pages). */
+typedef struct nva_prefix_group {
+  int32_t first_seq;
+  int32_t num_seqs;
+  int32_t num_tokens;
+} nva_prefix_group;
+
+/* Finds them: groups (room for num_seqs / 2) receives the runs of adjacent sequences, in order, that
+ * save the most page reads over the tables, *num_groups their number.  Only full pages of cached
+ * tokens count: cached_tokens[b] is context_lens[b] - 1 in a decode step, num_cached_tokens in a
+ * prefill.  Pure host code. */
+nva_status nva_find_shared_prefixes(const int32_t *block_tables, int num_seqs, int bt_stride,
+                                    const int32_t *cached_tokens, int block_size,
+                                    nva_prefix_group *groups, int *num_groups);
+/* Attention of a batch that shares prefixes: from this call to the next nva_step_set (or call), every
+ * attention call over the step's pages reads the tokens of a group once for all rows of its
+ * sequences and joins the result with each sequence's own keys; outputs agree with those of the
+ * separate reads to fp32 rounding.  (Layers with a sliding window, which see too little of a prefix,
+ * are computed as before, as is a group of one row.)  Groups are in order and do not overlap; a
+ * group's tokens are cached ones of each of its sequences, which hold them in the same pages: tables
+ * that differ there fail the attention call with NVA_E_ARG, before anything is written.  num_groups
+ * 0 ends the sharing. */
+nva_status nva_step_share_prefixes(nva_ctx *ctx, const nva_prefix_group *groups, int num_groups);
+
+/* The encoder rows that cross attention reads in this step: sequence b of the step sees rows
+ * kv_start[b] .. kv_start[b] + kv_len[b] - 1 of the pool given to nva_cross_attention_forward
+ * (kv_len 0: none).  Host arrays of num_seqs entries, the step's number of sequences; call it after
+ * nva_step_set, which forgets them. */
+nva_status nva_step_set_encoder(nva_ctx *ctx, const int32_t *kv_start, const int32_t *kv_len,
+                                int num_seqs);
+
 /* Replaces the step's positions only (the positions tensor RotaryEmbedding.forward receives,
  * Norms.java:275, rounded with Math.round as at Norms.java:317).  Valid after nva_step_set. */
 nva_status nva_step_positions(nva_ctx *ctx, const float *positions, int num_tokens);
@@ -269,6 +303,28 @@ nva_status nva_attention_forward(nva_ctx *ctx, nva_kv *kv, const nva_attn_desc *
 nva_status nva_attention_forward_noalloc(nva_ctx *ctx, nva_kv *kv, const nva_attn_desc *desc,
                                          const float *q, const float *k, const float *v,
                                          int num_tokens, float *out);
+
+/* Cross attention: every query of a sequence over all keys of its encoder's states, whose number is
+ * independent of the queries'.  out [num_tokens, num_heads, head_dim] = softmax(q k^T scale) v per
+ * head, KV head h / (num_heads / num_kv_heads); zeros where a sequence has no encoder rows and for
+ * rows behind the last sequence.  Also the full attention of an encoder's own layers (the
+ * reference's layers/BidirectionalAttention.java), with each sequence's rows as its keys.
+ *   q        [num_tokens, num_heads, head_dim]: row b per sequence in a decode step, the step's
+ *            cu_q otherwise
+ *   k, v     row r of the pool, [num_kv_heads, head_dim], starts kv_stride * r floats in: a pool of
+ *            kv_rows rows, or a view of a packed projection (kv_stride >= num_kv_heads * head_dim,
+ *            % 4 == 0, < 4194304); NULL if kv_rows is 0
+ * Rows come from nva_step_set_encoder.  Sequences in a row that read the same ones (beams) read them
+ * once.  sliding_window must be 0; kv_layer_index and write_kv are not used.  d = 64, 128, 256 and
+ * 512 run on matrix units, other head dims row by row.  Not under stream capture: the second form,
+ * with the rules and the scratch array of nva_attention_forward_noalloc, is for that. */
+nva_status nva_cross_attention_forward(nva_ctx *ctx, const nva_attn_desc *desc, const float *q,
+                                       const float *k, const float *v, int64_t kv_rows,
+                                       int64_t kv_stride, int num_tokens, float *out);
+nva_status nva_cross_attention_forward_noalloc(nva_ctx *ctx, const nva_attn_desc *desc,
+                                               const float *q, const float *k, const float *v,
+                                               int64_t kv_rows, int64_t kv_stride, int num_tokens,
+                                               float *out);
 
 /* The pair RotaryEmbedding.forward + Attention.forward as one call, the way the model layers
  * use them (models/internal/Qwen3ForCausalLM.java:207-222): one fused kernel rotates q and k

@@ -166,8 +166,16 @@ struct PlanKey {
   int paged;                   // keys through block tables (else dense k/v rows)
   int block_size, num_blocks;  // arena geometry the tables are checked against
   int head_dim, num_heads, num_kv_heads;  // size the work of a mixed plan's two kernels
+  int cross = 0;               // over the encoder's rows instead of the sequence's own keys
+  int64_t kv_rows = 0;         // cross: rows of the encoder pool
+  int col_heads = 0;           // spans: query heads of a column group
+  int span_cols = 0;           // most columns of a span item (0: the span kernel does not serve)
+  int span_tile_cols = 0;      // columns of a span tile (0: no tile kernel for this head dim)
+  int span_blocks_per_cu = 0;
   bool operator==(const PlanKey &o) const {
-    return window == o.window && mfma == o.mfma && fp32_tiles == o.fp32_tiles && tile_q == o.tile_q &&
+    return cross == o.cross && kv_rows == o.kv_rows && col_heads == o.col_heads &&
+           span_cols == o.span_cols && span_tile_cols == o.span_tile_cols &&
+           span_blocks_per_cu == o.span_blocks_per_cu && window == o.window && mfma == o.mfma && fp32_tiles == o.fp32_tiles && tile_q == o.tile_q &&
            head_dim == o.head_dim && num_heads == o.num_heads && num_kv_heads == o.num_kv_heads &&
            wg_per_item == o.wg_per_item && blocks_per_cu == o.blocks_per_cu &&
            tile_groups == o.tile_groups && tokens == o.tokens && paged == o.paged &&
@@ -180,9 +188,12 @@ struct Plan {
   bool valid = false;
   int num_rows = 0, num_merge = 0, num_tiles = 0, num_parts = 0;
   int num_slots = 0;  // prefill stream-K slots (grid x)
+  int num_spans = 0, max_cols = 0;                // span items, and the most columns of one
+  int num_span_tiles = 0, num_span_slots = 0;     // span tiles and their stream-K slots
   int max_parts = 0;  // most partials any merged row has
   bool covers_all = true;  // every output row is written by some kernel
   size_t off_rows = 0, off_merge = 0, off_tiles = 0, off_slots = 0;
+  size_t off_spans = 0, off_span_tiles = 0, off_span_slots = 0, off_row_part = 0;
   std::vector<char> host;  // the packed lists at the offsets above
   uint64_t id = 0;         // unique per build (identifies the plan held in a scratch array)
   bool on_device = false;  // host bytes uploaded to dev
@@ -238,6 +249,13 @@ struct nva_ctx {
   bool has_cu = false, has_slots = false, has_ctx_lens = false, has_tables = false,
        has_pos = false;
   std::vector<int32_t> cu_q, cu_k, slots, ctx_lens, tables, seq_ids, pos;
+  // Shared prefixes of the step's sequences, and the page size their tables were compared at (0:
+  // not yet).
+  std::vector<nva_prefix_group> groups;
+  int groups_block_size = 0;
+  // The encoder rows each sequence's cross attention reads.
+  bool has_encoder = false;
+  std::vector<int32_t> enc_start, enc_len;
   DevBuf d_step;
   Staging step_stage;
   size_t off_cu_q = 0, off_cu_k = 0, off_slots = 0, off_ctx = 0, off_tables = 0, off_pos = 0;
@@ -336,6 +354,14 @@ int ctx_prefill_blocks_per_cu(nva_ctx *ctx, int head_dim, int hpw, bool fp32) {
   const int n = fp32 ? prefill_fp32_blocks_per_cu(head_dim, hpw) : prefill_blocks_per_cu(head_dim, hpw);
   ctx->occupancy[key] = n;
   return n;
+}
+
+int ctx_span_blocks_per_cu(nva_ctx *ctx, int head_dim) {
+  const int key = -head_dim;  // beside the prefill kernels' keys, which are positive
+  auto it = ctx->occupancy.find(key);
+  if (it == ctx->occupancy.end())
+    it = ctx->occupancy.emplace(key, span_tile_blocks_per_cu(head_dim)).first;
+  return it->second;
 }
 
 hipEvent_t take_event(nva_ctx *ctx) {
@@ -458,6 +484,218 @@ int64_t mixed_tile_cus(int num_cus, double row_bytes, double tile_flops, int hea
   return (int64_t)num_cus * best_s / 16;
 }
 
+// One piece of a tile's keys, on one slot.
+struct Piece {
+  int tile, slot, k0, k1;
+};
+
+// Cuts the 32-key tiles of all query tiles into equal runs, one per slot; tile i writes rows[i] rows
+// per piece, and a piece has at most cap_tiles key tiles.  The pieces come grouped by tile, in key
+// order.
+//
+// Two ways to cut the tiles into equal runs; the plan keeps the one that splits fewer
+// query rows (each split row writes and re-reads one partial per segment), unless that one
+// cuts a tile into more segments than the row-wide merge folds:
+//  (a) the query tiles in sequence order, laid end to end, cut at every slot boundary;
+//  (b) tiles longer than a run (cap = ceil(total / slots) key tiles) first, largest first,
+//      each filling whole empty slots and its remainder going to the fullest slot it fits;
+//      then the other tiles whole, largest first, each into the fullest slot it fits; what
+//      is left goes, piece by piece, to the emptiest slot.
+// Both give every slot the same number of key tiles (to one).  Measured splits (rows):
+// Qwen3-0.6B varlen prefill 512/1024/1536/2048 6784 (a) / 5696 (b), Gemma3 d = 256 global
+// 11648 / 8192, with a 512-key window 9472 / 8832.
+// Pieces of both cuts are flat arrays (the plan is rebuilt every step, so it avoids a small
+// allocation per tile).
+std::vector<Piece> cut_tiles(const std::vector<TileItem> &tiles, const std::vector<int> &rows_of,
+                             int slots, int64_t cap_tiles) {
+  constexpr int KT = 32;
+  int64_t total = 0;
+  const int nt = (int)tiles.size();
+  std::vector<int64_t> ntile(nt);
+  for (int i = 0; i < nt; i++) total += ntile[i] = (tiles[i].ke - tiles[i].ks + KT - 1) / KT;
+  // Rows written as partials, and the most segments of one tile.
+  auto score = [&](const std::vector<Piece> &pc, int64_t *rows, int *most) {
+    *rows = 0;
+    *most = 1;
+    for (size_t a = 0; a < pc.size();) {
+      size_t b = a;
+      while (b < pc.size() && pc[b].tile == pc[a].tile) b++;
+      const int np = (int)(b - a);
+      if (np > 1) *rows += (int64_t)np * rows_of[pc[a].tile];
+      *most = std::max(*most, np);
+      a = b;
+    }
+  };
+  std::vector<Piece> cut_a, cut_b;
+  cut_a.reserve(nt + slots);
+  {
+    int64_t pos = 0;  // first key tile of the current query tile in the flattened order
+    for (int i = 0; i < nt; i++) {
+      const TileItem &t = tiles[i];
+      const int64_t n = ntile[i];
+      int64_t j = 0;
+      while (j < n) {
+        const int64_t g = pos + j;
+        const int s_of = (int)std::min<int64_t>(slots - 1, g * slots / total);
+        const int64_t s_end = ((int64_t)(s_of + 1) * total + slots - 1) / slots;  // exclusive
+        int64_t take = std::min<int64_t>(n - j, s_end - g);
+        take = std::max<int64_t>(1, std::min<int64_t>(take, cap_tiles));
+        cut_a.push_back({i, s_of, t.ks + (int)(j * KT),
+                         std::min<int>(t.ke, t.ks + (int)((j + take) * KT))});
+        j += take;
+      }
+      pos += n;
+    }
+  }
+  {
+    const int64_t cap = (total + slots - 1) / slots;
+    std::vector<int64_t> load(slots, 0), rem(nt, 0);
+    struct Run {
+      int tile, slot;
+      int64_t n;
+    };
+    std::vector<Run> runs;
+    runs.reserve(nt + 2 * slots);
+    std::vector<int> order(nt);
+    for (int i = 0; i < nt; i++) order[i] = i;
+    std::stable_sort(order.begin(), order.end(),
+                     [&](int x, int y) { return ntile[x] > ntile[y]; });
+    auto fullest_fit = [&](int64_t n) {
+      int best = -1;
+      for (int b = 0; b < slots; b++)
+        if (load[b] + n <= cap && (best < 0 || load[b] > load[best])) best = b;
+      return best;
+    };
+    int empty = 0;  // slots below this index are not empty
+    for (int i : order) {
+      if (ntile[i] <= cap) continue;
+      rem[i] = ntile[i];
+      while (rem[i] >= cap) {
+        while (empty < slots && load[empty] != 0) empty++;
+        if (empty == slots) break;
+        load[empty] = cap;
+        runs.push_back({i, empty, cap});
+        rem[i] -= cap;
+      }
+      if (rem[i] > 0) {
+        const int b = fullest_fit(rem[i]);
+        if (b >= 0) {
+          load[b] += rem[i];
+          runs.push_back({i, b, rem[i]});
+          rem[i] = 0;
+        }
+      }
+    }
+    for (int i : order) {
+      if (ntile[i] > cap) continue;
+      const int b = fullest_fit(ntile[i]);
+      if (b >= 0) {
+        load[b] += ntile[i];
+        runs.push_back({i, b, ntile[i]});
+      } else {
+        rem[i] = ntile[i];
+      }
+    }
+    for (int i : order)
+      while (rem[i] > 0) {
+        int b = 0;
+        for (int x = 1; x < slots; x++)
+          if (load[x] < load[b]) b = x;
+        const int64_t take = load[b] < cap ? std::min<int64_t>(rem[i], cap - load[b]) : rem[i];
+        load[b] += take;
+        runs.push_back({i, b, take});
+        rem[i] -= take;
+      }
+    // Runs to key ranges, in key order; runs longer than the page cap split in their slot.
+    std::stable_sort(runs.begin(), runs.end(),
+                     [](const Run &x, const Run &y) { return x.tile < y.tile; });
+    cut_b.reserve(runs.size());
+    int64_t off = 0;
+    for (size_t r = 0; r < runs.size(); r++) {
+      if (r == 0 || runs[r].tile != runs[r - 1].tile) off = 0;
+      const TileItem &t = tiles[runs[r].tile];
+      int64_t c = runs[r].n;
+      while (c > 0) {
+        const int64_t take = std::min<int64_t>(c, cap_tiles);
+        cut_b.push_back({runs[r].tile, runs[r].slot, t.ks + (int)(off * KT),
+                         std::min<int>(t.ke, t.ks + (int)((off + take) * KT))});
+        off += take;
+        c -= take;
+      }
+    }
+  }
+  int64_t rows_a = 0, rows_b = 0;
+  int most_a = 1, most_b = 1;
+  score(cut_a, &rows_a, &most_a);
+  score(cut_b, &rows_b, &most_b);
+  return rows_b < rows_a && most_b <= std::max(kMergeRowsMaxParts, most_a) ? cut_b : cut_a;
+}
+
+// The segments of a cut, grouped by slot and in tile order within each (counting sort); seg_off[s]
+// is slot s's first.  make(tile, pieces, piece, first piece) gives one segment.
+template <typename F>
+std::vector<TileItem> segments_by_slot(const std::vector<Piece> &cut, int slots,
+                                       std::vector<int32_t> *seg_off, F make) {
+  std::vector<int32_t> fill(slots + 1, 0);
+  for (const Piece &pc : cut) fill[pc.slot + 1]++;
+  for (int sl = 0; sl < slots; sl++) fill[sl + 1] += fill[sl];
+  seg_off->assign(fill.begin(), fill.end());
+  std::vector<TileItem> segs(cut.size());
+  for (size_t a = 0; a < cut.size();) {
+    size_t b = a;
+    while (b < cut.size() && cut[b].tile == cut[a].tile) b++;
+    const int np = (int)(b - a);
+    for (int pi = 0; pi < np; pi++) {
+      TileItem c = make(cut[a].tile, np, pi);
+      c.ks = cut[a + pi].k0;
+      c.ke = cut[a + pi].k1;
+      segs[fill[cut[a + pi].slot]++] = c;
+    }
+    a = b;
+  }
+  return segs;
+}
+
+// The key chunk of split rows: the largest of 4096..64 keys that still gives the grid at least
+// `many` workgroups, else the largest multiple of 64 that gives it `few`.  len(i) is the keys of row
+// i of n, workgroups the grid's workgroups per chunk.
+template <typename F>
+int key_chunk(int n, F len, int64_t workgroups, int64_t many, int64_t few) {
+  auto items_at = [&](int c) {
+    int64_t items = 0;
+    for (int i = 0; i < n; i++)
+      if (len(i) > 0) items += (len(i) + c - 1) / c;
+    return items * workgroups;
+  };
+  for (int c = 4096; c >= 64; c >>= 1)
+    if (items_at(c) >= many) return c;
+  // items_at falls as the chunk grows: binary search over multiples of 64 in [64, 4096].
+  int lo = 1, hi = 64;  // in units of 64 keys; lo satisfies the bound or is the fallback
+  if (items_at(64) >= few) {
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (items_at(64 * mid) >= few) lo = mid;
+      else hi = mid - 1;
+    }
+  }
+  return 64 * lo;
+}
+
+// A run of query rows that all see the keys [0, len) (nva_internal.h, SpanItem).
+struct Span {
+  int row0, rows, seq, kbase, len;
+};
+
+// How a run of that many rows is computed: the span kernel up to two items of columns, span tiles
+// beyond, row by row where neither serves.
+enum class SpanKernel { rows, items, tiles };
+SpanKernel span_kernel_of(const PlanKey &key, int rows) {
+  const int64_t cols = (int64_t)rows * key.col_heads;
+  if (key.span_cols > 0 && (cols <= 2 * key.span_cols || key.span_tile_cols == 0))
+    return SpanKernel::items;
+  return key.span_tile_cols > 0 ? SpanKernel::tiles : SpanKernel::rows;
+}
+
 // One query row of the row kernel before splitting.
 struct Row {
   int qrow, seq, kbase, kbeg, kend;
@@ -487,6 +725,7 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
   const bool paged = key.paged != 0;
   std::vector<Row> rows;
   std::vector<TileItem> tiles;
+  std::vector<Span> spans;
   int covered = 0;
   // Every page a sequence reads must be a real block of the arena: the reference would throw
   // (ArrayIndexOutOfBounds) where a kernel would read out of bounds.
@@ -503,7 +742,54 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
                     j, t[j], key.num_blocks);
     return NVA_OK;
   };
-  if (!ctx->is_prefill) {
+  // Rows of q of a sequence.
+  auto first_row = [&](int b) {
+    return ctx->is_prefill ? ctx->cu_q[b] : std::min(b, key.tokens);
+  };
+  // Shared prefixes: the rows of a group's sequences see its first keys as one span, and each
+  // sequence's own lists start behind them.  A sliding window sees too little of them.
+  std::vector<int32_t> prefix_len(ctx->num_seqs, 0);
+  if (!key.cross && paged && W == 0)
+    for (const nva_prefix_group &gr : ctx->groups) {
+      const int row0 = first_row(gr.first_seq);
+      const int n = first_row(gr.first_seq + gr.num_seqs) - row0;
+      if (n < 2 || gr.num_tokens <= 0 || span_kernel_of(key, n) == SpanKernel::rows) continue;
+      int seq = gr.first_seq;
+      while (first_row(seq + 1) == row0) seq++;  // the first that has rows
+      spans.push_back({row0, n, seq, 0, gr.num_tokens});
+      for (int b = 0; b < gr.num_seqs; b++) prefix_len[gr.first_seq + b] = gr.num_tokens;
+    }
+  if (key.cross) {
+    // The rows of sequence b see its encoder's keys; sequences in a row that read the same ones
+    // make one span.
+    for (int b = 0; b < ctx->num_seqs; b++) {
+      const int row0 = first_row(b), n = first_row(b + 1) - row0;
+      const int start = ctx->enc_start[b], len = ctx->enc_len[b];
+      if (row0 < 0 || row0 + n > key.tokens)
+        return fail(ctx, NVA_E_ARG, "sequence %d has rows [%d, %d) but q has %d", b, row0, row0 + n,
+                    key.tokens);
+      if ((int64_t)start + len > key.kv_rows)
+        return fail(ctx, NVA_E_ARG, "sequence %d reads encoder rows [%d, %lld) of %lld", b, start,
+                    (long long)start + len, (long long)key.kv_rows);
+      covered += n;
+      if (n == 0) continue;
+      if (!spans.empty()) {
+        Span &last = spans.back();
+        if (last.kbase == start && last.len == len && last.row0 + last.rows == row0) {
+          last.rows += n;
+          continue;
+        }
+      }
+      spans.push_back({row0, n, 0, start, len});
+    }
+    std::vector<Span> kept;
+    for (const Span &sp : spans)
+      if (sp.len > 0 && span_kernel_of(key, sp.rows) != SpanKernel::rows)
+        kept.push_back(sp);
+      else
+        for (int r = 0; r < sp.rows; r++) rows.push_back({sp.row0 + r, 0, sp.kbase, 0, sp.len});
+    spans.swap(kept);
+  } else if (!ctx->is_prefill) {
     // Decode, Attention.java:285-299: row b, kLen = contextLens[b], absQ = kLen - 1.
     const int n = key.tokens;
     rows.reserve(n);
@@ -512,7 +798,7 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
       nva_status st = check_pages(b, klen);
       if (st != NVA_OK) return st;
       const int aq = klen - 1;
-      const int kbeg = W > 0 ? std::max(0, aq - W + 1) : 0;
+      const int kbeg = W > 0 ? std::max(0, aq - W + 1) : prefix_len[b];
       rows.push_back({b, b, 0, kbeg, klen});
     }
     covered = n;
@@ -546,10 +832,10 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
           ti.q0 = t0;
           ti.klen = klen;
           ti.kbase = kbase;
-          ti.ks = W > 0 ? std::max(0, aq0 - W + 1) : 0;
+          ti.ks = W > 0 ? std::max(0, aq0 - W + 1) : prefix_len[b];
           // Over pages of 8 and 16 tokens key tiles start at multiples of 8 keys, where the split
           // kernel reads whole runs of rows from one page (the window masks the keys before it).
-          if (paged && (key.block_size == 8 || key.block_size == 16) && !key.fp32_tiles)
+          if (W > 0 && paged && (key.block_size == 8 || key.block_size == 16) && !key.fp32_tiles)
             ti.ks &= ~7;
           ti.ke = aq1 + 1;
           ti.part = -1;
@@ -562,7 +848,7 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
         for (int qi = 0; qi < qlen; qi++) {
           const int aq = klen - qlen + qi;
           const int kend = aq + 1;
-          const int kbeg = W > 0 ? std::max(0, aq - W + 1) : 0;
+          const int kbeg = W > 0 ? std::max(0, aq - W + 1) : prefix_len[b];
           rows.push_back({q0 + qi, b, kbase, kbeg, kend});
         }
       }
@@ -570,16 +856,134 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
   }
   plan->covers_all = covered == key.tokens;
 
+  std::vector<MergeItem> merges;
+  int parts = 0;
+  const int64_t page_cap =  // most keys of one tile segment, in whole key tiles
+      paged ? (int64_t)(kPrefillTablePages - 2) * key.block_size / 32 * 32 : INT32_MAX;
+
+  // Spans.  span_parts[r] partials of row r come from its span, the first at row_part[r]; its own
+  // keys, if any, add theirs below and the merge joins them.  Rows without own keys (cross attention)
+  // whose span is not split are written at once.
+  std::vector<int32_t> row_part, span_parts;
+  auto prefix_parts = [&](int row) { return span_parts.empty() ? 0 : span_parts[row]; };
+  std::vector<SpanItem> span_items;
+  std::vector<TileItem> span_tiles;
+  std::vector<int32_t> span_off;
+  int span_slots = 0;
+  if (!spans.empty()) {
+    row_part.assign(key.tokens, 0);
+    span_parts.assign(key.tokens, 0);
+    const int groups = key.num_heads / key.num_kv_heads / key.col_heads;
+    // Row r has `pieces` partials from its span (none if it is written at once).
+    auto split_row = [&](int r, int pieces) {
+      if (key.cross && pieces == 1) return;
+      span_parts[r] = pieces;
+      if (!key.cross) return;  // placed with the row's own
+      row_part[r] = parts;
+      merges.push_back({r, parts, pieces, 0});
+      parts += pieces;
+    };
+    double tile_keys = 0.0;
+    for (const Span &sp : spans)
+      if (span_kernel_of(key, sp.rows) == SpanKernel::tiles) {
+        const int cols = sp.rows * key.col_heads;
+        const int per_tile = key.span_tile_cols / key.col_heads * key.col_heads;  // whole rows
+        for (int c = 0; c < cols; c += per_tile)
+          span_tiles.push_back({sp.seq, sp.row0, std::min(cols, c + per_tile), c, 0, sp.kbase, 0,
+                                sp.len, -1, 1, 0, 0});
+        tile_keys += (double)sp.rows * sp.len;
+      } else {
+        const int per_item = key.span_cols / key.col_heads;  // rows
+        for (int r = 0; r < sp.rows; r += per_item) {
+          const int n = std::min(per_item, sp.rows - r);
+          span_items.push_back({sp.row0 + r, n * key.col_heads, sp.seq, sp.kbase, 0, sp.len, 0, 0});
+        }
+      }
+    // Beside span items, and with no span tiles, the rows of the step are items too: one launch.
+    const size_t own_items = span_items.size();
+    const bool rows_join = !span_items.empty() && span_tiles.empty() && !key.cross;
+    if (rows_join) {
+      for (const Row &r : rows)
+        span_items.push_back({r.qrow, key.col_heads, r.seq, r.kbase, r.kbeg, r.kend, 0, 0});
+      rows.clear();
+    }
+    if (!span_tiles.empty()) {
+      int64_t total = 0;
+      for (const TileItem &t : span_tiles) total += (t.ke + 31) / 32;
+      const int grid_y = key.num_kv_heads * groups;
+      int64_t resident = (int64_t)ctx->num_cus * key.span_blocks_per_cu;
+      if (!rows.empty() || !span_items.empty()) {
+        // The rows and items run beside the tiles, as in a mixed step.
+        double keys = 0.0;
+        for (const Row &r : rows) keys += std::max(0, r.kend - r.kbeg);
+        for (const SpanItem &it : span_items) keys += it.kend - it.kbeg;
+        resident = std::max<int64_t>(
+            grid_y, mixed_tile_cus(ctx->num_cus, keys * 8.0 * key.num_kv_heads * key.head_dim,
+                                   4.0 * key.head_dim * key.num_heads * tile_keys, key.head_dim,
+                                   false));
+      }
+      span_slots = (int)std::max<int64_t>(1, std::min<int64_t>(total, resident / grid_y));
+      std::vector<int> tile_rows(span_tiles.size());
+      for (size_t i = 0; i < span_tiles.size(); i++)
+        tile_rows[i] = (span_tiles[i].qlen - span_tiles[i].q0) / key.col_heads;
+      const std::vector<Piece> cut =
+          cut_tiles(span_tiles, tile_rows, span_slots, std::max<int64_t>(1, page_cap / 32));
+      span_tiles = segments_by_slot(cut, span_slots, &span_off, [&](int i, int np, int pi) {
+        TileItem c = span_tiles[i];
+        if (pi == 0)
+          for (int r = 0; r < tile_rows[i]; r++)
+            split_row(c.qstart + c.q0 / key.col_heads + r, np);
+        c.part = key.cross && np == 1 ? -1 : 0;
+        c.nsplit = np;
+        c.split = pi;
+        return c;
+      });
+    }
+    if (!span_items.empty()) {
+      int chunk = key_chunk(
+          (int)span_items.size(), [&](int i) { return span_items[i].kend - span_items[i].kbeg; },
+          (int64_t)key.num_kv_heads * groups, (int64_t)ctx->num_cus * 8, ctx->num_cus);
+      if (paged) chunk = std::min(chunk, (kRowTablePages - 1) * key.block_size);
+      std::vector<SpanItem> cut;
+      for (size_t i = 0; i < span_items.size(); i++) {
+        SpanItem it = span_items[i];
+        const int len = it.kend - it.kbeg, n = (len + chunk - 1) / chunk;
+        int first = 0;  // of the pieces' partials, behind row_part
+        if (i < own_items) {
+          for (int r = 0; r < it.cols / key.col_heads; r++) split_row(it.row0 + r, n);
+          if (key.cross && n == 1) first = -1;
+        } else {  // a row's own keys
+          const int prefix = span_parts[it.row0];
+          first = prefix > 0 || n > 1 ? prefix : -1;
+          if (len <= 0 || first >= 0) merges.push_back({it.row0, parts, len <= 0 ? 0 : prefix + n, 0});
+          row_part[it.row0] = parts;
+          if (len > 0 && first >= 0) parts += prefix + n;
+        }
+        const int kbeg = it.kbeg, kend = it.kend;
+        for (int j = 0; j < n; j++) {
+          it.kbeg = kbeg + j * chunk;
+          it.kend = std::min(kend, it.kbeg + chunk);
+          it.split = first < 0 ? -1 : first + j;
+          cut.push_back(it);
+        }
+      }
+      span_items.swap(cut);
+      std::stable_sort(span_items.begin(), span_items.end(),
+                       [](const SpanItem &x, const SpanItem &y) {
+                         return x.kend - x.kbeg > y.kend - y.kbeg;
+                       });
+    }
+  }
+
   // Stream-K schedule of the MFMA tiles.  The grid has exactly as many workgroups per head
   // group ("slots") as can be resident at once; the 32-key tiles of all query tiles are cut
   // into equal runs, one per slot, so every slot finishes at the same time.  A query tile whose
   // keys fall into several runs becomes several segments; they write partials (query-major,
   // segment-minor) that the merge kernel combines.  A segment also never spans more pages than
   // the kernel's LDS copy of the block table holds.
-  std::vector<MergeItem> merges;
   std::vector<int32_t> seg_off;
-  int parts = 0;
   int slots = 0;
+  int tile_part = -1;
   if (!tiles.empty()) {
     constexpr int KT = 32;
     int64_t total = 0;
@@ -587,15 +991,16 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
     // A mixed plan runs its rows on a second stream beside the tiles; the tile grid then has
     // one workgroup on each of a share of the CUs, and the rows take the rest.
     int64_t resident = (int64_t)ctx->num_cus * key.blocks_per_cu;
-    if (!rows.empty()) {
+    if (!rows.empty() || !span_items.empty()) {
       double row_bytes = 0.0, pairs = 0.0;
       for (const Row &r : rows) row_bytes += std::max(0, r.kend - r.kbeg);
+      for (const SpanItem &it : span_items) row_bytes += it.kend - it.kbeg;
       row_bytes *= 8.0 * key.num_kv_heads * key.head_dim;
       for (const TileItem &t : tiles) {
         const int n = std::min(key.tile_q, t.qlen - t.q0);
         for (int i = 0; i < n; i++) {
           const int aq = t.klen - t.qlen + t.q0 + i;
-          pairs += W > 0 ? std::min(aq + 1, W) : aq + 1;
+          pairs += W > 0 ? std::min(aq + 1, W) : aq + 1 - t.ks;
         }
       }
       const double flops = 4.0 * key.head_dim * key.num_heads * pairs;
@@ -604,173 +1009,33 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
                                                 key.fp32_tiles != 0));
     }
     slots = (int)std::max<int64_t>(1, std::min<int64_t>(total, resident / key.tile_groups));
-    const int64_t page_cap =
-        paged ? (int64_t)(kPrefillTablePages - 2) * key.block_size / KT * KT : INT32_MAX;
-    // Two ways to cut the tiles into equal runs; the plan keeps the one that splits fewer
-    // query rows (each split row writes and re-reads one partial per segment), unless that one
-    // cuts a tile into more segments than the row-wide merge folds:
-    //  (a) the query tiles in sequence order, laid end to end, cut at every slot boundary;
-    //  (b) tiles longer than a run (cap = ceil(total / slots) key tiles) first, largest first,
-    //      each filling whole empty slots and its remainder going to the fullest slot it fits;
-    //      then the other tiles whole, largest first, each into the fullest slot it fits; what
-    //      is left goes, piece by piece, to the emptiest slot.
-    // Both give every slot the same number of key tiles (to one).  Measured splits (rows):
-    // Qwen3-0.6B varlen prefill 512/1024/1536/2048 6784 (a) / 5696 (b), Gemma3 d = 256 global
-    // 11648 / 8192, with a 512-key window 9472 / 8832.
-    // Pieces of both cuts in flat arrays, grouped by tile in key order (the plan is rebuilt
-    // every step, so it avoids a small allocation per tile).
-    struct Piece {
-      int tile, slot, k0, k1;
-    };
     const int64_t cap_tiles = std::max<int64_t>(1, page_cap / KT);
-    const int nt = (int)tiles.size();
-    std::vector<int64_t> ntile(nt);
-    for (int i = 0; i < nt; i++) ntile[i] = (tiles[i].ke - tiles[i].ks + KT - 1) / KT;
-    // Rows written as partials, and the most segments of one tile.
-    auto score = [&](const std::vector<Piece> &pc, int64_t *rows, int *most) {
-      *rows = 0;
-      *most = 1;
-      for (size_t a = 0; a < pc.size();) {
-        size_t b = a;
-        while (b < pc.size() && pc[b].tile == pc[a].tile) b++;
-        const int np = (int)(b - a);
-        const TileItem &t = tiles[pc[a].tile];
-        if (np > 1) *rows += (int64_t)np * std::min(key.tile_q, t.qlen - t.q0);
-        *most = std::max(*most, np);
-        a = b;
-      }
-    };
-    std::vector<Piece> cut_a, cut_b;
-    cut_a.reserve(nt + slots);
-    {
-      int64_t pos = 0;  // first key tile of the current query tile in the flattened order
-      for (int i = 0; i < nt; i++) {
-        const TileItem &t = tiles[i];
-        const int64_t n = ntile[i];
-        int64_t j = 0;
-        while (j < n) {
-          const int64_t g = pos + j;
-          const int s_of = (int)std::min<int64_t>(slots - 1, g * slots / total);
-          const int64_t s_end = ((int64_t)(s_of + 1) * total + slots - 1) / slots;  // exclusive
-          int64_t take = std::min<int64_t>(n - j, s_end - g);
-          take = std::max<int64_t>(1, std::min<int64_t>(take, cap_tiles));
-          cut_a.push_back({i, s_of, t.ks + (int)(j * KT),
-                           std::min<int>(t.ke, t.ks + (int)((j + take) * KT))});
-          j += take;
-        }
-        pos += n;
-      }
-    }
-    {
-      const int64_t cap = (total + slots - 1) / slots;
-      std::vector<int64_t> load(slots, 0), rem(nt, 0);
-      struct Run {
-        int tile, slot;
-        int64_t n;
-      };
-      std::vector<Run> runs;
-      runs.reserve(nt + 2 * slots);
-      std::vector<int> order(nt);
-      for (int i = 0; i < nt; i++) order[i] = i;
-      std::stable_sort(order.begin(), order.end(),
-                       [&](int x, int y) { return ntile[x] > ntile[y]; });
-      auto fullest_fit = [&](int64_t n) {
-        int best = -1;
-        for (int b = 0; b < slots; b++)
-          if (load[b] + n <= cap && (best < 0 || load[b] > load[best])) best = b;
-        return best;
-      };
-      int empty = 0;  // slots below this index are not empty
-      for (int i : order) {
-        if (ntile[i] <= cap) continue;
-        rem[i] = ntile[i];
-        while (rem[i] >= cap) {
-          while (empty < slots && load[empty] != 0) empty++;
-          if (empty == slots) break;
-          load[empty] = cap;
-          runs.push_back({i, empty, cap});
-          rem[i] -= cap;
-        }
-        if (rem[i] > 0) {
-          const int b = fullest_fit(rem[i]);
-          if (b >= 0) {
-            load[b] += rem[i];
-            runs.push_back({i, b, rem[i]});
-            rem[i] = 0;
+    std::vector<int> tile_rows(tiles.size());
+    for (size_t i = 0; i < tiles.size(); i++)
+      tile_rows[i] = std::min(key.tile_q, tiles[i].qlen - tiles[i].q0);
+    const std::vector<Piece> cut = cut_tiles(tiles, tile_rows, slots, cap_tiles);
+    std::vector<TileItem> segs =
+        segments_by_slot(cut, slots, &seg_off, [&](int i, int np, int pi) {
+          TileItem c = tiles[i];
+          const int first = c.qstart + c.q0;
+          // Beside its own pieces a row has the partials of its prefix.
+          int prefix = 0;
+          for (int r = 0; r < tile_rows[i]; r++) prefix = std::max(prefix, prefix_parts(first + r));
+          const int stride = np + prefix;
+          if (pi == 0) {
+            tile_part = stride > 1 ? parts : -1;
+            for (int r = 0; stride > 1 && r < tile_rows[i]; r++) {
+              merges.push_back(
+                  {first + r, parts + r * stride, np + prefix_parts(first + r), 0});
+              if (prefix > 0) row_part[first + r] = parts + r * stride + np;
+            }
+            if (stride > 1) parts += tile_rows[i] * stride;
           }
-        }
-      }
-      for (int i : order) {
-        if (ntile[i] > cap) continue;
-        const int b = fullest_fit(ntile[i]);
-        if (b >= 0) {
-          load[b] += ntile[i];
-          runs.push_back({i, b, ntile[i]});
-        } else {
-          rem[i] = ntile[i];
-        }
-      }
-      for (int i : order)
-        while (rem[i] > 0) {
-          int b = 0;
-          for (int x = 1; x < slots; x++)
-            if (load[x] < load[b]) b = x;
-          const int64_t take = load[b] < cap ? std::min<int64_t>(rem[i], cap - load[b]) : rem[i];
-          load[b] += take;
-          runs.push_back({i, b, take});
-          rem[i] -= take;
-        }
-      // Runs to key ranges, in key order; runs longer than the page cap split in their slot.
-      std::stable_sort(runs.begin(), runs.end(),
-                       [](const Run &x, const Run &y) { return x.tile < y.tile; });
-      cut_b.reserve(runs.size());
-      int64_t off = 0;
-      for (size_t r = 0; r < runs.size(); r++) {
-        if (r == 0 || runs[r].tile != runs[r - 1].tile) off = 0;
-        const TileItem &t = tiles[runs[r].tile];
-        int64_t c = runs[r].n;
-        while (c > 0) {
-          const int64_t take = std::min<int64_t>(c, cap_tiles);
-          cut_b.push_back({runs[r].tile, runs[r].slot, t.ks + (int)(off * KT),
-                           std::min<int>(t.ke, t.ks + (int)((off + take) * KT))});
-          off += take;
-          c -= take;
-        }
-      }
-    }
-    int64_t rows_a = 0, rows_b = 0;
-    int most_a = 1, most_b = 1;
-    score(cut_a, &rows_a, &most_a);
-    score(cut_b, &rows_b, &most_b);
-    const std::vector<Piece> &cut =
-        rows_b < rows_a && most_b <= std::max(kMergeRowsMaxParts, most_a) ? cut_b : cut_a;
-    // Segments grouped by slot (counting sort), each slot's in tile order.
-    std::vector<int32_t> fill(slots + 1, 0);
-    for (const Piece &pc : cut) fill[pc.slot + 1]++;
-    for (int sl = 0; sl < slots; sl++) fill[sl + 1] += fill[sl];
-    seg_off.assign(fill.begin(), fill.end());
-    std::vector<TileItem> segs(cut.size());
-    for (size_t a = 0; a < cut.size();) {
-      size_t b = a;
-      while (b < cut.size() && cut[b].tile == cut[a].tile) b++;
-      const TileItem &t = tiles[cut[a].tile];
-      const int np = (int)(b - a);
-      const int rows = std::min(key.tile_q, t.qlen - t.q0);
-      for (int pi = 0; pi < np; pi++) {
-        TileItem c = t;
-        c.ks = cut[a + pi].k0;
-        c.ke = cut[a + pi].k1;
-        c.part = np > 1 ? parts : -1;
-        c.nsplit = np;
-        c.split = pi;
-        segs[fill[cut[a + pi].slot]++] = c;
-      }
-      if (np > 1) {
-        for (int r = 0; r < rows; r++) merges.push_back({t.qstart + t.q0 + r, parts + r * np, np, 0});
-        parts += rows * np;
-      }
-      a = b;
-    }
+          c.part = tile_part;
+          c.nsplit = stride;
+          c.split = pi;
+          return c;
+        });
     tiles.swap(segs);
   }
 
@@ -787,29 +1052,9 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
   // keeps 64.
   int64_t total = 0;
   for (const Row &r : rows) total += std::max(0, r.kend - r.kbeg);
-  auto items_at = [&](int c) {
-    int64_t items = 0;
-    for (const Row &r : rows) {
-      const int len = r.kend - r.kbeg;
-      if (len > 0) items += (len + c - 1) / c;
-    }
-    return items * key.wg_per_item;
-  };
-  int chunk = 0;
-  for (int c = 4096; c >= 64 && !chunk; c >>= 1)
-    if (items_at(c) >= (int64_t)ctx->num_cus * 8) chunk = c;
-  if (!chunk) {
-    // items_at falls as the chunk grows: binary search over multiples of 64 in [64, 4096].
-    int lo = 1, hi = 64;  // in units of 64 keys; lo satisfies the bound or is the fallback
-    if (items_at(64) >= (int64_t)ctx->num_cus) {
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (items_at(64 * mid) >= (int64_t)ctx->num_cus) lo = mid;
-        else hi = mid - 1;
-      }
-    }
-    chunk = 64 * lo;
-  }
+  int chunk = key_chunk(
+      (int)rows.size(), [&](int i) { return rows[i].kend - rows[i].kbeg; }, key.wg_per_item,
+      (int64_t)ctx->num_cus * 8, ctx->num_cus);
   // A paged item of `chunk` keys spans at most (chunk - 1) / BS + 2 pages; the row kernel
   // stages at most kRowTablePages of them.
   if (key.paged) chunk = std::min(chunk, (kRowTablePages - 1) * key.block_size);
@@ -822,19 +1067,20 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
       merges.push_back({r.qrow, 0, 0, 0});
       continue;
     }
-    const int rchunk = chunk;
-    if (len <= rchunk) {
+    const int prefix = prefix_parts(r.qrow);
+    if (len <= chunk && prefix == 0) {
       items.push_back({r.qrow, r.seq, r.kbase, r.kbeg, r.kend, -1, 0, 0});
       continue;
     }
-    const int n = (len + rchunk - 1) / rchunk;
+    const int n = (len + chunk - 1) / chunk;
     for (int j = 0; j < n; j++) {
-      const int b0 = r.kbeg + j * rchunk;
-      const int b1 = std::min(r.kend, b0 + rchunk);
+      const int b0 = r.kbeg + j * chunk;
+      const int b1 = std::min(r.kend, b0 + chunk);
       items.push_back({r.qrow, r.seq, r.kbase, b0, b1, parts + j, 0, 0});
     }
-    merges.push_back({r.qrow, parts, n, 0});
-    parts += n;
+    merges.push_back({r.qrow, parts, n + prefix, 0});
+    if (prefix > 0) row_part[r.qrow] = parts + n;
+    parts += n + prefix;
   }
   // Items within at most two pages carry the pages' block ids (RowItem::blk_a / blk_b).
   if (key.paged) {
@@ -861,7 +1107,12 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
     for (const RowItem &it : items)
       if (it.kend > it.kbeg && (it.kend - 1) / bs - it.kbeg / bs + 1 > kRowTablePages)
         return fail(ctx, NVA_E_UNSUPPORTED, "row item spans more than %d pages", kRowTablePages);
-    for (const TileItem &t : tiles)
+    for (const SpanItem &it : span_items)
+      if (it.kend <= it.kbeg || (it.kend - 1) / bs - it.kbeg / bs + 1 > kRowTablePages)
+        return fail(ctx, NVA_E_UNSUPPORTED, "span item is empty or spans more than %d pages",
+                    kRowTablePages);
+    for (const std::vector<TileItem> *list : {&tiles, &span_tiles})
+     for (const TileItem &t : *list)
       if (t.ke > t.ks && (t.ke - 1) / bs - t.ks / bs + 1 > kPrefillTablePages)
         return fail(ctx, NVA_E_UNSUPPORTED, "prefill segment spans more than %d pages",
                     kPrefillTablePages);
@@ -875,18 +1126,26 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
   plan->num_slots = slots;
   plan->max_parts = 0;
   for (const MergeItem &mi : merges) plan->max_parts = std::max(plan->max_parts, mi.nparts);
-  plan->off_rows = 0;
-  plan->off_merge = plan->off_rows + items.size() * sizeof(RowItem);
-  plan->off_tiles = plan->off_merge + merges.size() * sizeof(MergeItem);
-  plan->off_slots = plan->off_tiles + tiles.size() * sizeof(TileItem);
-  plan->host.resize(plan->off_slots + seg_off.size() * sizeof(int32_t));
-  char *h = plan->host.data();
-  if (!items.empty()) memcpy(h + plan->off_rows, items.data(), items.size() * sizeof(RowItem));
-  if (!merges.empty())
-    memcpy(h + plan->off_merge, merges.data(), merges.size() * sizeof(MergeItem));
-  if (!tiles.empty()) memcpy(h + plan->off_tiles, tiles.data(), tiles.size() * sizeof(TileItem));
-  if (!seg_off.empty())
-    memcpy(h + plan->off_slots, seg_off.data(), seg_off.size() * sizeof(int32_t));
+  plan->num_spans = (int)span_items.size();
+  plan->max_cols = 0;
+  for (const SpanItem &it : span_items) plan->max_cols = std::max(plan->max_cols, it.cols);
+  plan->num_span_tiles = (int)span_tiles.size();
+  plan->num_span_slots = span_slots;
+  plan->host.clear();
+  auto pack = [&](const auto &list) {
+    const size_t off = plan->host.size();
+    const char *p = reinterpret_cast<const char *>(list.data());
+    plan->host.insert(plan->host.end(), p, p + list.size() * sizeof(list[0]));
+    return off;
+  };
+  plan->off_rows = pack(items);
+  plan->off_merge = pack(merges);
+  plan->off_tiles = pack(tiles);
+  plan->off_slots = pack(seg_off);
+  plan->off_spans = pack(span_items);
+  plan->off_span_tiles = pack(span_tiles);
+  plan->off_span_slots = pack(span_off);
+  plan->off_row_part = pack(row_part);
   static std::atomic<uint64_t> next_id{1};
   plan->id = next_id.fetch_add(1);
   plan->on_device = false;
@@ -917,10 +1176,11 @@ KvView make_paged_view(nva_ctx *ctx, nva_kv *kv, int layer) {
   v.block_size = kv->block_size;
   v.bs_shift = pow2_shift(kv->block_size);
   v.paged = 1;
+  v.ld = kv->num_kv_heads * kv->head_dims[layer];
   return v;
 }
 
-KvView make_dense_view(const float *k, const float *v) {
+KvView make_dense_view(const float *k, const float *v, int ld) {
   KvView view;
   view.k = k;
   view.v = v;
@@ -929,6 +1189,7 @@ KvView make_dense_view(const float *k, const float *v) {
   view.block_size = 1;
   view.bs_shift = 0;
   view.paged = 0;
+  view.ld = ld;
   return view;
 }
 
@@ -947,6 +1208,12 @@ KvView make_dense_view(const float *k, const float *v) {
 // tokens 23.0 / 27.1, 14+295 35.7 / 33.6; 4 q / 1 KV, d = 256, 22 and 3+7 15.7 / 16.3, 400 33.8 /
 // 32.0, 3736+100 43.6 / 36.6; 8 q / 1 KV, d = 512, 663+23 and 22 28.2 / 29.9, 300 42.2 / 39.0, 400
 // 52.0 / 44.6.
+int prefix_tokens(const nva_ctx *ctx, int seq) {
+  for (const nva_prefix_group &gr : ctx->groups)
+    if (seq >= gr.first_seq && seq < gr.first_seq + gr.num_seqs) return gr.num_tokens;
+  return 0;
+}
+
 bool use_fp32_tiles(nva_ctx *ctx, const nva_attn_desc &d, int hpw_fp32, int hpw_split, int window) {
   struct Cost {
     double floor, per_wave;  // CU us per key tile: at least, and per active wave
@@ -964,7 +1231,7 @@ bool use_fp32_tiles(nva_ctx *ctx, const nva_attn_desc &d, int hpw_fp32, int hpw_
       for (int t0 = 0; t0 < qlen; t0 += tile_q) {
         const int n = std::min(tile_q, qlen - t0);
         const int first = klen - qlen + t0;
-        const int ks = window > 0 ? std::max(0, first - window + 1) : 0;
+        const int ks = window > 0 ? std::max(0, first - window + 1) : prefix_tokens(ctx, b);
         const double work = c.per_wave * hpw * ((n + c.queries - 1) / c.queries);
         sum += std::max(c.floor, work) * ((first + n - ks + 31) / 32);
         longest = std::max(longest, std::max(c.floor * c.per_cu, work));
@@ -992,13 +1259,18 @@ bool fp32_tiles(nva_ctx *ctx, const nva_attn_desc &d, int hpw_fp32, int hpw_spli
   return fp32;
 }
 
+// What a cross attention call reads: a pool of kv_rows rows.
+struct CrossRows {
+  int64_t kv_rows;
+};
+
 // The plan of one attention call (the descriptor, the step, and whether keys are paged over
 // an arena of num_blocks pages of block_size tokens or dense rows), plus the query heads per
 // workgroup of the row and tile kernels.
 nva_status attention_plan(nva_ctx *ctx, const nva_attn_desc &d, int paged, int block_size,
                           int num_blocks, int num_tokens, Plan **plan, int *hpw_row,
                           int *hpw_tile, bool *rows_mfma = nullptr,
-                          bool *tiles_fp32 = nullptr) {
+                          bool *tiles_fp32 = nullptr, const CrossRows *cross = nullptr) {
   const int rep = d.num_heads / d.num_kv_heads;
   // Query heads per row workgroup: the largest divisor of the GQA ratio the row kernel is built
   // for, so each K/V byte crosses HBM once per KV head (one head per workgroup at a ratio of 5
@@ -1014,7 +1286,8 @@ nva_status attention_plan(nva_ctx *ctx, const nva_attn_desc &d, int paged, int b
   // than with 4, Gemma 4 d = 512 3% faster with 1 than with 4, Qwen3-4B shape 4% faster with 2
   // than with 4).
   *hpw_tile = largest_pow2_divisor_upto(rep, prefill_max_heads(d.head_dim));
-  const bool mfma = ctx->is_prefill && prefill_kernel_supports(d.head_dim, *hpw_tile);
+  const bool mfma =
+      ctx->is_prefill && !cross && prefill_kernel_supports(d.head_dim, *hpw_tile);
   const int window = d.sliding_window > 0 ? d.sliding_window : 0;
   const int hpw_fp32 = largest_pow2_divisor_upto(rep, prefill_fp32_max_heads(d.head_dim));
   const bool fp32 = mfma && fp32_tiles(ctx, d, hpw_fp32, *hpw_tile, window);
@@ -1056,6 +1329,19 @@ nva_status attention_plan(nva_ctx *ctx, const nva_attn_desc &d, int paged, int b
   key.head_dim = d.head_dim;
   key.num_heads = d.num_heads;
   key.num_kv_heads = d.num_kv_heads;
+  if (cross || (!ctx->groups.empty() && paged && window == 0)) {
+    key.cross = cross ? 1 : 0;
+    key.kv_rows = cross ? cross->kv_rows : 0;
+    const bool tiles = prefill_kernel_supports(d.head_dim, 1);
+    const bool items = span_kernel_supports(d.head_dim, paged, block_size);
+    key.span_tile_cols = tiles ? span_tile_cols(d.head_dim) : 0;
+    key.span_cols = items ? span_max_cols(d.head_dim) : 0;
+    // A column group holds whole rows of a tile and of an item.
+    const int most = std::min(tiles ? key.span_tile_cols : rep, items ? key.span_cols : rep);
+    key.col_heads = std::min(rep, most);
+    while (rep % key.col_heads) key.col_heads--;
+    key.span_blocks_per_cu = tiles ? ctx_span_blocks_per_cu(ctx, d.head_dim) : 0;
+  }
   return get_plan(ctx, key, plan);
 }
 
@@ -1087,6 +1373,23 @@ bool stream_capturing(hipStream_t s) {
   return hipStreamIsCapturing(s, &cs) == hipSuccess && cs != hipStreamCaptureStatusNone;
 }
 
+// Whether a plan's call fits the array and, under stream capture, finds its plan there.
+nva_status noalloc_fits(nva_ctx *ctx, const Plan &plan, const nva_attn_desc &d, size_t gather) {
+  const ScratchLayout l = scratch_layout(gather, plan, d);
+  if (l.end > kScratchBytes)
+    return fail(ctx, NVA_E_ARG,
+                "this call needs %zu bytes of device scratch (plan %zu, partials %zu, gather "
+                "%zu); the no-allocation entry point has %zu",
+                l.end, plan.host.size(), l.part_bytes, gather, kScratchBytes);
+  const ScratchTag &tag = scratch_tag(ctx->device);
+  if (!plan.host.empty() && (tag.plan_id != plan.id || tag.offset != l.plan_off) &&
+      stream_capturing(ctx->stream))
+    return fail(ctx, NVA_E_ARG,
+                "under stream capture the step's plan must already be in the device scratch "
+                "array: make one call with this configuration outside capture first");
+  return NVA_OK;
+}
+
 // Checks of a no-allocation call made before it launches anything (so a rejected call leaves
 // the pages and the array untouched): the array must hold the call's gather rows, plan and
 // partials, and under stream capture the plan must already be in it (a captured copy would
@@ -1108,31 +1411,19 @@ nva_status noalloc_prepare(nva_ctx *ctx, nva_kv *kv, const nva_attn_desc &d, int
                                  dense ? 0 : kv->num_blocks, num_tokens, &plan, &hpw_row,
                                  &hpw_tile);
   if (st != NVA_OK) return st;
-  const ScratchLayout l = scratch_layout(gather, *plan, d);
-  if (l.end > kScratchBytes)
-    return fail(ctx, NVA_E_ARG,
-                "this call needs %zu bytes of device scratch (plan %zu, partials %zu, gather "
-                "%zu); the no-allocation entry point has %zu",
-                l.end, plan->host.size(), l.part_bytes, gather, kScratchBytes);
-  const ScratchTag &tag = scratch_tag(ctx->device);
-  if (!plan->host.empty() && (tag.plan_id != plan->id || tag.offset != l.plan_off) &&
-      stream_capturing(ctx->stream))
-    return fail(ctx, NVA_E_ARG,
-                "under stream capture the step's plan must already be in the device scratch "
-                "array: make one call with this configuration outside capture first");
-  return NVA_OK;
+  return noalloc_fits(ctx, *plan, d, gather);
 }
 
 // The attention part of Attention.forward once the store (if any) is done.  With scr null the
 // plan and partials use the context's buffers; otherwise the scratch array's regions.
 nva_status run_attention(nva_ctx *ctx, const nva_attn_desc &d, const KvView &view,
                          int num_blocks, const float *q, int num_tokens, float *out,
-                         Scratch *scr) {
+                         Scratch *scr, const CrossRows *cross = nullptr) {
   Plan *plan = nullptr;
   int hpw_row = 0, hpw_tile = 0;
   bool rows_mfma = false, tiles_fp32 = false;
   nva_status st = attention_plan(ctx, d, view.paged, view.block_size, num_blocks, num_tokens,
-                                 &plan, &hpw_row, &hpw_tile, &rows_mfma, &tiles_fp32);
+                                 &plan, &hpw_row, &hpw_tile, &rows_mfma, &tiles_fp32, cross);
   if (st != NVA_OK) return st;
   const int window = d.sliding_window > 0 ? d.sliding_window : 0;
 
@@ -1178,25 +1469,39 @@ nva_status run_attention(nva_ctx *ctx, const nva_attn_desc &d, const KvView &vie
   // main stream waits for the side stream before the merge.  The tiles are issued first: the
   // plan sized their grid to a share of the CUs, which it only gets if the rows do not fill
   // the chip before it.
-  const bool fork = plan->num_tiles > 0 && plan->num_rows > 0;
+  const bool fork = (plan->num_tiles > 0 || plan->num_span_tiles > 0) &&
+                    (plan->num_rows > 0 || plan->num_spans > 0);
+  const int32_t *row_part = reinterpret_cast<const int32_t *>(pbase + plan->off_row_part);
   if (fork) HIP_TRY(ctx, hipEventRecord(ctx->fork_ev, ctx->stream), "fork record");
+  TileLaunch t;
+  t.q = q;
+  t.out = out;
+  t.kv = view;
+  t.hq = d.num_heads;
+  t.hkv = d.num_kv_heads;
+  t.head_dim = d.head_dim;
+  t.scale = d.scale;
+  t.part_m = pm;
+  t.part_l = pm + parts;
+  t.part_acc = pm + 2 * parts;
+  if (plan->num_span_tiles > 0) {
+    t.items = reinterpret_cast<const TileItem *>(pbase + plan->off_span_tiles);
+    t.seg_off = reinterpret_cast<const int32_t *>(pbase + plan->off_span_slots);
+    t.num_items = plan->num_span_tiles;
+    t.num_slots = plan->num_span_slots;
+    t.window = 0;
+    t.col_heads = plan->key.col_heads;
+    t.row_part = row_part;
+    Timed tm(ctx, "span_tiles");
+    HIP_TRY(ctx, launch_span_tiles(t, ctx->stream), "span tile kernel launch");
+    tm.done();
+  }
   if (plan->num_tiles > 0) {
-    TileLaunch t;
-    t.q = q;
-    t.out = out;
-    t.kv = view;
     t.items = reinterpret_cast<const TileItem *>(pbase + plan->off_tiles);
     t.seg_off = reinterpret_cast<const int32_t *>(pbase + plan->off_slots);
     t.num_items = plan->num_tiles;
     t.num_slots = plan->num_slots;
-    t.hq = d.num_heads;
-    t.hkv = d.num_kv_heads;
-    t.head_dim = d.head_dim;
     t.window = window;
-    t.scale = d.scale;
-    t.part_m = pm;
-    t.part_l = pm + parts;
-    t.part_acc = pm + 2 * parts;
     Timed tm(ctx, "prefill", nullptr, tiles_fp32 ? "prefill_fp32" : "prefill_split");
     HIP_TRY(ctx,
             tiles_fp32 ? launch_prefill_fp32(t, hpw_tile, ctx->stream)
@@ -1204,12 +1509,32 @@ nva_status run_attention(nva_ctx *ctx, const nva_attn_desc &d, const KvView &vie
             "prefill kernel launch");
     tm.done();
   }
+  hipStream_t row_stream = ctx->stream;
+  if (fork) {
+    HIP_TRY(ctx, hipStreamWaitEvent(ctx->side_stream, ctx->fork_ev, 0), "fork wait");
+    row_stream = ctx->side_stream;
+  }
+  if (plan->num_spans > 0) {
+    SpanLaunch sp;
+    sp.q = q;
+    sp.out = out;
+    sp.kv = view;
+    sp.items = reinterpret_cast<const SpanItem *>(pbase + plan->off_spans);
+    sp.num_items = plan->num_spans;
+    sp.hq = d.num_heads;
+    sp.hkv = d.num_kv_heads;
+    sp.head_dim = d.head_dim;
+    sp.col_heads = plan->key.col_heads;
+    sp.scale = d.scale;
+    sp.row_part = row_part;
+    sp.part_m = pm;
+    sp.part_l = pm + parts;
+    sp.part_acc = pm + 2 * parts;
+    Timed tm(ctx, "span", row_stream);
+    HIP_TRY(ctx, launch_spans(sp, plan->max_cols, row_stream), "span kernel launch");
+    tm.done();
+  }
   if (plan->num_rows > 0) {
-    hipStream_t row_stream = ctx->stream;
-    if (fork) {
-      HIP_TRY(ctx, hipStreamWaitEvent(ctx->side_stream, ctx->fork_ev, 0), "fork wait");
-      row_stream = ctx->side_stream;
-    }
     RowLaunch r;
     r.q = q;
     r.out = out;
@@ -1288,6 +1613,26 @@ nva_status check_desc(nva_ctx *ctx, const nva_attn_desc *d) {
   return NVA_OK;
 }
 
+// The sequences of a prefix group must hold its tokens in the same pages (checked once per step).
+nva_status check_groups(nva_ctx *ctx, int block_size) {
+  if (ctx->groups.empty() || ctx->groups_block_size == block_size) return NVA_OK;
+  for (size_t i = 0; i < ctx->groups.size(); i++) {
+    const nva_prefix_group &g = ctx->groups[i];
+    const int pages = (int)(((int64_t)g.num_tokens + block_size - 1) / block_size);
+    if (pages > ctx->bt_stride)
+      return fail(ctx, NVA_E_ARG, "prefix group %d needs %d pages but the block tables have %d",
+                  (int)i, pages, ctx->bt_stride);
+    const int32_t *t = ctx->tables.data() + (size_t)g.first_seq * ctx->bt_stride;
+    for (int b = 1; b < g.num_seqs; b++)
+      if (memcmp(t, t + (size_t)b * ctx->bt_stride, pages * sizeof(int32_t)) != 0)
+        return fail(ctx, NVA_E_ARG,
+                    "prefix group %d: sequences %d and %d differ within the first %d pages", (int)i,
+                    g.first_seq, g.first_seq + b, pages);
+  }
+  ctx->groups_block_size = block_size;
+  return NVA_OK;
+}
+
 // Shared prologue of nva_attention_forward / nva_rope_attention_forward.
 nva_status check_forward(nva_ctx *ctx, nva_kv *kv, const nva_attn_desc *desc, int num_tokens) {
   nva_status st = check_desc(ctx, desc);
@@ -1314,7 +1659,7 @@ nva_status check_forward(nva_ctx *ctx, nva_kv *kv, const nva_attn_desc *desc, in
   } else if (!ctx->has_cu) {
     return fail(ctx, NVA_E_ARG, "prefill needs cu_seqlens");
   }
-  return NVA_OK;
+  return check_groups(ctx, kv->block_size);
 }
 
 // Which K/V the attention reads, Attention.java:161-170 and :176-195.  scr selects the
@@ -1327,7 +1672,7 @@ nva_status attention_after_store(nva_ctx *ctx, nva_kv *kv, const nva_attn_desc &
   if (ctx->is_prefill && !ctx->has_tables) {
     if (d.write_kv) {
       if (!k || !v) return fail(ctx, NVA_E_ARG, "dense prefill needs k and v");
-      return run_attention(ctx, d, make_dense_view(k, v), 0, q, num_tokens, out, scr);
+      return run_attention(ctx, d, make_dense_view(k, v, d.num_kv_heads * d.head_dim), 0, q, num_tokens, out, scr);
     }
     // Shared-KV dense prefill: gather the producer's rows at the step's slots.
     if (!ctx->has_slots || ctx->num_slots != num_tokens)
@@ -1361,7 +1706,7 @@ nva_status attention_after_store(nva_ctx *ctx, nva_kv *kv, const nva_attn_desc &
     Timed tm(ctx, "gather");
     HIP_TRY(ctx, launch_gather(g, ctx->stream), "gather kernel launch");
     tm.done();
-    return run_attention(ctx, d, make_dense_view(gk, gv), 0, q, num_tokens, out, scr);
+    return run_attention(ctx, d, make_dense_view(gk, gv, (int)row), 0, q, num_tokens, out, scr);
   }
   if (!allocated) return fail(ctx, NVA_E_ARG, "layer %d has no pages to attend over", layer);
   if (!ctx->has_tables) return fail(ctx, NVA_E_ARG, "paged attention needs block tables");
@@ -1742,6 +2087,8 @@ nva_status nva_step_set(nva_ctx *ctx, int is_prefill, const int32_t *cu_q, const
     return fail(ctx, NVA_E_ARG, "block tables need bt_stride > 0");
   for (Plan *p : ctx->plans) p->valid = false;
   ctx->tile_choices.clear();
+  ctx->groups.clear();
+  ctx->has_encoder = false;
   ctx->has_step = true;
   ctx->is_prefill = is_prefill != 0;
   ctx->num_seqs = num_seqs;
@@ -1847,6 +2194,64 @@ nva_status nva_step_clear(nva_ctx *ctx) {
   ctx->has_step = false;
   for (Plan *p : ctx->plans) p->valid = false;
   ctx->tile_choices.clear();
+  ctx->groups.clear();
+  ctx->has_encoder = false;
+  return NVA_OK;
+}
+
+nva_status nva_step_share_prefixes(nva_ctx *ctx, const nva_prefix_group *groups, int num_groups) {
+  if (!ctx) return NVA_E_ARG;
+  if (!ctx->has_step) return fail(ctx, NVA_E_NO_STEP, "no step metadata set on the context");
+  if (num_groups < 0 || (num_groups > 0 && !groups))
+    return fail(ctx, NVA_E_ARG, "prefix groups required");
+  if (num_groups > 0 && !ctx->has_tables)
+    return fail(ctx, NVA_E_ARG, "shared prefixes need block tables");
+  if (num_groups > 0 && !ctx->is_prefill && !ctx->has_ctx_lens)
+    return fail(ctx, NVA_E_ARG, "shared prefixes need context lengths");
+  if (num_groups > 0 && ctx->is_prefill && ctx->num_seqs > 0 && ctx->cu_q[0] != 0)
+    return fail(ctx, NVA_E_ARG, "cuSeqlensQ must start at 0");
+  int next = 0;
+  for (int i = 0; i < num_groups; i++) {
+    const nva_prefix_group &g = groups[i];
+    if (g.first_seq < next || g.num_seqs < 1 || g.num_seqs > ctx->num_seqs - g.first_seq)
+      return fail(ctx, NVA_E_ARG,
+                  "prefix group %d: sequences [%d, +%d) are not a run behind the group before it, of "
+                  "%d",
+                  i, g.first_seq, g.num_seqs, ctx->num_seqs);
+    next = g.first_seq + g.num_seqs;
+    for (int b = g.first_seq; b < next; b++) {
+      const int cached =
+          ctx->is_prefill ? (ctx->cu_k[b + 1] - ctx->cu_k[b]) - (ctx->cu_q[b + 1] - ctx->cu_q[b])
+                          : ctx->ctx_lens[b] - 1;
+      if (g.num_tokens < 0 || g.num_tokens > cached)
+        return fail(ctx, NVA_E_ARG, "prefix group %d: %d tokens, but sequence %d has %d cached", i,
+                    g.num_tokens, b, cached);
+    }
+  }
+  ctx->groups.assign(groups, groups + num_groups);
+  ctx->groups_block_size = 0;
+  for (Plan *p : ctx->plans) p->valid = false;
+  ctx->tile_choices.clear();
+  return NVA_OK;
+}
+
+nva_status nva_step_set_encoder(nva_ctx *ctx, const int32_t *kv_start, const int32_t *kv_len,
+                                int num_seqs) {
+  if (!ctx) return NVA_E_ARG;
+  if (!ctx->has_step) return fail(ctx, NVA_E_NO_STEP, "no step metadata set on the context");
+  if (num_seqs != ctx->num_seqs)
+    return fail(ctx, NVA_E_ARG, "encoder rows of %d sequences, but the step has %d", num_seqs,
+                ctx->num_seqs);
+  if (num_seqs > 0 && (!kv_start || !kv_len))
+    return fail(ctx, NVA_E_ARG, "encoder starts and lengths required");
+  for (int b = 0; b < num_seqs; b++)
+    if (kv_start[b] < 0 || kv_len[b] < 0)
+      return fail(ctx, NVA_E_ARG, "sequence %d: encoder rows [%d, +%d)", b, kv_start[b], kv_len[b]);
+  ctx->enc_start.assign(kv_start, kv_start + num_seqs);
+  ctx->enc_len.assign(kv_len, kv_len + num_seqs);
+  ctx->has_encoder = true;
+  for (Plan *p : ctx->plans)
+    if (p->key.cross) p->valid = false;
   return NVA_OK;
 }
 
@@ -1949,6 +2354,71 @@ nva_status nva_attention_forward_noalloc(nva_ctx *ctx, nva_kv *kv, const nva_att
   Scratch scr;
   scr.base = ctx->scratch;
   return attention_forward(ctx, kv, desc, q, k, v, num_tokens, out, &scr);
+}
+
+static nva_status cross_attention_forward(nva_ctx *ctx, const nva_attn_desc *desc, const float *q,
+                                          const float *k, const float *v, int64_t kv_rows,
+                                          int64_t kv_stride, int num_tokens, float *out,
+                                          Scratch *scr) {
+  nva_status st = check_desc(ctx, desc);
+  if (st != NVA_OK) return st;
+  const nva_attn_desc d = *desc;
+  if (d.sliding_window > 0)
+    return fail(ctx, NVA_E_UNSUPPORTED, "cross attention has no sliding window");
+  if (!ctx->has_step) return fail(ctx, NVA_E_NO_STEP, "no step metadata set on the context");
+  if (!ctx->has_encoder) return fail(ctx, NVA_E_NO_STEP, "no encoder rows set for this step");
+  if (num_tokens < 0 || kv_rows < 0) return fail(ctx, NVA_E_ARG, "negative count");
+  if (ctx->is_prefill ? !ctx->has_cu : num_tokens > ctx->num_seqs)
+    return fail(ctx, NVA_E_ARG, "%d tokens do not fit the step's %d sequences", num_tokens,
+                ctx->num_seqs);
+  if (num_tokens == 0) return NVA_OK;  // empty batch
+  if (!q || !out) return fail(ctx, NVA_E_ARG, "q and out are required");
+  if (kv_rows > 0 && (!k || !v)) return fail(ctx, NVA_E_ARG, "k and v are required");
+  if (!aligned16(q) || !aligned16(out) || !aligned16(k) || !aligned16(v))
+    return fail(ctx, NVA_E_ARG, "device pointers must be 16-byte aligned");
+  // The kernels address a key block's 32 rows with 32-bit byte offsets.
+  const int64_t width = (int64_t)d.num_kv_heads * d.head_dim;
+  if (kv_rows > 0 && (kv_stride < width || kv_stride % 4 || kv_stride >= (1 << 22)))
+    return fail(ctx, NVA_E_ARG,
+                "rows of %lld floats: the stride must be a multiple of 4 from %lld to below 4194304",
+                (long long)kv_stride, (long long)width);
+  const CrossRows rows{kv_rows};
+  if (scr) {
+    Plan *plan = nullptr;
+    int hpw_row = 0, hpw_tile = 0;
+    st = attention_plan(ctx, d, 0, 1, 0, num_tokens, &plan, &hpw_row, &hpw_tile, nullptr, nullptr,
+                        &rows);
+    if (st == NVA_OK) st = noalloc_fits(ctx, *plan, d, 0);
+    if (st != NVA_OK) return st;
+  } else if (stream_capturing(ctx->stream)) {
+    return fail(ctx, NVA_E_ARG,
+                "under stream capture use the no-allocation entry point: this one's buffers may move "
+                "before the graph runs");
+  }
+  return run_attention(ctx, d, make_dense_view(k, v, (int)std::max<int64_t>(kv_stride, width)), 0, q,
+                       num_tokens, out, scr, &rows);
+}
+
+nva_status nva_cross_attention_forward(nva_ctx *ctx, const nva_attn_desc *desc, const float *q,
+                                       const float *k, const float *v, int64_t kv_rows,
+                                       int64_t kv_stride, int num_tokens, float *out) {
+  if (!ctx) return NVA_E_ARG;
+  DeviceGuard dg(ctx);
+  return cross_attention_forward(ctx, desc, q, k, v, kv_rows, kv_stride, num_tokens, out, nullptr);
+}
+
+nva_status nva_cross_attention_forward_noalloc(nva_ctx *ctx, const nva_attn_desc *desc,
+                                               const float *q, const float *k, const float *v,
+                                               int64_t kv_rows, int64_t kv_stride, int num_tokens,
+                                               float *out) {
+  if (!ctx) return NVA_E_ARG;
+  DeviceGuard dg(ctx);
+  if (!ctx->scratch)
+    return fail(ctx, NVA_E_HIP, "device scratch array unavailable on device %d: %s",
+                ctx->device, hipGetErrorString(ctx->scratch_err));
+  Scratch scr;
+  scr.base = ctx->scratch;
+  return cross_attention_forward(ctx, desc, q, k, v, kv_rows, kv_stride, num_tokens, out, &scr);
 }
 
 nva_status nva_rope_attention_forward(nva_ctx *ctx, nva_kv *kv, const nva_rope *rope,

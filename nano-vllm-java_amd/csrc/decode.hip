@@ -31,6 +31,7 @@
 // HBM bytes per work item: chunk * 2 * D * 4 per KV head (+ q, + the partial or output row).
 #include "nva_internal.h"
 #include "nva_device.h"
+#include "row_lanes.h"
 
 namespace nva {
 
@@ -64,57 +65,14 @@ __device__ __forceinline__ void st4(float *p, float4 v) { *reinterpret_cast<floa
 
 // K/V rows are read once per step: non-temporal loads stream them past the caches, which
 // sustains a higher HBM read rate than ordinary loads.
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ float4 ld4_stream(const float *p) {
   const f32x4 t = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(p));
   return make_float4(t.x, t.y, t.z, t.w);
 }
-// The same non-temporal load from a wave-uniform base plus a 32-bit lane offset (floats), as a
-// buffer load: the base stays in scalar registers, so no per-lane 64-bit address is formed
-// (headline decode 2.160-2.162 against 2.166-2.171 ms with the pointer form).  The cache policy
-// matters, the form little: without the non-temporal bit the same loads take 2.40 ms, and
-// adding the L1-bypass (sc0) or device-scope (sc1) bits changes nothing.
-__device__ __forceinline__ float4 ld4_stream_at(const float *base, uint32_t off) {
-  constexpr int kNonTemporal = 2;  // the nt bit of the buffer instructions' cache policy
-  const uint64_t b = (uint64_t)(size_t)base;
-  const uint64_t u = ((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32)) << 32) |
-                     (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b);
-  const __amdgpu_buffer_rsrc_t r =
-      __builtin_amdgcn_make_buffer_rsrc((void *)(size_t)u, (short)0, 0x7fffffff, kBufferWord3);
-  const f32x4 t = __builtin_amdgcn_raw_buffer_load_b128(r, off * 4, 0, kNonTemporal);
-  return make_float4(t.x, t.y, t.z, t.w);
-}
-
 template <int CTRL>
 __device__ __forceinline__ float dpp(float x) {
   return __builtin_amdgcn_update_dpp(0.0f, x, CTRL, 0xF, 0xF, false);
 }
-
-// x[lane] + x[lane ^ 16] (resp. lane ^ 32) in every lane, by gfx950's row-swap instructions:
-// the swap of x with itself leaves one of the two values in each output, and the sum of the
-// two is the same bits in both lanes of a pair.  No LDS round trip, unlike ds_swizzle or
-// ds_bpermute.
-__device__ __forceinline__ float add_xor16(float x) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false,
-                                                  false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-__device__ __forceinline__ float add_xor32(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
-                                                  false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
-// Max and sum over the four lanes {l, l ^ 16, l ^ 32, l ^ 48}; every lane gets the same bits.
-__device__ __forceinline__ float max4_lanes(float x) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false,
-                                                  false);
-  const float m = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-  const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false,
-                                                  false);
-  return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
-}
-__device__ __forceinline__ float sum4_lanes(float x) { return add_xor32(add_xor16(x)); }
 
 // Sum of x over aligned groups of LPT lanes; every lane of the group receives the sum.
 template <int LPT>
@@ -215,7 +173,7 @@ __global__ void __launch_bounds__(256) row_attention_kernel(RowLaunch a) {
       }
   }
 
-  const size_t rs = (size_t)a.hkv * D;
+  const size_t rs = (size_t)a.kv.ld;
   // Stage the item's block ids in LDS once (the host caps items at kRowTablePages pages), so
   // a row address waits on an LDS read instead of on every K/V load issued before it.
   int blk0 = 0;
@@ -541,7 +499,7 @@ __global__ void __launch_bounds__(256) row_mfma_kernel(RowLaunch a, int hpw) {
     for (int s = 0; s < DQ; s++) q[s] = 0.0f;
   }
 
-  const size_t rs = (size_t)a.hkv * D;
+  const size_t rs = (size_t)a.kv.ld;
   const int bs_shift = a.kv.bs_shift;
   const int blk0 = it.kbeg >> bs_shift;
   const bool inl = it.blk_a != 0;

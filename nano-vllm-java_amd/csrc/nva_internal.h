@@ -64,6 +64,7 @@ struct KvView {
   int32_t block_size;
   int32_t bs_shift;      // log2(block_size) when a power of two, else -1
   int32_t paged;
+  int32_t ld;            // floats from one key's row to the next (hkv * head_dim in the arena)
 };
 
 struct RowLaunch {
@@ -104,6 +105,42 @@ struct TileLaunch {
   int32_t window;  // 0 = none
   float scale;
   float *part_m, *part_l, *part_acc;  // split tiles: [P, Hq], [P, Hq], [P, Hq, D]
+  // Span tiles (below) only: the query heads of a column group, and each q row's first partial of
+  // its span.
+  int32_t col_heads = 0;
+  const int32_t *row_part = nullptr;
+};
+
+// A span: a run of query rows that all see one whole key range (the rows of a step under a shared
+// prefix, or those that read one encoder's states).  The (row, query head) pairs of one KV head
+// are its columns: column c is row c / col_heads of the run and query head c % col_heads of the
+// column group, where col_heads is the GQA ratio (or a divisor of it that fits a tile), so a key
+// tile is read once for the rows and heads of the whole run.  Spans of many columns run as span
+// tiles on the tile kernel of prefill.hip: a TileItem whose qstart is the run's first row, qlen its
+// columns, q0 the tile's first column and klen unused, whose queries all see [ks, ke), and whose
+// partial (part >= 0) of row r is row_part[r] + split.  Spans of few columns are SpanItems.
+struct SpanItem {
+  int32_t row0;   // first query row
+  int32_t cols;   // columns, at most kSpanCols
+  int32_t seq;    // block-table row (paged K/V)
+  int32_t kbase;  // dense K/V: row of key 0; paged: unused
+  int32_t kbeg;   // first key
+  int32_t kend;   // one past the last key
+  int32_t split;  // partial row_part[row] + split, or -1: the whole range, written to out
+  int32_t pad;
+};
+
+struct SpanLaunch {
+  const float *q;
+  float *out;
+  KvView kv;
+  const SpanItem *items;
+  int32_t num_items;
+  int32_t hq, hkv, head_dim;
+  int32_t col_heads;
+  float scale;
+  const int32_t *row_part;
+  float *part_m, *part_l, *part_acc;
 };
 
 // RMSNorm of every head row of one tensor (RMSNorm.forward over [T*H, d], Ops.java:444-500).
@@ -215,6 +252,19 @@ int prefill_fp32_max_heads(int head_dim);
 int prefill_fp32_tile_queries(int head_dim, int heads_per_wg);
 int prefill_fp32_blocks_per_cu(int head_dim, int heads_per_wg);
 hipError_t launch_prefill_fp32(const TileLaunch &a, int heads_per_wg, hipStream_t s);
+
+// Span tiles: columns per workgroup, resident workgroups per CU, and the launch (a grid of
+// num_slots x hkv * (rep / col_heads)).
+int span_tile_cols(int head_dim);
+int span_tile_blocks_per_cu(int head_dim);
+hipError_t launch_span_tiles(const TileLaunch &a, hipStream_t s);
+
+// The span kernel of few columns (span.hip): most columns of an item, and the shapes it is built
+// for (paged: pages of a power of two of at least 16 tokens).
+constexpr int kSpanCols = 32;
+int span_max_cols(int head_dim);
+bool span_kernel_supports(int head_dim, int paged, int block_size);
+hipError_t launch_spans(const SpanLaunch &a, int max_cols, hipStream_t s);
 
 // Most query heads one prefill workgroup carries at this head dim.
 int prefill_max_heads(int head_dim);

@@ -117,25 +117,63 @@ __device__ __forceinline__ int64_t key_row(const KvView &kv, const int32_t *stab
 
 __device__ __forceinline__ float4 ld4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
 
+// Row of q (and out) and head of query qi of a tile; h0 is the workgroup's (wave's) first head.
+// The queries of a span tile are its columns, head by head within a row.
+struct QueryPos {
+  size_t row;
+  int h;
+};
+template <bool SPAN>
+__device__ __forceinline__ QueryPos query_pos(const TileLaunch &a, const TileItem &it, int qi, int h0) {
+  if constexpr (!SPAN) return QueryPos{(size_t)(it.qstart + qi), h0};
+  const int r = qi / a.col_heads;
+  return QueryPos{(size_t)(it.qstart + r), h0 + qi - r * a.col_heads};
+}
+
 // Where a query's results go: the output row, or the partial of one key chunk (rows of the tile
-// are laid out query-major, chunk-minor).
+// are laid out query-major, chunk-minor; a span's rows each have their own first partial).
 struct Dest {
   float *row;
   size_t pidx;
   bool partial;
 };
-__device__ __forceinline__ Dest destination(const TileLaunch &a, const TileItem &it, int qi, int h,
+template <bool SPAN>
+__device__ __forceinline__ Dest destination(const TileLaunch &a, const TileItem &it, int qi, int h0,
                                             int D) {
+  const QueryPos at = query_pos<SPAN>(a, it, qi, h0);
   Dest d;
   d.partial = it.part >= 0;
   d.pidx = 0;
   if (!d.partial) {
-    d.row = a.out + ((size_t)(it.qstart + qi) * a.hq + h) * D;
+    d.row = a.out + (at.row * a.hq + at.h) * D;
   } else {
-    d.pidx = ((size_t)it.part + (size_t)(qi - it.q0) * it.nsplit + it.split) * a.hq + h;
+    const size_t part = SPAN ? (size_t)a.row_part[at.row] + it.split
+                             : (size_t)it.part + (size_t)(qi - it.q0) * it.nsplit + it.split;
+    d.pidx = part * a.hq + at.h;
     d.row = a.part_acc + d.pidx * D;
   }
   return d;
+}
+
+// Visible keys of the queries [q0, q1] of a tile: of every one [all_lo, all_hi), of some
+// [any_lo, any_hi), and the last key + 1 of query qi.  All queries of a span see the segment's keys.
+struct Seen {
+  int all_lo, all_hi, any_lo, any_hi;
+};
+template <bool SPAN>
+__device__ __forceinline__ Seen seen_keys(const TileItem &it, int window, int q0, int q1) {
+  if constexpr (SPAN) return Seen{0, it.ke, 0, it.ke};
+  const int off = it.klen - it.qlen;  // absolute position of query 0
+  return Seen{window > 0 ? max(0, off + q1 - window + 1) : 0, off + q0 + 1,
+              window > 0 ? max(0, off + q0 - window + 1) : 0, off + q1 + 1};
+}
+template <bool SPAN>
+__device__ __forceinline__ int seen_from(const TileItem &it, int window, int qi) {
+  return !SPAN && window > 0 ? max(0, it.klen - it.qlen + qi - window + 1) : 0;
+}
+template <bool SPAN>
+__device__ __forceinline__ int seen_to(const TileItem &it, int qi) {
+  return SPAN ? it.ke : it.klen - it.qlen + qi + 1;
 }
 
 // The segment's result for a wave's 32 queries (from tile query q0 on) and dims [v0, v0 + 32 NB) of V
@@ -143,25 +181,22 @@ __device__ __forceinline__ Dest destination(const TileLaunch &a, const TileItem 
 // fit.  Lanes and registers of S^T and O^T are those of the split products; a step of PV contracts
 // the keys of one S^T register.  Scores are added up over sums of 64 dims and O^T over the tiles' own,
 // which leaves 2.2e-7 of a row where the split leaves 2.2e-7 to 2.9e-7.
-template <int D, int NB>
-__device__ void fp32_segment(const TileLaunch &a, const TileItem &it, int kvh, int h, int q0, int v0) {
+template <int D, int NB, bool SPAN>
+__device__ void fp32_segment(const TileLaunch &a, const TileItem &it, int kvh, int h0, int q0, int v0) {
   const int lane = threadIdx.x & 63;
   const int i = lane & 31, half = lane >> 5;
-  const int W = a.window;
-  const int off = it.klen - it.qlen;
   const int qi = q0 + i;
   const bool qvalid = qi < it.qlen;
-  const int aq = off + (qvalid ? qi : it.qlen - 1);
-  const int vis_lo = W > 0 ? max(0, aq - W + 1) : 0;
-  const int q1 = min(q0 + QW, it.qlen) - 1;
-  const int all_lo = W > 0 ? max(0, off + q1 - W + 1) : 0;  // keys that every query sees
-  const int all_hi = off + q0 + 1;
-  const int any_lo = W > 0 ? max(0, off + q0 - W + 1) : 0;
-  const int any_hi = min(it.ke, off + q1 + 1);
+  const int qic = qvalid ? qi : it.qlen - 1;
+  const int vis_lo = seen_from<SPAN>(it, a.window, qic);
+  const int vis_hi = seen_to<SPAN>(it, qic);
+  const Seen seen_by = seen_keys<SPAN>(it, a.window, q0, min(q0 + QW, it.qlen) - 1);
+  const int any_hi = min(it.ke, seen_by.any_hi);
   const int32_t *table = a.kv.table + (size_t)it.seq * a.kv.bt_stride;
   const float sl2 = a.scale * kLog2e;
-  const size_t rs = (size_t)a.hkv * D;
-  const float *qp = a.q + ((size_t)(it.qstart + aq - off) * a.hq + h) * D + 4 * half;
+  const size_t rs = (size_t)a.kv.ld;
+  const QueryPos at = query_pos<SPAN>(a, it, qic, h0);
+  const float *qp = a.q + (at.row * a.hq + at.h) * D + 4 * half;
   const float *kbase = a.kv.k + (size_t)kvh * D + 4 * half;
   const float *vbase = a.kv.v + (size_t)kvh * D + v0;
   f32x16 o[NB];
@@ -172,8 +207,8 @@ __device__ void fp32_segment(const TileLaunch &a, const TileItem &it, int kvh, i
   float m = -INFINITY, l = 0.0f;
 #pragma unroll 1
   for (int kt = it.ks; kt < any_hi; kt += KT) {
-    if (kt + KT <= any_lo) continue;
-    const bool full = kt >= all_lo && kt + KT <= min(all_hi, it.ke);
+    if (kt + KT <= seen_by.any_lo) continue;
+    const bool full = kt >= seen_by.all_lo && kt + KT <= min(seen_by.all_hi, it.ke);
     const int64_t row = key_row(a.kv, table, 0, it.kbase, min(kt + i, it.ke - 1));
     const float *kp = kbase + (size_t)row * rs;
     f32x16 st;
@@ -202,7 +237,7 @@ __device__ void fp32_segment(const TileLaunch &a, const TileItem &it, int kvh, i
 #pragma unroll
     for (int r = 0; r < 16; r++) {
       const int key = kt + 8 * (r >> 2) + 4 * half + (r & 3);
-      st[r] = full || (key >= vis_lo && key <= aq && key < it.ke) ? st[r] * sl2 : -INFINITY;
+      st[r] = full || (key >= vis_lo && key < vis_hi && key < it.ke) ? st[r] * sl2 : -INFINITY;
       mx = fmaxf(mx, st[r]);
     }
     const float mn = fmaxf(m, max_halves(mx));
@@ -246,7 +281,7 @@ __device__ void fp32_segment(const TileLaunch &a, const TileItem &it, int kvh, i
         for (int r = 1; r < 16; r++) p = r == 4 * (k >> 3) + (k & 3) ? st[r] : p;
         p = __shfl(p, i + 32 * ((k >> 2) & 1), 64);
         const float *vp = vbase + (size_t)__shfl((long long)row, k, 64) * rs + 4 * half;
-        const bool seen = kt + k >= vis_lo && kt + k <= aq;
+        const bool seen = kt + k >= vis_lo && kt + k < vis_hi;
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -267,7 +302,7 @@ __device__ void fp32_segment(const TileLaunch &a, const TileItem &it, int kvh, i
   }
   l = sum_halves(l);
   if (!qvalid) return;
-  const Dest d = destination(a, it, qi, h, D);
+  const Dest d = destination<SPAN>(a, it, qi, h0, D);
   const float f = d.partial ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
   for (int b = 0; b < NB; b++)
@@ -523,7 +558,7 @@ __device__ __forceinline__ int stage_table(const TileLaunch &a, const TileItem &
 
 // NW waves per workgroup.  At most 256 registers and two waves per SIMD at d = 128, 168 and three
 // at d = 64.
-template <int D, int HPW, int NW>
+template <int D, int HPW, int NW, bool SPAN = false>
 __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2)))
 prefill_split_kernel(TileLaunch a) {
   constexpr int KS = D / 16;         // contraction steps of QK
@@ -539,21 +574,20 @@ prefill_split_kernel(TileLaunch a) {
   const int slot = blockIdx.x;
   const int seg_end = a.seg_off[slot + 1];
   const int rep = a.hq / a.hkv;
-  const int groups = rep / HPW;
+  const int groups = rep / (SPAN ? a.col_heads : HPW);
   const int kvh = blockIdx.y / groups;
   // Wave-uniform, and known to be: every value derived from it lives in scalar registers.
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int h = kvh * rep + (blockIdx.y - kvh * groups) * HPW + wave % HPW;
+  const int h = kvh * rep + (blockIdx.y - kvh * groups) * (SPAN ? a.col_heads : HPW) + wave % HPW;
   const int qb = wave / HPW;
   const int lane = threadIdx.x & 63;
   const int i = lane & 31;     // MFMA row / column index of this lane
   const int half = lane >> 5;  // MFMA k-slot
-  const int W = a.window;
   // Scores are kept unscaled until the exponential; a negative scale goes into q's sign, so that
   // the largest product is the largest score.
   const float sl2 = fabsf(a.scale) * kLog2e;
   const float qsign = a.scale < 0.0f ? -1.0f : 1.0f;
-  const size_t rs = (size_t)a.hkv * D;
+  const size_t rs = (size_t)a.kv.ld;
   const float *kbase = a.kv.k + (size_t)kvh * D;
   const float *vbase = a.kv.v + (size_t)kvh * D;
 
@@ -563,22 +597,16 @@ prefill_split_kernel(TileLaunch a) {
     __syncthreads();
     if (threadIdx.x == 0) uneven = 0;
     const TileItem it = a.items[seg];
-    const int off = it.klen - it.qlen;  // absolute position of query 0
     // This lane's query (column i of S^T) and its visible key range.
     const int wq0 = it.q0 + qb * QW;
     const int qi = wq0 + i;
     const bool qvalid = qi < it.qlen;
     const int qic = qvalid ? qi : it.qlen - 1;
-    const int aq = off + qic;
-    const int vis_lo = W > 0 ? max(0, aq - W + 1) : 0;
-    const int vis_hi = aq + 1;
+    const int vis_lo = seen_from<SPAN>(it, a.window, qic);
+    const int vis_hi = seen_to<SPAN>(it, qic);
     // The wave's 32 queries: bounds of their visible ranges.
     const bool wave_active = wq0 < it.qlen;
-    const int wq1 = min(wq0 + QW - 1, it.qlen - 1);
-    const int wlo_min = W > 0 ? max(0, off + wq0 - W + 1) : 0;
-    const int wlo_max = W > 0 ? max(0, off + wq1 - W + 1) : 0;
-    const int whi_min = off + wq0 + 1;
-    const int whi_max = off + wq1 + 1;
+    const Seen seen = seen_keys<SPAN>(it, a.window, wq0, min(wq0 + QW - 1, it.qlen - 1));
 
     // The first tile's loads are issued before Q is read: a short segment waits once for both.
     TileShare<D, NW> share{a.kv, kbase, vbase, rs, stab, stage_table(a, it, stab), it.kbase, it.ks, it.ke,
@@ -595,7 +623,8 @@ prefill_split_kernel(TileLaunch a) {
     Split8 q[KS];
     float qscale;  // takes a product of scaled q and k (of exponent 0) to log2 units
     {
-      const float *qp = a.q + ((size_t)(it.qstart + qic) * a.hq + h) * D + 8 * half;
+      const QueryPos at = query_pos<SPAN>(a, it, qic, h);
+      const float *qp = a.q + (at.row * a.hq + at.h) * D + 8 * half;
       f32x8 x[KS];
       float mx = 0.0f;
 #pragma unroll
@@ -650,12 +679,12 @@ prefill_split_kernel(TileLaunch a) {
     // the one after it loaded (next_kt; none if < 0).
     auto compute_tile = [&](int kt, const _Float16 *tk, const _Float16 *tv, int k_exp, int v_exp,
                             int nb, int next_kt) {
-      if (!wave_active || kt >= whi_max || kt + KT <= wlo_min) {
+      if (!wave_active || kt >= seen.any_hi || kt + KT <= seen.any_lo) {
         store_tile(nb);
         if (next_kt >= 0) load_tile(next_kt);
         return;
       }
-      const bool full = (kt + KT <= whi_min) && (kt >= wlo_max);
+      const bool full = (kt + KT <= seen.all_hi) && (kt >= seen.all_lo);
 
       // S^T = K Q^T: register r of st holds key kt + 8 (r / 4) + 4 half + r % 4 of query i.
       f32x16 st;
@@ -761,7 +790,7 @@ prefill_split_kernel(TileLaunch a) {
       continue;
     }
     if (!qvalid) continue;
-    const Dest d = destination(a, it, qi, h, D);
+    const Dest d = destination<SPAN>(a, it, qi, h, D);
     const float f = result_factor(d, l_tot, m_run, m_top);
     // Register r of o[b] is dim 32 b + 8 (r / 4) + 4 half + r % 4.
 #pragma unroll
@@ -777,7 +806,7 @@ prefill_split_kernel(TileLaunch a) {
   }
   for (int seg = again.next(again.first, seg_end); seg < seg_end; seg = again.next(seg + 1, seg_end)) {
     const TileItem it = a.items[seg];
-    if (it.q0 + qb * QW < it.qlen) fp32_segment<D, NB>(a, it, kvh, h, it.q0 + qb * QW, 0);
+    if (it.q0 + qb * QW < it.qlen) fp32_segment<D, NB, SPAN>(a, it, kvh, h, it.q0 + qb * QW, 0);
   }
 }
 
@@ -791,7 +820,7 @@ prefill_split_kernel(TileLaunch a) {
 // split and stored during QK of tile t, K of tile t + 1 during PV of tile t.  At d = 512 the
 // tiles take 128 KB, so the partial scores are added pairwise in place (16 KB instead of 32),
 // which costs one more barrier.
-template <int D, int HPW>
+template <int D, int HPW, bool SPAN = false>
 __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2)))
 prefill_split_wide_kernel(TileLaunch a) {
   constexpr int NW = 8, DW = 128, DS = D / DW;
@@ -809,40 +838,33 @@ prefill_split_wide_kernel(TileLaunch a) {
   const int slot = blockIdx.x;
   const int seg_end = a.seg_off[slot + 1];
   const int rep = a.hq / a.hkv;
-  const int groups = rep / HPW;
+  const int groups = rep / (SPAN ? a.col_heads : HPW);
   const int kvh = blockIdx.y / groups;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ds = wave % DS, qg = wave / DS;  // dims [128 ds, 128 ds + 128) of query group qg
-  const int h = kvh * rep + (blockIdx.y - kvh * groups) * HPW + qg % HPW;
+  const int h = kvh * rep + (blockIdx.y - kvh * groups) * (SPAN ? a.col_heads : HPW) + qg % HPW;
   const int qb = qg / HPW;
   const int lane = threadIdx.x & 63;
   const int i = lane & 31, half = lane >> 5;
-  const int W = a.window;
   // Scores are kept unscaled until the exponential; a negative scale goes into q's sign.  (Not 0:
   // 0 * -inf is NaN.)
   const float sl2 = fmaxf(fabsf(a.scale) * kLog2e, 0x1p-126f);
   const float qsign = a.scale < 0.0f ? -1.0f : 1.0f;
-  const size_t rs = (size_t)a.hkv * D;
+  const size_t rs = (size_t)a.kv.ld;
 
   Again again{a.seg_off[slot], 0};
   for (int seg = again.first; seg < seg_end; seg++) {
     __syncthreads();
     if (threadIdx.x == 0) uneven = 0;
     const TileItem it = a.items[seg];
-    const int off = it.klen - it.qlen;
     const int wq0 = it.q0 + qb * QW;
     const int qi = wq0 + i;
     const bool qvalid = qi < it.qlen;
     const int qic = qvalid ? qi : it.qlen - 1;
-    const int aq = off + qic;
-    const int vis_lo = W > 0 ? max(0, aq - W + 1) : 0;
-    const int vis_hi = aq + 1;
+    const int vis_lo = seen_from<SPAN>(it, a.window, qic);
+    const int vis_hi = seen_to<SPAN>(it, qic);
     const bool group_active = wq0 < it.qlen;
-    const int wq1 = min(wq0 + QW - 1, it.qlen - 1);
-    const int wlo_min = W > 0 ? max(0, off + wq0 - W + 1) : 0;
-    const int wlo_max = W > 0 ? max(0, off + wq1 - W + 1) : 0;
-    const int whi_min = off + wq0 + 1;
-    const int whi_max = off + wq1 + 1;
+    const Seen seen = seen_keys<SPAN>(it, a.window, wq0, min(wq0 + QW - 1, it.qlen - 1));
 
     // The first tile's loads are issued before Q is read: a short segment waits once for both.
     TileShare<D, NW> share{a.kv, a.kv.k + (size_t)kvh * D, a.kv.v + (size_t)kvh * D, rs, stab,
@@ -854,7 +876,8 @@ prefill_split_wide_kernel(TileLaunch a) {
     Split8 q[KS];  // lane (i, half): the parts of Q[query i][128 ds + 16 s + 8 half + 0..7]
     float qscale;
     {
-      const float *qp = a.q + ((size_t)(it.qstart + qic) * a.hq + h) * D + DW * ds + 8 * half;
+      const QueryPos at = query_pos<SPAN>(a, it, qic, h);
+      const float *qp = a.q + (at.row * a.hq + at.h) * D + DW * ds + 8 * half;
       f32x8 x[KS];
       float mx = 0.0f;
 #pragma unroll
@@ -916,7 +939,7 @@ prefill_split_wide_kernel(TileLaunch a) {
     for (int t = 0; t < ntiles; t++) {
       const int kt = it.ks + t * KT;
       const bool more = t + 1 < ntiles;
-      const bool active = group_active && kt < whi_max && kt + KT > wlo_min;
+      const bool active = group_active && kt < seen.any_hi && kt + KT > seen.any_lo;
       const float c = qscale * split_unscale(k_exp_in);
 
       // K of tile t is in LDS; V of tile t is in rv, its maxima in smax[1]; PV of tile t - 1 is
@@ -987,7 +1010,7 @@ prefill_split_wide_kernel(TileLaunch a) {
         if (t + 2 < ntiles) share.load_k(kt + 2 * KT, rk);
       }
       if (active) {
-        const bool full = (kt + KT <= whi_min) && (kt >= wlo_max);
+        const bool full = (kt + KT <= seen.all_hi) && (kt >= seen.all_lo);
         if (!full) {
 #pragma unroll
           for (int r = 0; r < 16; r++) {
@@ -1063,7 +1086,7 @@ prefill_split_wide_kernel(TileLaunch a) {
       continue;
     }
     if (!qvalid) continue;
-    const Dest d = destination(a, it, qi, h, D);
+    const Dest d = destination<SPAN>(a, it, qi, h, D);
     const float f = result_factor(d, l_tot, m_run, m_top);
 #pragma unroll
     for (int b = 0; b < NB; b++)
@@ -1078,7 +1101,7 @@ prefill_split_wide_kernel(TileLaunch a) {
   }
   for (int seg = again.next(again.first, seg_end); seg < seg_end; seg = again.next(seg + 1, seg_end)) {
     const TileItem it = a.items[seg];
-    if (it.q0 + qb * QW < it.qlen) fp32_segment<D, NB>(a, it, kvh, h, it.q0 + qb * QW, DW * ds);
+    if (it.q0 + qb * QW < it.qlen) fp32_segment<D, NB, SPAN>(a, it, kvh, h, it.q0 + qb * QW, DW * ds);
   }
 }
 
@@ -1101,6 +1124,18 @@ hipError_t with_kernel(int head_dim, int hpw, F f) {
     case 256 * 8 + 1: return f(prefill_split_wide_kernel<256, 1>);
     case 256 * 8 + 2: return f(prefill_split_wide_kernel<256, 2>);
     case 512 * 8 + 1: return f(prefill_split_wide_kernel<512, 1>);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+// The same for span tiles.
+template <typename F>
+hipError_t with_span_kernel(int head_dim, F f) {
+  switch (head_dim) {
+    case 64: return f(prefill_split_kernel<64, 1, split_waves<64>(), true>);
+    case 128: return f(prefill_split_kernel<128, 1, split_waves<128>(), true>);
+    case 256: return f(prefill_split_wide_kernel<256, 1, true>);
+    case 512: return f(prefill_split_wide_kernel<512, 1, true>);
     default: return hipErrorInvalidValue;
   }
 }
@@ -1132,6 +1167,27 @@ int prefill_blocks_per_cu(int head_dim, int heads_per_wg) {
       b < 1)
     b = 1;
   return b;
+}
+
+int span_tile_cols(int head_dim) { return prefill_tile_queries(head_dim, 1); }
+
+int span_tile_blocks_per_cu(int head_dim) {
+  int b = 0;
+  if (with_span_kernel(head_dim, [&](auto k) {
+        return hipOccupancyMaxActiveBlocksPerMultiprocessor(&b, k, 64 * waves(head_dim), 0);
+      }) != hipSuccess ||
+      b < 1)
+    b = 1;
+  return b;
+}
+
+hipError_t launch_span_tiles(const TileLaunch &a, hipStream_t s) {
+  if (a.num_items <= 0 || a.num_slots <= 0) return hipSuccess;
+  const dim3 grid(a.num_slots, a.hkv * ((a.hq / a.hkv) / a.col_heads)), block(64 * waves(a.head_dim));
+  return with_span_kernel(a.head_dim, [&](auto k) {
+    hipLaunchKernelGGL(k, grid, block, 0, s, a);
+    return hipGetLastError();
+  });
 }
 
 hipError_t launch_prefill_tiles(const TileLaunch &a, int hpw, hipStream_t s) {

@@ -1,0 +1,305 @@
+// Attention of runs of query rows that all see one whole key range, for runs of few columns: the
+// rows of a step under a shared prefix, or those that read one encoder's states (a row of a step
+// alone, too).  Runs of many columns are span tiles (prefill.hip).
+//
+// Mathematics: column c of a run is query row r = c / H and query head h of one KV head
+// (H = col_heads heads of it).  For the keys t of the item,
+//   s_ct = q_rh . k_t * scale,  m_c = max_t s_ct,  l_c = sum_t e^(s_ct - m_c),
+//   a_c = sum_t e^(s_ct - m_c) v_t;
+// an item over the whole range writes a_c / l_c (0 where l_c = 0), a split one or one of a prefix
+// leaves (m_c, l_c, a_c), and the merge joins what a row has from its prefix and from its own keys.
+//
+// Mapping onto CDNA4.  Bound by HBM: a key costs 8 D bytes of K and V, which the whole run uses, and
+// 4 D operations a column, so fp32 matrix instructions (which need no scaling and take any value)
+// stay ahead of the memory up to about 48 columns.  One workgroup of 4 waves per (item, KV head,
+// head group); each wave takes 16-key blocks of the item in turn, so that 4 waves read 64
+// consecutive keys at a time, two register buffers deep, with no barrier and no LDS until the end:
+//   S^T[key][col] = K Q^T    D/4 v_mfma_f32_16x16x4_f32 per block and 16 columns: at step 4v + c
+//                            lane (i, g) supplies K[t0 + i][16v + 4g + c] (A) and
+//                            Q[col i][16v + 4g + c] (B), i = lane % 16, g = lane / 16;
+//                            lane (j, g) then holds column j's scores of keys t0 + 4g + r;
+//   O^T[dim][col] += V^T P^T 4 x D/16 per block: step s contracts key t0 + 4g + s, whose
+//                            probability is the lane's own (B), against V[key][64w + 4i + c] (A) in
+//                            block b = 4w + c, so P never leaves the registers.
+// K operands serve both blocks of 16 columns.  The four waves' states meet in LDS in wave order.
+#include "nva_internal.h"
+#include "nva_device.h"
+#include "row_lanes.h"
+
+namespace nva {
+
+namespace {
+__device__ __forceinline__ float4 ld4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
+__device__ __forceinline__ void st4(float *p, float4 v) { *reinterpret_cast<float4 *>(p) = v; }
+}  // namespace
+
+template <int D, int NCB, bool PAGED>
+__global__ void __launch_bounds__(256) span_kernel(SpanLaunch a) {
+  constexpr int DQ = D / 4;   // QK steps per block
+  constexpr int NB = D / 16;  // O^T blocks; block b = 4w + c, row i is dim 64w + 4i + c
+  constexpr int NQ = DQ / 4;  // float4 loads of a K row part per lane
+  constexpr int NV = NB / 4;  // float4 loads of a V row part per lane per key (one per 64 dims)
+  constexpr int COLS = 16 * NCB;
+  __shared__ float sm_m[4][COLS];
+  __shared__ float sm_l[4][COLS];
+  __shared__ float4 sm_acc[4][COLS][D / 4];
+  __shared__ int32_t stab[kRowTablePages];
+
+  const int rep = a.hq / a.hkv;
+  const int groups = rep / a.col_heads;
+  const int per_item = a.hkv * groups;
+  const int item = blockIdx.x / per_item;
+  const int gy = blockIdx.x - item * per_item;
+  const SpanItem it = a.items[item];
+  const int kvh = gy / groups;
+  const int h0 = kvh * rep + (gy - kvh * groups) * a.col_heads;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i = lane & 15;
+  const int g = lane >> 4;
+
+  // B operand of QK: this lane's columns i and 16 + i, dims 16v + 4g + [0, 4), in log2 units.
+  const float sl2 = a.scale * 1.4426950408889634f;
+  float q[NCB][DQ];
+#pragma unroll
+  for (int n = 0; n < NCB; n++) {
+    const int c = 16 * n + i;
+    if (c < it.cols) {
+      const int r = c / a.col_heads;
+      const float *qp =
+          a.q + ((size_t)(it.row0 + r) * a.hq + h0 + c - r * a.col_heads) * D + 4 * g;
+#pragma unroll
+      for (int v = 0; v < NQ; v++) {
+        const float4 x = ld4(qp + 16 * v);
+        q[n][4 * v] = x.x * sl2;
+        q[n][4 * v + 1] = x.y * sl2;
+        q[n][4 * v + 2] = x.z * sl2;
+        q[n][4 * v + 3] = x.w * sl2;
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < DQ; s++) q[n][s] = 0.0f;
+    }
+  }
+
+  const size_t rs = (size_t)a.kv.ld;
+  const int bs_shift = a.kv.bs_shift;
+  const int blk0 = PAGED ? it.kbeg >> bs_shift : 0;
+  if constexpr (PAGED) {
+    const int32_t *table = a.kv.table + (size_t)it.seq * a.kv.bt_stride;
+    const int npages = ((it.kend - 1) >> bs_shift) - blk0 + 1;
+    for (int j = threadIdx.x; j < npages; j += blockDim.x) stab[j] = table[blk0 + j];
+    __syncthreads();
+  }
+  const float *kbase_h = a.kv.k + (size_t)kvh * D;
+  const float *vbase_h = a.kv.v + (size_t)kvh * D;
+  const int tfirst = it.kbeg & ~15;  // blocks of pages start at multiples of 16
+  // Fixed lane offsets (floats) from a block's first row: K row i, dims 16v + 4g; V rows
+  // 4g + s, dims 64w + 4i.
+  const uint32_t koff = (uint32_t)(i * rs + 4 * g);
+  const uint32_t voff = (uint32_t)(4 * g * rs + 4 * i);
+
+  float kra[DQ], krb[DQ];
+  float vra[4][NB], vrb[4][NB];
+  auto issue = [&](int t0, float(&kr)[DQ], float(&vr)[4][NB]) {
+    // A block past the item's end reloads its first block (never folded).
+    const int tb = t0 < it.kend ? t0 : tfirst;
+    int64_t row;
+    if constexpr (PAGED) {
+      const int p = tb >> bs_shift;
+      const int id = __builtin_amdgcn_readfirstlane(stab[p - blk0]);
+      row = (int64_t)id * a.kv.block_size + (tb - (p << bs_shift));
+    } else {
+      row = (int64_t)it.kbase + tb;
+    }
+    const float *kb = kbase_h + row * (int64_t)rs;
+    const float *vb = vbase_h + row * (int64_t)rs;
+    uint32_t ko = koff, vo[4];
+#pragma unroll
+    for (int s = 0; s < 4; s++) vo[s] = voff + (uint32_t)(s * rs);
+    if (tb < it.kbeg || tb + 16 > it.kend) {
+      // A partial block: every lane reads the block's key nearest its own inside the item (what
+      // lies outside could hold any bits, NaN included; a finite V row adds 0 at weight 0).
+      const int tk = min(max(tb + i, it.kbeg), it.kend - 1);
+      ko = (uint32_t)((tk - tb) * (int64_t)rs + 4 * g);
+#pragma unroll
+      for (int s = 0; s < 4; s++) {
+        const int tv = min(max(tb + 4 * g + s, it.kbeg), it.kend - 1);
+        vo[s] = (uint32_t)((tv - tb) * (int64_t)rs + 4 * i);
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < NQ; v++) {
+      const float4 x = ld4_stream_at(kb, ko + 16 * v);
+      kr[4 * v] = x.x;
+      kr[4 * v + 1] = x.y;
+      kr[4 * v + 2] = x.z;
+      kr[4 * v + 3] = x.w;
+    }
+#pragma unroll
+    for (int s = 0; s < 4; s++)
+#pragma unroll
+      for (int v = 0; v < NV; v++) {
+        const float4 x = ld4_stream_at(vb, vo[s] + 64 * v);
+        vr[s][4 * v] = x.x;
+        vr[s][4 * v + 1] = x.y;
+        vr[s][4 * v + 2] = x.z;
+        vr[s][4 * v + 3] = x.w;
+      }
+  };
+
+  f32x4 o[NCB][NB];
+  float m_run[NCB], l_run[NCB];  // column's max (log2 units, the same in its 4 lanes), lane's sum
+#pragma unroll
+  for (int n = 0; n < NCB; n++) {
+#pragma unroll
+    for (int b = 0; b < NB; b++) o[n][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    m_run[n] = -INFINITY;
+    l_run[n] = 0.0f;
+  }
+  auto fold = [&](int t0, const float(&kr)[DQ], const float(&vr)[4][NB]) {
+#pragma unroll
+    for (int n = 0; n < NCB; n++) {
+      if (n > 0 && it.cols <= 16 * n) break;  // an item of a launch with wider ones
+      f32x4 st = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int s = 0; s < DQ; s++)
+        st = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[s], q[n][s], st, 0, 0, 0);
+      float p[4];
+      float mx = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const int key = t0 + 4 * g + r;
+        p[r] = (key >= it.kbeg && key < it.kend) ? st[r] : -INFINITY;
+        mx = fmaxf(mx, p[r]);
+      }
+      mx = max4_lanes(mx);
+      // The max moves, and the sums with it, only where it grows by more than 2^8.
+      const bool need = mx > m_run[n] + 8.0f;
+      if (__any(need)) {
+        const float mn = need ? mx : m_run[n];
+        const float alpha = m_run[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[n] - mn);
+        l_run[n] *= alpha;
+#pragma unroll
+        for (int b = 0; b < NB; b++) o[n][b] *= alpha;
+        m_run[n] = mn;
+      }
+      const float ms = m_run[n] == -INFINITY ? 0.0f : m_run[n];
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        p[r] = __builtin_amdgcn_exp2f(p[r] - ms);
+        l_run[n] += p[r];
+      }
+#pragma unroll
+      for (int s = 0; s < 4; s++)
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+          o[n][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[s][b], p[s], o[n][b], 0, 0, 0);
+    }
+  };
+
+  int t0 = tfirst + 16 * wave;
+  if (t0 < it.kend) {
+    issue(t0, kra, vra);
+    for (;;) {
+      issue(t0 + 64, krb, vrb);
+      fold(t0, kra, vra);
+      t0 += 64;
+      if (t0 >= it.kend) break;
+      issue(t0 + 64, kra, vra);
+      fold(t0, krb, vrb);
+      t0 += 64;
+      if (t0 >= it.kend) break;
+    }
+  }
+
+#pragma unroll
+  for (int n = 0; n < NCB; n++) {
+    const int c = 16 * n + i;
+    const float l_tot = sum4_lanes(l_run[n]);
+    if (c < it.cols) {
+      if (g == 0) {
+        sm_m[wave][c] = m_run[n];
+        sm_l[wave][c] = l_tot;
+      }
+      // Lane (i, g) holds row 4g + r of block 4w + b: dim 64w + 16g + 4r + b.
+#pragma unroll
+      for (int w = 0; w < NV; w++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+          sm_acc[wave][c][16 * w + 4 * g + r] = make_float4(
+              o[n][4 * w][r], o[n][4 * w + 1][r], o[n][4 * w + 2][r], o[n][4 * w + 3][r]);
+    }
+  }
+  __syncthreads();
+  for (int idx = threadIdx.x; idx < it.cols * (D / 4); idx += blockDim.x) {
+    const int c = idx / (D / 4);
+    const int cc = idx - c * (D / 4);
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; w++) M = fmaxf(M, sm_m[w][c]);
+    const float Ms = M == -INFINITY ? 0.0f : M;
+    float L = 0.0f;
+    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      const float e = __builtin_amdgcn_exp2f(sm_m[w][c] - Ms);
+      L = fmaf(sm_l[w][c], e, L);
+      const float4 x = sm_acc[w][c][cc];
+      A.x = fmaf(x.x, e, A.x);
+      A.y = fmaf(x.y, e, A.y);
+      A.z = fmaf(x.z, e, A.z);
+      A.w = fmaf(x.w, e, A.w);
+    }
+    const int r = c / a.col_heads;
+    const int h = h0 + c - r * a.col_heads;
+    if (it.split < 0) {
+      const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+      st4(a.out + ((size_t)(it.row0 + r) * a.hq + h) * D + cc * 4,
+          make_float4(A.x * inv, A.y * inv, A.z * inv, A.w * inv));
+    } else {
+      const size_t pi = (size_t)(a.row_part[it.row0 + r] + it.split) * a.hq + h;
+      st4(a.part_acc + pi * D + cc * 4, A);
+      if (cc == 0) {
+        a.part_m[pi] = M;
+        a.part_l[pi] = L;
+      }
+    }
+  }
+}
+
+namespace {
+
+template <int D, int NCB>
+void launch_span(const SpanLaunch &a, hipStream_t s) {
+  const dim3 grid(a.num_items * (a.hkv * ((a.hq / a.hkv) / a.col_heads)));
+  if (a.kv.paged)
+    hipLaunchKernelGGL((span_kernel<D, NCB, true>), grid, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((span_kernel<D, NCB, false>), grid, dim3(256), 0, s, a);
+}
+
+}  // namespace
+
+// At d = 256 the registers hold 16 columns.
+int span_max_cols(int head_dim) { return head_dim == 256 ? 16 : kSpanCols; }
+
+bool span_kernel_supports(int head_dim, int paged, int block_size) {
+  return (head_dim == 64 || head_dim == 128 || head_dim == 256) &&
+         (!paged || (block_size >= 16 && (block_size & (block_size - 1)) == 0));
+}
+
+hipError_t launch_spans(const SpanLaunch &a, int max_cols, hipStream_t s) {
+  if (a.num_items <= 0) return hipSuccess;
+  switch (a.head_dim * 2 + (max_cols > 16)) {
+    case 64 * 2: launch_span<64, 1>(a, s); break;
+    case 64 * 2 + 1: launch_span<64, 2>(a, s); break;
+    case 128 * 2: launch_span<128, 1>(a, s); break;
+    case 128 * 2 + 1: launch_span<128, 2>(a, s); break;
+    case 256 * 2: launch_span<256, 1>(a, s); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace nva

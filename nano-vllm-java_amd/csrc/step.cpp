@@ -154,6 +154,54 @@ __attribute__((visibility("hidden"))) nva_status nva_internal_fail(nva_ctx *ctx,
 
 extern "C" {
 
+// Which runs of adjacent sequences to read as one: the cut of the step into runs that saves the most
+// page reads, sum over runs of (sequences - 1) * common full pages.  best[j] is the saving of the
+// first j sequences, run[j] where the last run of that cut starts.
+nva_status nva_find_shared_prefixes(const int32_t *block_tables, int num_seqs, int bt_stride,
+                                    const int32_t *cached_tokens, int block_size,
+                                    nva_prefix_group *groups, int *num_groups) {
+  if (!num_groups) return NVA_E_ARG;
+  *num_groups = 0;
+  if (num_seqs < 0 || bt_stride < 0 || block_size <= 0) return NVA_E_ARG;
+  if (num_seqs == 0) return NVA_OK;
+  if (!cached_tokens || !groups || (bt_stride > 0 && !block_tables)) return NVA_E_ARG;
+  std::vector<int32_t> full(num_seqs), same(num_seqs, 0);  // own full pages; shared with the next
+  for (int b = 0; b < num_seqs; b++) {
+    const int32_t *t = block_tables + (size_t)b * bt_stride;
+    int n = 0;
+    while (n < bt_stride && n < cached_tokens[b] / block_size && t[n] >= 0) n++;
+    full[b] = n;
+    if (b > 0) {
+      int c = 0;
+      const int most = std::min(full[b - 1], n);
+      while (c < most && t[c - bt_stride] == t[c]) c++;
+      same[b - 1] = c;
+    }
+  }
+  std::vector<int64_t> best(num_seqs + 1, 0);
+  std::vector<int32_t> run(num_seqs + 1, 0), pages(num_seqs + 1, 0);
+  for (int j = 1; j <= num_seqs; j++) {
+    best[j] = best[j - 1];
+    run[j] = j - 1;
+    int common = INT32_MAX;
+    for (int i = j - 2; i >= 0; i--) {  // the run [i, j)
+      common = std::min(common, same[i]);
+      if (common == 0) break;
+      const int64_t saved = best[i] + (int64_t)(j - i - 1) * common;
+      if (saved > best[j]) {
+        best[j] = saved;
+        run[j] = i;
+        pages[j] = common;
+      }
+    }
+  }
+  for (int j = num_seqs; j > 0; j = run[j])
+    if (j - run[j] > 1)
+      groups[(*num_groups)++] = {run[j], j - run[j], pages[j] * block_size};
+  std::reverse(groups, groups + *num_groups);
+  return NVA_OK;
+}
+
 nva_status nva_build_prefill_metadata(const nva_seq *seqs, int num_seqs, int block_size,
                                       nva_step_meta *out) {
   Built b;

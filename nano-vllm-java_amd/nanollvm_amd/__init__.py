@@ -6,6 +6,7 @@ from . import _native  # noqa: F401
 from .layers import (  # noqa: F401
     Attention,
     Context,
+    CrossAttention,
     IllegalArgumentException,
     IllegalStateException,
     KvCacheArena,

@@ -94,6 +94,17 @@ class StepMetaOut(ctypes.Structure):
     ]
 
 
+class PrefixGroup(ctypes.Structure):
+    """nva_prefix_group: a run of the step's sequences with the same first tokens."""
+
+    _fields_ = [
+        ("first_seq", ctypes.c_int32),
+        ("num_seqs", ctypes.c_int32),
+        ("num_tokens", ctypes.c_int32),
+    ]
+
+
+_pgroup = ctypes.POINTER(PrefixGroup)
 _pseq = ctypes.POINTER(Seq)
 _pmeta = ctypes.POINTER(StepMetaOut)
 
@@ -123,6 +134,13 @@ SIGNATURES = {
                      _st),
     "nva_step_positions": ([_vp, _vp, _ci], _st),
     "nva_step_clear": ([_vp], _st),
+    "nva_find_shared_prefixes": ([_vp, _ci, _ci, _vp, _ci, _pgroup, ctypes.POINTER(_ci)], _st),
+    "nva_step_share_prefixes": ([_vp, _pgroup, _ci], _st),
+    "nva_step_set_encoder": ([_vp, _vp, _vp, _ci], _st),
+    "nva_cross_attention_forward": ([_vp, ctypes.POINTER(AttnDesc), _vp, _vp, _vp, _i64, _i64, _ci,
+                                     _vp], _st),
+    "nva_cross_attention_forward_noalloc": ([_vp, ctypes.POINTER(AttnDesc), _vp, _vp, _vp, _i64,
+                                             _i64, _ci, _vp], _st),
     "nva_rope_forward": ([_vp, _vp, _vp, _vp, _ci, _ci, _ci, _vp, _vp], _st),
     "nva_attention_forward": ([_vp, _vp, ctypes.POINTER(AttnDesc), _vp, _vp, _vp, _ci, _vp], _st),
     "nva_attention_forward_noalloc": ([_vp, _vp, ctypes.POINTER(AttnDesc), _vp, _vp, _vp, _ci,

@@ -8,6 +8,8 @@ the reference's own code:
 * ``KvCacheArena``   -- engine/KvCacheArena.java (per-layer K/V pages, resident in HBM).
 * ``RotaryEmbedding``-- layers/Norms.java:158-388 (cos|sin table, ``forward``).
 * ``Attention``      -- layers/Attention.java (constructor arguments, ``forward``).
+* ``CrossAttention`` -- the encoder-decoder counterpart (layers/BidirectionalAttention.java for an
+                        encoder's own layers).
 * ``RMSNorm``        -- layers/Norms.java:32-97 (``forward``; ``weightless``), applied per head
                         by the model layers before RoPE.
 * ``Linear``         -- layers/Linear.java Linear.Row (``forward``): o_proj on the attention
@@ -187,6 +189,24 @@ class Context:
                "Transformer.prepareDecode")
         del keep
         self._positions_key = None
+
+    def share_prefixes(self, groups) -> None:
+        """Attention over the step set last reads the tokens that runs of its sequences share once
+        for each run: ``groups`` is a list of (first sequence, sequences, tokens), e.g. from
+        ``step.find_shared_prefixes``."""
+        arr = (N.PrefixGroup * max(1, len(groups)))(*(N.PrefixGroup(*(int(x) for x in g))
+                                                      for g in groups))
+        _check(self._h, N.load().nva_step_share_prefixes(self._h, arr, len(groups)),
+               "Context.share_prefixes")
+
+    def set_encoder(self, kv_start, kv_len) -> None:
+        """The encoder rows each sequence of the step set last sees in ``CrossAttention``: the first
+        row and the number of rows."""
+        start, lens = _i32(kv_start), _i32(kv_len)
+        if start.ndim != 1 or start.shape != lens.shape:
+            raise IllegalArgumentException("kv_start and kv_len must be 1-D and alike")
+        _check(self._h, N.load().nva_step_set_encoder(self._h, _ptr(start), _ptr(lens), len(lens)),
+               "Context.set_encoder")
 
     def set_positions(self, positions) -> None:
         pos = np.ascontiguousarray(
@@ -597,4 +617,48 @@ class Attention:
             None if v_norm is None else v_norm.desc(), ctypes.byref(self._desc),
             _dev(qkv, "qkv"), T, _dev(q_out, "q_out"), _dev(k_out, "k_out"), _dev(out, "out")),
             "Attention.forward (packed qkv)")
+        return out
+
+
+class CrossAttention:
+    """Attention of each sequence's queries over all keys of its encoder's states (encoder-decoder
+    models; with a sequence's own rows as its keys, an encoder's full attention,
+    layers/BidirectionalAttention.java)."""
+
+    def __init__(self, num_heads: int, head_dim: int, scale: float, num_kv_heads: int):
+        self.num_heads = num_heads
+        self.head_dim = head_dim
+        self.scale = float(np.float32(scale))
+        self.num_kv_heads = num_kv_heads
+        self._desc = N.AttnDesc(num_heads, head_dim, self.scale, num_kv_heads, 0, 0, 0)
+
+    def _pool(self, k, v):
+        """Pointers, rows and row stride of the encoder's keys and values."""
+        for name, t in (("k", k), ("v", v)):
+            if t.dim() != 3 or tuple(t.shape[1:]) != (self.num_kv_heads, self.head_dim):
+                raise IllegalArgumentException(
+                    f"{name} must be [rows, {self.num_kv_heads}, {self.head_dim}], "
+                    f"got {tuple(t.shape)}")
+            if not (t.is_cuda and t.dtype == torch.float32 and
+                    (t.numel() == 0 or t[0].is_contiguous())):
+                raise IllegalArgumentException(
+                    f"{name} must be a float32 device tensor with contiguous rows")
+        if k.shape[0] != v.shape[0] or (k.shape[0] > 1 and k.stride(0) != v.stride(0)):
+            raise IllegalArgumentException("k and v must have the same rows and row stride")
+        stride = k.stride(0) if k.shape[0] > 1 else self.num_kv_heads * self.head_dim
+        return k.data_ptr(), v.data_ptr(), k.shape[0], stride
+
+    def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                ctx: Context) -> torch.Tensor:
+        """softmax(q k^T scale) v over the rows of ``ctx.set_encoder``: q [tokens, numHeads, headDim]
+        as the step has it, k and v [rows, numKvHeads, headDim], whose rows may lie apart (views of
+        one packed projection); returns a new [tokens, numHeads, headDim]."""
+        if q.dim() != 3 or tuple(q.shape[1:]) != (self.num_heads, self.head_dim):
+            raise IllegalArgumentException(
+                f"q must be [tokens, {self.num_heads}, {self.head_dim}], got {tuple(q.shape)}")
+        kp, vp, rows, stride = self._pool(k, v)
+        out = torch.empty(q.shape, dtype=torch.float32, device=q.device)
+        _check(ctx.handle, N.load().nva_cross_attention_forward(
+            ctx.handle, ctypes.byref(self._desc), _dev(q, "q"), kp, vp, rows, stride, q.shape[0],
+            _dev(out, "out")), "CrossAttention.forward")
         return out

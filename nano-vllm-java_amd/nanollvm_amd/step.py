@@ -11,7 +11,7 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
-from typing import List, Optional, Sequence
+from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
 
@@ -96,3 +96,22 @@ def build_prefill_metadata(seqs, block_size: int) -> StepMeta:
 def build_decode_metadata(seqs, block_size: int) -> StepMeta:
     """nva_build_decode_metadata (Transformer.prepareDecode) over Sequence-like objects."""
     return _build(seqs, block_size, False)
+
+
+def find_shared_prefixes(block_tables, cached_tokens, block_size: int) -> List[Tuple[int, int, int]]:
+    """nva_find_shared_prefixes: the runs of adjacent sequences of a step whose cached tokens start
+    in the same pages, as (first sequence, sequences, tokens) for ``Context.share_prefixes``;
+    ``block_tables`` is the step's 2-D table, -1 padded."""
+    table = np.ascontiguousarray(block_tables, dtype=np.int32)
+    cached = np.ascontiguousarray(cached_tokens, dtype=np.int32)
+    if table.ndim != 2 or cached.shape != (table.shape[0],):
+        raise MetadataError("block tables must be 2-D, with one cached length per row")
+    n = len(cached)
+    groups = (N.PrefixGroup * max(1, n // 2))()
+    count = ctypes.c_int()
+    st = N.load().nva_find_shared_prefixes(table.ctypes.data if table.size else None, n,
+                                           table.shape[1], cached.ctypes.data, block_size, groups,
+                                           ctypes.byref(count))
+    if st != N.NVA_OK:
+        raise MetadataError(N.load().nva_status_string(st).decode())
+    return [(g.first_seq, g.num_seqs, g.num_tokens) for g in groups[:count.value]]
