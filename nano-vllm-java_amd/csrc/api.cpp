@@ -191,6 +191,7 @@ struct Plan {
   int num_spans = 0, max_cols = 0;                // span items, and the most columns of one
   int num_span_tiles = 0, num_span_slots = 0;     // span tiles and their stream-K slots
   int max_parts = 0;  // most partials any merged row has
+  bool beside = false;     // rows and items run on the side stream, beside the tiles
   bool covers_all = true;  // every output row is written by some kernel
   size_t off_rows = 0, off_merge = 0, off_tiles = 0, off_slots = 0;
   size_t off_spans = 0, off_span_tiles = 0, off_span_slots = 0, off_row_part = 0;
@@ -463,7 +464,8 @@ int largest_pow2_divisor_upto(int rep, int cap) {
 // 8 KV heads at d = 64 down to half (8 rows beside 752 new tokens 374 -> 197 us).  At d = 128 rates
 // of 150 to 260 are within 1%: four 512-token chunks beside 64 rows of 4096-16384 keys at 32 q / 8 KV
 // heads take 1040 us at 100, 1005 at 150, 955 at 200, 988 at 250 and 1020 at 350.
-int64_t mixed_tile_cus(int num_cus, double row_bytes, double tile_flops, int head_dim, bool fp32) {
+int64_t mixed_tile_cus(int num_cus, double row_bytes, double tile_flops, int head_dim, bool fp32,
+                       double *seconds = nullptr) {
   const double tr = row_bytes / 6.5e12;
   const double rate = fp32              ? (head_dim == 512 ? 70e12 : 100e12)
                       : head_dim == 64  ? 60e12
@@ -481,7 +483,19 @@ int64_t mixed_tile_cus(int num_cus, double row_bytes, double tile_flops, int hea
       best_s = s;
     }
   }
+  if (seconds) *seconds = best;
   return (int64_t)num_cus * best_s / 16;
+}
+
+// Whether the rows (and items) of a step run beside its span tiles, on a share of the CUs as in a
+// mixed step, or behind them with all CUs for each.  Beside them the longer of the two counts, but
+// 8 us more go to the events; span tiles on all CUs reach 170 / 270 / 170 / 170 TFLOP/s at d = 64 /
+// 128 / 256 / 512, and the rows start 5 us later.
+bool rows_beside_tiles(int num_cus, double row_bytes, double tile_flops, int head_dim) {
+  double beside = 0.0;
+  mixed_tile_cus(num_cus, row_bytes, tile_flops, head_dim, false, &beside);
+  const double behind = row_bytes / 6.5e12 + tile_flops / (head_dim == 128 ? 270e12 : 170e12);
+  return beside + 8e-6 < behind + 5e-6;
 }
 
 // One piece of a tile's keys, on one slot.
@@ -681,19 +695,83 @@ int key_chunk(int n, F len, int64_t workgroups, int64_t many, int64_t few) {
   return 64 * lo;
 }
 
+// The key chunk of span items, each run by `workgroups` workgroups: the multiple of 64 keys whose
+// estimated time is least, in keys: what the resident workgroups (two on a CU) have to do each, but
+// at least one chunk, and half a chunk for the last round.  A workgroup's start and end (Q, the first
+// loads, the waves' meeting, partials) take as long as kFixed keys.
+int span_chunk(const std::vector<SpanItem> &items, int workgroups, int num_cus) {
+  constexpr double kFixed = 250;
+  const double resident = 2.0 * num_cus;
+  int best = 64;
+  double best_time = 1e300;
+  for (int c = 64; c <= 4096; c += 64) {
+    double keys = 0.0, pieces = 0.0;
+    for (const SpanItem &it : items) {
+      const int len = it.kend - it.kbeg, n = (len + c - 1) / c;
+      pieces += n;
+      keys += len;
+    }
+    const double each = (keys + pieces * kFixed) * workgroups / resident;
+    const double one = c + kFixed;
+    const double time = std::max(one, each) + (pieces * workgroups > resident ? 0.5 * one : 0.0);
+    if (time < best_time) {
+      best_time = time;
+      best = c;
+    }
+  }
+  return best;
+}
+
 // A run of query rows that all see the keys [0, len) (nva_internal.h, SpanItem).
 struct Span {
   int row0, rows, seq, kbase, len;
 };
 
-// How a run of that many rows is computed: the span kernel up to two items of columns, span tiles
-// beyond, row by row where neither serves.
-enum class SpanKernel { rows, items, tiles };
-SpanKernel span_kernel_of(const PlanKey &key, int rows) {
+// Estimated time of a span on each kernel, in us on all CUs: span items at 75 TFLOP/s over columns
+// padded to the items', span tiles at tile_rate() over whole tiles, of which idle columns cost 70%.
+// A launch of items takes kItemsUs, of tiles kTilesUs more.  (1e300: the kernel does not serve.)
+struct SpanCost {
+  double items, tiles;
+};
+constexpr double kItemsUs = 3.0, kTilesUs = 14.0;
+double tile_rate(int head_dim) {  // flops per us
+  return head_dim == 128 ? 270e6 : head_dim == 512 ? 100e6 : 170e6;
+}
+SpanCost span_cost(const PlanKey &key, int rows, int len) {
+  SpanCost c{1e300, 1e300};
   const int64_t cols = (int64_t)rows * key.col_heads;
-  if (key.span_cols > 0 && (cols <= 2 * key.span_cols || key.span_tile_cols == 0))
-    return SpanKernel::items;
-  return key.span_tile_cols > 0 ? SpanKernel::tiles : SpanKernel::rows;
+  const double flops = 4.0 * key.head_dim * (key.num_heads / key.col_heads) * len;  // a column
+  if (key.span_cols > 0) {
+    const int per = key.span_cols / key.col_heads * key.col_heads;
+    c.items = flops * (double)((cols + per - 1) / per) * key.span_cols / 75e6;
+  }
+  if (key.span_tile_cols > 0) {
+    const int per = key.span_tile_cols / key.col_heads * key.col_heads;
+    c.tiles = flops * (0.7 * key.span_tile_cols * ((cols + per - 1) / per) + 0.3 * cols) /
+              tile_rate(key.head_dim);
+  }
+  return c;
+}
+
+// Which spans run on span tiles (the others on the span kernel): those of the cheapest of three ways,
+// all on either kernel or each on the one it costs less on.
+std::vector<char> choose_tiles(const PlanKey &key, const std::vector<Span> &spans, double *us) {
+  std::vector<char> tiles(spans.size(), 0);
+  double items_us = kItemsUs, tiles_us = kTilesUs, each_us = 0.0;
+  bool any[2] = {false, false};
+  for (size_t i = 0; i < spans.size(); i++) {
+    const SpanCost c = span_cost(key, spans[i].rows, spans[i].len);
+    items_us += c.items;
+    tiles_us += c.tiles;
+    each_us += std::min(c.items, c.tiles);
+    tiles[i] = c.tiles < c.items;
+    any[(int)tiles[i]] = true;
+  }
+  each_us += (any[0] ? kItemsUs : 0.0) + (any[1] ? kTilesUs : 0.0);
+  *us = std::min({items_us, tiles_us, each_us});
+  if (*us == items_us) tiles.assign(spans.size(), 0);
+  else if (*us == tiles_us) tiles.assign(spans.size(), 1);
+  return tiles;
 }
 
 // One query row of the row kernel before splitting.
@@ -748,17 +826,52 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
   };
   // Shared prefixes: the rows of a group's sequences see its first keys as one span, and each
   // sequence's own lists start behind them.  A sliding window sees too little of them.
+  const bool spans_run = key.span_cols > 0 || key.span_tile_cols > 0;  // else row by row
   std::vector<int32_t> prefix_len(ctx->num_seqs, 0);
-  if (!key.cross && paged && W == 0)
-    for (const nva_prefix_group &gr : ctx->groups) {
+  if (!key.cross && paged && W == 0 && spans_run) {
+    // Sharing has to pay.  Read separately, a prefix costs its rows' share of HBM or whole query
+    // tiles; shared, its span, and in a prefill step another launch, a partial of each row and the
+    // merge, which took 10 us and 4 TB/s.  (Chunks that fill their tiles have nothing to gain: six
+    // chunks of 173 tokens behind 6400, 4 q / 1 KV heads at d = 256, took 193 us apart and 252 us
+    // shared; 24 questions of 1-160 tokens behind 8192, 32 q / 8 KV heads at d = 128, 1437 and 843.)
+    std::vector<size_t> gain;
+    double apart_us = 0.0, join_us = 0.0;
+    for (size_t gi = 0; gi < ctx->groups.size(); gi++) {
+      const nva_prefix_group &gr = ctx->groups[gi];
       const int row0 = first_row(gr.first_seq);
       const int n = first_row(gr.first_seq + gr.num_seqs) - row0;
-      if (n < 2 || gr.num_tokens <= 0 || span_kernel_of(key, n) == SpanKernel::rows) continue;
+      if (n < 2 || gr.num_tokens <= 0) continue;
+      double apart = 0.0, join = 0.0;
+      for (int b = gr.first_seq; b < gr.first_seq + gr.num_seqs; b++) {
+        const int q = first_row(b + 1) - first_row(b);
+        if (key.mfma && q >= 2) {
+          const int tiles_of = (q + key.tile_q - 1) / key.tile_q;
+          apart += 4.0 * key.head_dim * key.num_heads * gr.num_tokens *
+                   (0.7 * key.tile_q * tiles_of + 0.3 * q) / tile_rate(key.head_dim);
+        } else {
+          apart += (double)q * gr.num_tokens * key.num_kv_heads * key.head_dim * 8.0 / 6.5e6;
+        }
+      }
+      if (ctx->is_prefill) join = 16.0 * n * key.num_heads * key.head_dim / 4e6;
+      const SpanCost c = span_cost(key, n, gr.num_tokens);
+      if (std::min(c.items, c.tiles) + join >= apart) continue;
       int seq = gr.first_seq;
       while (first_row(seq + 1) == row0) seq++;  // the first that has rows
       spans.push_back({row0, n, seq, 0, gr.num_tokens});
-      for (int b = 0; b < gr.num_seqs; b++) prefix_len[gr.first_seq + b] = gr.num_tokens;
+      gain.push_back(gi);
+      apart_us += apart;
+      join_us += join;
     }
+    double span_us = 0.0;
+    choose_tiles(key, spans, &span_us);
+    if (ctx->is_prefill ? span_us + join_us + 10.0 >= apart_us : span_us > apart_us + kItemsUs)
+      spans.clear();
+    else
+      for (size_t gi : gain) {
+        const nva_prefix_group &gr = ctx->groups[gi];
+        for (int b = 0; b < gr.num_seqs; b++) prefix_len[gr.first_seq + b] = gr.num_tokens;
+      }
+  }
   if (key.cross) {
     // The rows of sequence b see its encoder's keys; sequences in a row that read the same ones
     // make one span.
@@ -784,7 +897,7 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
     }
     std::vector<Span> kept;
     for (const Span &sp : spans)
-      if (sp.len > 0 && span_kernel_of(key, sp.rows) != SpanKernel::rows)
+      if (sp.len > 0 && spans_run)
         kept.push_back(sp);
       else
         for (int r = 0; r < sp.rows; r++) rows.push_back({sp.row0 + r, 0, sp.kbase, 0, sp.len});
@@ -870,6 +983,28 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
   std::vector<TileItem> span_tiles;
   std::vector<int32_t> span_off;
   int span_slots = 0;
+  // Rows and items run on a second stream beside the tiles (a mixed plan): the tile grids then have
+  // one workgroup on each of tile_cus CUs, and the rows take the rest.  Where spans are, that has to
+  // pay.  pairs: (row, key) pairs of span tiles.
+  int64_t tile_cus = 0;
+  auto plan_beside = [&](double pairs) {
+    if ((tiles.empty() && pairs == 0.0) || (rows.empty() && span_items.empty())) return false;
+    double row_keys = 0.0;
+    for (const Row &r : rows) row_keys += std::max(0, r.kend - r.kbeg);
+    for (const SpanItem &it : span_items) row_keys += it.kend - it.kbeg;
+    for (const TileItem &t : tiles) {
+      const int n = std::min(key.tile_q, t.qlen - t.q0);
+      for (int i = 0; i < n; i++) {
+        const int aq = t.klen - t.qlen + t.q0 + i;
+        pairs += W > 0 ? std::min(aq + 1, W) : aq + 1 - t.ks;
+      }
+    }
+    const double bytes = row_keys * 8.0 * key.num_kv_heads * key.head_dim;
+    const double flops = 4.0 * key.head_dim * key.num_heads * pairs;
+    tile_cus = mixed_tile_cus(ctx->num_cus, bytes, flops, key.head_dim, key.fp32_tiles != 0);
+    return spans.empty() || rows_beside_tiles(ctx->num_cus, bytes, flops, key.head_dim);
+  };
+  bool beside = spans.empty() && plan_beside(0.0);
   if (!spans.empty()) {
     row_part.assign(key.tokens, 0);
     span_parts.assign(key.tokens, 0);
@@ -883,46 +1018,46 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
       merges.push_back({r, parts, pieces, 0});
       parts += pieces;
     };
-    double tile_keys = 0.0;
-    for (const Span &sp : spans)
-      if (span_kernel_of(key, sp.rows) == SpanKernel::tiles) {
+    double tile_pairs = 0.0;
+    double span_us = 0.0;
+    const std::vector<char> on_tiles = choose_tiles(key, spans, &span_us);
+    for (size_t i = 0; i < spans.size(); i++) {
+      const Span &sp = spans[i];
+      if (on_tiles[i]) {
         const int cols = sp.rows * key.col_heads;
         const int per_tile = key.span_tile_cols / key.col_heads * key.col_heads;  // whole rows
         for (int c = 0; c < cols; c += per_tile)
           span_tiles.push_back({sp.seq, sp.row0, std::min(cols, c + per_tile), c, 0, sp.kbase, 0,
                                 sp.len, -1, 1, 0, 0});
-        tile_keys += (double)sp.rows * sp.len;
+        tile_pairs += (double)sp.rows * sp.len;
       } else {
         const int per_item = key.span_cols / key.col_heads;  // rows
         for (int r = 0; r < sp.rows; r += per_item) {
           const int n = std::min(per_item, sp.rows - r);
-          span_items.push_back({sp.row0 + r, n * key.col_heads, sp.seq, sp.kbase, 0, sp.len, 0, 0});
+          span_items.push_back({sp.row0 + r, n * key.col_heads, sp.seq, sp.kbase, 0, sp.len, 0, 0, 0, 0});
         }
       }
+    }
     // Beside span items, and with no span tiles, the rows of the step are items too: one launch.
     const size_t own_items = span_items.size();
     const bool rows_join = !span_items.empty() && span_tiles.empty() && !key.cross;
     if (rows_join) {
       for (const Row &r : rows)
-        span_items.push_back({r.qrow, key.col_heads, r.seq, r.kbase, r.kbeg, r.kend, 0, 0});
+        span_items.push_back({r.qrow, key.col_heads, r.seq, r.kbase, r.kbeg, r.kend, 0, 0, 0, 0});
       rows.clear();
     }
+    beside = plan_beside(tile_pairs);
     if (!span_tiles.empty()) {
       int64_t total = 0;
       for (const TileItem &t : span_tiles) total += (t.ke + 31) / 32;
       const int grid_y = key.num_kv_heads * groups;
-      int64_t resident = (int64_t)ctx->num_cus * key.span_blocks_per_cu;
-      if (!rows.empty() || !span_items.empty()) {
-        // The rows and items run beside the tiles, as in a mixed step.
-        double keys = 0.0;
-        for (const Row &r : rows) keys += std::max(0, r.kend - r.kbeg);
-        for (const SpanItem &it : span_items) keys += it.kend - it.kbeg;
-        resident = std::max<int64_t>(
-            grid_y, mixed_tile_cus(ctx->num_cus, keys * 8.0 * key.num_kv_heads * key.head_dim,
-                                   4.0 * key.head_dim * key.num_heads * tile_keys, key.head_dim,
-                                   false));
-      }
+      const int64_t resident = beside ? std::max<int64_t>(grid_y, tile_cus)
+                                      : (int64_t)ctx->num_cus * key.span_blocks_per_cu;
       span_slots = (int)std::max<int64_t>(1, std::min<int64_t>(total, resident / grid_y));
+      // Where 30 pieces of a tile nearly fill the CUs, no more: with those of its own keys a row then
+      // has few enough for the merge of 4 waves a head (33 of them took it 16 us, 18 of them 9).
+      const int few = 30 * (int)std::min<size_t>(span_tiles.size(), INT32_MAX / 64);
+      if (span_slots > few && span_slots <= few + few / 8) span_slots = few;
       std::vector<int> tile_rows(span_tiles.size());
       for (size_t i = 0; i < span_tiles.size(); i++)
         tile_rows[i] = (span_tiles[i].qlen - span_tiles[i].q0) / key.col_heads;
@@ -940,9 +1075,7 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
       });
     }
     if (!span_items.empty()) {
-      int chunk = key_chunk(
-          (int)span_items.size(), [&](int i) { return span_items[i].kend - span_items[i].kbeg; },
-          (int64_t)key.num_kv_heads * groups, (int64_t)ctx->num_cus * 8, ctx->num_cus);
+      int chunk = span_chunk(span_items, key.num_kv_heads * groups, ctx->num_cus);
       if (paged) chunk = std::min(chunk, (kRowTablePages - 1) * key.block_size);
       std::vector<SpanItem> cut;
       for (size_t i = 0; i < span_items.size(); i++) {
@@ -988,26 +1121,8 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
     constexpr int KT = 32;
     int64_t total = 0;
     for (const TileItem &t : tiles) total += (t.ke - t.ks + KT - 1) / KT;
-    // A mixed plan runs its rows on a second stream beside the tiles; the tile grid then has
-    // one workgroup on each of a share of the CUs, and the rows take the rest.
-    int64_t resident = (int64_t)ctx->num_cus * key.blocks_per_cu;
-    if (!rows.empty() || !span_items.empty()) {
-      double row_bytes = 0.0, pairs = 0.0;
-      for (const Row &r : rows) row_bytes += std::max(0, r.kend - r.kbeg);
-      for (const SpanItem &it : span_items) row_bytes += it.kend - it.kbeg;
-      row_bytes *= 8.0 * key.num_kv_heads * key.head_dim;
-      for (const TileItem &t : tiles) {
-        const int n = std::min(key.tile_q, t.qlen - t.q0);
-        for (int i = 0; i < n; i++) {
-          const int aq = t.klen - t.qlen + t.q0 + i;
-          pairs += W > 0 ? std::min(aq + 1, W) : aq + 1 - t.ks;
-        }
-      }
-      const double flops = 4.0 * key.head_dim * key.num_heads * pairs;
-      resident = std::max<int64_t>(key.tile_groups,
-                                   mixed_tile_cus(ctx->num_cus, row_bytes, flops, key.head_dim,
-                                                key.fp32_tiles != 0));
-    }
+    const int64_t resident = beside ? std::max<int64_t>(key.tile_groups, tile_cus)
+                                    : (int64_t)ctx->num_cus * key.blocks_per_cu;
     slots = (int)std::max<int64_t>(1, std::min<int64_t>(total, resident / key.tile_groups));
     const int64_t cap_tiles = std::max<int64_t>(1, page_cap / KT);
     std::vector<int> tile_rows(tiles.size());
@@ -1083,9 +1198,9 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
     parts += n + prefix;
   }
   // Items within at most two pages carry the pages' block ids (RowItem::blk_a / blk_b).
-  if (key.paged) {
+  auto inline_pages = [&](auto &list) {
     const int bs = key.block_size;
-    for (RowItem &it : items) {
+    for (auto &it : list) {
       if (it.kend <= it.kbeg) continue;
       const int p0 = it.kbeg / bs, p1 = (it.kend - 1) / bs;
       if (p1 - p0 > 1) continue;
@@ -1093,6 +1208,10 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
       it.blk_a = t[p0] + 1;
       it.blk_b = p1 > p0 ? t[p1] : 0;
     }
+  };
+  if (key.paged) {
+    inline_pages(items);
+    inline_pages(span_items);
   }
   // Longest items first: the workgroups dispatched last are the short row tails, so the chip
   // drains quickly at the end of the launch.  Items carry their own partial slot, so the
@@ -1126,6 +1245,7 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
   plan->num_slots = slots;
   plan->max_parts = 0;
   for (const MergeItem &mi : merges) plan->max_parts = std::max(plan->max_parts, mi.nparts);
+  plan->beside = beside;
   plan->num_spans = (int)span_items.size();
   plan->max_cols = 0;
   for (const SpanItem &it : span_items) plan->max_cols = std::max(plan->max_cols, it.cols);
@@ -1335,7 +1455,7 @@ nva_status attention_plan(nva_ctx *ctx, const nva_attn_desc &d, int paged, int b
     const bool tiles = prefill_kernel_supports(d.head_dim, 1);
     const bool items = span_kernel_supports(d.head_dim, paged, block_size);
     key.span_tile_cols = tiles ? span_tile_cols(d.head_dim) : 0;
-    key.span_cols = items ? span_max_cols(d.head_dim) : 0;
+    key.span_cols = items ? kSpanCols : 0;
     // A column group holds whole rows of a tile and of an item.
     const int most = std::min(tiles ? key.span_tile_cols : rep, items ? key.span_cols : rep);
     key.col_heads = std::min(rep, most);
@@ -1469,8 +1589,7 @@ nva_status run_attention(nva_ctx *ctx, const nva_attn_desc &d, const KvView &vie
   // main stream waits for the side stream before the merge.  The tiles are issued first: the
   // plan sized their grid to a share of the CUs, which it only gets if the rows do not fill
   // the chip before it.
-  const bool fork = (plan->num_tiles > 0 || plan->num_span_tiles > 0) &&
-                    (plan->num_rows > 0 || plan->num_spans > 0);
+  const bool fork = plan->beside;
   const int32_t *row_part = reinterpret_cast<const int32_t *>(pbase + plan->off_row_part);
   if (fork) HIP_TRY(ctx, hipEventRecord(ctx->fork_ev, ctx->stream), "fork record");
   TileLaunch t;

@@ -127,6 +127,7 @@ struct SpanItem {
   int32_t kbeg;   // first key
   int32_t kend;   // one past the last key
   int32_t split;  // partial row_part[row] + split, or -1: the whole range, written to out
+  int32_t blk_a, blk_b;  // as in RowItem
   int32_t pad;
 };
 
@@ -262,7 +263,6 @@ hipError_t launch_span_tiles(const TileLaunch &a, hipStream_t s);
 // The span kernel of few columns (span.hip): most columns of an item, and the shapes it is built
 // for (paged: pages of a power of two of at least 16 tokens).
 constexpr int kSpanCols = 32;
-int span_max_cols(int head_dim);
 bool span_kernel_supports(int head_dim, int paged, int block_size);
 hipError_t launch_spans(const SpanLaunch &a, int max_cols, hipStream_t s);
 

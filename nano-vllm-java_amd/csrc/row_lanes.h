@@ -15,15 +15,23 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // (headline decode 2.160-2.162 against 2.166-2.171 ms with the pointer form).  The cache policy
 // matters, the form little: without the non-temporal bit the same loads take 2.40 ms, and
 // adding the L1-bypass (sc0) or device-scope (sc1) bits changes nothing.
-__device__ __forceinline__ float4 ld4_stream_at(const float *base, uint32_t off) {
-  constexpr int kNonTemporal = 2;  // the nt bit of the buffer instructions' cache policy
+template <int POLICY>
+__device__ __forceinline__ float4 ld4_buffer(const float *base, uint32_t off) {
   const uint64_t b = (uint64_t)(size_t)base;
   const uint64_t u = ((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32)) << 32) |
                      (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b);
   const __amdgpu_buffer_rsrc_t r =
       __builtin_amdgcn_make_buffer_rsrc((void *)(size_t)u, (short)0, 0x7fffffff, kBufferWord3);
-  const f32x4 t = __builtin_amdgcn_raw_buffer_load_b128(r, off * 4, 0, kNonTemporal);
+  const f32x4 t = __builtin_amdgcn_raw_buffer_load_b128(r, off * 4, 0, POLICY);
   return make_float4(t.x, t.y, t.z, t.w);
+}
+__device__ __forceinline__ float4 ld4_stream_at(const float *base, uint32_t off) {
+  constexpr int kNonTemporal = 2;  // the nt bit of the buffer instructions' cache policy
+  return ld4_buffer<kNonTemporal>(base, off);
+}
+// The same, cached.
+__device__ __forceinline__ float4 ld4_at(const float *base, uint32_t off) {
+  return ld4_buffer<0>(base, off);
 }
 
 // x[lane] + x[lane ^ 16] (resp. lane ^ 32) in every lane, by gfx950's row-swap instructions:

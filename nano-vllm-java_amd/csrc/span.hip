@@ -13,7 +13,7 @@
 // 4 D operations a column, so fp32 matrix instructions (which need no scaling and take any value)
 // stay ahead of the memory up to about 48 columns.  One workgroup of 4 waves per (item, KV head,
 // head group); each wave takes 16-key blocks of the item in turn, so that 4 waves read 64
-// consecutive keys at a time, two register buffers deep, with no barrier and no LDS until the end:
+// consecutive keys at a time, with no barrier and no LDS until the end:
 //   S^T[key][col] = K Q^T    D/4 v_mfma_f32_16x16x4_f32 per block and 16 columns: at step 4v + c
 //                            lane (i, g) supplies K[t0 + i][16v + 4g + c] (A) and
 //                            Q[col i][16v + 4g + c] (B), i = lane % 16, g = lane / 16;
@@ -31,19 +31,32 @@ namespace nva {
 namespace {
 __device__ __forceinline__ float4 ld4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
 __device__ __forceinline__ void st4(float *p, float4 v) { *reinterpret_cast<float4 *>(p) = v; }
+// This wave's LDS writes, then the workgroup: unlike __syncthreads(), the loads in flight stay so.
+__device__ __forceinline__ void lds_writes_barrier() {
+  wait_lds_reads();
+  lds_barrier();
+}
 }  // namespace
 
 template <int D, int NCB, bool PAGED>
-__global__ void __launch_bounds__(256) span_kernel(SpanLaunch a) {
-  constexpr int DQ = D / 4;   // QK steps per block
-  constexpr int NB = D / 16;  // O^T blocks; block b = 4w + c, row i is dim 64w + 4i + c
-  constexpr int NQ = DQ / 4;  // float4 loads of a K row part per lane
-  constexpr int NV = NB / 4;  // float4 loads of a V row part per lane per key (one per 64 dims)
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
+span_kernel(SpanLaunch a) {
+  constexpr int DW = D < 128 ? D : 128;  // dims of a wave
+  constexpr int DS = D / DW;             // waves that share a key block, by dims
+  constexpr int KG = 4 / DS;             // key blocks in turn
+  constexpr int DQ = DW / 4;   // QK steps per block
+  constexpr int NB = DW / 16;  // O^T blocks; block b = 4w + c, row i is dim 64w + 4i + c of the wave's
+  constexpr int NQ = DQ / 4;   // float4 loads of a K row part per lane
+  constexpr int NV = NB / 4;   // float4 loads of a V row part per lane per key (one per 64 dims)
   constexpr int COLS = 16 * NCB;
-  __shared__ float sm_m[4][COLS];
-  __shared__ float sm_l[4][COLS];
-  __shared__ float4 sm_acc[4][COLS][D / 4];
+  __shared__ float sm_m[KG][COLS];
+  __shared__ float sm_l[KG][COLS];
+  __shared__ float4 sm_acc[KG][COLS][D / 4];
   __shared__ int32_t stab[kRowTablePages];
+
+  // Partial scores [turn][wave][column block][lane], until the waves' results meet.
+  float4 *const spart = &sm_acc[0][0][0];
+  static_assert(DS == 1 || 2 * 4 * NCB * 64 <= KG * COLS * (D / 4), "spart lies in sm_acc");
 
   const int rep = a.hq / a.hkv;
   const int groups = rep / a.col_heads;
@@ -55,6 +68,7 @@ __global__ void __launch_bounds__(256) span_kernel(SpanLaunch a) {
   const int h0 = kvh * rep + (gy - kvh * groups) * a.col_heads;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kg = wave / DS, ds = wave % DS;
   const int i = lane & 15;
   const int g = lane >> 4;
 
@@ -66,8 +80,8 @@ __global__ void __launch_bounds__(256) span_kernel(SpanLaunch a) {
     const int c = 16 * n + i;
     if (c < it.cols) {
       const int r = c / a.col_heads;
-      const float *qp =
-          a.q + ((size_t)(it.row0 + r) * a.hq + h0 + c - r * a.col_heads) * D + 4 * g;
+      const float *qp = a.q + ((size_t)(it.row0 + r) * a.hq + h0 + c - r * a.col_heads) * D +
+                        DW * ds + 4 * g;
 #pragma unroll
       for (int v = 0; v < NQ; v++) {
         const float4 x = ld4(qp + 16 * v);
@@ -85,62 +99,75 @@ __global__ void __launch_bounds__(256) span_kernel(SpanLaunch a) {
   const size_t rs = (size_t)a.kv.ld;
   const int bs_shift = a.kv.bs_shift;
   const int blk0 = PAGED ? it.kbeg >> bs_shift : 0;
-  if constexpr (PAGED) {
+  // An item within at most two pages carries their block ids: no table read before its first loads.
+  const bool inl = PAGED && it.blk_a != 0;
+  if (PAGED && !inl) {
     const int32_t *table = a.kv.table + (size_t)it.seq * a.kv.bt_stride;
     const int npages = ((it.kend - 1) >> bs_shift) - blk0 + 1;
     for (int j = threadIdx.x; j < npages; j += blockDim.x) stab[j] = table[blk0 + j];
     __syncthreads();
   }
-  const float *kbase_h = a.kv.k + (size_t)kvh * D;
-  const float *vbase_h = a.kv.v + (size_t)kvh * D;
+  const float *kbase_h = a.kv.k + (size_t)kvh * D + DW * ds;
+  const float *vbase_h = a.kv.v + (size_t)kvh * D + DW * ds;
   const int tfirst = it.kbeg & ~15;  // blocks of pages start at multiples of 16
   // Fixed lane offsets (floats) from a block's first row: K row i, dims 16v + 4g; V rows
   // 4g + s, dims 64w + 4i.
   const uint32_t koff = (uint32_t)(i * rs + 4 * g);
   const uint32_t voff = (uint32_t)(4 * g * rs + 4 * i);
 
-  float kra[DQ], krb[DQ];
-  float vra[4][NB], vrb[4][NB];
-  auto issue = [&](int t0, float(&kr)[DQ], float(&vr)[4][NB]) {
-    // A block past the item's end reloads its first block (never folded).
+  // The wave's block t0: its rows' base, and this lane's offsets in it (floats).
+  struct Block {
+    const float *k, *v;
+    uint32_t ko, vo[4];
+  };
+  auto locate = [&](int t0) {
+    Block b;
+    // A block past the item's end is the item's first (never used).
     const int tb = t0 < it.kend ? t0 : tfirst;
     int64_t row;
     if constexpr (PAGED) {
       const int p = tb >> bs_shift;
-      const int id = __builtin_amdgcn_readfirstlane(stab[p - blk0]);
+      const int id = inl ? (p == blk0 ? it.blk_a - 1 : it.blk_b)
+                         : __builtin_amdgcn_readfirstlane(stab[p - blk0]);
       row = (int64_t)id * a.kv.block_size + (tb - (p << bs_shift));
     } else {
       row = (int64_t)it.kbase + tb;
     }
-    const float *kb = kbase_h + row * (int64_t)rs;
-    const float *vb = vbase_h + row * (int64_t)rs;
-    uint32_t ko = koff, vo[4];
+    b.k = kbase_h + row * (int64_t)rs;
+    b.v = vbase_h + row * (int64_t)rs;
+    b.ko = koff;
 #pragma unroll
-    for (int s = 0; s < 4; s++) vo[s] = voff + (uint32_t)(s * rs);
+    for (int s = 0; s < 4; s++) b.vo[s] = voff + (uint32_t)(s * rs);
     if (tb < it.kbeg || tb + 16 > it.kend) {
       // A partial block: every lane reads the block's key nearest its own inside the item (what
       // lies outside could hold any bits, NaN included; a finite V row adds 0 at weight 0).
       const int tk = min(max(tb + i, it.kbeg), it.kend - 1);
-      ko = (uint32_t)((tk - tb) * (int64_t)rs + 4 * g);
+      b.ko = (uint32_t)((tk - tb) * (int64_t)rs + 4 * g);
 #pragma unroll
       for (int s = 0; s < 4; s++) {
         const int tv = min(max(tb + 4 * g + s, it.kbeg), it.kend - 1);
-        vo[s] = (uint32_t)((tv - tb) * (int64_t)rs + 4 * i);
+        b.vo[s] = (uint32_t)((tv - tb) * (int64_t)rs + 4 * i);
       }
     }
+    return b;
+  };
+  float kr[DQ], vr[4][NB];
+  auto load_k = [&](const Block &b) {
 #pragma unroll
     for (int v = 0; v < NQ; v++) {
-      const float4 x = ld4_stream_at(kb, ko + 16 * v);
+      const float4 x = ld4_at(b.k, b.ko + 16 * v);
       kr[4 * v] = x.x;
       kr[4 * v + 1] = x.y;
       kr[4 * v + 2] = x.z;
       kr[4 * v + 3] = x.w;
     }
+  };
+  auto load_v = [&](const Block &b) {
 #pragma unroll
     for (int s = 0; s < 4; s++)
 #pragma unroll
       for (int v = 0; v < NV; v++) {
-        const float4 x = ld4_stream_at(vb, vo[s] + 64 * v);
+        const float4 x = ld4_at(b.v, b.vo[s] + 64 * v);
         vr[s][4 * v] = x.x;
         vr[s][4 * v + 1] = x.y;
         vr[s][4 * v + 2] = x.z;
@@ -157,77 +184,97 @@ __global__ void __launch_bounds__(256) span_kernel(SpanLaunch a) {
     m_run[n] = -INFINITY;
     l_run[n] = 0.0f;
   }
-  auto fold = [&](int t0, const float(&kr)[DQ], const float(&vr)[4][NB]) {
+
+  int t0 = tfirst + 16 * kg;
+  // Waves that share a key block meet at every one, so all of the workgroup's make the same turns.
+  const int tend = DS == 1 ? it.kend : it.kend + 16 * kg;
+  if (t0 < tend) {
+    Block at = locate(t0);
+    load_k(at);
+    load_v(at);
+    for (int turn = 0; t0 < tend; t0 += 16 * KG, turn ^= 1) {
+      f32x4 p[NCB];
 #pragma unroll
-    for (int n = 0; n < NCB; n++) {
-      if (n > 0 && it.cols <= 16 * n) break;  // an item of a launch with wider ones
-      f32x4 st = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int n = 0; n < NCB; n++) p[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int s = 0; s < DQ; s++)
-        st = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[s], q[n][s], st, 0, 0, 0);
-      float p[4];
-      float mx = -INFINITY;
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const int key = t0 + 4 * g + r;
-        p[r] = (key >= it.kbeg && key < it.kend) ? st[r] : -INFINITY;
-        mx = fmaxf(mx, p[r]);
+        for (int n = 0; n < NCB; n++)
+          p[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[s], q[n][s], p[n], 0, 0, 0);
+      // The next block's K is in flight during the softmax and PV, its V during the next QK.
+      const Block next = locate(t0 + 16 * KG);
+      load_k(next);
+      if constexpr (DS > 1) {
+        // Scores of all dims, added in the waves' order (so that they hold the same bits).
+#pragma unroll
+        for (int n = 0; n < NCB; n++)
+          spart[((turn * 4 + wave) * NCB + n) * 64 + lane] = make_float4(p[n][0], p[n][1], p[n][2], p[n][3]);
+        lds_writes_barrier();
+#pragma unroll
+        for (int n = 0; n < NCB; n++) {
+          const float4 x = spart[((turn * 4 + kg * DS) * NCB + n) * 64 + lane];
+          p[n] = f32x4{x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int w = 1; w < DS; w++) {
+            const float4 y = spart[((turn * 4 + kg * DS + w) * NCB + n) * 64 + lane];
+            p[n] += f32x4{y.x, y.y, y.z, y.w};
+          }
+        }
       }
-      mx = max4_lanes(mx);
-      // The max moves, and the sums with it, only where it grows by more than 2^8.
-      const bool need = mx > m_run[n] + 8.0f;
-      if (__any(need)) {
-        const float mn = need ? mx : m_run[n];
-        const float alpha = m_run[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[n] - mn);
-        l_run[n] *= alpha;
 #pragma unroll
-        for (int b = 0; b < NB; b++) o[n][b] *= alpha;
-        m_run[n] = mn;
-      }
-      const float ms = m_run[n] == -INFINITY ? 0.0f : m_run[n];
+      for (int n = 0; n < NCB; n++) {
+        float mx = -INFINITY;
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        p[r] = __builtin_amdgcn_exp2f(p[r] - ms);
-        l_run[n] += p[r];
+        for (int r = 0; r < 4; r++) {
+          const int key = t0 + 4 * g + r;
+          p[n][r] = (key >= it.kbeg && key < it.kend) ? p[n][r] : -INFINITY;
+          mx = fmaxf(mx, p[n][r]);
+        }
+        mx = max4_lanes(mx);
+        // The max moves, and the sums with it, only where it grows by more than 2^8.
+        const bool need = mx > m_run[n] + 8.0f;
+        if (__any(need)) {
+          const float mn = need ? mx : m_run[n];
+          const float alpha = m_run[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[n] - mn);
+          l_run[n] *= alpha;
+#pragma unroll
+          for (int b = 0; b < NB; b++) o[n][b] *= alpha;
+          m_run[n] = mn;
+        }
+        const float ms = m_run[n] == -INFINITY ? 0.0f : m_run[n];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          p[n][r] = __builtin_amdgcn_exp2f(p[n][r] - ms);
+          l_run[n] += p[n][r];
+        }
       }
 #pragma unroll
       for (int s = 0; s < 4; s++)
 #pragma unroll
         for (int b = 0; b < NB; b++)
-          o[n][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[s][b], p[s], o[n][b], 0, 0, 0);
-    }
-  };
-
-  int t0 = tfirst + 16 * wave;
-  if (t0 < it.kend) {
-    issue(t0, kra, vra);
-    for (;;) {
-      issue(t0 + 64, krb, vrb);
-      fold(t0, kra, vra);
-      t0 += 64;
-      if (t0 >= it.kend) break;
-      issue(t0 + 64, kra, vra);
-      fold(t0, krb, vrb);
-      t0 += 64;
-      if (t0 >= it.kend) break;
+#pragma unroll
+          for (int n = 0; n < NCB; n++)
+            o[n][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[s][b], p[n][s], o[n][b], 0, 0, 0);
+      load_v(next);
     }
   }
 
+  if constexpr (DS > 1) __syncthreads();  // every wave is done with spart
 #pragma unroll
   for (int n = 0; n < NCB; n++) {
     const int c = 16 * n + i;
     const float l_tot = sum4_lanes(l_run[n]);
     if (c < it.cols) {
-      if (g == 0) {
-        sm_m[wave][c] = m_run[n];
-        sm_l[wave][c] = l_tot;
+      if (g == 0 && ds == 0) {
+        sm_m[kg][c] = m_run[n];
+        sm_l[kg][c] = l_tot;
       }
-      // Lane (i, g) holds row 4g + r of block 4w + b: dim 64w + 16g + 4r + b.
+      // Lane (i, g) holds row 4g + r of block 4w + b: dim 64w + 16g + 4r + b of the wave's.
 #pragma unroll
       for (int w = 0; w < NV; w++)
 #pragma unroll
         for (int r = 0; r < 4; r++)
-          sm_acc[wave][c][16 * w + 4 * g + r] = make_float4(
+          sm_acc[kg][c][DW / 4 * ds + 16 * w + 4 * g + r] = make_float4(
               o[n][4 * w][r], o[n][4 * w + 1][r], o[n][4 * w + 2][r], o[n][4 * w + 3][r]);
     }
   }
@@ -237,12 +284,12 @@ __global__ void __launch_bounds__(256) span_kernel(SpanLaunch a) {
     const int cc = idx - c * (D / 4);
     float M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < 4; w++) M = fmaxf(M, sm_m[w][c]);
+    for (int w = 0; w < KG; w++) M = fmaxf(M, sm_m[w][c]);
     const float Ms = M == -INFINITY ? 0.0f : M;
     float L = 0.0f;
     float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < 4; w++) {
+    for (int w = 0; w < KG; w++) {
       const float e = __builtin_amdgcn_exp2f(sm_m[w][c] - Ms);
       L = fmaf(sm_l[w][c], e, L);
       const float4 x = sm_acc[w][c][cc];
@@ -281,11 +328,8 @@ void launch_span(const SpanLaunch &a, hipStream_t s) {
 
 }  // namespace
 
-// At d = 256 the registers hold 16 columns.
-int span_max_cols(int head_dim) { return head_dim == 256 ? 16 : kSpanCols; }
-
 bool span_kernel_supports(int head_dim, int paged, int block_size) {
-  return (head_dim == 64 || head_dim == 128 || head_dim == 256) &&
+  return (head_dim == 64 || head_dim == 128 || head_dim == 256 || head_dim == 512) &&
          (!paged || (block_size >= 16 && (block_size & (block_size - 1)) == 0));
 }
 
@@ -297,6 +341,9 @@ hipError_t launch_spans(const SpanLaunch &a, int max_cols, hipStream_t s) {
     case 128 * 2: launch_span<128, 1>(a, s); break;
     case 128 * 2 + 1: launch_span<128, 2>(a, s); break;
     case 256 * 2: launch_span<256, 1>(a, s); break;
+    case 256 * 2 + 1: launch_span<256, 2>(a, s); break;
+    case 512 * 2: launch_span<512, 1>(a, s); break;
+    case 512 * 2 + 1: launch_span<512, 2>(a, s); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();

@@ -634,31 +634,32 @@ class CrossAttention:
 
     def _pool(self, k, v):
         """Pointers, rows and row stride of the encoder's keys and values."""
+        row = (self.num_kv_heads, self.head_dim)
+        rows, stride = k.shape[0] if k.dim() else 0, k.stride(0) if k.dim() else 0
         for name, t in (("k", k), ("v", v)):
-            if t.dim() != 3 or tuple(t.shape[1:]) != (self.num_kv_heads, self.head_dim):
+            if t.dim() != 3 or t.shape[1:] != row:
                 raise IllegalArgumentException(
-                    f"{name} must be [rows, {self.num_kv_heads}, {self.head_dim}], "
-                    f"got {tuple(t.shape)}")
-            if not (t.is_cuda and t.dtype == torch.float32 and
-                    (t.numel() == 0 or t[0].is_contiguous())):
+                    f"{name} must be [rows, {row[0]}, {row[1]}], got {tuple(t.shape)}")
+            if not (t.is_cuda and t.dtype is torch.float32 and
+                    (rows == 0 or t.stride()[1:] == (self.head_dim, 1))):
                 raise IllegalArgumentException(
                     f"{name} must be a float32 device tensor with contiguous rows")
-        if k.shape[0] != v.shape[0] or (k.shape[0] > 1 and k.stride(0) != v.stride(0)):
+        if v.shape[0] != rows or (rows > 1 and v.stride(0) != stride):
             raise IllegalArgumentException("k and v must have the same rows and row stride")
-        stride = k.stride(0) if k.shape[0] > 1 else self.num_kv_heads * self.head_dim
-        return k.data_ptr(), v.data_ptr(), k.shape[0], stride
+        return k.data_ptr(), v.data_ptr(), rows, stride if rows > 1 else row[0] * row[1]
 
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                 ctx: Context) -> torch.Tensor:
         """softmax(q k^T scale) v over the rows of ``ctx.set_encoder``: q [tokens, numHeads, headDim]
         as the step has it, k and v [rows, numKvHeads, headDim], whose rows may lie apart (views of
         one packed projection); returns a new [tokens, numHeads, headDim]."""
-        if q.dim() != 3 or tuple(q.shape[1:]) != (self.num_heads, self.head_dim):
+        if q.dim() != 3 or q.shape[1:] != (self.num_heads, self.head_dim):
             raise IllegalArgumentException(
                 f"q must be [tokens, {self.num_heads}, {self.head_dim}], got {tuple(q.shape)}")
         kp, vp, rows, stride = self._pool(k, v)
-        out = torch.empty(q.shape, dtype=torch.float32, device=q.device)
+        qp = _dev(q, "q")
+        out = torch.empty_like(q)
         _check(ctx.handle, N.load().nva_cross_attention_forward(
-            ctx.handle, ctypes.byref(self._desc), _dev(q, "q"), kp, vp, rows, stride, q.shape[0],
-            _dev(out, "out")), "CrossAttention.forward")
+            ctx.handle, ctypes.byref(self._desc), qp, kp, vp, rows, stride, q.shape[0],
+            out.data_ptr()), "CrossAttention.forward")
         return out

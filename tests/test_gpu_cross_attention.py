@@ -170,6 +170,35 @@ def test_infinities(ctx, queries, shape):
     ctx.clear()
 
 
+@pytest.mark.parametrize("shape", [(16, 8, 128), (12, 12, 64), (4, 1, 256), (8, 1, 512)], ids=str)
+def test_infinities_on_span_tiles(ctx, shape):
+    """Prompts long enough for span tiles: -inf scores, one sequence that has nothing else, and
+    lengths around the tiles'."""
+    hq, hkv, d = shape
+    lens, queries = [3000, 2049, 31], [700, 300, 260]
+    pool = Pool(shape, lens, 14, True)
+    q = torch.randn(sum(queries), hq, d, device="cuda")
+    q[..., 0] = q[..., 0].abs() + 0.5
+    s0, s2 = int(pool.start[0]), int(pool.start[2])
+    pool.k[s0 + 1030:s0 + 1070, :, 0] = -float("inf")
+    pool.v[s0 + 1030] = 1e30
+    pool.k[s2:s2 + 31, :, 0] = -float("inf")
+    set_step(ctx, queries, lens, pool.start)
+    scale = float(np.float32(d ** -0.5))
+    ctx.set_timing(True)
+    try:
+        ctx.reset_stats()
+        out = CrossAttention(hq, d, scale, hkv).forward(q, pool.k, pool.v, ctx)
+        ctx.sync()
+        assert ctx.kernel_stats("span_tiles")[0] == 1
+    finally:
+        ctx.set_timing(False)
+    want = reference(q, pool, queries, lens, pool.start, scale)
+    close(out, want, f"infinities on span tiles {shape}")
+    assert torch.equal(out[1000:], torch.zeros_like(out[1000:]))
+    ctx.clear()
+
+
 @pytest.mark.parametrize("queries", [1, 30])
 def test_large_scores_and_negative_scale(ctx, queries):
     """Scores of some hundreds, where one key has nearly all the weight; a negative scale."""

@@ -135,6 +135,55 @@ def test_prefill_and_mixed(ctx, shape, chunks):
         s.arena.close()
 
 
+@pytest.mark.parametrize("shape", [(16, 8, 128), (32, 8, 64), (4, 1, 256), (8, 1, 512), (40, 8, 128),
+                                   (12, 12, 64), (34, 2, 64), (71, 1, 64)], ids=str)
+@pytest.mark.parametrize("chunks", [(2, 1, 3), (9,) * 30 + (1, 40, 70)], ids=["few", "many"])
+def test_prefill_over_long_prefixes(ctx, shape, chunks):
+    """Prefixes long enough that a prefill step reads them as spans, of few and of many columns,
+    beside query tiles and rows of its own and a sequence that shares nothing."""
+    own = [(i % 3, n) for i, n in enumerate(chunks)] + [(70, 50)]
+    st = SharedStep([(len(chunks), 8192), (1, 0)], own, 256, seed=20, decode=False)
+    s = Setup(ctx, st, shape, seed=20)
+    ctx.set_timing(True)
+    try:
+        ctx.reset_stats()
+        s.check(ctx, f"prefill over 8192 tokens {shape} {len(chunks)} chunks")
+        ran = dict(zip(("span", "span_tiles"), launches(ctx, "span", "span_tiles")))
+        assert sum(ran.values()) >= 1, ran
+    finally:
+        ctx.set_timing(False)
+        ctx.clear()
+        s.arena.close()
+
+
+def test_prefill_chunks_that_fill_their_tiles_are_read_apart(ctx):
+    st = SharedStep([(2, 1536)], [(0, 256), (0, 256)], 256, seed=21, decode=False)
+    s = Setup(ctx, st, (16, 8, 128), seed=21)
+    ctx.set_timing(True)
+    try:
+        ctx.reset_stats()
+        s.check(ctx, "full chunks")
+        assert launches(ctx, "span", "span_tiles") == [0, 0]
+    finally:
+        ctx.set_timing(False)
+        ctx.clear()
+        s.arena.close()
+
+
+@pytest.mark.parametrize("shape", [(16, 8, 128), (32, 8, 64), (4, 1, 256), (8, 1, 512)], ids=str)
+def test_groups_on_both_kernels(ctx, shape):
+    """Groups of few and of many columns in one decode step, beside long rows of their own: the span
+    kernel, span tiles, and the rows on the second stream."""
+    st = SharedStep([(3, 4096), (200, 2048), (2, 1024), (9, 0)],
+                    [(i * 7 % 900, 1) for i in range(214)], 256, seed=22)
+    s = Setup(ctx, st, shape, seed=22)
+    try:
+        s.check(ctx, f"few and many columns {shape}")
+    finally:
+        ctx.clear()
+        s.arena.close()
+
+
 def test_long_prefix_many_rows(ctx):
     st = SharedStep([(130, 20480), (60, 5120)], [(i % 300, 1) for i in range(190)], 256, seed=5)
     s = Setup(ctx, st, (16, 8, 128), seed=5)
@@ -146,13 +195,13 @@ def test_long_prefix_many_rows(ctx):
 
 
 def test_found_groups_use_both_kernels(ctx):
-    """find_shared_prefixes gives the groups; 3 rows run on the span kernel, 150 on span tiles, and
-    without sharing neither runs."""
+    """find_shared_prefixes gives the groups; a few rows and a short prefix run on the span kernel,
+    many over a long one on span tiles, and without sharing neither runs."""
     ctx.set_timing(True)
     try:
-        for rows, name in ((3, "span"), (150, "span_tiles")):
-            st = SharedStep([(rows, 512)], [(3, 1)] * rows, 256, seed=6)
-            assert st.found() == [(0, rows, 512)]
+        for rows, tokens, name in ((3, 512, "span"), (150, 512, "span"), (150, 8192, "span_tiles")):
+            st = SharedStep([(rows, tokens)], [(3, 1)] * rows, 256, seed=6)
+            assert st.found() == [(0, rows, tokens)]
             s = Setup(ctx, st, (16, 8, 128), seed=6, groups=st.found())
             try:
                 ctx.reset_stats()
@@ -246,6 +295,37 @@ def test_infinities_and_unlike_sizes(ctx, rows, shape):
             say(f"unlike sizes {shape} {rows} rows, dims {dims}: rel_l2={rel:.3e}")
             assert rel <= 1e-5
     finally:
+        ctx.clear()
+        s.arena.close()
+
+
+@pytest.mark.parametrize("shape", [(16, 8, 128), (32, 8, 64), (4, 1, 256), (8, 1, 512)], ids=str)
+def test_infinities_and_unlike_sizes_on_span_tiles(ctx, shape):
+    """The same over a prefix and rows that run on span tiles, whose segments with such keys are
+    taken again on fp32 instructions."""
+    st = SharedStep([(210, 4096)], [(i % 9, 1) for i in range(210)], 64, seed=23)
+    s = Setup(ctx, st, shape, seed=23)
+    ctx.set_timing(True)
+    try:
+        at = torch.from_numpy(st.slots[0]).cuda()
+        s.q[..., 0] = s.q[..., 0].abs() + 0.5
+        s.kp[at[70], :, 0] = -float("inf")
+        s.kp[at[2071]] *= 30
+        s.vp[:, :, 3] *= 1e6
+        s.vp[at[3100], :, 1] = float("inf")
+        want, _, _ = s.reference()
+        ctx.reset_stats()
+        out = s.attn.forward(s.q, s.k, s.v, ctx)
+        ctx.sync()
+        assert launches(ctx, "span_tiles") == [1]
+        assert torch.equal(torch.isfinite(out), torch.isfinite(want))
+        for dims in (slice(4, None), slice(3, 4), slice(2, 3)):
+            x, y = out[..., dims].double(), want[..., dims]
+            rel = float((x - y).norm() / y.norm())
+            say(f"unlike sizes on span tiles {shape}, dims {dims}: rel_l2={rel:.3e}")
+            assert rel <= 1e-5
+    finally:
+        ctx.set_timing(False)
         ctx.clear()
         s.arena.close()
 
