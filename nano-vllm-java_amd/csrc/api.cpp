@@ -21,6 +21,7 @@
 #include <cstring>
 #include <map>
 #include <mutex>
+#include <queue>
 #include <string>
 #include <vector>
 
@@ -645,6 +646,37 @@ std::vector<Piece> cut_tiles(const std::vector<TileItem> &tiles, const std::vect
   return rows_b < rows_a && most_b <= std::max(kMergeRowsMaxParts, most_a) ? cut_b : cut_a;
 }
 
+// Every tile whole on a slot of its own, longest first, so that the workgroups take them as they come
+// free: no partials and no merge.  Empty (then the tiles are cut) unless that ends within 1.1 times
+// the equal shares' time (1.2 with three workgroups on a CU, which speed up when one of them ends), or
+// a tile is longer than a segment may be.  (48 spans of 9-512 keys by as many rows, 12 heads, d = 64,
+// 1.13 times: 86 us cut, 79 us whole; 29 spans of 17-138 keys, 40 q / 8 KV heads, d = 128, 1.15 times:
+// 40 and 46 us.)
+std::vector<Piece> whole_tiles(const std::vector<TileItem> &tiles, int slots, int64_t total,
+                               int64_t cap_tiles, int per_cu) {
+  std::vector<Piece> whole;
+  if ((int64_t)tiles.size() < slots) return whole;
+  std::vector<int> order(tiles.size());
+  for (size_t i = 0; i < order.size(); i++) order[i] = (int)i;
+  std::stable_sort(order.begin(), order.end(),
+                   [&](int x, int y) { return tiles[x].ke - tiles[x].ks > tiles[y].ke - tiles[y].ks; });
+  std::priority_queue<int64_t, std::vector<int64_t>, std::greater<int64_t>> free_at;
+  for (int i = 0; i < slots; i++) free_at.push(0);
+  int64_t end = 0;
+  for (int i : order) {
+    const int64_t n = (tiles[i].ke - tiles[i].ks + 31) / 32;
+    if (n > cap_tiles) return whole;
+    const int64_t t = free_at.top() + n;
+    free_at.pop();
+    free_at.push(t);
+    end = std::max(end, t);
+  }
+  if ((double)end * slots > (1.05 + 0.05 * per_cu) * (double)total) return whole;
+  for (size_t i = 0; i < order.size(); i++)
+    whole.push_back({order[i], (int)i, tiles[order[i]].ks, tiles[order[i]].ke});
+  return whole;
+}
+
 // The segments of a cut, grouped by slot and in tile order within each (counting sort); seg_off[s]
 // is slot s's first.  make(tile, pieces, piece, first piece) gives one segment.
 template <typename F>
@@ -1054,15 +1086,13 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
       const int64_t resident = beside ? std::max<int64_t>(grid_y, tile_cus)
                                       : (int64_t)ctx->num_cus * key.span_blocks_per_cu;
       span_slots = (int)std::max<int64_t>(1, std::min<int64_t>(total, resident / grid_y));
-      // Where 30 pieces of a tile nearly fill the CUs, no more: with those of its own keys a row then
-      // has few enough for the merge of 4 waves a head (33 of them took it 16 us, 18 of them 9).
-      const int few = 30 * (int)std::min<size_t>(span_tiles.size(), INT32_MAX / 64);
-      if (span_slots > few && span_slots <= few + few / 8) span_slots = few;
       std::vector<int> tile_rows(span_tiles.size());
       for (size_t i = 0; i < span_tiles.size(); i++)
         tile_rows[i] = (span_tiles[i].qlen - span_tiles[i].q0) / key.col_heads;
-      const std::vector<Piece> cut =
-          cut_tiles(span_tiles, tile_rows, span_slots, std::max<int64_t>(1, page_cap / 32));
+      const int64_t cap = std::max<int64_t>(1, page_cap / 32);
+      std::vector<Piece> cut = whole_tiles(span_tiles, span_slots, total, cap, beside ? 1 : key.span_blocks_per_cu);
+      if (cut.empty()) cut = cut_tiles(span_tiles, tile_rows, span_slots, cap);
+      else span_slots = (int)cut.size();
       span_tiles = segments_by_slot(cut, span_slots, &span_off, [&](int i, int np, int pi) {
         TileItem c = span_tiles[i];
         if (pi == 0)
@@ -1691,7 +1721,11 @@ nva_status run_attention(nva_ctx *ctx, const nva_attn_desc &d, const KvView &vie
     mg.part_l = pm + parts;
     mg.part_acc = pm + 2 * parts;
     Timed tm(ctx, "merge");
-    HIP_TRY(ctx, launch_merge(mg, plan->max_parts, ctx->stream), "merge kernel launch");
+    const bool spans = plan->num_spans > 0 || plan->num_span_tiles > 0;
+    HIP_TRY(ctx,
+            spans && d.head_dim <= 256 && plan->max_parts > 4 ? launch_merge_spans(mg, ctx->stream)
+                                         : launch_merge(mg, plan->max_parts, ctx->stream),
+            "merge kernel launch");
     tm.done();
   }
   span.done();

@@ -265,6 +265,8 @@ hipError_t launch_span_tiles(const TileLaunch &a, hipStream_t s);
 constexpr int kSpanCols = 32;
 bool span_kernel_supports(int head_dim, int paged, int block_size);
 hipError_t launch_spans(const SpanLaunch &a, int max_cols, hipStream_t s);
+// The merge of plans with spans, d = 64, 128 and 256.
+hipError_t launch_merge_spans(const MergeLaunch &a, hipStream_t s);
 
 // Most query heads one prefill workgroup carries at this head dim.
 int prefill_max_heads(int head_dim);

@@ -328,6 +328,81 @@ void launch_span(const SpanLaunch &a, hipStream_t s) {
 
 }  // namespace
 
+// Joins the partials of each row of a plan with spans: a workgroup per (row, head), whose groups of
+// D / 4 lanes take every G-th partial, four of them in flight, and meet in LDS in order, so the result
+// does not depend on timing.  (The decode merge gives a partial a wave of 64 lanes: of 97 partials at
+// d = 64 three quarters of 16 waves idle, in two rounds of workgroups: 10 us for 20 rows of 32 heads,
+// 5.0 here.  At d = 512, where four groups are left, it is the faster one, 33 against 35 us a decode
+// call, as for at most four partials, where it takes all heads of a row at once.)  Rows without
+// partials are zero.
+template <int D>
+__global__ void __launch_bounds__(256) merge_spans_kernel(MergeLaunch a) {
+  constexpr int D4 = D / 4, G = 256 / D4;
+  __shared__ float sm[G], sl[G];
+  __shared__ float4 sacc[G][D4];
+  const MergeItem it = a.items[blockIdx.x];
+  const int h = blockIdx.y;
+  const int g = threadIdx.x / D4, c = threadIdx.x % D4;
+  float4 *out = reinterpret_cast<float4 *>(a.out + ((size_t)it.qrow * a.hq + h) * D);
+  float M = -INFINITY, L = 0.0f;
+  float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p0 = g; p0 < it.nparts; p0 += 4 * G) {
+    float pm[4], pl[4];
+    float4 x[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const int p = p0 + G * u;
+      const bool ok = p < it.nparts;
+      const size_t pi = (size_t)(it.first + (ok ? p : p0)) * a.hq + h;
+      pm[u] = ok ? a.part_m[pi] : -INFINITY;
+      pl[u] = ok ? a.part_l[pi] : 0.0f;
+      x[u] = ok ? ld4(a.part_acc + pi * D + 4 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    const float Mn = fmaxf(fmaxf(M, fmaxf(pm[0], pm[1])), fmaxf(pm[2], pm[3]));
+    const float Ms = Mn == -INFINITY ? 0.0f : Mn;
+    const float alpha = __builtin_amdgcn_exp2f(M - Ms);  // 0 while M is -inf
+    L *= alpha;
+    A = make_float4(A.x * alpha, A.y * alpha, A.z * alpha, A.w * alpha);
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const float e = __builtin_amdgcn_exp2f(pm[u] - Ms);
+      L = fmaf(pl[u], e, L);
+      A.x = fmaf(x[u].x, e, A.x);
+      A.y = fmaf(x[u].y, e, A.y);
+      A.z = fmaf(x[u].z, e, A.z);
+      A.w = fmaf(x[u].w, e, A.w);
+    }
+    M = Mn;
+  }
+  if (c == 0) {
+    sm[g] = M;
+    sl[g] = L;
+  }
+  sacc[g][c] = A;
+  __syncthreads();
+  float T = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < G; w++) T = fmaxf(T, sm[w]);
+  const float Ts = T == -INFINITY ? 0.0f : T;
+  float LT = 0.0f;
+#pragma unroll
+  for (int w = 0; w < G; w++) LT = fmaf(sl[w], __builtin_amdgcn_exp2f(sm[w] - Ts), LT);
+  const float inv = LT == 0.0f ? 0.0f : 1.0f / LT;
+  for (int cc = threadIdx.x; cc < D4; cc += blockDim.x) {
+    float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < G; w++) {
+      const float e = __builtin_amdgcn_exp2f(sm[w] - Ts);
+      const float4 x = sacc[w][cc];
+      r.x = fmaf(x.x, e, r.x);
+      r.y = fmaf(x.y, e, r.y);
+      r.z = fmaf(x.z, e, r.z);
+      r.w = fmaf(x.w, e, r.w);
+    }
+    out[cc] = make_float4(r.x * inv, r.y * inv, r.z * inv, r.w * inv);
+  }
+}
+
 bool span_kernel_supports(int head_dim, int paged, int block_size) {
   return (head_dim == 64 || head_dim == 128 || head_dim == 256 || head_dim == 512) &&
          (!paged || (block_size >= 16 && (block_size & (block_size - 1)) == 0));
@@ -344,6 +419,18 @@ hipError_t launch_spans(const SpanLaunch &a, int max_cols, hipStream_t s) {
     case 256 * 2 + 1: launch_span<256, 2>(a, s); break;
     case 512 * 2: launch_span<512, 1>(a, s); break;
     case 512 * 2 + 1: launch_span<512, 2>(a, s); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_merge_spans(const MergeLaunch &a, hipStream_t s) {
+  if (a.num_items <= 0) return hipSuccess;
+  const dim3 grid(a.num_items, a.hq);
+  switch (a.head_dim) {
+    case 64: hipLaunchKernelGGL(merge_spans_kernel<64>, grid, dim3(256), 0, s, a); break;
+    case 128: hipLaunchKernelGGL(merge_spans_kernel<128>, grid, dim3(256), 0, s, a); break;
+    case 256: hipLaunchKernelGGL(merge_spans_kernel<256>, grid, dim3(256), 0, s, a); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
