@@ -169,13 +169,13 @@ struct PlanKey {
   int head_dim, num_heads, num_kv_heads;  // size the work of a mixed plan's two kernels
   int cross = 0;               // over the encoder's rows instead of the sequence's own keys
   int64_t kv_rows = 0;         // cross: rows of the encoder pool
-  int col_heads = 0;           // spans: query heads of a column group
-  int span_cols = 0;           // most columns of a span item (0: the span kernel does not serve)
-  int span_tile_cols = 0;      // columns of a span tile (0: no tile kernel for this head dim)
+  int item_heads = 0;          // query heads of a column group of a span item (0: no span kernel)
+  int tile_heads = 0;          // and of a span tile (0: no tile kernel for this head dim)
+  int span_tile_cols = 0;      // columns of a span tile
   int span_blocks_per_cu = 0;
   bool operator==(const PlanKey &o) const {
-    return cross == o.cross && kv_rows == o.kv_rows && col_heads == o.col_heads &&
-           span_cols == o.span_cols && span_tile_cols == o.span_tile_cols &&
+    return cross == o.cross && kv_rows == o.kv_rows && item_heads == o.item_heads &&
+           tile_heads == o.tile_heads && span_tile_cols == o.span_tile_cols &&
            span_blocks_per_cu == o.span_blocks_per_cu && window == o.window && mfma == o.mfma && fp32_tiles == o.fp32_tiles && tile_q == o.tile_q &&
            head_dim == o.head_dim && num_heads == o.num_heads && num_kv_heads == o.num_kv_heads &&
            wg_per_item == o.wg_per_item && blocks_per_cu == o.blocks_per_cu &&
@@ -731,11 +731,12 @@ int key_chunk(int n, F len, int64_t workgroups, int64_t many, int64_t few) {
 // estimated time is least, in keys: what the resident workgroups (two on a CU) have to do each, but
 // at least one chunk, and half a chunk for the last round.  A workgroup's start and end (Q, the first
 // loads, the waves' meeting, partials) take as long as kFixed keys.
-int span_chunk(const std::vector<SpanItem> &items, int workgroups, int num_cus) {
+int span_chunk(const std::vector<SpanItem> &items, int workgroups, int num_cus, double *keys_time) {
   constexpr double kFixed = 250;
   const double resident = 2.0 * num_cus;
   int best = 64;
-  double best_time = 1e300;
+  double &best_time = *keys_time;
+  best_time = 1e300;
   for (int c = 64; c <= 4096; c += 64) {
     double keys = 0.0, pieces = 0.0;
     for (const SpanItem &it : items) {
@@ -760,7 +761,7 @@ struct Span {
 };
 
 // Estimated time of a span on each kernel, in us on all CUs: span items at 75 TFLOP/s over columns
-// padded to the items', span tiles at tile_rate() over whole tiles, of which idle columns cost 70%.
+// padded to the items', span tiles at tile_rate() over whole tiles, of which idle columns cost 55%.
 // A launch of items takes kItemsUs, of tiles kTilesUs more.  (1e300: the kernel does not serve.)
 struct SpanCost {
   double items, tiles;
@@ -771,17 +772,16 @@ double tile_rate(int head_dim) {  // flops per us
 }
 SpanCost span_cost(const PlanKey &key, int rows, int len) {
   SpanCost c{1e300, 1e300};
-  const int64_t cols = (int64_t)rows * key.col_heads;
-  const double flops = 4.0 * key.head_dim * (key.num_heads / key.col_heads) * len;  // a column
-  if (key.span_cols > 0) {
-    const int per = key.span_cols / key.col_heads * key.col_heads;
-    c.items = flops * (double)((cols + per - 1) / per) * key.span_cols / 75e6;
-  }
-  if (key.span_tile_cols > 0) {
-    const int per = key.span_tile_cols / key.col_heads * key.col_heads;
-    c.tiles = flops * (0.7 * key.span_tile_cols * ((cols + per - 1) / per) + 0.3 * cols) /
-              tile_rate(key.head_dim);
-  }
+  auto padded = [&](int heads, int cols_of, double idle) {  // columns of all heads, idle ones counted
+    const int64_t cols = (int64_t)rows * heads;
+    const int per = cols_of / heads * heads;
+    return (double)(key.num_heads / heads) *
+           (idle * cols_of * ((cols + per - 1) / per) + (1.0 - idle) * cols);
+  };
+  const double flops = 4.0 * key.head_dim * len;  // a column
+  if (key.item_heads > 0) c.items = flops * padded(key.item_heads, kSpanCols, 1.0) / 75e6;
+  if (key.tile_heads > 0)
+    c.tiles = flops * padded(key.tile_heads, key.span_tile_cols, 0.55) / tile_rate(key.head_dim);
   return c;
 }
 
@@ -858,7 +858,7 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
   };
   // Shared prefixes: the rows of a group's sequences see its first keys as one span, and each
   // sequence's own lists start behind them.  A sliding window sees too little of them.
-  const bool spans_run = key.span_cols > 0 || key.span_tile_cols > 0;  // else row by row
+  const bool spans_run = key.item_heads > 0 || key.tile_heads > 0;  // else row by row
   std::vector<int32_t> prefix_len(ctx->num_seqs, 0);
   if (!key.cross && paged && W == 0 && spans_run) {
     // Sharing has to pay.  Read separately, a prefix costs its rows' share of HBM or whole query
@@ -879,7 +879,7 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
         if (key.mfma && q >= 2) {
           const int tiles_of = (q + key.tile_q - 1) / key.tile_q;
           apart += 4.0 * key.head_dim * key.num_heads * gr.num_tokens *
-                   (0.7 * key.tile_q * tiles_of + 0.3 * q) / tile_rate(key.head_dim);
+                   (0.55 * key.tile_q * tiles_of + 0.45 * q) / tile_rate(key.head_dim);
         } else {
           apart += (double)q * gr.num_tokens * key.num_kv_heads * key.head_dim * 8.0 / 6.5e6;
         }
@@ -1040,7 +1040,6 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
   if (!spans.empty()) {
     row_part.assign(key.tokens, 0);
     span_parts.assign(key.tokens, 0);
-    const int groups = key.num_heads / key.num_kv_heads / key.col_heads;
     // Row r has `pieces` partials from its span (none if it is written at once).
     auto split_row = [&](int r, int pieces) {
       if (key.cross && pieces == 1) return;
@@ -1053,42 +1052,62 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
     double tile_pairs = 0.0;
     double span_us = 0.0;
     const std::vector<char> on_tiles = choose_tiles(key, spans, &span_us);
+    std::vector<Span> on_items;
     for (size_t i = 0; i < spans.size(); i++) {
       const Span &sp = spans[i];
       if (on_tiles[i]) {
-        const int cols = sp.rows * key.col_heads;
-        const int per_tile = key.span_tile_cols / key.col_heads * key.col_heads;  // whole rows
+        const int cols = sp.rows * key.tile_heads;
+        const int per_tile = key.span_tile_cols / key.tile_heads * key.tile_heads;  // whole rows
         for (int c = 0; c < cols; c += per_tile)
           span_tiles.push_back({sp.seq, sp.row0, std::min(cols, c + per_tile), c, 0, sp.kbase, 0,
                                 sp.len, -1, 1, 0, 0});
         tile_pairs += (double)sp.rows * sp.len;
       } else {
-        const int per_item = key.span_cols / key.col_heads;  // rows
-        for (int r = 0; r < sp.rows; r += per_item) {
-          const int n = std::min(per_item, sp.rows - r);
-          span_items.push_back({sp.row0 + r, n * key.col_heads, sp.seq, sp.kbase, 0, sp.len, 0, 0, 0, 0});
-        }
+        on_items.push_back(sp);
       }
     }
     // Beside span items, and with no span tiles, the rows of the step are items too: one launch.
-    const size_t own_items = span_items.size();
-    const bool rows_join = !span_items.empty() && span_tiles.empty() && !key.cross;
-    if (rows_join) {
-      for (const Row &r : rows)
-        span_items.push_back({r.qrow, key.col_heads, r.seq, r.kbase, r.kbeg, r.kend, 0, 0, 0, 0});
-      rows.clear();
+    const bool rows_join = !on_items.empty() && span_tiles.empty() && !key.cross;
+    // Items of 16 columns, or of 32 (which read the keys of wide spans half as often, but run two
+    // workgroups on a CU where those of 16 run three, and 1.4 times as long a key, 1.6 at d = 64).  32 q /
+    // 8 KV heads, d = 128, 210 queries by as many keys: 28 us on 16, 20 on 32; 20 rows of 40 q / 8 KV
+    // heads under 256 tokens: 15.6 and 18 us.
+    int chunk = 0;
+    size_t own_items = 0;
+    double best_time = 1e300;
+    for (int cols = kSpanCols; cols <= (key.head_dim <= 128 ? 2 : 1) * kSpanCols && !on_items.empty();
+         cols *= 2) {
+      const int per_item = cols / key.item_heads;  // rows
+      std::vector<SpanItem> list;
+      for (const Span &sp : on_items)
+        for (int r = 0; r < sp.rows; r += per_item)
+          list.push_back({sp.row0 + r, std::min(per_item, sp.rows - r) * key.item_heads, sp.seq,
+                          sp.kbase, 0, sp.len, 0, 0, 0, 0});
+      const size_t of_spans = list.size();
+      if (rows_join)
+        for (const Row &r : rows)
+          list.push_back({r.qrow, key.item_heads, r.seq, r.kbase, r.kbeg, r.kend, 0, 0, 0, 0});
+      double time = 0.0;
+      const int c = span_chunk(list, key.num_heads / key.item_heads, ctx->num_cus, &time);
+      if (cols > kSpanCols) time *= key.head_dim == 64 ? 1.6 : 1.4;
+      if (time >= best_time) continue;
+      best_time = time;
+      chunk = c;
+      own_items = of_spans;
+      span_items.swap(list);
     }
+    if (rows_join) rows.clear();
     beside = plan_beside(tile_pairs);
     if (!span_tiles.empty()) {
       int64_t total = 0;
       for (const TileItem &t : span_tiles) total += (t.ke + 31) / 32;
-      const int grid_y = key.num_kv_heads * groups;
+      const int grid_y = key.num_heads / key.tile_heads;
       const int64_t resident = beside ? std::max<int64_t>(grid_y, tile_cus)
                                       : (int64_t)ctx->num_cus * key.span_blocks_per_cu;
       span_slots = (int)std::max<int64_t>(1, std::min<int64_t>(total, resident / grid_y));
       std::vector<int> tile_rows(span_tiles.size());
       for (size_t i = 0; i < span_tiles.size(); i++)
-        tile_rows[i] = (span_tiles[i].qlen - span_tiles[i].q0) / key.col_heads;
+        tile_rows[i] = (span_tiles[i].qlen - span_tiles[i].q0) / key.tile_heads;
       const int64_t cap = std::max<int64_t>(1, page_cap / 32);
       std::vector<Piece> cut = whole_tiles(span_tiles, span_slots, total, cap, beside ? 1 : key.span_blocks_per_cu);
       if (cut.empty()) cut = cut_tiles(span_tiles, tile_rows, span_slots, cap);
@@ -1097,7 +1116,7 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
         TileItem c = span_tiles[i];
         if (pi == 0)
           for (int r = 0; r < tile_rows[i]; r++)
-            split_row(c.qstart + c.q0 / key.col_heads + r, np);
+            split_row(c.qstart + c.q0 / key.tile_heads + r, np);
         c.part = key.cross && np == 1 ? -1 : 0;
         c.nsplit = np;
         c.split = pi;
@@ -1105,7 +1124,6 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
       });
     }
     if (!span_items.empty()) {
-      int chunk = span_chunk(span_items, key.num_kv_heads * groups, ctx->num_cus);
       if (paged) chunk = std::min(chunk, (kRowTablePages - 1) * key.block_size);
       std::vector<SpanItem> cut;
       for (size_t i = 0; i < span_items.size(); i++) {
@@ -1113,7 +1131,7 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
         const int len = it.kend - it.kbeg, n = (len + chunk - 1) / chunk;
         int first = 0;  // of the pieces' partials, behind row_part
         if (i < own_items) {
-          for (int r = 0; r < it.cols / key.col_heads; r++) split_row(it.row0 + r, n);
+          for (int r = 0; r < it.cols / key.item_heads; r++) split_row(it.row0 + r, n);
           if (key.cross && n == 1) first = -1;
         } else {  // a row's own keys
           const int prefix = span_parts[it.row0];
@@ -1484,12 +1502,15 @@ nva_status attention_plan(nva_ctx *ctx, const nva_attn_desc &d, int paged, int b
     key.kv_rows = cross ? cross->kv_rows : 0;
     const bool tiles = prefill_kernel_supports(d.head_dim, 1);
     const bool items = span_kernel_supports(d.head_dim, paged, block_size);
+    // A column group holds whole rows of an item, or a tile.
+    auto group = [&](int cols) {
+      int h = std::min(rep, cols);
+      while (rep % h) h--;
+      return h;
+    };
     key.span_tile_cols = tiles ? span_tile_cols(d.head_dim) : 0;
-    key.span_cols = items ? kSpanCols : 0;
-    // A column group holds whole rows of a tile and of an item.
-    const int most = std::min(tiles ? key.span_tile_cols : rep, items ? key.span_cols : rep);
-    key.col_heads = std::min(rep, most);
-    while (rep % key.col_heads) key.col_heads--;
+    key.tile_heads = tiles ? group(key.span_tile_cols) : 0;
+    key.item_heads = items ? group(kSpanCols) : 0;
     key.span_blocks_per_cu = tiles ? ctx_span_blocks_per_cu(ctx, d.head_dim) : 0;
   }
   return get_plan(ctx, key, plan);
@@ -1639,7 +1660,7 @@ nva_status run_attention(nva_ctx *ctx, const nva_attn_desc &d, const KvView &vie
     t.num_items = plan->num_span_tiles;
     t.num_slots = plan->num_span_slots;
     t.window = 0;
-    t.col_heads = plan->key.col_heads;
+    t.col_heads = plan->key.tile_heads;
     t.row_part = row_part;
     Timed tm(ctx, "span_tiles");
     HIP_TRY(ctx, launch_span_tiles(t, ctx->stream), "span tile kernel launch");
@@ -1673,7 +1694,7 @@ nva_status run_attention(nva_ctx *ctx, const nva_attn_desc &d, const KvView &vie
     sp.hq = d.num_heads;
     sp.hkv = d.num_kv_heads;
     sp.head_dim = d.head_dim;
-    sp.col_heads = plan->key.col_heads;
+    sp.col_heads = plan->key.item_heads;
     sp.scale = d.scale;
     sp.row_part = row_part;
     sp.part_m = pm;

@@ -121,7 +121,7 @@ struct TileLaunch {
 // partial (part >= 0) of row r is row_part[r] + split.  Spans of few columns are SpanItems.
 struct SpanItem {
   int32_t row0;   // first query row
-  int32_t cols;   // columns, at most kSpanCols
+  int32_t cols;   // columns, at most 2 kSpanCols (kSpanCols from d = 256 on)
   int32_t seq;    // block-table row (paged K/V)
   int32_t kbase;  // dense K/V: row of key 0; paged: unused
   int32_t kbeg;   // first key
@@ -260,9 +260,9 @@ int span_tile_cols(int head_dim);
 int span_tile_blocks_per_cu(int head_dim);
 hipError_t launch_span_tiles(const TileLaunch &a, hipStream_t s);
 
-// The span kernel of few columns (span.hip): most columns of an item, and the shapes it is built
-// for (paged: pages of a power of two of at least 16 tokens).
-constexpr int kSpanCols = 32;
+// The span kernel of few columns (span.hip): columns of an item, and the shapes it is built for
+// (paged: pages of a power of two of at least 16 tokens).
+constexpr int kSpanCols = 16;
 bool span_kernel_supports(int head_dim, int paged, int block_size);
 hipError_t launch_spans(const SpanLaunch &a, int max_cols, hipStream_t s);
 // The merge of plans with spans, d = 64, 128 and 256.

@@ -410,15 +410,13 @@ bool span_kernel_supports(int head_dim, int paged, int block_size) {
 
 hipError_t launch_spans(const SpanLaunch &a, int max_cols, hipStream_t s) {
   if (a.num_items <= 0) return hipSuccess;
-  switch (a.head_dim * 2 + (max_cols > 16)) {
+  switch (a.head_dim * 2 + (max_cols > kSpanCols)) {
     case 64 * 2: launch_span<64, 1>(a, s); break;
     case 64 * 2 + 1: launch_span<64, 2>(a, s); break;
     case 128 * 2: launch_span<128, 1>(a, s); break;
     case 128 * 2 + 1: launch_span<128, 2>(a, s); break;
     case 256 * 2: launch_span<256, 1>(a, s); break;
-    case 256 * 2 + 1: launch_span<256, 2>(a, s); break;
     case 512 * 2: launch_span<512, 1>(a, s); break;
-    case 512 * 2 + 1: launch_span<512, 2>(a, s); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
