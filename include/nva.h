@@ -251,7 +251,9 @@ nva_status nva_find_shared_prefixes(const int32_t *block_tables, int num_seqs, i
  * attention call over the step's pages reads the tokens of a group once for all rows of its
  * sequences and joins the result with each sequence's own keys; outputs agree with those of the
  * separate reads to fp32 rounding.  (Layers with a sliding window, which see too little of a prefix,
- * are computed as before, as is a group of one row.)  Groups are in order and do not overlap; a
+ * are computed as before, and so are groups that would not gain: one row, or prefill chunks that fill
+ * their query tiles.  Joining takes more partials, which the no-allocation entry point's array has to
+ * hold.)  Groups are in order and do not overlap; a
  * group's tokens are cached ones of each of its sequences, which hold them in the same pages: tables
  * that differ there fail the attention call with NVA_E_ARG, before anything is written.  num_groups
  * 0 ends the sharing. */
@@ -317,7 +319,9 @@ nva_status nva_attention_forward_noalloc(nva_ctx *ctx, nva_kv *kv, const nva_att
  * Rows come from nva_step_set_encoder.  Sequences in a row that read the same ones (beams) read them
  * once.  sliding_window must be 0; kv_layer_index and write_kv are not used.  d = 64, 128, 256 and
  * 512 run on matrix units, other head dims row by row.  Not under stream capture: the second form,
- * with the rules and the scratch array of nva_attention_forward_noalloc, is for that. */
+ * with the rules and the scratch array of nva_attention_forward_noalloc, is for that (its plan lies
+ * at the array's end, so that a decoder layer's calls of both kinds fit one graph; replays need the
+ * plans they were captured with, so no call of another step or configuration may come between). */
 nva_status nva_cross_attention_forward(nva_ctx *ctx, const nva_attn_desc *desc, const float *q,
                                        const float *k, const float *v, int64_t kv_rows,
                                        int64_t kv_stride, int num_tokens, float *out);

@@ -21,6 +21,7 @@
 #include <cstring>
 #include <map>
 #include <mutex>
+#include <new>
 #include <queue>
 #include <string>
 #include <vector>
@@ -45,7 +46,9 @@ static __device__ __align__(256) unsigned char scratch[kScratchBytes];
 
 namespace {
 
-// The scratch plan held by one device's array, so a call can skip copying the same plan again.
+// A scratch plan held by one device's array, so a call can skip copying the same plan again: a
+// sequence attention call's at its front, a cross attention call's at its end, so that the two of a
+// decoder layer need not displace each other.
 struct ScratchTag {
   uint64_t plan_id = 0;  // 0: no plan known to be held
   size_t offset = 0, bytes = 0;
@@ -57,7 +60,7 @@ struct ScratchSlot {
   bool looked_up = false;
   hipError_t err = hipSuccess;
   char *ptr = nullptr;
-  ScratchTag tag;
+  ScratchTag tags[2];
 };
 std::mutex g_scratch_mu;
 ScratchSlot g_scratch[kScratchDevices];
@@ -80,7 +83,7 @@ char *scratch_address(int device, hipError_t *err) {
   return slot.ptr;
 }
 
-ScratchTag &scratch_tag(int device) { return g_scratch[device].tag; }
+ScratchTag &scratch_tag(int device, bool cross) { return g_scratch[device].tags[cross ? 1 : 0]; }
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
@@ -1524,27 +1527,36 @@ nva_status attention_plan(nva_ctx *ctx, const nva_attn_desc &d, int paged, int b
   return get_plan(ctx, key, plan);
 }
 
-// Regions of the no-allocation array one call uses: [gather rows | plan lists | partials],
-// each 256-byte aligned.
+// Regions of the no-allocation array one call uses, each 256-byte aligned: [gather rows | plan lists |
+// partials] from the front, or, for cross attention, [partials | plan lists] up to the end.
 struct ScratchLayout {
-  size_t plan_off = 0, part_off = 0, part_bytes = 0, end = 0;
+  size_t plan_off = 0, part_off = 0, part_bytes = 0;
+  size_t bytes = 0;  // in all; the offsets hold only if the array has them
 };
 
 ScratchLayout scratch_layout(size_t gather_bytes, const Plan &plan, const nva_attn_desc &d) {
   ScratchLayout l;
-  const size_t parts = (size_t)plan.num_parts * d.num_heads;
-  l.plan_off = align256(gather_bytes);
-  l.part_off = align256(l.plan_off + plan.host.size());
+  const size_t parts = (size_t)plan.num_parts * d.num_heads, plan_bytes = align256(plan.host.size());
   l.part_bytes = parts * (2 + (size_t)d.head_dim) * sizeof(float);
-  l.end = l.part_off + l.part_bytes;
+  l.bytes = align256(gather_bytes) + plan_bytes + l.part_bytes;
+  if (plan.key.cross) {
+    l.bytes = plan_bytes + align256(l.part_bytes);
+    l.plan_off = kScratchBytes - plan_bytes;
+    l.part_off = l.plan_off - align256(l.part_bytes);
+  } else {
+    l.plan_off = align256(gather_bytes);
+    l.part_off = l.plan_off + plan_bytes;
+  }
   return l;
 }
 
-// A kernel is about to write [begin, end) of this device's array: the plan recorded as held
-// there no longer is, if the ranges meet.
+// A call is about to write [begin, end) of this device's array: a plan recorded as held there no
+// longer is, if the ranges meet.
 void scratch_overwritten(int device, size_t begin, size_t end) {
-  ScratchTag &tag = scratch_tag(device);
-  if (tag.plan_id != 0 && begin < tag.offset + tag.bytes && tag.offset < end) tag = ScratchTag{};
+  for (bool cross : {false, true}) {
+    ScratchTag &tag = scratch_tag(device, cross);
+    if (tag.plan_id != 0 && begin < tag.offset + tag.bytes && tag.offset < end) tag = ScratchTag{};
+  }
 }
 
 bool stream_capturing(hipStream_t s) {
@@ -1555,12 +1567,12 @@ bool stream_capturing(hipStream_t s) {
 // Whether a plan's call fits the array and, under stream capture, finds its plan there.
 nva_status noalloc_fits(nva_ctx *ctx, const Plan &plan, const nva_attn_desc &d, size_t gather) {
   const ScratchLayout l = scratch_layout(gather, plan, d);
-  if (l.end > kScratchBytes)
+  if (l.bytes > kScratchBytes)
     return fail(ctx, NVA_E_ARG,
                 "this call needs %zu bytes of device scratch (plan %zu, partials %zu, gather "
                 "%zu); the no-allocation entry point has %zu",
-                l.end, plan.host.size(), l.part_bytes, gather, kScratchBytes);
-  const ScratchTag &tag = scratch_tag(ctx->device);
+                l.bytes, plan.host.size(), l.part_bytes, gather, kScratchBytes);
+  const ScratchTag &tag = scratch_tag(ctx->device, plan.key.cross);
   if (!plan.host.empty() && (tag.plan_id != plan.id || tag.offset != l.plan_off) &&
       stream_capturing(ctx->stream))
     return fail(ctx, NVA_E_ARG,
@@ -1623,8 +1635,9 @@ nva_status run_attention(nva_ctx *ctx, const nva_attn_desc &d, const KvView &vie
     pbase = scr->base + l.plan_off;
     pm = reinterpret_cast<float *>(scr->base + l.part_off);
     // Skip the copy when this device's array already holds this very plan at this offset.
-    ScratchTag &tag = scratch_tag(ctx->device);
+    ScratchTag &tag = scratch_tag(ctx->device, plan->key.cross);
     if (!plan->host.empty() && (tag.plan_id != plan->id || tag.offset != l.plan_off)) {
+      scratch_overwritten(ctx->device, l.plan_off, l.plan_off + plan->host.size());
       tag = ScratchTag{};
       HIP_TRY(ctx, hipMemcpyAsync(pbase, plan->host.data(), plan->host.size(),
                                   hipMemcpyHostToDevice, ctx->stream),
@@ -1633,7 +1646,7 @@ nva_status run_attention(nva_ctx *ctx, const nva_attn_desc &d, const KvView &vie
       tag.offset = l.plan_off;
       tag.bytes = plan->host.size();
     }
-    if (l.part_bytes > 0) scratch_overwritten(ctx->device, l.part_off, l.end);
+    if (l.part_bytes > 0) scratch_overwritten(ctx->device, l.part_off, l.part_off + l.part_bytes);
   }
 
   // "attention" times the whole part below, kernels that overlap counted once.
@@ -1921,6 +1934,12 @@ int32_t java_round(float x) {
 }
 
 }  // namespace
+
+// Host memory ran out in an entry point (no exception may leave it).
+static nva_status no_memory(nva_ctx *ctx) {
+  ctx->err = "out of memory";  // short: needs no allocation
+  return NVA_E_OOM;
+}
 
 // Records msg as the context's last error (the step producers in step.cpp report through it).
 __attribute__((visibility("hidden"))) nva_status nva_internal_fail(nva_ctx *ctx, nva_status st,
@@ -2381,7 +2400,7 @@ nva_status nva_step_clear(nva_ctx *ctx) {
   return NVA_OK;
 }
 
-nva_status nva_step_share_prefixes(nva_ctx *ctx, const nva_prefix_group *groups, int num_groups) {
+nva_status nva_step_share_prefixes(nva_ctx *ctx, const nva_prefix_group *groups, int num_groups) try {
   if (!ctx) return NVA_E_ARG;
   if (!ctx->has_step) return fail(ctx, NVA_E_NO_STEP, "no step metadata set on the context");
   if (num_groups < 0 || (num_groups > 0 && !groups))
@@ -2415,10 +2434,12 @@ nva_status nva_step_share_prefixes(nva_ctx *ctx, const nva_prefix_group *groups,
   for (Plan *p : ctx->plans) p->valid = false;
   ctx->tile_choices.clear();
   return NVA_OK;
+} catch (const std::bad_alloc &) {
+  return no_memory(ctx);
 }
 
 nva_status nva_step_set_encoder(nva_ctx *ctx, const int32_t *kv_start, const int32_t *kv_len,
-                                int num_seqs) {
+                                int num_seqs) try {
   if (!ctx) return NVA_E_ARG;
   if (!ctx->has_step) return fail(ctx, NVA_E_NO_STEP, "no step metadata set on the context");
   if (num_seqs != ctx->num_seqs)
@@ -2435,6 +2456,8 @@ nva_status nva_step_set_encoder(nva_ctx *ctx, const int32_t *kv_start, const int
   for (Plan *p : ctx->plans)
     if (p->key.cross) p->valid = false;
   return NVA_OK;
+} catch (const std::bad_alloc &) {
+  return no_memory(ctx);
 }
 
 // ------------------------------------------------------------------------------- compute
@@ -2541,7 +2564,7 @@ nva_status nva_attention_forward_noalloc(nva_ctx *ctx, nva_kv *kv, const nva_att
 static nva_status cross_attention_forward(nva_ctx *ctx, const nva_attn_desc *desc, const float *q,
                                           const float *k, const float *v, int64_t kv_rows,
                                           int64_t kv_stride, int num_tokens, float *out,
-                                          Scratch *scr) {
+                                          Scratch *scr) try {
   nva_status st = check_desc(ctx, desc);
   if (st != NVA_OK) return st;
   const nva_attn_desc d = *desc;
@@ -2579,6 +2602,8 @@ static nva_status cross_attention_forward(nva_ctx *ctx, const nva_attn_desc *des
   }
   return run_attention(ctx, d, make_dense_view(k, v, (int)std::max<int64_t>(kv_stride, width)), 0, q,
                        num_tokens, out, scr, &rows);
+} catch (const std::bad_alloc &) {
+  return no_memory(ctx);
 }
 
 nva_status nva_cross_attention_forward(nva_ctx *ctx, const nva_attn_desc *desc, const float *q,

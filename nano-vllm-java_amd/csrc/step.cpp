@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <cstdio>
+#include <new>
 #include <vector>
 
 #include "../../include/nva.h"
@@ -156,10 +157,11 @@ extern "C" {
 
 // Which runs of adjacent sequences to read as one: the cut of the step into runs that saves the most
 // page reads, sum over runs of (sequences - 1) * common full pages.  best[j] is the saving of the
-// first j sequences, run[j] where the last run of that cut starts.
+// first j sequences, run[j] where the last run of that cut starts.  Runs are of at most 1024 sequences,
+// which bounds the search (a longer one would save less than a thousandth more).
 nva_status nva_find_shared_prefixes(const int32_t *block_tables, int num_seqs, int bt_stride,
                                     const int32_t *cached_tokens, int block_size,
-                                    nva_prefix_group *groups, int *num_groups) {
+                                    nva_prefix_group *groups, int *num_groups) try {
   if (!num_groups) return NVA_E_ARG;
   *num_groups = 0;
   if (num_seqs < 0 || bt_stride < 0 || block_size <= 0) return NVA_E_ARG;
@@ -184,7 +186,7 @@ nva_status nva_find_shared_prefixes(const int32_t *block_tables, int num_seqs, i
     best[j] = best[j - 1];
     run[j] = j - 1;
     int common = INT32_MAX;
-    for (int i = j - 2; i >= 0; i--) {  // the run [i, j)
+    for (int i = j - 2; i >= std::max(0, j - 1024); i--) {  // the run [i, j)
       common = std::min(common, same[i]);
       if (common == 0) break;
       const int64_t saved = best[i] + (int64_t)(j - i - 1) * common;
@@ -200,6 +202,9 @@ nva_status nva_find_shared_prefixes(const int32_t *block_tables, int num_seqs, i
       groups[(*num_groups)++] = {run[j], j - run[j], pages[j] * block_size};
   std::reverse(groups, groups + *num_groups);
   return NVA_OK;
+} catch (const std::bad_alloc &) {
+  *num_groups = 0;
+  return NVA_E_OOM;
 }
 
 nva_status nva_build_prefill_metadata(const nva_seq *seqs, int num_seqs, int block_size,

@@ -632,7 +632,7 @@ class CrossAttention:
         self.num_kv_heads = num_kv_heads
         self._desc = N.AttnDesc(num_heads, head_dim, self.scale, num_kv_heads, 0, 0, 0)
 
-    def _pool(self, k, v):
+    def _pool(self, k, v, device):
         """Pointers, rows and row stride of the encoder's keys and values."""
         row = (self.num_kv_heads, self.head_dim)
         rows, stride = k.shape[0] if k.dim() else 0, k.stride(0) if k.dim() else 0
@@ -640,10 +640,10 @@ class CrossAttention:
             if t.dim() != 3 or t.shape[1:] != row:
                 raise IllegalArgumentException(
                     f"{name} must be [rows, {row[0]}, {row[1]}], got {tuple(t.shape)}")
-            if not (t.is_cuda and t.dtype is torch.float32 and
+            if not (t.is_cuda and t.get_device() == device and t.dtype is torch.float32 and
                     (rows == 0 or t.stride()[1:] == (self.head_dim, 1))):
                 raise IllegalArgumentException(
-                    f"{name} must be a float32 device tensor with contiguous rows")
+                    f"{name} must be a float32 tensor with contiguous rows on the context's device")
         if v.shape[0] != rows or (rows > 1 and v.stride(0) != stride):
             raise IllegalArgumentException("k and v must have the same rows and row stride")
         return k.data_ptr(), v.data_ptr(), rows, stride if rows > 1 else row[0] * row[1]
@@ -656,8 +656,10 @@ class CrossAttention:
         if q.dim() != 3 or q.shape[1:] != (self.num_heads, self.head_dim):
             raise IllegalArgumentException(
                 f"q must be [tokens, {self.num_heads}, {self.head_dim}], got {tuple(q.shape)}")
-        kp, vp, rows, stride = self._pool(k, v)
+        kp, vp, rows, stride = self._pool(k, v, ctx.device)
         qp = _dev(q, "q")
+        if q.get_device() != ctx.device:
+            raise IllegalArgumentException("q must be on the context's device")
         out = torch.empty_like(q)
         _check(ctx.handle, N.load().nva_cross_attention_forward(
             ctx.handle, ctypes.byref(self._desc), qp, kp, vp, rows, stride, q.shape[0],

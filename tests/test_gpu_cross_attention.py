@@ -259,6 +259,58 @@ def test_no_alloc_graph_replays(queries, lens, beams):
         ctx.clear()
 
 
+def test_decoder_layer_in_one_graph():
+    """Self attention over pages that share a prefix and cross attention on its output, captured as
+    one graph: both plans stay in the device's scratch array, and replays give the eager bits."""
+    from nanollvm_amd import Attention, KvCacheArena
+    from span_checks import SharedStep
+    lib = N.load()
+    s1 = torch.cuda.Stream()
+    with torch.cuda.stream(s1), Context(0, stream=s1) as ctx:
+        st = SharedStep([(40, 1024)], [(i, 1) for i in range(40)], 64, seed=15)
+        arena = KvCacheArena(ctx, 1, st.num_blocks, 64, 8, 128)
+        try:
+            lens = [50 + 20 * i for i in range(40)]
+            pool = Pool((16, 8, 128), lens, 16, True)
+            q = torch.randn(40, 16, 128, device="cuda")
+            k, v = (torch.randn(40, 8, 128, device="cuda") for _ in range(2))
+            ctx.set(**st.context_args())
+            ctx.share_prefixes(st.groups)
+            ctx.set_encoder(pool.start, lens)
+            ctx.bind_kv_cache(arena)
+            own, cross = Attention(16, 128, 0.09, 8), CrossAttention(16, 128, 0.09, 8)
+            x, y = torch.empty_like(q), torch.empty_like(q)
+
+            def layer():
+                return [lib.nva_attention_forward_noalloc(
+                            ctx.handle, arena.handle, ctypes.byref(own._desc), q.data_ptr(),
+                            k.data_ptr(), v.data_ptr(), 40, x.data_ptr()),
+                        lib.nva_cross_attention_forward_noalloc(
+                            ctx.handle, ctypes.byref(cross._desc), x.data_ptr(), pool.k.data_ptr(),
+                            pool.v.data_ptr(), pool.rows, pool.k.stride(0), 40, y.data_ptr())]
+
+            assert layer() == [N.NVA_OK, N.NVA_OK]
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s1):
+                got = layer()
+            assert got == [N.NVA_OK, N.NVA_OK], lib.nva_last_error(ctx.handle)
+            for r in range(4):
+                for t in (q, k, v):
+                    t.normal_()
+                want_x = own.forward(q, k, v, ctx)
+                want_y = cross.forward(want_x, pool.k, pool.v, ctx)
+                x.fill_(float("nan"))
+                y.fill_(float("nan"))
+                s1.synchronize()
+                g.replay()
+                s1.synchronize()
+                say(f"decoder layer graph: replay {r}")
+                assert torch.equal(x, want_x) and torch.equal(y, want_y), f"replay {r}"
+        finally:
+            ctx.clear()
+            arena.close()
+
+
 def test_beside_the_decoder_layer(ctx):
     """A decoder step's self attention and cross attention in turn on one step: each keeps its plan,
     and new encoder rows replace the old."""
