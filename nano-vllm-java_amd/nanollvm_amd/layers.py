@@ -84,7 +84,7 @@ def _ptr(a: Optional[np.ndarray]):
 def _dev(t: Optional[torch.Tensor], name: str):
     if t is None:
         return None
-    if not (t.is_cuda and t.dtype == torch.float32 and t.is_contiguous()):
+    if not (t.is_cuda and t.dtype is torch.float32 and t.is_contiguous()):
         raise IllegalArgumentException(f"{name} must be a contiguous float32 device tensor")
     return t.data_ptr()
 
@@ -508,11 +508,12 @@ class Attention:
                                 self.sliding_window, kv_layer_index, int(self.write_kv))
 
     def _check_shapes(self, q, k, v) -> None:
-        if q.dim() != 3 or tuple(q.shape[1:]) != (self.num_heads, self.head_dim):
+        if q.dim() != 3 or q.shape[1:] != (self.num_heads, self.head_dim):
             raise IllegalArgumentException(
                 f"q must be [tokens, {self.num_heads}, {self.head_dim}], got {tuple(q.shape)}")
+        want = (q.shape[0], self.num_kv_heads, self.head_dim)
         for name, t in (("k", k), ("v", v)):
-            if t is not None and tuple(t.shape) != (q.shape[0], self.num_kv_heads, self.head_dim):
+            if t is not None and t.shape != want:
                 raise IllegalArgumentException(
                     f"{name} must be [{q.shape[0]}, {self.num_kv_heads}, {self.head_dim}], "
                     f"got {tuple(t.shape)}")
@@ -523,12 +524,11 @@ class Attention:
         arena at the step's slots, then attends; returns a new [tokens, numHeads, headDim]."""
         self._check_shapes(q, k, v)
         arena = ctx.kv_cache()
-        out = torch.empty((q.shape[0], self.num_heads, self.head_dim), dtype=torch.float32,
-                          device=q.device)
+        qp = _dev(q, "q")
+        out = torch.empty_like(q)
         _check(ctx.handle, N.load().nva_attention_forward(
             ctx.handle, arena.handle if arena is not None else None, ctypes.byref(self._desc),
-            _dev(q, "q"), _dev(k, "k"), _dev(v, "v"), q.shape[0], _dev(out, "out")),
-            "Attention.forward")
+            qp, _dev(k, "k"), _dev(v, "v"), q.shape[0], out.data_ptr()), "Attention.forward")
         return out
 
     def forward_with_rope(self, rope: RotaryEmbedding, positions, q: torch.Tensor,
