@@ -1763,10 +1763,12 @@ nva_status run_attention(nva_ctx *ctx, const nva_attn_desc &d, const KvView &vie
     mg.part_l = pm + parts;
     mg.part_acc = pm + 2 * parts;
     Timed tm(ctx, "merge");
-    const bool spans = plan->num_spans > 0 || plan->num_span_tiles > 0;
+    // Plans with spans take the merge of lane groups where launch_merge would a wave per partial.
+    const bool spans = (plan->num_spans > 0 || plan->num_span_tiles > 0) && d.head_dim <= 256 &&
+                       plan->max_parts > (plan->num_merge >= 512 ? kMergeRowsMaxParts : 4);
     HIP_TRY(ctx,
-            spans && d.head_dim <= 256 && plan->max_parts > 4 ? launch_merge_spans(mg, ctx->stream)
-                                         : launch_merge(mg, plan->max_parts, ctx->stream),
+            spans ? launch_merge_spans(mg, ctx->stream)
+                  : launch_merge(mg, plan->max_parts, ctx->stream),
             "merge kernel launch");
     tm.done();
   }

@@ -340,9 +340,9 @@ void launch_span(const SpanLaunch &a, hipStream_t s) {
 // D / 4 lanes take every G-th partial, four of them in flight, and meet in LDS in order, so the result
 // does not depend on timing.  (The decode merge gives a partial a wave of 64 lanes: of 97 partials at
 // d = 64 three quarters of 16 waves idle, in two rounds of workgroups: 10 us for 20 rows of 32 heads,
-// 5.0 here.  At d = 512, where four groups are left, it is the faster one, 33 against 35 us a decode
-// call, as for at most four partials, where it takes all heads of a row at once.)  Rows without
-// partials are zero.
+// 5.0 here.  At d = 512, where two groups would be left, it is the faster one, 33 against 35 us a
+// decode call, and so is the row-wide merge where it serves: 1280 rows of 32 heads and 8 partials 13
+// against 26 us.)  Rows without partials are zero.
 template <int D>
 __global__ void __launch_bounds__(256) merge_spans_kernel(MergeLaunch a) {
   constexpr int D4 = D / 4, G = 256 / D4;

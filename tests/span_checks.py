@@ -19,7 +19,7 @@ class SharedStep:
     """A step over pages.  ``groups`` lists (sequences, prefix tokens), whole pages that the sequences
     share; sequence i of the step has own[i] = (cached, new) tokens behind its group's prefix."""
 
-    def __init__(self, groups, own, block, seed, decode=None):
+    def __init__(self, groups, own, block, seed, decode=None, first_block=0):
         r = np.random.default_rng(seed)
         self.block = block
         self.prefix = [p for n, p in groups for _ in range(n)]
@@ -29,8 +29,8 @@ class SharedStep:
         self.keys = [p + c + n for p, (c, n) in zip(self.prefix, self.own)]
         self.new = [n for _, n in self.own]
         need = sum(-(-k // block) for k in self.keys) + 2
-        ids = iter(r.permutation(need + 3).tolist())
-        self.num_blocks = need + 3
+        ids = iter((first_block + r.permutation(need + 3)).tolist())
+        self.num_blocks = first_block + need + 3
         tables, b = [], 0
         for n, p in groups:
             assert p % block == 0

@@ -117,6 +117,19 @@ def test_full_attention_of_an_encoder(ctx, shape):
     check(ctx, "full attention", shape, lens, lens, seed=4)
 
 
+@pytest.mark.parametrize("seed", range(48))
+def test_drawn_steps(ctx, seed):
+    """Any head shape, numbers of requests, beams, queries and keys."""
+    r = np.random.default_rng(2000 + seed)
+    shape = SHAPES[int(r.integers(len(SHAPES)))]
+    lens = [int(np.exp(r.uniform(0, np.log(3000)))) - 1 for _ in range(int(r.integers(1, 25)))]
+    beams = int(r.choice([1, 1, 2, 3, 6]))
+    most = int(r.choice([1, 4, 90]))
+    queries = [int(r.integers(0 if most > 1 else 1, most + 1)) for _ in range(len(lens) * beams)]
+    check(ctx, f"drawn step {seed}", shape, queries, lens, beams=beams, packed=bool(r.integers(2)),
+          seed=seed, tail=int(r.integers(0, 3)) if any(n != 1 for n in queries) else 0)
+
+
 def test_many_sequences_of_one_key(ctx):
     check(ctx, "one key each", (16, 16, 64), [1] * 700, [1] * 700, seed=5)
 

@@ -194,6 +194,45 @@ def test_long_prefix_many_rows(ctx):
         s.arena.close()
 
 
+@pytest.mark.parametrize("rows", [3, 200])
+def test_pages_behind_four_gib(ctx, rows):
+    """Pages whose rows lie beyond 32-bit byte and float offsets, on the span kernel and the tiles."""
+    st = SharedStep([(rows, 4096)], [(i % 50, 1) for i in range(rows)], 256, seed=24,
+                    first_block=16500)
+    s = Setup(ctx, st, (2, 2, 128), seed=24)
+    assert s.arena.shape(0)[0] * 256 * 2 * 128 > 2 ** 30
+    try:
+        s.check(ctx, f"pages behind 4 GiB, {rows} rows")
+    finally:
+        ctx.clear()
+        s.arena.close()
+
+
+@pytest.mark.parametrize("seed", range(48))
+def test_drawn_steps(ctx, seed):
+    """Steps of any shape: groups of one to many sequences, prefixes of one page to many, page sizes,
+    own lengths, decode or prefill, groups that name part of what the pages share."""
+    r = np.random.default_rng(1000 + seed)
+    shape = SHAPES[int(r.integers(len(SHAPES)))]
+    block = int(r.choice([4, 16, 24, 64, 256]))
+    decode = bool(r.integers(2))
+    groups, own = [], []
+    for _ in range(int(r.integers(1, 5))):
+        n = int(r.integers(1, 3 if r.integers(2) else 70))
+        pages = int(np.exp(r.uniform(0, np.log(max(2, 6000 // block)))))
+        groups.append((n, pages * block))
+        own += [(int(r.integers(0, 90)), 1 if decode else int(r.integers(1, 60)) if n < 30 else
+                 int(r.integers(1, 9))) for _ in range(n)]
+    st = SharedStep(groups, own, block, seed=seed, decode=decode)
+    named = [(a, n, int(r.integers(0, p + 1)) if r.integers(2) else p) for a, n, p in st.groups]
+    s = Setup(ctx, st, shape, seed=seed, groups=named)
+    try:
+        s.check(ctx, f"drawn step {seed}: {shape} pages of {block} {groups} decode={decode}")
+    finally:
+        ctx.clear()
+        s.arena.close()
+
+
 def test_found_groups_use_both_kernels(ctx):
     """find_shared_prefixes gives the groups; a few rows and a short prefix run on the span kernel,
     many over a long one on span tiles, and without sharing neither runs."""
