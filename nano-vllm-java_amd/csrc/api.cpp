@@ -179,7 +179,8 @@ struct PlanKey {
   bool operator==(const PlanKey &o) const {
     return cross == o.cross && kv_rows == o.kv_rows && item_heads == o.item_heads &&
            tile_heads == o.tile_heads && span_tile_cols == o.span_tile_cols &&
-           span_blocks_per_cu == o.span_blocks_per_cu && window == o.window && mfma == o.mfma && fp32_tiles == o.fp32_tiles && tile_q == o.tile_q &&
+           span_blocks_per_cu == o.span_blocks_per_cu && window == o.window && mfma == o.mfma &&
+           fp32_tiles == o.fp32_tiles && tile_q == o.tile_q &&
            head_dim == o.head_dim && num_heads == o.num_heads && num_kv_heads == o.num_kv_heads &&
            wg_per_item == o.wg_per_item && blocks_per_cu == o.blocks_per_cu &&
            tile_groups == o.tile_groups && tokens == o.tokens && paged == o.paged &&
@@ -1112,9 +1113,12 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
       for (size_t i = 0; i < span_tiles.size(); i++)
         tile_rows[i] = (span_tiles[i].qlen - span_tiles[i].q0) / key.tile_heads;
       const int64_t cap = std::max<int64_t>(1, page_cap / 32);
-      std::vector<Piece> cut = whole_tiles(span_tiles, span_slots, total, cap, beside ? 1 : key.span_blocks_per_cu);
-      if (cut.empty()) cut = cut_tiles(span_tiles, tile_rows, span_slots, cap);
-      else span_slots = (int)cut.size();
+      std::vector<Piece> cut =
+          whole_tiles(span_tiles, span_slots, total, cap, beside ? 1 : key.span_blocks_per_cu);
+      if (cut.empty())
+        cut = cut_tiles(span_tiles, tile_rows, span_slots, cap);
+      else
+        span_slots = (int)cut.size();
       span_tiles = segments_by_slot(cut, span_slots, &span_off, [&](int i, int np, int pi) {
         TileItem c = span_tiles[i];
         if (pi == 0)
@@ -1290,10 +1294,10 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
         return fail(ctx, NVA_E_UNSUPPORTED, "span item is empty or spans more than %d pages",
                     kRowTablePages);
     for (const std::vector<TileItem> *list : {&tiles, &span_tiles})
-     for (const TileItem &t : *list)
-      if (t.ke > t.ks && (t.ke - 1) / bs - t.ks / bs + 1 > kPrefillTablePages)
-        return fail(ctx, NVA_E_UNSUPPORTED, "prefill segment spans more than %d pages",
-                    kPrefillTablePages);
+      for (const TileItem &t : *list)
+        if (t.ke > t.ks && (t.ke - 1) / bs - t.ks / bs + 1 > kPrefillTablePages)
+          return fail(ctx, NVA_E_UNSUPPORTED, "prefill segment spans more than %d pages",
+                      kPrefillTablePages);
   }
 
   plan->key = key;
@@ -1372,6 +1376,13 @@ KvView make_dense_view(const float *k, const float *v, int ld) {
   return view;
 }
 
+// Tokens of the group that sequence seq is in.
+int prefix_tokens(const nva_ctx *ctx, int seq) {
+  for (const nva_prefix_group &gr : ctx->groups)
+    if (seq >= gr.first_seq && seq < gr.first_seq + gr.num_seqs) return gr.num_tokens;
+  return 0;
+}
+
 // Whether a prefill step runs on the fp32 tile kernel (prefill_fp32.hip) rather than the split one.
 // The split kernel multiplies 2.5 times as fast, but its tiles cover twice the queries, with half
 // the workgroups per CU, and a segment starts later; steps of a few short prompts or chunks leave
@@ -1387,12 +1398,6 @@ KvView make_dense_view(const float *k, const float *v, int ld) {
 // tokens 23.0 / 27.1, 14+295 35.7 / 33.6; 4 q / 1 KV, d = 256, 22 and 3+7 15.7 / 16.3, 400 33.8 /
 // 32.0, 3736+100 43.6 / 36.6; 8 q / 1 KV, d = 512, 663+23 and 22 28.2 / 29.9, 300 42.2 / 39.0, 400
 // 52.0 / 44.6.
-int prefix_tokens(const nva_ctx *ctx, int seq) {
-  for (const nva_prefix_group &gr : ctx->groups)
-    if (seq >= gr.first_seq && seq < gr.first_seq + gr.num_seqs) return gr.num_tokens;
-  return 0;
-}
-
 bool use_fp32_tiles(nva_ctx *ctx, const nva_attn_desc &d, int hpw_fp32, int hpw_split, int window) {
   struct Cost {
     double floor, per_wave;  // CU us per key tile: at least, and per active wave
@@ -1407,10 +1412,11 @@ bool use_fp32_tiles(nva_ctx *ctx, const nva_attn_desc &d, int hpw_fp32, int hpw_
       const int qlen = ctx->cu_q[b + 1] - ctx->cu_q[b];
       const int klen = ctx->cu_k[b + 1] - ctx->cu_k[b];
       if (qlen < 2 || klen < qlen) continue;  // row kernel
+      const int prefix = prefix_tokens(ctx, b);
       for (int t0 = 0; t0 < qlen; t0 += tile_q) {
         const int n = std::min(tile_q, qlen - t0);
         const int first = klen - qlen + t0;
-        const int ks = window > 0 ? std::max(0, first - window + 1) : prefix_tokens(ctx, b);
+        const int ks = window > 0 ? std::max(0, first - window + 1) : prefix;
         const double work = c.per_wave * hpw * ((n + c.queries - 1) / c.queries);
         sum += std::max(c.floor, work) * ((first + n - ks + 31) / 32);
         longest = std::max(longest, std::max(c.floor * c.per_cu, work));
@@ -1550,12 +1556,16 @@ ScratchLayout scratch_layout(size_t gather_bytes, const Plan &plan, const nva_at
   return l;
 }
 
+bool tag_meets(const ScratchTag &tag, size_t begin, size_t end) {
+  return tag.plan_id != 0 && begin < tag.offset + tag.bytes && tag.offset < end;
+}
+
 // A call is about to write [begin, end) of this device's array: a plan recorded as held there no
 // longer is, if the ranges meet.
 void scratch_overwritten(int device, size_t begin, size_t end) {
   for (bool cross : {false, true}) {
     ScratchTag &tag = scratch_tag(device, cross);
-    if (tag.plan_id != 0 && begin < tag.offset + tag.bytes && tag.offset < end) tag = ScratchTag{};
+    if (tag_meets(tag, begin, end)) tag = ScratchTag{};
   }
 }
 
@@ -1564,7 +1574,8 @@ bool stream_capturing(hipStream_t s) {
   return hipStreamIsCapturing(s, &cs) == hipSuccess && cs != hipStreamCaptureStatusNone;
 }
 
-// Whether a plan's call fits the array and, under stream capture, finds its plan there.
+// Whether a plan's call fits the array and, under stream capture, finds its plan there and leaves the
+// other kind's alone (a graph of both would overwrite that plan at every replay).
 nva_status noalloc_fits(nva_ctx *ctx, const Plan &plan, const nva_attn_desc &d, size_t gather) {
   const ScratchLayout l = scratch_layout(gather, plan, d);
   if (l.bytes > kScratchBytes)
@@ -1578,6 +1589,13 @@ nva_status noalloc_fits(nva_ctx *ctx, const Plan &plan, const nva_attn_desc &d, 
     return fail(ctx, NVA_E_ARG,
                 "under stream capture the step's plan must already be in the device scratch "
                 "array: make one call with this configuration outside capture first");
+  const ScratchTag &other = scratch_tag(ctx->device, !plan.key.cross);
+  if ((tag_meets(other, 0, gather) || tag_meets(other, l.part_off, l.part_off + l.part_bytes)) &&
+      stream_capturing(ctx->stream))
+    return fail(ctx, NVA_E_ARG,
+                "this call's %zu bytes of the device scratch array meet the plan that the step's %s "
+                "attention holds there: the two do not fit one graph",
+                l.bytes, plan.key.cross ? "sequence" : "cross");
   return NVA_OK;
 }
 
@@ -1869,7 +1887,8 @@ nva_status attention_after_store(nva_ctx *ctx, nva_kv *kv, const nva_attn_desc &
   if (ctx->is_prefill && !ctx->has_tables) {
     if (d.write_kv) {
       if (!k || !v) return fail(ctx, NVA_E_ARG, "dense prefill needs k and v");
-      return run_attention(ctx, d, make_dense_view(k, v, d.num_kv_heads * d.head_dim), 0, q, num_tokens, out, scr);
+      return run_attention(ctx, d, make_dense_view(k, v, d.num_kv_heads * d.head_dim), 0, q,
+                           num_tokens, out, scr);
     }
     // Shared-KV dense prefill: gather the producer's rows at the step's slots.
     if (!ctx->has_slots || ctx->num_slots != num_tokens)
@@ -2503,7 +2522,7 @@ nva_status nva_rope_forward(nva_ctx *ctx, const nva_rope *rope, const float *q, 
 // workspace (null: the context's buffers).
 static nva_status attention_forward(nva_ctx *ctx, nva_kv *kv, const nva_attn_desc *desc,
                                     const float *q, const float *k, const float *v,
-                                    int num_tokens, float *out, Scratch *scr) {
+                                    int num_tokens, float *out, Scratch *scr) try {
   nva_status st = check_forward(ctx, kv, desc, num_tokens);
   if (st != NVA_OK) return st;
   if (num_tokens == 0) return NVA_OK;  // empty batch: an empty output, as Tensor.zeros(0, ...)
@@ -2540,6 +2559,8 @@ static nva_status attention_forward(nva_ctx *ctx, nva_kv *kv, const nva_attn_des
     tm.done();
   }
   return attention_after_store(ctx, kv, d, q, k, v, num_tokens, out, scr);
+} catch (const std::bad_alloc &) {
+  return no_memory(ctx);
 }
 
 nva_status nva_attention_forward(nva_ctx *ctx, nva_kv *kv, const nva_attn_desc *desc,
@@ -2645,7 +2666,7 @@ static nva_status norm_rope_attention(nva_ctx *ctx, nva_kv *kv, const nva_rope *
                                       const nva_rms_norm *v_norm, const nva_attn_desc *desc,
                                       const float *q, const float *k, const float *v, int q_ld,
                                       int k_ld, int v_ld, int num_tokens, float *q_out,
-                                      float *k_out, float *out) {
+                                      float *k_out, float *out) try {
   if (!ctx) return NVA_E_ARG;
   DeviceGuard dg(ctx);
   nva_status st = check_forward(ctx, kv, desc, num_tokens);
@@ -2723,6 +2744,8 @@ static nva_status norm_rope_attention(nva_ctx *ctx, nva_kv *kv, const nva_rope *
     tm.done();
   }
   return attention_after_store(ctx, kv, d, q_out, k_out, v_out ? v_out : v, num_tokens, out);
+} catch (const std::bad_alloc &) {
+  return no_memory(ctx);
 }
 
 nva_status nva_norm_rope_attention_forward(nva_ctx *ctx, nva_kv *kv, const nva_rope *rope,

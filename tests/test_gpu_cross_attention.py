@@ -324,6 +324,61 @@ def test_decoder_layer_in_one_graph():
             arena.close()
 
 
+def test_calls_that_do_not_fit_one_graph():
+    """Under capture a call whose partials would overwrite the plan that the other attention holds in
+    the scratch array is refused; outside capture both run and agree with the allocating forms."""
+    from nanollvm_amd import Attention, KvCacheArena
+    lib = N.load()
+    tokens, keys, block = 1250, 6 * 4096, 64
+    s1 = torch.cuda.Stream()
+    with torch.cuda.stream(s1), Context(0, stream=s1) as ctx:
+        arena = KvCacheArena(ctx, 1, (tokens + block - 1) // block, block, 64, 128)
+        try:
+            torch.manual_seed(18)
+            q, k, v = (torch.randn(tokens, 64, 128, device="cuda") for _ in range(3))
+            ctx.set(is_prefill=True, cu_seqlens_q=[0, tokens], cu_seqlens_k=[0, tokens],
+                    slot_mapping=list(range(tokens)))
+            ctx.set_encoder([0], [keys])
+            ctx.bind_kv_cache(arena)
+            # Head dim 32 runs row by row: six partials a row, 65 MB at the array's end.  The gathered
+            # rows of a layer that shares another's pages put its plan 82 MB behind the array's start.
+            cross, own = CrossAttention(64, 32, 0.1, 1), Attention(64, 128, 0.09, 64)
+            shared = N.AttnDesc(64, 128, own.scale, 64, 0, 0, 0)
+            x = torch.randn(tokens, 64, 32, device="cuda")
+            pool = torch.randn(2, keys, 1, 32, device="cuda")
+            out, y = torch.empty_like(q), torch.empty_like(x)
+            want = own.forward(q, k, v, ctx)
+            want_y = cross.forward(x, pool[0], pool[1], ctx)
+
+            def self_call():
+                return lib.nva_attention_forward_noalloc(
+                    ctx.handle, arena.handle, ctypes.byref(shared), q.data_ptr(), None, None, tokens,
+                    out.data_ptr())
+
+            def cross_call():
+                return lib.nva_cross_attention_forward_noalloc(
+                    ctx.handle, ctypes.byref(cross._desc), x.data_ptr(), pool[0].data_ptr(),
+                    pool[1].data_ptr(), keys, 32, tokens, y.data_ptr())
+
+            for r in range(2):
+                assert cross_call() == N.NVA_OK and self_call() == N.NVA_OK
+                s1.synchronize()
+                assert torch.equal(out, want) and torch.equal(y, want_y), f"turn {r}"
+            y.zero_()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s1):
+                refused = cross_call()
+                message = lib.nva_last_error(ctx.handle)
+                y.fill_(1.0)
+            assert refused == N.NVA_E_ARG and b"do not fit one graph" in message
+            assert cross_call() == N.NVA_OK and self_call() == N.NVA_OK
+            s1.synchronize()
+            assert torch.equal(out, want) and torch.equal(y, want_y), "after the refusal"
+        finally:
+            ctx.clear()
+            arena.close()
+
+
 def test_beside_the_decoder_layer(ctx):
     """A decoder step's self attention and cross attention in turn on one step: each keeps its plan,
     and new encoder rows replace the old."""
