@@ -634,6 +634,13 @@ class CrossAttention:
 
     def _pool(self, k, v, device):
         """Pointers, rows and row stride of the encoder's keys and values."""
+        shape, strides = k.shape, k.stride()
+        if (shape == v.shape and strides == v.stride() and len(shape) == 3 and shape[0] > 1 and
+                shape[1] == self.num_kv_heads and shape[2] == strides[1] == self.head_dim and
+                strides[2] == 1 and k.dtype is v.dtype is torch.float32 and
+                k.get_device() == v.get_device() == device):
+            return k.data_ptr(), v.data_ptr(), shape[0], strides[0]
+        # Few rows, whose strides need not agree, or a mistake.
         row = (self.num_kv_heads, self.head_dim)
         rows, stride = k.shape[0] if k.dim() else 0, k.stride(0) if k.dim() else 0
         for name, t in (("k", k), ("v", v)):
@@ -653,15 +660,17 @@ class CrossAttention:
         """softmax(q k^T scale) v over the rows of ``ctx.set_encoder``: q [tokens, numHeads, headDim]
         as the step has it, k and v [rows, numKvHeads, headDim], whose rows may lie apart (views of
         one packed projection); returns a new [tokens, numHeads, headDim]."""
-        if q.dim() != 3 or q.shape[1:] != (self.num_heads, self.head_dim):
+        shape = q.shape
+        if len(shape) != 3 or shape[1] != self.num_heads or shape[2] != self.head_dim:
             raise IllegalArgumentException(
-                f"q must be [tokens, {self.num_heads}, {self.head_dim}], got {tuple(q.shape)}")
-        kp, vp, rows, stride = self._pool(k, v, ctx.device)
+                f"q must be [tokens, {self.num_heads}, {self.head_dim}], got {tuple(shape)}")
+        device, handle = ctx.device, ctx.handle
+        kp, vp, rows, stride = self._pool(k, v, device)
         qp = _dev(q, "q")
-        if q.get_device() != ctx.device:
+        if q.get_device() != device:
             raise IllegalArgumentException("q must be on the context's device")
         out = torch.empty_like(q)
-        _check(ctx.handle, N.load().nva_cross_attention_forward(
-            ctx.handle, ctypes.byref(self._desc), qp, kp, vp, rows, stride, q.shape[0],
+        _check(handle, N.load().nva_cross_attention_forward(
+            handle, ctypes.byref(self._desc), qp, kp, vp, rows, stride, shape[0],
             out.data_ptr()), "CrossAttention.forward")
         return out
