@@ -681,6 +681,41 @@ std::vector<Piece> whole_tiles(const std::vector<TileItem> &tiles, int slots, in
   return whole;
 }
 
+// One piece of a tile on every slot: the tiles cut into at most `slots` pieces, as even as that allows,
+// so that no workgroup starts a second segment (its queries, first key tile and results cost as much
+// as about 4 key tiles, and partials are fewer).  Empty if the longest piece then is more than 1.4 equal
+// shares and 4 key tiles, or than a segment may be.  Over 87 drawn steps of 2-20 spans of 12-10000 keys
+// (d = 64 to 512) calls take 0.83 times as long on average as with equal shares, 1.05 at most but for
+// one: nine prompts of 2-500 queries over 147-2567 keys, 4 q / 1 KV heads, d = 256, 96 -> 83 us.
+std::vector<Piece> even_tiles(const std::vector<TileItem> &tiles, int slots, int64_t total,
+                              int64_t cap_tiles) {
+  std::vector<Piece> cut;
+  if ((int64_t)tiles.size() > slots) return cut;
+  auto key_tiles = [](const TileItem &t) { return (int64_t)(t.ke - t.ks + 31) / 32; };
+  auto fits = [&](int64_t longest) {
+    int64_t n = 0;
+    for (const TileItem &t : tiles) n += (key_tiles(t) + longest - 1) / longest;
+    return n <= slots;
+  };
+  int64_t longest = (total + slots - 1) / slots;
+  int64_t most = std::min(cap_tiles, (int64_t)(1.4 * (double)total / slots) + 4);
+  if (longest > most || !fits(most)) return cut;
+  while (longest < most) {
+    const int64_t mid = (longest + most) / 2;
+    if (fits(mid))
+      most = mid;
+    else
+      longest = mid + 1;
+  }
+  for (int i = 0; i < (int)tiles.size(); i++) {
+    const int64_t n = key_tiles(tiles[i]), pieces = (n + longest - 1) / longest;
+    for (int64_t j = 0; j < pieces; j++)
+      cut.push_back({i, (int)cut.size(), tiles[i].ks + (int)(n * j / pieces * 32),
+                     std::min(tiles[i].ke, tiles[i].ks + (int)(n * (j + 1) / pieces * 32))});
+  }
+  return cut;
+}
+
 // The segments of a cut, grouped by slot and in tile order within each (counting sort); seg_off[s]
 // is slot s's first.  make(tile, pieces, piece, first piece) gives one segment.
 template <typename F>
@@ -1115,6 +1150,7 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
       const int64_t cap = std::max<int64_t>(1, page_cap / 32);
       std::vector<Piece> cut =
           whole_tiles(span_tiles, span_slots, total, cap, beside ? 1 : key.span_blocks_per_cu);
+      if (cut.empty()) cut = even_tiles(span_tiles, span_slots, total, cap);
       if (cut.empty())
         cut = cut_tiles(span_tiles, tile_rows, span_slots, cap);
       else
