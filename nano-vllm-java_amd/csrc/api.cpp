@@ -683,10 +683,11 @@ std::vector<Piece> whole_tiles(const std::vector<TileItem> &tiles, int slots, in
 
 // One piece of a tile on every slot: the tiles cut into at most `slots` pieces, as even as that allows,
 // so that no workgroup starts a second segment (its queries, first key tile and results cost as much
-// as about 4 key tiles, and partials are fewer).  Empty if the longest piece then is more than 1.4 equal
-// shares and 4 key tiles, or than a segment may be.  Over 87 drawn steps of 2-20 spans of 12-10000 keys
-// (d = 64 to 512) calls take 0.83 times as long on average as with equal shares, 1.05 at most but for
-// one: nine prompts of 2-500 queries over 147-2567 keys, 4 q / 1 KV heads, d = 256, 96 -> 83 us.
+// as about 4 key tiles, and partials are fewer).  Empty if the longest piece then passes the equal share
+// by more than 4 key tiles and 0.4 shares, or 24 key tiles, or is more than a segment may be.  Over 90
+// drawn steps of 2-20 spans of 12-10000 keys (d = 64 to 512) calls take 0.85 times as long on average as
+// with equal shares, the best 0.48 and the worst 1.08 times; nine prompts of 253-486 queries over 147-2567
+// keys, 4 q / 1 KV heads, d = 256, 96 -> 83 us.
 std::vector<Piece> even_tiles(const std::vector<TileItem> &tiles, int slots, int64_t total,
                               int64_t cap_tiles) {
   std::vector<Piece> cut;
@@ -698,7 +699,8 @@ std::vector<Piece> even_tiles(const std::vector<TileItem> &tiles, int slots, int
     return n <= slots;
   };
   int64_t longest = (total + slots - 1) / slots;
-  int64_t most = std::min(cap_tiles, (int64_t)(1.4 * (double)total / slots) + 4);
+  const double share = (double)total / slots;
+  int64_t most = std::min(cap_tiles, (int64_t)(share + std::min(0.4 * share + 4.0, 24.0)));
   if (longest > most || !fits(most)) return cut;
   while (longest < most) {
     const int64_t mid = (longest + most) / 2;
