@@ -718,6 +718,60 @@ std::vector<Piece> even_tiles(const std::vector<TileItem> &tiles, int slots, int
   return cut;
 }
 
+// Tiles whole or in up to 8 pieces each, every piece on a slot of its own and longest first, where the
+// workgroups, which take them as they come free at 4 key tiles more a piece, end less than `slack` key
+// tiles behind the equal share.  (Equal shares start a second and third tile in most workgroups.)  Empty
+// otherwise.  Of 110 drawn steps the ones that qualify take 0.44-1.06 times as long as with equal shares
+// (48 spans of 100 queries over 13-99 keys, 4 q / 1 KV heads, d = 256, 173 -> 76 us), and without the
+// bound up to 1.25 times.
+std::vector<Piece> packed_tiles(const std::vector<TileItem> &tiles, int slots, int64_t total,
+                                int64_t cap_tiles, double slack) {
+  std::vector<Piece> cut;
+  auto key_tiles = [](const TileItem &t) { return (int64_t)(t.ke - t.ks + 31) / 32; };
+  int64_t most = 0;
+  for (const TileItem &t : tiles) most = std::max(most, key_tiles(t));
+  double best = (double)total / slots + slack;
+  int64_t best_longest = 0;
+  std::vector<int64_t> sizes;
+  for (int k = 1; k <= 8; k++) {
+    const int64_t longest = (most + k - 1) / k;
+    if (longest > cap_tiles || (double)longest + 4.0 >= best) continue;
+    sizes.clear();
+    for (const TileItem &t : tiles) {
+      const int64_t n = key_tiles(t), p = (n + longest - 1) / longest;
+      for (int64_t j = 0; j < p; j++) sizes.push_back(n * (j + 1) / p - n * j / p);
+    }
+    if (sizes.size() > 1024) break;
+    std::sort(sizes.begin(), sizes.end(), std::greater<int64_t>());
+    std::priority_queue<int64_t, std::vector<int64_t>, std::greater<int64_t>> free_at;
+    for (int i = 0; i < slots; i++) free_at.push(0);
+    int64_t end = 0;
+    for (int64_t n : sizes) {
+      const int64_t t = free_at.top() + n + 4;
+      free_at.pop();
+      free_at.push(t);
+      end = std::max(end, t);
+    }
+    if ((double)end < best) {
+      best = (double)end;
+      best_longest = longest;
+    }
+  }
+  if (best_longest == 0) return cut;
+  for (int i = 0; i < (int)tiles.size(); i++) {
+    const int64_t n = key_tiles(tiles[i]), p = (n + best_longest - 1) / best_longest;
+    for (int64_t j = 0; j < p; j++)
+      cut.push_back({i, 0, tiles[i].ks + (int)(n * j / p * 32),
+                     std::min(tiles[i].ke, tiles[i].ks + (int)(n * (j + 1) / p * 32))});
+  }
+  std::vector<int> order(cut.size());
+  for (size_t i = 0; i < order.size(); i++) order[i] = (int)i;
+  std::stable_sort(order.begin(), order.end(),
+                   [&](int x, int y) { return cut[x].k1 - cut[x].k0 > cut[y].k1 - cut[y].k0; });
+  for (size_t i = 0; i < order.size(); i++) cut[order[i]].slot = (int)i;
+  return cut;
+}
+
 // The segments of a cut, grouped by slot and in tile order within each (counting sort); seg_off[s]
 // is slot s's first.  make(tile, pieces, piece, first piece) gives one segment.
 template <typename F>
@@ -1153,6 +1207,9 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
       std::vector<Piece> cut =
           whole_tiles(span_tiles, span_slots, total, cap, beside ? 1 : key.span_blocks_per_cu);
       if (cut.empty()) cut = even_tiles(span_tiles, span_slots, total, cap);
+      if (cut.empty())
+        cut = packed_tiles(span_tiles, span_slots, total, cap,
+                           key.head_dim == 64 ? 10.0 : key.head_dim == 128 ? 8.5 : 16.0);
       if (cut.empty())
         cut = cut_tiles(span_tiles, tile_rows, span_slots, cap);
       else
