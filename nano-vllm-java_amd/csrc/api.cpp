@@ -173,6 +173,7 @@ struct PlanKey {
   int cross = 0;               // over the encoder's rows instead of the sequence's own keys
   int64_t kv_rows = 0;         // cross: rows of the encoder pool
   int item_heads = 0;          // query heads of a column group of a span item (0: no span kernel)
+  int split_tile_q = 0;        // queries of a split tile
   int tile_heads = 0;          // and of a span tile (0: no tile kernel for this head dim)
   int span_tile_cols = 0;      // columns of a span tile
   int span_blocks_per_cu = 0;
@@ -901,6 +902,124 @@ std::vector<char> choose_tiles(const PlanKey &key, const std::vector<Span> &span
   return tiles;
 }
 
+// First row of q of sequence b.
+int first_row_of(const nva_ctx *ctx, const PlanKey &key, int b) {
+  return ctx->is_prefill ? ctx->cu_q[b] : std::min(b, key.tokens);
+}
+
+// What of a step's prefix groups is read as spans.
+struct Sharing {
+  std::vector<Span> spans;
+  std::vector<int32_t> prefix;  // keys of each sequence that a span reads
+  bool tiles_run = true;        // chunks run on query tiles (else row by row)
+};
+
+// Sharing has to pay.  Read separately, a prefix costs its rows' share of HBM or whole query tiles;
+// shared, its span, and in a prefill step another launch, a partial of each row and the merge, which
+// took 10 us and 4 TB/s.  (Chunks that fill their tiles have nothing to gain: six chunks of 173 tokens
+// behind 6400, 4 q / 1 KV heads at d = 256, took 193 us apart and 252 us shared; 24 questions of 1-160
+// tokens behind 8192, 32 q / 8 KV heads at d = 128, 1437 and 843.)
+// A prefill step of few tokens is read without tiles, shared or not: in place of tiles, rows on the side
+// stream and their events (20 us), every row is an item, beside the spans' where they are items too,
+// else behind them (10 us and a tenth more).  (12 chunks of 1-5 tokens behind 544, 16 q / 8 KV heads at
+// d = 128, 50 -> 17 us; three behind 4096 70 -> 22.)
+Sharing choose_sharing(const nva_ctx *ctx, const PlanKey &key) {
+  auto first_row = [&](int b) { return first_row_of(ctx, key, b); };
+  auto is_chunk = [&](int q, int klen) { return key.mfma && q >= 2 && klen >= q; };
+  auto row_us = [&](double q, double keys) {  // a workgroup reads a KV head's keys for its heads
+    return q * keys * key.wg_per_item * key.head_dim * 8.0 / 6.5e6;
+  };
+  auto tile_us = [&](int q, double keys) {
+    const int tiles_of = (q + key.split_tile_q - 1) / key.split_tile_q;
+    return 4.0 * key.head_dim * key.num_heads * keys *
+           (0.55 * key.split_tile_q * tiles_of + 0.45 * q) / tile_rate(key.head_dim);
+  };
+  struct Way {
+    std::vector<Span> spans;
+    std::vector<size_t> groups;
+    double apart_us = 0.0;  // all prefixes apart
+    double saves_us = 0.0;  // of that, by sharing
+    bool on_items = true;   // all spans are
+  };
+  auto way = [&](bool chunks_on_tiles) {
+    Way w;
+    double shared_us = 0.0, join_us = 0.0, span_us = 0.0;  // of the shared prefixes: apart, and joined
+    for (size_t gi = 0; gi < ctx->groups.size(); gi++) {
+      const nva_prefix_group &gr = ctx->groups[gi];
+      const int row0 = first_row(gr.first_seq);
+      const int n = first_row(gr.first_seq + gr.num_seqs) - row0;
+      double apart = 0.0, join = 0.0;
+      for (int b = gr.first_seq; b < gr.first_seq + gr.num_seqs; b++) {
+        const int q = first_row(b + 1) - first_row(b);  // (behind a prefix, so never more than its keys)
+        apart += chunks_on_tiles && is_chunk(q, q) ? tile_us(q, gr.num_tokens) : row_us(q, gr.num_tokens);
+      }
+      w.apart_us += apart;
+      if (n < 2 || gr.num_tokens <= 0) continue;
+      if (ctx->is_prefill) join = 16.0 * n * key.num_heads * key.head_dim / 4e6;
+      const SpanCost c = span_cost(key, n, gr.num_tokens);
+      if (std::min(c.items, c.tiles) + join >= apart) continue;
+      int seq = gr.first_seq;
+      while (first_row(seq + 1) == row0) seq++;  // the first that has rows
+      w.spans.push_back({row0, n, seq, 0, gr.num_tokens});
+      w.groups.push_back(gi);
+      shared_us += apart;
+      join_us += join;
+    }
+    const std::vector<char> on_tiles = choose_tiles(key, w.spans, &span_us);
+    w.on_items = std::find(on_tiles.begin(), on_tiles.end(), 1) == on_tiles.end();
+    w.saves_us = shared_us - span_us - join_us;
+    if (ctx->is_prefill)
+      w.saves_us -= chunks_on_tiles ? 10.0 : 3.0;
+    else
+      w.saves_us += kItemsUs;
+    if (w.spans.empty() || w.saves_us < 0.0) {
+      w.spans.clear();
+      w.groups.clear();
+      w.saves_us = 0.0;
+    }
+    return w;
+  };
+  Sharing s;
+  Way chosen = way(true);
+  if (key.mfma) {
+    Way rows = way(false);
+    double own_tiles_us = 0.0, own_rows_us = 0.0;  // the chunks' keys behind their prefixes
+    bool singles = false, chunks = false;
+    size_t g = 0;
+    for (int b = 0; b < ctx->num_seqs; b++) {
+      const int q = first_row(b + 1) - first_row(b), klen = ctx->cu_k[b + 1] - ctx->cu_k[b];
+      while (g < ctx->groups.size() && b >= ctx->groups[g].first_seq + ctx->groups[g].num_seqs) g++;
+      const bool in_group = g < ctx->groups.size() && b >= ctx->groups[g].first_seq;
+      if (is_chunk(q, klen)) {
+        const double keys = klen - (in_group ? ctx->groups[g].num_tokens : 0) - 0.5 * q;
+        chunks = true;
+        own_tiles_us += tile_us(q, keys);
+        own_rows_us += row_us(q, keys);
+      } else {
+        singles |= q > 0;
+      }
+    }
+    const double tiles_us =
+        chosen.apart_us - chosen.saves_us + own_tiles_us + kTilesUs + (singles ? 20.0 : 0.0);
+    double rows_us = rows.apart_us - rows.saves_us + own_rows_us;
+    if (rows.spans.empty())
+      rows_us += 5.0;
+    else if (!rows.on_items)
+      rows_us = 1.1 * rows_us + 10.0;
+    if (chunks && rows_us < tiles_us) {
+      chosen = std::move(rows);
+      s.tiles_run = false;
+    }
+  }
+  s.spans = std::move(chosen.spans);
+  s.prefix.assign(ctx->num_seqs, 0);
+  for (size_t gi : chosen.groups) {
+    const nva_prefix_group &gr = ctx->groups[gi];
+    for (int b = 0; b < gr.num_seqs; b++) s.prefix[gr.first_seq + b] = gr.num_tokens;
+  }
+  return s;
+}
+
 // One query row of the row kernel before splitting.
 struct Row {
   int qrow, seq, kbase, kbeg, kend;
@@ -947,57 +1066,17 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
                     j, t[j], key.num_blocks);
     return NVA_OK;
   };
-  // Rows of q of a sequence.
-  auto first_row = [&](int b) {
-    return ctx->is_prefill ? ctx->cu_q[b] : std::min(b, key.tokens);
-  };
+  auto first_row = [&](int b) { return first_row_of(ctx, key, b); };
   // Shared prefixes: the rows of a group's sequences see its first keys as one span, and each
   // sequence's own lists start behind them.  A sliding window sees too little of them.
   const bool spans_run = key.item_heads > 0 || key.tile_heads > 0;  // else row by row
   std::vector<int32_t> prefix_len(ctx->num_seqs, 0);
-  if (!key.cross && paged && W == 0 && spans_run) {
-    // Sharing has to pay.  Read separately, a prefix costs its rows' share of HBM or whole query
-    // tiles; shared, its span, and in a prefill step another launch, a partial of each row and the
-    // merge, which took 10 us and 4 TB/s.  (Chunks that fill their tiles have nothing to gain: six
-    // chunks of 173 tokens behind 6400, 4 q / 1 KV heads at d = 256, took 193 us apart and 252 us
-    // shared; 24 questions of 1-160 tokens behind 8192, 32 q / 8 KV heads at d = 128, 1437 and 843.)
-    std::vector<size_t> gain;
-    double apart_us = 0.0, join_us = 0.0;
-    for (size_t gi = 0; gi < ctx->groups.size(); gi++) {
-      const nva_prefix_group &gr = ctx->groups[gi];
-      const int row0 = first_row(gr.first_seq);
-      const int n = first_row(gr.first_seq + gr.num_seqs) - row0;
-      if (n < 2 || gr.num_tokens <= 0) continue;
-      double apart = 0.0, join = 0.0;
-      for (int b = gr.first_seq; b < gr.first_seq + gr.num_seqs; b++) {
-        const int q = first_row(b + 1) - first_row(b);
-        if (key.mfma && q >= 2) {
-          const int tiles_of = (q + key.tile_q - 1) / key.tile_q;
-          apart += 4.0 * key.head_dim * key.num_heads * gr.num_tokens *
-                   (0.55 * key.tile_q * tiles_of + 0.45 * q) / tile_rate(key.head_dim);
-        } else {
-          apart += (double)q * gr.num_tokens * key.num_kv_heads * key.head_dim * 8.0 / 6.5e6;
-        }
-      }
-      if (ctx->is_prefill) join = 16.0 * n * key.num_heads * key.head_dim / 4e6;
-      const SpanCost c = span_cost(key, n, gr.num_tokens);
-      if (std::min(c.items, c.tiles) + join >= apart) continue;
-      int seq = gr.first_seq;
-      while (first_row(seq + 1) == row0) seq++;  // the first that has rows
-      spans.push_back({row0, n, seq, 0, gr.num_tokens});
-      gain.push_back(gi);
-      apart_us += apart;
-      join_us += join;
-    }
-    double span_us = 0.0;
-    choose_tiles(key, spans, &span_us);
-    if (ctx->is_prefill ? span_us + join_us + 10.0 >= apart_us : span_us > apart_us + kItemsUs)
-      spans.clear();
-    else
-      for (size_t gi : gain) {
-        const nva_prefix_group &gr = ctx->groups[gi];
-        for (int b = 0; b < gr.num_seqs; b++) prefix_len[gr.first_seq + b] = gr.num_tokens;
-      }
+  bool tiles_run = key.mfma != 0;  // chunks run on query tiles
+  if (!key.cross && paged && W == 0 && spans_run && !ctx->groups.empty()) {
+    Sharing sharing = choose_sharing(ctx, key);
+    spans.swap(sharing.spans);
+    prefix_len.swap(sharing.prefix);
+    tiles_run = sharing.tiles_run;
   }
   if (key.cross) {
     // The rows of sequence b see its encoder's keys; sequences in a row that read the same ones
@@ -1061,7 +1140,7 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
         if (st != NVA_OK) return st;
       }
       covered += qlen;
-      if (key.mfma && qlen >= 2 && klen >= qlen) {
+      if (tiles_run && qlen >= 2 && klen >= qlen) {
         for (int t0 = 0; t0 < qlen; t0 += key.tile_q) {
           const int t1 = std::min(qlen, t0 + key.tile_q) - 1;
           const int aq0 = klen - qlen + t0, aq1 = klen - qlen + t1;
@@ -1471,13 +1550,6 @@ KvView make_dense_view(const float *k, const float *v, int ld) {
   return view;
 }
 
-// Tokens of the group that sequence seq is in.
-int prefix_tokens(const nva_ctx *ctx, int seq) {
-  for (const nva_prefix_group &gr : ctx->groups)
-    if (seq >= gr.first_seq && seq < gr.first_seq + gr.num_seqs) return gr.num_tokens;
-  return 0;
-}
-
 // Whether a prefill step runs on the fp32 tile kernel (prefill_fp32.hip) rather than the split one.
 // The split kernel multiplies 2.5 times as fast, but its tiles cover twice the queries, with half
 // the workgroups per CU, and a segment starts later; steps of a few short prompts or chunks leave
@@ -1493,7 +1565,8 @@ int prefix_tokens(const nva_ctx *ctx, int seq) {
 // tokens 23.0 / 27.1, 14+295 35.7 / 33.6; 4 q / 1 KV, d = 256, 22 and 3+7 15.7 / 16.3, 400 33.8 /
 // 32.0, 3736+100 43.6 / 36.6; 8 q / 1 KV, d = 512, 663+23 and 22 28.2 / 29.9, 300 42.2 / 39.0, 400
 // 52.0 / 44.6.
-bool use_fp32_tiles(nva_ctx *ctx, const nva_attn_desc &d, int hpw_fp32, int hpw_split, int window) {
+bool use_fp32_tiles(nva_ctx *ctx, const nva_attn_desc &d, int hpw_fp32, int hpw_split, int window,
+                    const std::vector<int32_t> &prefix) {
   struct Cost {
     double floor, per_wave;  // CU us per key tile: at least, and per active wave
     int per_cu;              // workgroups sharing the CU, so one tile's latency is floor * per_cu
@@ -1507,11 +1580,11 @@ bool use_fp32_tiles(nva_ctx *ctx, const nva_attn_desc &d, int hpw_fp32, int hpw_
       const int qlen = ctx->cu_q[b + 1] - ctx->cu_q[b];
       const int klen = ctx->cu_k[b + 1] - ctx->cu_k[b];
       if (qlen < 2 || klen < qlen) continue;  // row kernel
-      const int prefix = prefix_tokens(ctx, b);
+      const int own = prefix.empty() ? 0 : prefix[b];  // first key that a span does not read
       for (int t0 = 0; t0 < qlen; t0 += tile_q) {
         const int n = std::min(tile_q, qlen - t0);
         const int first = klen - qlen + t0;
-        const int ks = window > 0 ? std::max(0, first - window + 1) : prefix;
+        const int ks = window > 0 ? std::max(0, first - window + 1) : own;
         const double work = c.per_wave * hpw * ((n + c.queries - 1) / c.queries);
         sum += std::max(c.floor, work) * ((first + n - ks + 31) / 32);
         longest = std::max(longest, std::max(c.floor * c.per_cu, work));
@@ -1529,12 +1602,15 @@ bool use_fp32_tiles(nva_ctx *ctx, const nva_attn_desc &d, int hpw_fp32, int hpw_
 }
 
 // The same for a layer, estimated once per step and configuration.
-bool fp32_tiles(nva_ctx *ctx, const nva_attn_desc &d, int hpw_fp32, int hpw_split, int window) {
+bool fp32_tiles(nva_ctx *ctx, const nva_attn_desc &d, int hpw_fp32, int hpw_split, int window,
+                const PlanKey &key) {
   for (const TileChoice &c : ctx->tile_choices)
     if (c.head_dim == d.head_dim && c.num_heads == d.num_heads &&
         c.num_kv_heads == d.num_kv_heads && c.window == window)
       return c.fp32;
-  const bool fp32 = use_fp32_tiles(ctx, d, hpw_fp32, hpw_split, window);
+  std::vector<int32_t> prefix;
+  if (key.tile_heads > 0) prefix = choose_sharing(ctx, key).prefix;
+  const bool fp32 = use_fp32_tiles(ctx, d, hpw_fp32, hpw_split, window, prefix);
   ctx->tile_choices.push_back({d.head_dim, d.num_heads, d.num_kv_heads, window, fp32});
   return fp32;
 }
@@ -1570,9 +1646,6 @@ nva_status attention_plan(nva_ctx *ctx, const nva_attn_desc &d, int paged, int b
       ctx->is_prefill && !cross && prefill_kernel_supports(d.head_dim, *hpw_tile);
   const int window = d.sliding_window > 0 ? d.sliding_window : 0;
   const int hpw_fp32 = largest_pow2_divisor_upto(rep, prefill_fp32_max_heads(d.head_dim));
-  const bool fp32 = mfma && fp32_tiles(ctx, d, hpw_fp32, *hpw_tile, window);
-  if (fp32) *hpw_tile = hpw_fp32;
-  if (tiles_fp32) *tiles_fp32 = fp32;
   // The MFMA row kernel carries up to 16 heads of one KV head (it is used from 5).  Rows that
   // run beside MFMA prefill tiles (a mixed step) share the matrix pipes with them: there the row
   // kernel keeps 5 heads per KV head (40 query heads over 8 KV heads, Qwen3-4B-like mixed step:
@@ -1595,13 +1668,6 @@ nva_status attention_plan(nva_ctx *ctx, const nva_attn_desc &d, int paged, int b
   PlanKey key;
   key.window = window;
   key.mfma = mfma ? 1 : 0;
-  key.fp32_tiles = fp32 ? 1 : 0;
-  key.tile_q = !mfma  ? 0
-               : fp32 ? prefill_fp32_tile_queries(d.head_dim, *hpw_tile)
-                      : prefill_tile_queries(d.head_dim, *hpw_tile);
-  key.wg_per_item = d.num_kv_heads * (rep / *hpw_row);
-  key.blocks_per_cu = mfma ? ctx_prefill_blocks_per_cu(ctx, d.head_dim, *hpw_tile, fp32) : 0;
-  key.tile_groups = mfma ? d.num_kv_heads * (rep / *hpw_tile) : 0;
   key.tokens = num_tokens;
   key.paged = paged;
   key.block_size = paged ? block_size : 0;
@@ -1609,6 +1675,7 @@ nva_status attention_plan(nva_ctx *ctx, const nva_attn_desc &d, int paged, int b
   key.head_dim = d.head_dim;
   key.num_heads = d.num_heads;
   key.num_kv_heads = d.num_kv_heads;
+  key.wg_per_item = d.num_kv_heads * (rep / *hpw_row);
   if (cross || (!ctx->groups.empty() && paged && window == 0)) {
     key.cross = cross ? 1 : 0;
     key.kv_rows = cross ? cross->kv_rows : 0;
@@ -1620,11 +1687,21 @@ nva_status attention_plan(nva_ctx *ctx, const nva_attn_desc &d, int paged, int b
       while (rep % h) h--;
       return h;
     };
+    key.split_tile_q = mfma ? prefill_tile_queries(d.head_dim, *hpw_tile) : 0;
     key.span_tile_cols = tiles ? span_tile_cols(d.head_dim) : 0;
     key.tile_heads = tiles ? group(key.span_tile_cols) : 0;
     key.item_heads = items ? group(kSpanCols) : 0;
     key.span_blocks_per_cu = tiles ? ctx_span_blocks_per_cu(ctx, d.head_dim) : 0;
   }
+  const bool fp32 = mfma && fp32_tiles(ctx, d, hpw_fp32, *hpw_tile, window, key);
+  if (fp32) *hpw_tile = hpw_fp32;
+  if (tiles_fp32) *tiles_fp32 = fp32;
+  key.fp32_tiles = fp32 ? 1 : 0;
+  key.tile_q = !mfma  ? 0
+               : fp32 ? prefill_fp32_tile_queries(d.head_dim, *hpw_tile)
+                      : prefill_tile_queries(d.head_dim, *hpw_tile);
+  key.blocks_per_cu = mfma ? ctx_prefill_blocks_per_cu(ctx, d.head_dim, *hpw_tile, fp32) : 0;
+  key.tile_groups = mfma ? d.num_kv_heads * (rep / *hpw_tile) : 0;
   return get_plan(ctx, key, plan);
 }
 

@@ -156,6 +156,32 @@ def test_prefill_over_long_prefixes(ctx, shape, chunks):
         s.arena.close()
 
 
+@pytest.mark.parametrize("shape", [(16, 8, 128), (32, 8, 64), (4, 1, 256), (8, 1, 512), (40, 8, 128),
+                                   (34, 2, 64)], ids=str)
+@pytest.mark.parametrize("prefix,chunks,shared", [(2048, (5, 3, 1, 2, 4, 5), True),
+                                                  (64, (2, 1), False)], ids=["shared", "apart"])
+def test_prefill_of_few_tokens_runs_row_by_row(ctx, shape, prefix, chunks, shared):
+    """A step of a few tokens behind a prefix takes no query tiles: its rows, masked one by one, run as
+    rows, beside the prefix's span where that pays."""
+    st = SharedStep([(len(chunks), prefix)], [(3 * i, n) for i, n in enumerate(chunks)], 64, seed=22,
+                    decode=False)
+    s = Setup(ctx, st, shape, seed=22)
+    ctx.set_timing(True)
+    try:
+        ctx.reset_stats()
+        s.check(ctx, f"few tokens {shape} {prefix} {chunks}")
+        tiles, rows, span = launches(ctx, "prefill", "decode", "span")
+        assert tiles == 0 and rows + span >= 1, (tiles, rows, span)
+        if not shared:
+            assert (rows, span) == (1, 0)
+        elif shape == (16, 8, 128):
+            assert (rows, span) == (0, 1)
+    finally:
+        ctx.set_timing(False)
+        ctx.clear()
+        s.arena.close()
+
+
 def test_prefill_chunks_that_fill_their_tiles_are_read_apart(ctx):
     st = SharedStep([(2, 1536)], [(0, 256), (0, 256)], 256, seed=21, decode=False)
     s = Setup(ctx, st, (16, 8, 128), seed=21)
