@@ -9,9 +9,13 @@
 // an item over the whole range writes a_c / l_c (0 where l_c = 0), a split one or one of a prefix
 // leaves (m_c, l_c, a_c), and the merge joins what a row has from its prefix and from its own keys.
 //
-// Mapping onto CDNA4.  Bound by HBM: a key costs 8 D bytes of K and V, which the whole run uses, and
-// 4 D operations a column, so fp32 matrix instructions (which need no scaling and take any value)
-// stay ahead of the memory up to about 48 columns.  One workgroup of 4 waves per (item, KV head,
+// Mapping onto CDNA4.  A key costs 8 D bytes of K and V and 4 D operations a column, 8 operations a byte
+// on the 16 columns of a matrix instruction: fp32 matrix instructions (which need no scaling and take
+// any value; 155 TFLOP/s) keep up with HBM to 32 columns.  Measured: 128 single tokens over 300-1500
+// encoder rows (16 heads, d = 64, 0.96 GB) 172 us, 5.6 TB/s; 40 x 5 beams over 500-4000 rows (32 q / 8
+// KV heads, d = 128, 0.73 GB) 151 us, 4.9 TB/s; 256 rows under three prefixes with 2.1 GB of own keys
+// 363 us, 6.3 TB/s.  Runs of more columns are bound by their items' number (33 rows of 4 heads under 6144
+// tokens, d = 256: 26 us, 40% of the matrix unit, 5.5 turns a wave).  One workgroup of 4 waves per (item, KV head,
 // head group); each wave takes 16-key blocks of the item in turn, so that 4 waves read 64
 // consecutive keys at a time, with no barrier and no LDS until the end:
 //   S^T[key][col] = K Q^T    D/4 v_mfma_f32_16x16x4_f32 per block and 16 columns: at step 4v + c
@@ -21,7 +25,10 @@
 //   O^T[dim][col] += V^T P^T 4 x D/16 per block: step s contracts key t0 + 4g + s, whose
 //                            probability is the lane's own (B), against V[key][64w + 4i + c] (A) in
 //                            block b = 4w + c, so P never leaves the registers.
-// K operands serve both blocks of 16 columns.  The four waves' states meet in LDS in wave order.
+// From D = 256 on, 2 or 4 waves share a block by 128 dims each and add their partial scores in LDS.
+// K and V have one register buffer, so that two waves share a SIMD on items of 32 columns and three on
+// those of 16 (a second buffer leaves one on 32: beams 189 -> 219 us).  K operands serve both blocks of
+// 16 columns.  The waves' states meet in LDS in wave order.
 #include "nva_internal.h"
 #include "nva_device.h"
 #include "row_lanes.h"
