@@ -130,6 +130,16 @@ def test_drawn_steps(ctx, seed):
           seed=seed, tail=int(r.integers(0, 3)) if any(n != 1 for n in queries) else 0)
 
 
+@pytest.mark.parametrize("shape", [(4, 1, 256), (16, 8, 128), (12, 12, 64), (8, 1, 512)], ids=str)
+@pytest.mark.parametrize("queries,lens", [
+    ([333, 410, 250, 301, 377], [1777, 900, 1300, 33, 650]),                   # few tiles, one piece each
+    ([90 + 7 * (i % 5) for i in range(40)], [13 + 37 * i % 97 for i in range(40)]),  # many short ones
+    ([700, 20, 520], [5000, 129, 64]),                                        # one far longer
+], ids=["even", "short", "uneven"])
+def test_cuts_of_span_tiles(ctx, shape, queries, lens):
+    check(ctx, "cuts", shape, queries, lens, packed=False, seed=23)
+
+
 def test_many_sequences_of_one_key(ctx):
     check(ctx, "one key each", (16, 16, 64), [1] * 700, [1] * 700, seed=5)
 
