@@ -320,8 +320,9 @@ nva_status nva_attention_forward_noalloc(nva_ctx *ctx, nva_kv *kv, const nva_att
  * once.  sliding_window must be 0; kv_layer_index and write_kv are not used.  d = 64, 128, 256 and
  * 512 run on matrix units, other head dims row by row.  Not under stream capture: the second form,
  * with the rules and the scratch array of nva_attention_forward_noalloc, is for that (its plan lies
- * at the array's end, so that a decoder layer's calls of both kinds fit one graph; replays need the
- * plans they were captured with, so no call of another step or configuration may come between). */
+ * at the array's end, so that a decoder layer's calls of both kinds fit one graph; a captured call
+ * whose work would overwrite the plan the other kind holds there fails with NVA_E_ARG; replays need
+ * the plans they were captured with, so no call of another step or configuration may come between). */
 nva_status nva_cross_attention_forward(nva_ctx *ctx, const nva_attn_desc *desc, const float *q,
                                        const float *k, const float *v, int64_t kv_rows,
                                        int64_t kv_stride, int num_tokens, float *out);

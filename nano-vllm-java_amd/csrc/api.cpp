@@ -1076,7 +1076,7 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
     Sharing sharing = choose_sharing(ctx, key);
     spans.swap(sharing.spans);
     prefix_len.swap(sharing.prefix);
-    tiles_run = sharing.tiles_run;
+    tiles_run = tiles_run && sharing.tiles_run;
   }
   if (key.cross) {
     // The rows of sequence b see its encoder's keys; sequences in a row that read the same ones
@@ -1283,10 +1283,10 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
       for (size_t i = 0; i < span_tiles.size(); i++)
         tile_rows[i] = (span_tiles[i].qlen - span_tiles[i].q0) / key.tile_heads;
       const int64_t cap = std::max<int64_t>(1, page_cap / 32);
-      std::vector<Piece> cut =
-          whole_tiles(span_tiles, span_slots, total, cap, beside ? 1 : key.span_blocks_per_cu);
+      std::vector<Piece> cut;  // beside rows the grid stays within its share of the CUs
+      if (!beside) cut = whole_tiles(span_tiles, span_slots, total, cap, key.span_blocks_per_cu);
       if (cut.empty()) cut = even_tiles(span_tiles, span_slots, total, cap);
-      if (cut.empty())
+      if (cut.empty() && !beside)
         cut = packed_tiles(span_tiles, span_slots, total, cap,
                            key.head_dim == 64 ? 10.0 : key.head_dim == 128 ? 8.5 : 16.0);
       if (cut.empty())
