@@ -29,6 +29,9 @@ __device__ __forceinline__ float4 ld4_stream_at(const float *base, uint32_t off)
   constexpr int kNonTemporal = 2;  // the nt bit of the buffer instructions' cache policy
   return ld4_buffer<kNonTemporal>(base, off);
 }
+// An offset (floats) behind the range of the loads above, which they answer with zeros: the V of a
+// masked key, whose weight of 0 must not meet an infinity.
+constexpr uint32_t kOutside = 0x20000000;
 // The same, cached.
 __device__ __forceinline__ float4 ld4_at(const float *base, uint32_t off) {
   return ld4_buffer<0>(base, off);

@@ -104,7 +104,8 @@ span_kernel(SpanLaunch a) {
   };
   auto locate = [&](int t0) {
     Block b;
-    // A block past the item's end is the item's first (never used).
+    // A block past the item's end is the item's first: never used up to d = 128, multiplied by weights
+    // of 0 from d = 256 on, where the waves of a key group make the same turns.
     const int tb = t0 < it.kend ? t0 : tfirst;
     int64_t row;
     if constexpr (PAGED) {
@@ -120,15 +121,15 @@ span_kernel(SpanLaunch a) {
     b.ko = koff;
 #pragma unroll
     for (int s = 0; s < 4; s++) b.vo[s] = voff + (uint32_t)(s * rs);
-    if (tb < it.kbeg || tb + 16 > it.kend) {
-      // A partial block: every lane reads the block's key nearest its own inside the item (what
-      // lies outside could hold any bits, NaN included; a finite V row adds 0 at weight 0).
+    if (t0 < it.kbeg || t0 + 16 > it.kend) {
+      // A partial block (what lies outside the item could hold any bits, NaN included): K is the block's
+      // key nearest the lane's own inside the item, whose score is masked, V is zero.
       const int tk = min(max(tb + i, it.kbeg), it.kend - 1);
       b.ko = (uint32_t)((tk - tb) * (int64_t)rs + 4 * g);
 #pragma unroll
       for (int s = 0; s < 4; s++) {
-        const int tv = min(max(tb + 4 * g + s, it.kbeg), it.kend - 1);
-        b.vo[s] = (uint32_t)((tv - tb) * (int64_t)rs + 4 * i);
+        const int tv = t0 + 4 * g + s;
+        if (tv < it.kbeg || tv >= it.kend) b.vo[s] = kOutside;
       }
     }
     return b;
