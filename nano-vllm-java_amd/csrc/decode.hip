@@ -100,6 +100,10 @@ __device__ __forceinline__ int64_t kv_row(const KvView &kv, const int32_t *stab,
   return (int64_t)stab[blk - blk0] * kv.block_size + off;
 }
 
+// A V row of zeros, for masked keys.  (Not const: in constant memory the choice between it and a real
+// row would be a flat load.)
+__device__ float zero_row[512];
+
 }  // namespace
 
 // Lane layout of the K/V rows, per head dim and heads per workgroup: a row is read by LPT lanes
@@ -228,14 +232,14 @@ __global__ void __launch_bounds__(256) row_attention_kernel(RowLaunch a) {
       const float *vb = vbase_h + row * rs;
       // Lane offsets (floats) of the group's rows.  In a partial group (the item's first or
       // last, or one past its end that reloads the first) masked keys may sit on page slots
-      // never written (any bits, NaN included), so each lane reads the group's key nearest its
-      // own inside [kbeg, kend) instead, whose finite V row adds exactly 0 at weight 0.
-      uint32_t off[UH];
+      // never written (any bits, NaN included): their lanes read K of the group's key nearest
+      // their own inside [kbeg, kend) instead, and zeros for V, which add exactly 0 at weight 0.
+      uint32_t off[UH], voff[UH];
       if (g0 >= it.kbeg && g0 + G <= it.kend) {
 #pragma unroll
         for (int u = 0; u < UH; u++) {
           ok[u] = true;
-          off[u] = lane_off + (uint32_t)(u * TPW * rs);
+          voff[u] = off[u] = lane_off + (uint32_t)(u * TPW * rs);
         }
       } else {
 #pragma unroll
@@ -246,6 +250,7 @@ __global__ void __launch_bounds__(256) row_attention_kernel(RowLaunch a) {
           const int tq = gq + u * TPW + sub;
           const int tc = g0 >= it.kend ? it.kbeg : min(max(tq, it.kbeg), it.kend - 1);
           off[u] = (uint32_t)__mul24(tc - gq, (int)rs) + c * 4;
+          voff[u] = ok[u] ? off[u] : kOutside;
         }
       }
 #pragma unroll
@@ -253,7 +258,7 @@ __global__ void __launch_bounds__(256) row_attention_kernel(RowLaunch a) {
 #pragma unroll
         for (int j = 0; j < VPL; j++) {
           kr[u][j] = ld4_stream_at(kb, off[u] + LPT * 4 * j);  // kb, vb: wave-uniform
-          vr[u][j] = ld4_stream_at(vb, off[u] + LPT * 4 * j);
+          vr[u][j] = ld4_stream_at(vb, voff[u] + LPT * 4 * j);
         }
     } else {
 #pragma unroll
@@ -269,10 +274,11 @@ __global__ void __launch_bounds__(256) row_attention_kernel(RowLaunch a) {
         } else {
           row = kv_row(a.kv, stab, blk0, it.kbase, tt);
         }
+        const float *vrow = ok[u] ? vbase_h + row * rs : zero_row;  // of a masked key, as above
 #pragma unroll
         for (int j = 0; j < VPL; j++) {
           kr[u][j] = ld4_stream(kbase_h + row * rs + c * 4 + LPT * 4 * j);
-          vr[u][j] = ld4_stream(vbase_h + row * rs + c * 4 + LPT * 4 * j);
+          vr[u][j] = ld4_stream(vrow + c * 4 + LPT * 4 * j);
         }
       }
     }
@@ -532,14 +538,14 @@ __global__ void __launch_bounds__(256) row_mfma_kernel(RowLaunch a, int hpw) {
 #pragma unroll
     for (int s = 0; s < 4; s++) vo[s] = voff + (uint32_t)(s * rs);
     if (tb < it.kbeg || tb + 16 > it.kend) {
-      // A partial block: every lane reads the block's key nearest its own inside the chunk (an
-      // unwritten slot could hold any bits, NaN included; a finite V row adds 0 at weight 0).
+      // A partial block (an unwritten slot could hold any bits, NaN included): K is the block's key
+      // nearest the lane's own inside the chunk, whose score is masked, V is zero.
       const int tk = min(max(tb + i, it.kbeg), it.kend - 1);
       ko = (uint32_t)((tk - tb) * rs + 4 * g);
 #pragma unroll
       for (int s = 0; s < 4; s++) {
-        const int tv = min(max(tb + 4 * g + s, it.kbeg), it.kend - 1);
-        vo[s] = (uint32_t)((tv - tb) * rs + 4 * i);
+        const int tv = tb + 4 * g + s;
+        if (tv < it.kbeg || tv >= it.kend) vo[s] = kOutside;
       }
     }
 #pragma unroll

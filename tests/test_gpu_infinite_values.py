@@ -57,9 +57,10 @@ def plant(v, first, last):
 
 
 SHAPES = [(12, 12, 64), (16, 8, 128), (40, 8, 128), (34, 2, 64), (4, 1, 256), (8, 1, 512)]
+BY_ROWS = [(12, 12, 32), (6, 3, 16)]  # head dims that run row by row
 
 
-@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("shape", SHAPES + BY_ROWS, ids=str)
 @pytest.mark.parametrize("queries", [1, 4, 130])
 def test_ends_of_encoder_states(ctx, shape, queries):
     hq, hkv, d = shape
@@ -99,6 +100,21 @@ def test_ends_of_shared_prefixes(ctx, shape, block, tokens, rows):
     ends(ctx, shape, block, [(rows, -(-tokens // block) * block)], rows, [(0, rows, tokens)])
 
 
+@pytest.mark.parametrize("shape", SHAPES + BY_ROWS, ids=str)
+@pytest.mark.parametrize("block,tokens,rows", [(64, 192, 60), (24, 31, 5), (256, 129, 90)])
+def test_ends_of_shared_prefixes_beside_rows(ctx, shape, block, tokens, rows):
+    """The same where the rows' own keys, or all, are read row by row."""
+    ends(ctx, shape, block, [(rows, -(-tokens // block) * block)], rows, [(0, rows, tokens)])
+
+
+@pytest.mark.parametrize("shape", SHAPES + BY_ROWS + [(4, 2, 8), (28, 4, 128), (6, 2, 256)], ids=str)
+@pytest.mark.parametrize("window", [0, 45])
+@pytest.mark.parametrize("block", [1, 24, 64])
+def test_ends_of_rows_read_apart(ctx, shape, window, block):
+    """The same without groups, and under a window whose first key lies inside a block."""
+    ends(ctx, shape, block, [(9, 0)], 9, [], window)
+
+
 def ends(ctx, shape, block, groups, rows, named, window=0):
     hq, hkv, d = shape
     st = SharedStep(groups, [(40 + 7 * i % 61, 1) for i in range(rows)], block, seed=32)
@@ -114,7 +130,7 @@ def ends(ctx, shape, block, groups, rows, named, window=0):
                                                             generator=g)
         q = torch.randn(rows, hq, d, device="cuda", generator=g)
         k, v = (torch.randn(rows, hkv, d, device="cuda", generator=g) for _ in range(2))
-        v[:, :, 9] = -INF
+        v[:, :, 3] = -INF
         for s in st.slots:
             first = max(0, len(s) - window) if window else 0
             plant(vp, s[first], s[(named[0][2] if named else len(s) - 1) - 1])
