@@ -48,7 +48,7 @@ enum {
   NVA_E_NO_ARENA = 5,   /* no KV arena bound (Java: NullPointerException), Attention.java:153 */
   NVA_E_NO_STEP = 6,    /* no step metadata set (Java: NullPointerException on Context) */
   NVA_E_HIP = 7,        /* HIP runtime error or no usable device */
-  NVA_E_OOM = 8,        /* device or pinned allocation failed */
+  NVA_E_OOM = 8,        /* device, pinned or host memory ran out */
   NVA_E_UNSUPPORTED = 9 /* shape this build has no kernel for (e.g. head_dim % 4 != 0) */
 };
 
@@ -165,7 +165,8 @@ nva_status nva_rope_destroy(nva_rope *rope);
  *   seq_ids          [num_tokens]  optional, kept for the caller
  *   positions        [num_tokens]  fp32 positions, rounded like Math.round; may be NULL when
  *                                  RoPE is not used this step
- * For decode, num_seqs is the number of rows (one query token per sequence). */
+ * For decode, num_seqs is the number of rows (one query token per sequence).  A call that fails for
+ * want of memory leaves the context without a step (NVA_E_NO_STEP until the next). */
 nva_status nva_step_set(nva_ctx *ctx, int is_prefill, const int32_t *cu_q, const int32_t *cu_k,
                         int num_seqs, int max_seqlen_q, int max_seqlen_k,
                         const int32_t *slot_mapping, int num_slots,

@@ -19,7 +19,9 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <exception>
 #include <map>
+#include <memory>
 #include <mutex>
 #include <new>
 #include <queue>
@@ -321,9 +323,19 @@ nva_status fail(nva_ctx *ctx, nva_status st, const char *fmt, ...) {
     va_start(ap, fmt);
     vsnprintf(buf, sizeof(buf), fmt, ap);
     va_end(ap);
-    ctx->err = buf;
+    try {
+      ctx->err = buf;
+    } catch (const std::exception &) {  // no memory for the text
+      ctx->err.clear();
+    }
   }
   return st;
+}
+
+// Host memory ran out in an entry point (no exception may leave it).
+nva_status no_memory(nva_ctx *ctx) {
+  ctx->err = "out of memory";  // short: needs no allocation
+  return NVA_E_OOM;
 }
 
 nva_status hip_fail(nva_ctx *ctx, hipError_t e, const char *what) {
@@ -371,6 +383,24 @@ int ctx_span_blocks_per_cu(nva_ctx *ctx, int head_dim) {
   return it->second;
 }
 
+// Timings that find no host memory are dropped: the call they time is not to fail for them.
+void give_event(nva_ctx *ctx, hipEvent_t e) {
+  try {
+    ctx->event_pool.push_back(e);
+  } catch (const std::exception &) {
+    (void)hipEventDestroy(e);
+  }
+}
+
+void add_stat(nva_ctx *ctx, const char *name, double ms) {
+  try {
+    KernelStat &s = ctx->stats[name];
+    s.launches++;
+    s.ms += ms;
+  } catch (const std::exception &) {
+  }
+}
+
 hipEvent_t take_event(nva_ctx *ctx) {
   if (!ctx->event_pool.empty()) {
     hipEvent_t e = ctx->event_pool.back();
@@ -401,7 +431,12 @@ struct Timed {
     hipEvent_t stop = take_event(ctx);
     if (!stop) return;
     (void)hipEventRecord(stop, stream);
-    ctx->pending.push_back({name, variant, start, stop});
+    try {
+      ctx->pending.push_back({name, variant, start, stop});
+    } catch (const std::exception &) {
+      give_event(ctx, start);
+      give_event(ctx, stop);
+    }
     start = nullptr;
   }
 };
@@ -411,15 +446,11 @@ void resolve_timings(nva_ctx *ctx) {
     float ms = 0.f;
     if (hipEventSynchronize(p.stop) == hipSuccess &&
         hipEventElapsedTime(&ms, p.start, p.stop) == hipSuccess) {
-      for (const char *n : {p.name, p.variant}) {
-        if (!n) continue;
-        auto &s = ctx->stats[n];
-        s.launches++;
-        s.ms += ms;
-      }
+      for (const char *n : {p.name, p.variant})
+        if (n) add_stat(ctx, n, ms);
     }
-    ctx->event_pool.push_back(p.start);
-    ctx->event_pool.push_back(p.stop);
+    give_event(ctx, p.start);
+    give_event(ctx, p.stop);
   }
   ctx->pending.clear();
 }
@@ -438,9 +469,7 @@ struct HostTimed {
     if (!on) return;
     const double ms =
         std::chrono::duration<double, std::milli>(std::chrono::steady_clock::now() - t0).count();
-    auto &s = ctx->stats[name];
-    s.launches++;
-    s.ms += ms;
+    add_stat(ctx, name, ms);
   }
 };
 
@@ -1041,8 +1070,9 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
       break;
     }
   if (!plan) {
-    plan = new Plan();
-    ctx->plans.push_back(plan);
+    std::unique_ptr<Plan> made(new Plan());
+    ctx->plans.push_back(made.get());
+    plan = made.release();
   }
 
   const int W = key.window;
@@ -2128,12 +2158,6 @@ int32_t java_round(float x) {
 
 }  // namespace
 
-// Host memory ran out in an entry point (no exception may leave it).
-static nva_status no_memory(nva_ctx *ctx) {
-  ctx->err = "out of memory";  // short: needs no allocation
-  return NVA_E_OOM;
-}
-
 // Records msg as the context's last error (the step producers in step.cpp report through it).
 __attribute__((visibility("hidden"))) nva_status nva_internal_fail(nva_ctx *ctx, nva_status st,
                                                                  const char *msg) {
@@ -2167,7 +2191,8 @@ nva_status nva_ctx_create(int device, nva_ctx **out) {
   DeviceGuard dg(device);
   int cur = -1;
   if (hipGetDevice(&cur) != hipSuccess || cur != device) return NVA_E_HIP;
-  nva_ctx *ctx = new nva_ctx();
+  nva_ctx *ctx = new (std::nothrow) nva_ctx();
+  if (!ctx) return NVA_E_OOM;
   ctx->device = device;
   hipDeviceProp_t prop;
   if (hipGetDeviceProperties(&prop, device) == hipSuccess && prop.multiProcessorCount > 0)
@@ -2263,7 +2288,8 @@ nva_status nva_ctx_kernel_stats(nva_ctx *ctx, const char *kernel, int64_t *launc
     return NVA_OK;
   }
   resolve_timings(ctx);
-  auto it = ctx->stats.find(kernel);
+  auto it = ctx->stats.begin();
+  while (it != ctx->stats.end() && it->first != kernel) ++it;
   if (launches) *launches = it == ctx->stats.end() ? 0 : it->second.launches;
   if (total_ms) *total_ms = it == ctx->stats.end() ? 0.0 : it->second.ms;
   return NVA_OK;
@@ -2288,16 +2314,22 @@ nva_status nva_kv_create(nva_ctx *ctx, int num_layers, int num_blocks, int block
   if (num_blocks <= 0) return fail(ctx, NVA_E_ARG, "numBlocks must be > 0");
   if (block_size <= 0 || num_kv_heads <= 0 || !head_dims)
     return fail(ctx, NVA_E_ARG, "blockSize, numKvHeads must be > 0 and headDims non-null");
-  nva_kv *kv = new nva_kv();
+  nva_kv *kv = new (std::nothrow) nva_kv();
+  if (!kv) return no_memory(ctx);
   kv->ctx = ctx;
   kv->num_layers = num_layers;
   kv->num_blocks = num_blocks;
   kv->block_size = block_size;
   kv->num_kv_heads = num_kv_heads;
-  kv->head_dims.assign(head_dims, head_dims + num_layers);
-  kv->k.assign(num_layers, nullptr);
-  kv->v.assign(num_layers, nullptr);
-  kv->bytes.assign(num_layers, 0);
+  try {
+    kv->head_dims.assign(head_dims, head_dims + num_layers);
+    kv->k.assign(num_layers, nullptr);
+    kv->v.assign(num_layers, nullptr);
+    kv->bytes.assign(num_layers, 0);
+  } catch (const std::exception &) {
+    delete kv;
+    return no_memory(ctx);
+  }
   for (int i = 0; i < num_layers; i++) {
     if (allocate && !allocate[i]) continue;
     if (head_dims[i] <= 0) {
@@ -2425,7 +2457,11 @@ nva_status nva_rope_create(nva_ctx *ctx, const float *cos_sin, int max_pos, int 
     (void)hipFree(p);
     return hip_fail(ctx, e, "RoPE table upload");
   }
-  nva_rope *r = new nva_rope();
+  nva_rope *r = new (std::nothrow) nva_rope();
+  if (!r) {
+    (void)hipFree(p);
+    return no_memory(ctx);
+  }
   r->ctx = ctx;
   r->max_pos = max_pos;
   r->head_size = head_size;
@@ -2435,7 +2471,7 @@ nva_status nva_rope_create(nva_ctx *ctx, const float *cos_sin, int max_pos, int 
 }
 
 nva_status nva_rope_create_theta(nva_ctx *ctx, int head_size, int rotary_dim, int max_pos,
-                                 float base, nva_rope **out) {
+                                 float base, nva_rope **out) try {
   if (!ctx || !out) return NVA_E_ARG;
   if (rotary_dim != head_size) return fail(ctx, NVA_E_ARG, "rotaryDim must equal headSize");
   if (max_pos <= 0 || head_size <= 0 || head_size % 2)
@@ -2453,6 +2489,8 @@ nva_status nva_rope_create_theta(nva_ctx *ctx, int head_size, int rotary_dim, in
       table[(size_t)pos * head_size + half + i] = (float)std::sin(freq);
     }
   return nva_rope_create(ctx, table.data(), max_pos, head_size, out);
+} catch (const std::exception &) {
+  return no_memory(ctx);
 }
 
 nva_status nva_rope_destroy(nva_rope *rope) {
@@ -2470,7 +2508,7 @@ nva_status nva_step_set(nva_ctx *ctx, int is_prefill, const int32_t *cu_q, const
                         const int32_t *slot_mapping, int num_slots,
                         const int32_t *context_lens, const int32_t *block_tables,
                         int bt_stride, const int32_t *seq_ids, const float *positions,
-                        int num_tokens) {
+                        int num_tokens) try {
   if (!ctx) return NVA_E_ARG;
   DeviceGuard dg(ctx);
   if (num_seqs < 0 || num_slots < 0 || num_tokens < 0 || bt_stride < 0)
@@ -2483,7 +2521,7 @@ nva_status nva_step_set(nva_ctx *ctx, int is_prefill, const int32_t *cu_q, const
   ctx->tile_choices.clear();
   ctx->groups.clear();
   ctx->has_encoder = false;
-  ctx->has_step = true;
+  ctx->has_step = false;  // until all of it is set
   ctx->is_prefill = is_prefill != 0;
   ctx->num_seqs = num_seqs;
   ctx->num_tokens = num_tokens;
@@ -2511,10 +2549,8 @@ nva_status nva_step_set(nva_ctx *ctx, int is_prefill, const int32_t *cu_q, const
   for (int t = 0; positions && t < num_tokens; t++) ctx->pos[t] = java_round(positions[t]);
   if (ctx->is_prefill) {
     for (int b = 0; b < num_seqs; b++)
-      if (cu_q[b + 1] < cu_q[b] || cu_k[b + 1] < cu_k[b]) {
-        ctx->has_step = false;
+      if (cu_q[b + 1] < cu_q[b] || cu_k[b + 1] < cu_k[b])
         return fail(ctx, NVA_E_ARG, "cu_seqlens must be non-decreasing");
-      }
   }
 
   // One device blob: cu_q | cu_k | slots | ctx_lens | tables | positions (16-byte aligned).
@@ -2546,10 +2582,13 @@ nva_status nva_step_set(nva_ctx *ctx, int is_prefill, const int32_t *cu_q, const
   put(ctx->off_tables, ctx->tables);
   put(ctx->off_pos, ctx->pos);
   HIP_TRY(ctx, ctx->step_stage.upload(ctx->d_step, bytes, ctx->stream), "step upload");
+  ctx->has_step = true;
   return NVA_OK;
+} catch (const std::exception &) {
+  return no_memory(ctx);
 }
 
-nva_status nva_step_positions(nva_ctx *ctx, const float *positions, int num_tokens) {
+nva_status nva_step_positions(nva_ctx *ctx, const float *positions, int num_tokens) try {
   if (!ctx) return NVA_E_ARG;
   DeviceGuard dg(ctx);
   if (!ctx->has_step) return fail(ctx, NVA_E_NO_STEP, "no step metadata set on the context");
@@ -2581,6 +2620,8 @@ nva_status nva_step_positions(nva_ctx *ctx, const float *positions, int num_toke
   }
   HIP_TRY(ctx, ctx->step_stage.upload(ctx->d_step, bytes, ctx->stream), "step upload");
   return NVA_OK;
+} catch (const std::exception &) {
+  return no_memory(ctx);
 }
 
 nva_status nva_step_clear(nva_ctx *ctx) {

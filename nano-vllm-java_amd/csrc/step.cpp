@@ -7,7 +7,7 @@
 
 #include <algorithm>
 #include <cstdio>
-#include <new>
+#include <exception>
 #include <vector>
 
 #include "../../include/nva.h"
@@ -180,8 +180,8 @@ nva_status nva_find_shared_prefixes(const int32_t *block_tables, int num_seqs, i
       same[b - 1] = c;
     }
   }
-  std::vector<int64_t> best(num_seqs + 1, 0);
-  std::vector<int32_t> run(num_seqs + 1, 0), pages(num_seqs + 1, 0);
+  std::vector<int64_t> best((size_t)num_seqs + 1, 0);
+  std::vector<int32_t> run((size_t)num_seqs + 1, 0), pages((size_t)num_seqs + 1, 0);
   for (int j = 1; j <= num_seqs; j++) {
     best[j] = best[j - 1];
     run[j] = j - 1;
@@ -202,43 +202,51 @@ nva_status nva_find_shared_prefixes(const int32_t *block_tables, int num_seqs, i
       groups[(*num_groups)++] = {run[j], j - run[j], pages[j] * block_size};
   std::reverse(groups, groups + *num_groups);
   return NVA_OK;
-} catch (const std::bad_alloc &) {
+} catch (const std::exception &) {
   *num_groups = 0;
   return NVA_E_OOM;
 }
 
 nva_status nva_build_prefill_metadata(const nva_seq *seqs, int num_seqs, int block_size,
-                                      nva_step_meta *out) {
+                                      nva_step_meta *out) try {
   Built b;
   nva_status st = build_prefill(seqs, num_seqs, block_size, b);
   if (st != NVA_OK) return st;
   return export_to(b, num_seqs, true, out);
+} catch (const std::exception &) {
+  return NVA_E_OOM;
 }
 
 nva_status nva_build_decode_metadata(const nva_seq *seqs, int num_seqs, int block_size,
-                                     nva_step_meta *out) {
+                                     nva_step_meta *out) try {
   Built b;
   nva_status st = build_decode(seqs, num_seqs, block_size, b);
   if (st != NVA_OK) return st;
   return export_to(b, num_seqs, false, out);
+} catch (const std::exception &) {
+  return NVA_E_OOM;
 }
 
 nva_status nva_step_prepare_prefill(nva_ctx *ctx, const nva_seq *seqs, int num_seqs,
-                                    int block_size) {
+                                    int block_size) try {
   if (!ctx) return NVA_E_ARG;
   Built b;
   nva_status st = build_prefill(seqs, num_seqs, block_size, b);
   if (st != NVA_OK) return nva_internal_fail(ctx, st, b.err);
   return upload(ctx, b, num_seqs, true);
+} catch (const std::exception &) {
+  return nva_internal_fail(ctx, NVA_E_OOM, "out of memory");
 }
 
 nva_status nva_step_prepare_decode(nva_ctx *ctx, const nva_seq *seqs, int num_seqs,
-                                   int block_size) {
+                                   int block_size) try {
   if (!ctx) return NVA_E_ARG;
   Built b;
   nva_status st = build_decode(seqs, num_seqs, block_size, b);
   if (st != NVA_OK) return nva_internal_fail(ctx, st, b.err);
   return upload(ctx, b, num_seqs, false);
+} catch (const std::exception &) {
+  return nva_internal_fail(ctx, NVA_E_OOM, "out of memory");
 }
 
 }  // extern "C"
