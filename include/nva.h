@@ -268,7 +268,8 @@ nva_status nva_step_set_encoder(nva_ctx *ctx, const int32_t *kv_start, const int
                                 int num_seqs);
 
 /* Replaces the step's positions only (the positions tensor RotaryEmbedding.forward receives,
- * Norms.java:275, rounded with Math.round as at Norms.java:317).  Valid after nva_step_set. */
+ * Norms.java:275, rounded with Math.round as at Norms.java:317).  Valid after nva_step_set; without
+ * memory for them the context has no step left. */
 nva_status nva_step_positions(nva_ctx *ctx, const float *positions, int num_tokens);
 /* Context.clear(), Context.java:61-74. */
 nva_status nva_step_clear(nva_ctx *ctx);

@@ -2598,6 +2598,7 @@ nva_status nva_step_positions(nva_ctx *ctx, const float *positions, int num_toke
   for (int t = 0; t < num_tokens; t++) pos[t] = java_round(positions[t]);
   if (ctx->has_pos && pos == ctx->pos) return NVA_OK;
   // Re-pack the step blob with the new positions at the end (the other arrays are unchanged).
+  ctx->has_step = false;  // until all of it is set again
   ctx->pos.swap(pos);
   ctx->has_pos = true;
   const size_t bytes = std::max<size_t>(ctx->off_pos + ctx->pos.size() * 4, 16);
@@ -2619,6 +2620,7 @@ nva_status nva_step_positions(nva_ctx *ctx, const float *positions, int num_toke
     HIP_TRY(ctx, ctx->d_step.reserve(bytes), "step buffer");
   }
   HIP_TRY(ctx, ctx->step_stage.upload(ctx->d_step, bytes, ctx->stream), "step upload");
+  ctx->has_step = true;
   return NVA_OK;
 } catch (const std::exception &) {
   return no_memory(ctx);

@@ -254,6 +254,56 @@ def host_memory():
             stub.stub_fail_host_after(-1)
 
 
+def device_memory():
+    """A step or positions that find no device (or pinned) memory leave no step behind: nothing is
+    launched over the buffers of the one before, until a step is set whole."""
+    small, big = (Step(*a, 1, heads=(4, 2, 64)) for a in ((3, 128, 10), (60, 1024, 100)))
+    for what in ("step", "positions"):
+        failed = 0
+        for n in range(6):
+            ctx = context()
+            st, kv = big.arena(ctx)
+            assert st == N.NVA_OK
+            rope = ctypes.c_void_p()
+            assert lib.nva_rope_create_theta(ctx, 64, 64, 4096, 1e6, ctypes.byref(rope)) == N.NVA_OK
+            assert small.set(ctx) == small.attend(ctx, kv) == N.NVA_OK
+            many = np.arange(4000, dtype=np.float32)
+            stub.stub_fail_device_after(n)
+            st = (big.set(ctx) if what == "step" else
+                  lib.nva_step_positions(ctx, ptr(many), len(many)))
+            stub.stub_fail_device_after(-1)
+            if st != N.NVA_OK:
+                failed += 1
+                assert st == N.NVA_E_OOM, (what, n, st)
+                before, p = stub.stub_launches(), big.aligned()
+                got = [big.attend(ctx, kv), big.attend(ctx, kv, True), big.attend_encoder(ctx),
+                       big.share(ctx), big.encode(ctx),
+                       lib.nva_rope_forward(ctx, rope, p, p, 3, 4, 2, p, p),
+                       lib.nva_step_positions(ctx, ptr(many), 3)]
+                assert got == [N.NVA_E_NO_STEP] * len(got), (what, n, got)
+                assert stub.stub_launches() == before, (what, n)
+            assert big.set(ctx) == big.attend(ctx, kv) == N.NVA_OK
+            lib.nva_rope_destroy(rope)
+            lib.nva_kv_destroy(kv)
+            lib.nva_ctx_destroy(ctx)
+        assert failed >= 2, (what, failed)
+    # A call that finds none can be made again.
+    for noalloc in (False, True):
+        for call in ("attend", "attend_encoder"):
+            for n in range(8):
+                ctx = context()
+                st, kv = big.arena(ctx)
+                assert big.set(ctx) == big.share(ctx) == big.encode(ctx) == N.NVA_OK
+                args = (kv,) if call == "attend" else ()
+                stub.stub_fail_device_after(n)
+                st = getattr(big, call)(ctx, *args, noalloc)
+                stub.stub_fail_device_after(-1)
+                assert st in (N.NVA_OK, N.NVA_E_OOM), (call, n, st)
+                assert getattr(big, call)(ctx, *args, noalloc) == N.NVA_OK
+                lib.nva_kv_destroy(kv)
+                lib.nva_ctx_destroy(ctx)
+
+
 if __name__ == "__main__":
     globals()[sys.argv[2]]()
     print("ok", flush=True)

@@ -26,3 +26,7 @@ def run(stand_in, scenario):
 
 def test_no_exception_leaves_an_entry_point(stand_in):
     run(stand_in, "host_memory")
+
+
+def test_a_step_without_device_memory_is_none(stand_in):
+    run(stand_in, "device_memory")
