@@ -251,13 +251,13 @@ nva_status nva_find_shared_prefixes(const int32_t *block_tables, int num_seqs, i
 /* Attention of a batch that shares prefixes: from this call to the next nva_step_set (or call), every
  * attention call over the step's pages reads the tokens of a group once for all rows of its
  * sequences and joins the result with each sequence's own keys; outputs agree with those of the
- * separate reads to fp32 rounding.  (Layers with a sliding window, which see too little of a prefix,
+ * separate reads to fp32 rounding.  Layers with a sliding window, which see too little of a prefix,
  * are computed as before, and groups that would not gain are read apart: one row, or prefill chunks
- * that fill their query tiles.  Prefill steps of few tokens run row by row.  Joining takes more partials, which the no-allocation entry point's array has to
- * hold.)  Groups are in order and do not overlap; a
- * group's tokens are cached ones of each of its sequences, which hold them in the same pages: tables
- * that differ there fail the attention call with NVA_E_ARG, before anything is written.  num_groups
- * 0 ends the sharing. */
+ * that fill their query tiles.  Prefill steps of few tokens run row by row.  Joining takes more
+ * partials: in the no-allocation form, groups whose work its array does not hold are read apart.
+ * Groups are in order and do not overlap; a group's tokens are cached ones of each of its sequences,
+ * which hold them in the same pages: tables that differ there fail the attention call with NVA_E_ARG,
+ * before anything is written.  num_groups 0 ends the sharing. */
 nva_status nva_step_share_prefixes(nva_ctx *ctx, const nva_prefix_group *groups, int num_groups);
 
 /* The encoder rows that cross attention reads in this step: sequence b of the step sees rows

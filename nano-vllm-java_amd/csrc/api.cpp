@@ -227,6 +227,7 @@ struct PendingTiming {
 // Which tile kernel a layer configuration's prefill runs on in the current step.
 struct TileChoice {
   int head_dim, num_heads, num_kv_heads, window;
+  int tile_heads;  // of its spans (0: no prefix is shared)
   bool fp32;
 };
 
@@ -1636,13 +1637,37 @@ bool fp32_tiles(nva_ctx *ctx, const nva_attn_desc &d, int hpw_fp32, int hpw_spli
                 const PlanKey &key) {
   for (const TileChoice &c : ctx->tile_choices)
     if (c.head_dim == d.head_dim && c.num_heads == d.num_heads &&
-        c.num_kv_heads == d.num_kv_heads && c.window == window)
+        c.num_kv_heads == d.num_kv_heads && c.window == window && c.tile_heads == key.tile_heads)
       return c.fp32;
   std::vector<int32_t> prefix;
   if (key.tile_heads > 0) prefix = choose_sharing(ctx, key).prefix;
   const bool fp32 = use_fp32_tiles(ctx, d, hpw_fp32, hpw_split, window, prefix);
-  ctx->tile_choices.push_back({d.head_dim, d.num_heads, d.num_kv_heads, window, fp32});
+  ctx->tile_choices.push_back(
+      {d.head_dim, d.num_heads, d.num_kv_heads, window, key.tile_heads, fp32});
   return fp32;
+}
+
+// Regions of the no-allocation array one call uses, each 256-byte aligned: [gather rows | plan lists |
+// partials] from the front, or, for cross attention, [partials | plan lists] up to the end.
+struct ScratchLayout {
+  size_t plan_off = 0, part_off = 0, part_bytes = 0;
+  size_t bytes = 0;  // in all; the offsets hold only if the array has them
+};
+
+ScratchLayout scratch_layout(size_t gather_bytes, const Plan &plan, const nva_attn_desc &d) {
+  ScratchLayout l;
+  const size_t parts = (size_t)plan.num_parts * d.num_heads, plan_bytes = align256(plan.host.size());
+  l.part_bytes = parts * (2 + (size_t)d.head_dim) * sizeof(float);
+  l.bytes = align256(gather_bytes) + plan_bytes + l.part_bytes;
+  if (plan.key.cross) {
+    l.bytes = plan_bytes + align256(l.part_bytes);
+    l.plan_off = kScratchBytes - plan_bytes;
+    l.part_off = l.plan_off - align256(l.part_bytes);
+  } else {
+    l.plan_off = align256(gather_bytes);
+    l.part_off = l.plan_off + plan_bytes;
+  }
+  return l;
 }
 
 // What a cross attention call reads: a pool of kv_rows rows.
@@ -1652,11 +1677,10 @@ struct CrossRows {
 
 // The plan of one attention call (the descriptor, the step, and whether keys are paged over
 // an arena of num_blocks pages of block_size tokens or dense rows), plus the query heads per
-// workgroup of the row and tile kernels.
-nva_status attention_plan(nva_ctx *ctx, const nva_attn_desc &d, int paged, int block_size,
-                          int num_blocks, int num_tokens, Plan **plan, int *hpw_row,
-                          int *hpw_tile, bool *rows_mfma = nullptr,
-                          bool *tiles_fp32 = nullptr, const CrossRows *cross = nullptr) {
+// workgroup of the row and tile kernels.  share: the step's prefix groups count.
+nva_status plan_of(nva_ctx *ctx, const nva_attn_desc &d, int paged, int block_size, int num_blocks,
+                   int num_tokens, bool share, Plan **plan, int *hpw_row, int *hpw_tile,
+                   bool *rows_mfma, bool *tiles_fp32, const CrossRows *cross) {
   const int rep = d.num_heads / d.num_kv_heads;
   // Query heads per row workgroup: the largest divisor of the GQA ratio the row kernel is built
   // for, so each K/V byte crosses HBM once per KV head (one head per workgroup at a ratio of 5
@@ -1706,7 +1730,7 @@ nva_status attention_plan(nva_ctx *ctx, const nva_attn_desc &d, int paged, int b
   key.num_heads = d.num_heads;
   key.num_kv_heads = d.num_kv_heads;
   key.wg_per_item = d.num_kv_heads * (rep / *hpw_row);
-  if (cross || (!ctx->groups.empty() && paged && window == 0)) {
+  if (cross || (share && !ctx->groups.empty() && paged && window == 0)) {
     key.cross = cross ? 1 : 0;
     key.kv_rows = cross ? cross->kv_rows : 0;
     const bool tiles = prefill_kernel_supports(d.head_dim, 1);
@@ -1735,27 +1759,20 @@ nva_status attention_plan(nva_ctx *ctx, const nva_attn_desc &d, int paged, int b
   return get_plan(ctx, key, plan);
 }
 
-// Regions of the no-allocation array one call uses, each 256-byte aligned: [gather rows | plan lists |
-// partials] from the front, or, for cross attention, [partials | plan lists] up to the end.
-struct ScratchLayout {
-  size_t plan_off = 0, part_off = 0, part_bytes = 0;
-  size_t bytes = 0;  // in all; the offsets hold only if the array has them
-};
-
-ScratchLayout scratch_layout(size_t gather_bytes, const Plan &plan, const nva_attn_desc &d) {
-  ScratchLayout l;
-  const size_t parts = (size_t)plan.num_parts * d.num_heads, plan_bytes = align256(plan.host.size());
-  l.part_bytes = parts * (2 + (size_t)d.head_dim) * sizeof(float);
-  l.bytes = align256(gather_bytes) + plan_bytes + l.part_bytes;
-  if (plan.key.cross) {
-    l.bytes = plan_bytes + align256(l.part_bytes);
-    l.plan_off = kScratchBytes - plan_bytes;
-    l.part_off = l.plan_off - align256(l.part_bytes);
-  } else {
-    l.plan_off = align256(gather_bytes);
-    l.part_off = l.plan_off + plan_bytes;
-  }
-  return l;
+// The same; in the no-allocation array (noalloc) groups whose plan does not fit it are read apart,
+// which takes fewer partials.
+nva_status attention_plan(nva_ctx *ctx, const nva_attn_desc &d, int paged, int block_size,
+                          int num_blocks, int num_tokens, bool noalloc, Plan **plan, int *hpw_row,
+                          int *hpw_tile, bool *rows_mfma = nullptr, bool *tiles_fp32 = nullptr,
+                          const CrossRows *cross = nullptr) {
+  const nva_status st = plan_of(ctx, d, paged, block_size, num_blocks, num_tokens, true, plan, hpw_row,
+                                hpw_tile, rows_mfma, tiles_fp32, cross);
+  if (st != NVA_OK || !noalloc || cross) return st;
+  if ((*plan)->num_spans + (*plan)->num_span_tiles == 0 ||
+      scratch_layout(0, **plan, d).bytes <= kScratchBytes)  // (paged calls gather nothing)
+    return st;
+  return plan_of(ctx, d, paged, block_size, num_blocks, num_tokens, false, plan, hpw_row, hpw_tile,
+                 rows_mfma, tiles_fp32, cross);
 }
 
 bool tag_meets(const ScratchTag &tag, size_t begin, size_t end) {
@@ -1819,7 +1836,7 @@ nva_status noalloc_prepare(nva_ctx *ctx, nva_kv *kv, const nva_attn_desc &d, int
   Plan *plan = nullptr;
   int hpw_row = 0, hpw_tile = 0;
   nva_status st = attention_plan(ctx, d, dense ? 0 : 1, dense ? 1 : kv->block_size,
-                                 dense ? 0 : kv->num_blocks, num_tokens, &plan, &hpw_row,
+                                 dense ? 0 : kv->num_blocks, num_tokens, true, &plan, &hpw_row,
                                  &hpw_tile);
   if (st != NVA_OK) return st;
   return noalloc_fits(ctx, *plan, d, gather);
@@ -1834,7 +1851,8 @@ nva_status run_attention(nva_ctx *ctx, const nva_attn_desc &d, const KvView &vie
   int hpw_row = 0, hpw_tile = 0;
   bool rows_mfma = false, tiles_fp32 = false;
   nva_status st = attention_plan(ctx, d, view.paged, view.block_size, num_blocks, num_tokens,
-                                 &plan, &hpw_row, &hpw_tile, &rows_mfma, &tiles_fp32, cross);
+                                 scr != nullptr, &plan, &hpw_row, &hpw_tile, &rows_mfma, &tiles_fp32,
+                                 cross);
   if (st != NVA_OK) return st;
   const int window = d.sliding_window > 0 ? d.sliding_window : 0;
 
@@ -2829,8 +2847,8 @@ static nva_status cross_attention_forward(nva_ctx *ctx, const nva_attn_desc *des
   if (scr) {
     Plan *plan = nullptr;
     int hpw_row = 0, hpw_tile = 0;
-    st = attention_plan(ctx, d, 0, 1, 0, num_tokens, &plan, &hpw_row, &hpw_tile, nullptr, nullptr,
-                        &rows);
+    st = attention_plan(ctx, d, 0, 1, 0, num_tokens, true, &plan, &hpw_row, &hpw_tile, nullptr,
+                        nullptr, &rows);
     if (st == NVA_OK) st = noalloc_fits(ctx, *plan, d, 0);
     if (st != NVA_OK) return st;
   } else if (stream_capturing(ctx->stream)) {

@@ -304,6 +304,39 @@ def device_memory():
                 lib.nva_ctx_destroy(ctx)
 
 
+def stat(ctx, name):
+    n = ctypes.c_int64()
+    assert lib.nva_ctx_kernel_stats(ctx, name, ctypes.byref(n), None) == N.NVA_OK
+    return n.value
+
+
+def shared_work_area():
+    """Naming prefix groups takes nothing away from the no-allocation form: a step whose shared plan
+    is larger than the array is read apart if that fits, and shared up to there."""
+    ctx = context()
+    lib.nva_ctx_set_timing(ctx, 1)
+    seen = set()
+    for new in (60, 70, 80, 90, 100, 110, 120, 200):
+        step = Step(24, 8192, 0, new, heads=(32, 8, 128))
+        step.desc.write_kv = 0
+        step.num_blocks = 1  # nothing reads the pages here: one for all
+        step.table[:] = np.where(step.table >= 0, 0, -1)
+        st, kv = step.arena(ctx)
+        assert st == step.set(ctx) == N.NVA_OK
+        apart = step.attend(ctx, kv, True)
+        lib.nva_ctx_reset_stats(ctx)
+        assert step.share(ctx) == N.NVA_OK
+        shared = step.attend(ctx, kv, True)
+        spans = stat(ctx, b"span_tiles") + stat(ctx, b"span")
+        seen.add((apart, shared, spans))
+        print(new, apart, shared, spans, flush=True)
+        assert (shared == N.NVA_OK) == (apart == N.NVA_OK), (new, apart, shared)
+        assert step.attend(ctx, kv) == N.NVA_OK  # and the allocating form shares
+        lib.nva_kv_destroy(kv)
+    assert {(N.NVA_OK, N.NVA_OK, 1), (N.NVA_OK, N.NVA_OK, 0)} <= seen, seen
+    lib.nva_ctx_destroy(ctx)
+
+
 if __name__ == "__main__":
     globals()[sys.argv[2]]()
     print("ok", flush=True)

@@ -30,3 +30,7 @@ def test_no_exception_leaves_an_entry_point(stand_in):
 
 def test_a_step_without_device_memory_is_none(stand_in):
     run(stand_in, "device_memory")
+
+
+def test_shared_plans_that_do_not_fit_the_work_area_are_read_apart(stand_in):
+    run(stand_in, "shared_work_area")
