@@ -24,6 +24,7 @@
 #include <memory>
 #include <mutex>
 #include <new>
+#include <optional>
 #include <queue>
 #include <string>
 #include <vector>
@@ -181,7 +182,8 @@ struct PlanKey {
   int span_blocks_per_cu = 0;
   bool operator==(const PlanKey &o) const {
     return cross == o.cross && kv_rows == o.kv_rows && item_heads == o.item_heads &&
-           tile_heads == o.tile_heads && span_tile_cols == o.span_tile_cols &&
+           split_tile_q == o.split_tile_q && tile_heads == o.tile_heads &&
+           span_tile_cols == o.span_tile_cols &&
            span_blocks_per_cu == o.span_blocks_per_cu && window == o.window && mfma == o.mfma &&
            fp32_tiles == o.fp32_tiles && tile_q == o.tile_q &&
            head_dim == o.head_dim && num_heads == o.num_heads && num_kv_heads == o.num_kv_heads &&
@@ -773,6 +775,7 @@ std::vector<Piece> packed_tiles(const std::vector<TileItem> &tiles, int slots, i
       for (int64_t j = 0; j < p; j++) sizes.push_back(n * (j + 1) / p - n * j / p);
     }
     if (sizes.size() > 1024) break;
+    if ((double)(total + 4 * (int64_t)sizes.size()) / slots >= best) continue;  // no end is before that
     std::sort(sizes.begin(), sizes.end(), std::greater<int64_t>());
     std::priority_queue<int64_t, std::vector<int64_t>, std::greater<int64_t>> free_at;
     for (int i = 0; i < slots; i++) free_at.push(0);
@@ -857,25 +860,51 @@ int key_chunk(int n, F len, int64_t workgroups, int64_t many, int64_t few) {
 // estimated time is least, in keys: what the resident workgroups (two on a CU) have to do each, but
 // at least one chunk, and half a chunk for the last round.  A workgroup's start and end (Q, the first
 // loads, the waves' meeting, partials) take as long as kFixed keys.
-int span_chunk(const std::vector<SpanItem> &items, int workgroups, int num_cus, double *keys_time) {
+template <typename F>
+int span_chunk(int n, F len, int workgroups, int num_cus, double *keys_time) {
   constexpr double kFixed = 250;
+  constexpr int kUnits = 64;  // chunks of up to 64 units of 64 keys
   const double resident = 2.0 * num_cus;
+  // count[k]: pieces of k units.  An item of u units has as many as there are multiples of k (0 among
+  // them) below u, so the items above each number of units tell them all, without a division for every
+  // item and chunk (the plan of 256 rows of up to 1500 own keys under a prefix: 60 -> 18 us).  Few items of
+  // very many keys are divided.
+  double keys = 0.0;
+  int most = 0;
+  auto units = [&](int i) { return (std::max(0, len(i)) + 63) / 64; };
+  for (int i = 0; i < n; i++) {
+    keys += std::max(0, len(i));
+    most = std::max(most, units(i));
+  }
+  int64_t count[kUnits + 1] = {};
+  if (5LL * most <= (int64_t)kUnits * n) {
+    std::vector<int> above(most + 1, 0);  // items of more than j units
+    for (int i = 0; i < n; i++) above[units(i)]++;
+    int64_t sum = 0;
+    for (int j = most; j >= 0; j--) {
+      const int at = above[j];
+      above[j] = (int)sum;
+      sum += at;
+    }
+    for (int k = 1; k <= kUnits; k++)
+      for (int j = 0; j < most; j += k) count[k] += above[j];
+  } else {
+    for (int i = 0; i < n; i++) {
+      const int u = units(i);
+      for (int k = 1; k <= kUnits; k++) count[k] += (u + k - 1) / k;
+    }
+  }
   int best = 64;
   double &best_time = *keys_time;
   best_time = 1e300;
-  for (int c = 64; c <= 4096; c += 64) {
-    double keys = 0.0, pieces = 0.0;
-    for (const SpanItem &it : items) {
-      const int len = it.kend - it.kbeg, n = (len + c - 1) / c;
-      pieces += n;
-      keys += len;
-    }
+  for (int k = 1; k <= kUnits; k++) {
+    const double pieces = (double)count[k];
     const double each = (keys + pieces * kFixed) * workgroups / resident;
-    const double one = c + kFixed;
+    const double one = 64 * k + kFixed;
     const double time = std::max(one, each) + (pieces * workgroups > resident ? 0.5 * one : 0.0);
     if (time < best_time) {
       best_time = time;
-      best = c;
+      best = 64 * k;
     }
   }
   return best;
@@ -1057,7 +1086,8 @@ struct Row {
 
 // Builds (or reuses) the host lists of the plan for this configuration of the current step;
 // upload_plan() or the scratch path puts them on the device.
-nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
+// sharing: what of the step's prefix groups is shared, if it was chosen already, else null.
+nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Sharing *sharing, Plan **out) {
   for (Plan *p : ctx->plans)
     if (p->valid && p->key == key) {
       *out = p;
@@ -1104,10 +1134,10 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
   std::vector<int32_t> prefix_len(ctx->num_seqs, 0);
   bool tiles_run = key.mfma != 0;  // chunks run on query tiles
   if (!key.cross && paged && W == 0 && spans_run && !ctx->groups.empty()) {
-    Sharing sharing = choose_sharing(ctx, key);
-    spans.swap(sharing.spans);
-    prefix_len.swap(sharing.prefix);
-    tiles_run = tiles_run && sharing.tiles_run;
+    Sharing chosen = sharing ? std::move(*sharing) : choose_sharing(ctx, key);
+    spans.swap(chosen.spans);
+    prefix_len.swap(chosen.prefix);
+    tiles_run = tiles_run && chosen.tiles_run;
   }
   if (key.cross) {
     // The rows of sequence b see its encoder's keys; sequences in a row that read the same ones
@@ -1293,7 +1323,9 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
         for (const Row &r : rows)
           list.push_back({r.qrow, key.item_heads, r.seq, r.kbase, r.kbeg, r.kend, 0, 0, 0, 0});
       double time = 0.0;
-      const int c = span_chunk(list, key.num_heads / key.item_heads, ctx->num_cus, &time);
+      const int c = span_chunk(
+          (int)list.size(), [&](int i) { return list[i].kend - list[i].kbeg; },
+          key.num_heads / key.item_heads, ctx->num_cus, &time);
       if (cols > kSpanCols) time *= key.head_dim == 64 ? 1.6 : 1.4;
       if (time >= best_time) continue;
       best_time = time;
@@ -1433,10 +1465,10 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Plan **out) {
   if (!spans.empty() && !rows.empty()) {
     // Beside spans the rows' chunk is the span items' (64 rows of 16-1500 own keys under 8192 shared
     // ones, 32 q / 8 KV heads: 125 -> 115 us a call).
-    std::vector<SpanItem> list;
-    for (const Row &r : rows) list.push_back({r.qrow, 0, r.seq, r.kbase, r.kbeg, r.kend, 0, 0, 0, 0});
     double time = 0.0;
-    chunk = span_chunk(list, key.wg_per_item, ctx->num_cus, &time);
+    chunk = span_chunk(
+        (int)rows.size(), [&](int i) { return rows[i].kend - rows[i].kbeg; }, key.wg_per_item,
+        ctx->num_cus, &time);
   }
   // A paged item of `chunk` keys spans at most (chunk - 1) / BS + 2 pages; the row kernel
   // stages at most kRowTablePages of them.
@@ -1632,16 +1664,18 @@ bool use_fp32_tiles(nva_ctx *ctx, const nva_attn_desc &d, int hpw_fp32, int hpw_
   return estimate(fp32, hpw_fp32, q_fp32) <= estimate(split, hpw_split, q_split) + later;
 }
 
-// The same for a layer, estimated once per step and configuration.
+// The same for a layer, estimated once per step and configuration; where that needs the choice of what
+// is shared, *sharing receives it.
 bool fp32_tiles(nva_ctx *ctx, const nva_attn_desc &d, int hpw_fp32, int hpw_split, int window,
-                const PlanKey &key) {
+                const PlanKey &key, std::optional<Sharing> *sharing) {
   for (const TileChoice &c : ctx->tile_choices)
     if (c.head_dim == d.head_dim && c.num_heads == d.num_heads &&
         c.num_kv_heads == d.num_kv_heads && c.window == window && c.tile_heads == key.tile_heads)
       return c.fp32;
-  std::vector<int32_t> prefix;
-  if (key.tile_heads > 0) prefix = choose_sharing(ctx, key).prefix;
-  const bool fp32 = use_fp32_tiles(ctx, d, hpw_fp32, hpw_split, window, prefix);
+  if (key.tile_heads > 0) *sharing = choose_sharing(ctx, key);
+  static const std::vector<int32_t> none;
+  const bool fp32 = use_fp32_tiles(ctx, d, hpw_fp32, hpw_split, window,
+                                   sharing->has_value() ? (*sharing)->prefix : none);
   ctx->tile_choices.push_back(
       {d.head_dim, d.num_heads, d.num_kv_heads, window, key.tile_heads, fp32});
   return fp32;
@@ -1747,7 +1781,8 @@ nva_status plan_of(nva_ctx *ctx, const nva_attn_desc &d, int paged, int block_si
     key.item_heads = items ? group(kSpanCols) : 0;
     key.span_blocks_per_cu = tiles ? ctx_span_blocks_per_cu(ctx, d.head_dim) : 0;
   }
-  const bool fp32 = mfma && fp32_tiles(ctx, d, hpw_fp32, *hpw_tile, window, key);
+  std::optional<Sharing> sharing;
+  const bool fp32 = mfma && fp32_tiles(ctx, d, hpw_fp32, *hpw_tile, window, key, &sharing);
   if (fp32) *hpw_tile = hpw_fp32;
   if (tiles_fp32) *tiles_fp32 = fp32;
   key.fp32_tiles = fp32 ? 1 : 0;
@@ -1756,7 +1791,7 @@ nva_status plan_of(nva_ctx *ctx, const nva_attn_desc &d, int paged, int block_si
                       : prefill_tile_queries(d.head_dim, *hpw_tile);
   key.blocks_per_cu = mfma ? ctx_prefill_blocks_per_cu(ctx, d.head_dim, *hpw_tile, fp32) : 0;
   key.tile_groups = mfma ? d.num_kv_heads * (rep / *hpw_tile) : 0;
-  return get_plan(ctx, key, plan);
+  return get_plan(ctx, key, sharing ? &*sharing : nullptr, plan);
 }
 
 // The same; in the no-allocation array (noalloc) groups whose plan does not fit it are read apart,

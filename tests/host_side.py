@@ -101,7 +101,7 @@ class Step:
         p = self.aligned()
         f = (lib.nva_cross_attention_forward_noalloc if noalloc else
              lib.nva_cross_attention_forward)
-        return f(ctx, ctypes.byref(self.cross), p, p, p, 50, self.hkv * self.d, self.tokens, p)
+        return f(ctx, ctypes.byref(self.cross), p, p, p, 2000, self.hkv * self.d, self.tokens, p)
 
 
 def create():
@@ -334,6 +334,42 @@ def shared_work_area():
         assert step.attend(ctx, kv) == N.NVA_OK  # and the allocating form shares
         lib.nva_kv_destroy(kv)
     assert {(N.NVA_OK, N.NVA_OK, 1), (N.NVA_OK, N.NVA_OK, 0)} <= seen, seen
+    lib.nva_ctx_destroy(ctx)
+
+
+def plan_time():
+    """Planning a decode step's spans costs the host no more than planning its rows read apart: the
+    least of 40 builds each, for rows under a shared prefix and for rows over encoder states."""
+    ctx = context()
+    lib.nva_ctx_set_timing(ctx, 1)
+
+    def least(step, call, *before):
+        times = []
+        for _ in range(40):
+            for f in (step.set, *before):
+                assert f(ctx) == N.NVA_OK
+            lib.nva_ctx_reset_stats(ctx)
+            assert call() == N.NVA_OK
+            ms, n = ctypes.c_double(), ctypes.c_int64()
+            lib.nva_ctx_kernel_stats(ctx, b"plan", ctypes.byref(n), ctypes.byref(ms))
+            assert n.value == 1
+            times.append(1e3 * ms.value)
+        return min(times)
+
+    for rows in (64, 256, 1024):
+        step = Step(rows, 8192, 211, 1, block=256)
+        step.desc.write_kv = 0
+        step.num_blocks = 1  # nothing reads the pages here: one for all
+        step.table[:] = np.where(step.table >= 0, 0, -1)
+        st, kv = step.arena(ctx)
+        assert st == N.NVA_OK
+        step.enc_len = i32(300 + 37 * np.arange(rows) % 1201)
+        apart = least(step, lambda: step.attend(ctx, kv))
+        shared = least(step, lambda: step.attend(ctx, kv), step.share)
+        cross = least(step, lambda: step.attend_encoder(ctx), step.encode)
+        print(f"{rows} rows: apart {apart:.1f}, shared {shared:.1f}, encoder {cross:.1f} us", flush=True)
+        assert shared <= 1.5 * apart and cross <= 1.5 * apart
+        lib.nva_kv_destroy(kv)
     lib.nva_ctx_destroy(ctx)
 
 

@@ -34,3 +34,7 @@ def test_a_step_without_device_memory_is_none(stand_in):
 
 def test_shared_plans_that_do_not_fit_the_work_area_are_read_apart(stand_in):
     run(stand_in, "shared_work_area")
+
+
+def test_planning_spans_costs_no_more_than_rows(stand_in):
+    run(stand_in, "plan_time")
