@@ -10,6 +10,8 @@ from __future__ import annotations
 import ctypes
 import os
 
+import numpy as np
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libnva.so")
 
@@ -160,6 +162,24 @@ SIGNATURES = {
                                              ctypes.POINTER(AttnDesc), _vp, _ci, _vp, _vp, _vp],
                                             _st),
 }
+
+
+
+def i32(a) -> np.ndarray:
+    """``a`` as a contiguous int32 array of at least one dimension; ValueError for values that int32 does not hold, which a
+    cast would replace by others."""
+    a = np.atleast_1d(np.asarray(a))
+    if a.dtype == np.int32:
+        return np.ascontiguousarray(a)
+    try:
+        with np.errstate(invalid="ignore"):
+            b = np.ascontiguousarray(a.astype(np.int32))
+    except (OverflowError, TypeError) as e:
+        raise ValueError(f"not whole numbers of 32 bits: {e}") from None
+    if a.size and not np.array_equal(a, b):
+        raise ValueError("not whole numbers of 32 bits")
+    return b
+
 
 _lib = None
 

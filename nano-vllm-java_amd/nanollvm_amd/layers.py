@@ -74,7 +74,10 @@ def _check(ctx_handle, status: int, what: str) -> None:
 def _i32(a) -> Optional[np.ndarray]:
     if a is None:
         return None
-    return np.ascontiguousarray(np.asarray(a), dtype=np.int32)
+    try:
+        return N.i32(a)
+    except ValueError as e:
+        raise IllegalArgumentException(str(e)) from None
 
 
 def _ptr(a: Optional[np.ndarray]):
@@ -143,7 +146,7 @@ class Context:
         stride = 0
         if block_tables is not None:
             if isinstance(block_tables, np.ndarray):
-                bt = np.ascontiguousarray(block_tables, dtype=np.int32)
+                bt = _i32(block_tables)
             else:
                 width = max((len(r) for r in block_tables), default=0)
                 bt = np.full((len(block_tables), max(width, 1)), -1, np.int32)
@@ -194,10 +197,12 @@ class Context:
         """Attention over the step set last reads the tokens that runs of its sequences share once
         for each run: ``groups`` is a list of (first sequence, sequences, tokens), e.g. from
         ``step.find_shared_prefixes``."""
-        arr = (N.PrefixGroup * max(1, len(groups)))(*(N.PrefixGroup(*(int(x) for x in g))
-                                                      for g in groups))
-        _check(self._h, N.load().nva_step_share_prefixes(self._h, arr, len(groups)),
-               "Context.share_prefixes")
+        arr = _i32(groups).reshape(-1, 3) if len(groups) == 0 else _i32(groups)
+        if arr.ndim != 2 or arr.shape[1] != 3:
+            raise IllegalArgumentException("groups must be (first sequence, sequences, tokens)")
+        _check(self._h, N.load().nva_step_share_prefixes(
+            self._h, arr.ctypes.data_as(ctypes.POINTER(N.PrefixGroup)), len(arr)),
+            "Context.share_prefixes")
 
     def set_encoder(self, kv_start, kv_len) -> None:
         """The encoder rows each sequence of the step set last sees in ``CrossAttention``: the first

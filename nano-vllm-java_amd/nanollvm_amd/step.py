@@ -102,8 +102,11 @@ def find_shared_prefixes(block_tables, cached_tokens, block_size: int) -> List[T
     """nva_find_shared_prefixes: the runs of adjacent sequences of a step whose cached tokens start
     in the same pages, as (first sequence, sequences, tokens) for ``Context.share_prefixes``;
     ``block_tables`` is the step's 2-D table, -1 padded."""
-    table = np.ascontiguousarray(block_tables, dtype=np.int32)
-    cached = np.ascontiguousarray(cached_tokens, dtype=np.int32)
+    try:
+        table, cached = N.i32(block_tables), N.i32(cached_tokens)
+        block_size = int(N.i32(block_size)[0])
+    except ValueError as e:
+        raise MetadataError(f"block tables, cached lengths or block size: {e}") from None
     if table.ndim != 2 or cached.shape != (table.shape[0],):
         raise MetadataError("block tables must be 2-D, with one cached length per row")
     n = len(cached)
