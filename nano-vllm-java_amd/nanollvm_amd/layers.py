@@ -652,8 +652,10 @@ class CrossAttention:
             if t.dim() != 3 or t.shape[1:] != row:
                 raise IllegalArgumentException(
                     f"{name} must be [rows, {row[0]}, {row[1]}], got {tuple(t.shape)}")
+            # (The stride of a single head means nothing: [rows, None, dims] gives it any.)
             if not (t.is_cuda and t.get_device() == device and t.dtype is torch.float32 and
-                    (rows == 0 or t.stride()[1:] == (self.head_dim, 1))):
+                    (rows == 0 or t.stride(2) == 1 and
+                     (row[0] == 1 or t.stride(1) == self.head_dim))):
                 raise IllegalArgumentException(
                     f"{name} must be a float32 tensor with contiguous rows on the context's device")
         if v.shape[0] != rows or (rows > 1 and v.stride(0) != stride):
