@@ -41,7 +41,8 @@
 //     running max is only moved -- and O rescaled -- when a tile's max exceeds it by more than
 //     2^8, which after the first tiles almost never happens.
 //   * Only tiles that cross the causal diagonal, the window edge or the end of the keys are
-//     masked.
+//     masked.  A wave whose results are not finite takes them again over the keys that each query sees
+//     (seen_keys_only).
 #include "nva_internal.h"
 #include "nva_device.h"
 
@@ -122,6 +123,69 @@ __device__ __forceinline__ int64_t tile_row(const KvView &kv, const int32_t *sta
   return (int64_t)stab[blk - blk0] * kv.block_size + off;
 }
 
+// Whether a lane's sums hold an infinity or NaN in any lane of the wave.
+template <int NB>
+__device__ __forceinline__ bool any_not_finite(const f32x4 (&o)[NB]) {
+  f32x4 zero = f32x4{0.0f, 0.0f, 0.0f, 0.0f};  // NaN if any is not finite
+#pragma unroll
+  for (int b = 0; b < NB; b++)
+#pragma unroll
+    for (int v = 0; v < 4; v++) zero[v] = fmaf(0.0f, o[b][v], zero[v]);
+  return __any(!((zero[0] + zero[1]) + (zero[2] + zero[3]) == 0.0f));
+}
+
+// The segment's results for a wave's 16 queries (from q0 on) and dims [d0, d0 + DN), query by query over
+// the keys that it sees alone: for waves whose sums are not finite.  In the tiles a masked key has weight
+// 0, and 0 times an infinity in its V is NaN, in the results of queries that do not see it.
+template <int D, int DN>
+__device__ void seen_keys_only(const TileLaunch &a, const TileItem &it, int kvh, int h, int q0, int d0) {
+  const int lane = threadIdx.x & 63;
+  const int32_t *table = a.kv.table + (size_t)it.seq * a.kv.bt_stride;
+  const size_t rs = (size_t)a.hkv * D;
+  const float sl2 = a.scale * kLog2e;
+  const float *kbase = a.kv.k + (size_t)kvh * D + lane;
+  const float *vbase = a.kv.v + (size_t)kvh * D + d0 + lane;
+#pragma unroll 1
+  for (int qi = q0; qi < min(q0 + 16, it.qlen); qi++) {
+    const int aq = it.klen - it.qlen + qi;
+    const int lo = max(it.ks, a.window > 0 ? aq - a.window + 1 : 0), hi = min(it.ke, aq + 1);
+    const float *qp = a.q + ((size_t)(it.qstart + qi) * a.hq + h) * D + lane;
+    float q[D / 64], acc[DN / 64], m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int u = 0; u < D / 64; u++) q[u] = qp[64 * u];
+#pragma unroll
+    for (int u = 0; u < DN / 64; u++) acc[u] = 0.0f;
+#pragma unroll 1
+    for (int t = lo; t < hi; t++) {
+      const size_t at = (size_t)tile_row(a.kv, table, 0, it.kbase, t) * rs;
+      float x = 0.0f;
+#pragma unroll
+      for (int u = 0; u < D / 64; u++) x = fmaf(q[u], kbase[at + 64 * u], x);
+#pragma unroll
+      for (int dist = 32; dist; dist >>= 1) x += __shfl_xor(x, dist);
+      x *= sl2;
+      const float mn = fmaxf(m, x);
+      const float ms = mn == -INFINITY ? 0.0f : mn;
+      const float alpha = __builtin_amdgcn_exp2f(m - ms), w = __builtin_amdgcn_exp2f(x - ms);
+      l = fmaf(l, alpha, w);
+#pragma unroll
+      for (int u = 0; u < DN / 64; u++) acc[u] = fmaf(acc[u], alpha, w * vbase[at + 64 * u]);
+      m = mn;
+    }
+    const bool partial = it.part >= 0;
+    const size_t pidx = ((size_t)it.part + (size_t)(qi - it.q0) * it.nsplit + it.split) * a.hq + h;
+    const float inv = partial ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+    float *op = (partial ? a.part_acc + pidx * D
+                         : a.out + ((size_t)(it.qstart + qi) * a.hq + h) * D) + d0 + lane;
+#pragma unroll
+    for (int u = 0; u < DN / 64; u++) op[64 * u] = acc[u] * inv;
+    if (partial && lane == 0 && d0 == 0) {
+      a.part_m[pidx] = m;
+      a.part_l[pidx] = l;
+    }
+  }
+}
+
 }  // namespace
 
 // Head dims 64 and 128: four waves per SIMD (at most 128 VGPRs).
@@ -162,6 +226,7 @@ prefill_kernel(TileLaunch a) {
       voff[p] = (uint32_t)r * rsb + (uint32_t)pos * 16u;
     }
   }
+  uint64_t again = 0;  // the wave's segments to take again, by their number mod 64
   for (int seg = a.seg_off[slot]; seg < seg_end; seg++) {
   // Every wave is done with the previous segment's LDS tiles and table before they are reused.
   __syncthreads();
@@ -396,6 +461,10 @@ prefill_kernel(TileLaunch a) {
     compute_tile(kt + KT, sk1, sv1);
   }
 
+  if (wave_active && any_not_finite(o)) {
+    again |= 1ull << ((seg - a.seg_off[slot]) & 63);
+    continue;
+  }
   const float l_tot = sum4_lanes(l_run);
   if (!qvalid || !wave_active) continue;
   // Lane (i, g) holds O^T rows r = 4g + v of every block: dims 64*hh + 4r + bb.
@@ -424,6 +493,15 @@ prefill_kernel(TileLaunch a) {
     a.part_l[pidx] = l_tot;
   }
   }  // segments
+  __threadfence_block();  // (segments of one number mod 64 are taken again together)
+  for (int seg = a.seg_off[slot]; again && seg < seg_end; seg++) {
+    if (!(again >> ((seg - a.seg_off[slot]) & 63) & 1)) continue;
+    const int rep = a.hq / a.hkv, groups = rep / HPW, kvh = blockIdx.y / groups;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const TileItem it = a.items[seg];
+    seen_keys_only<D, D>(a, it, kvh, kvh * rep + (blockIdx.y - kvh * groups) * HPW + wave % HPW,
+                         it.q0 + wave / HPW * 16, 0);
+  }
 }
 
 // Head dim 512 (Gemma 4 global layers) with the head split over a wave pair: one 8-wave
@@ -452,10 +530,12 @@ prefill512_kernel(TileLaunch a) {
   __shared__ __attribute__((aligned(16))) float sk1[TILE];
   __shared__ __attribute__((aligned(16))) float sv1[TILE];
   __shared__ f32x4 spart[NW][64];  // each wave's partial S^T of the current tile
+  __shared__ uint64_t to_do[NW];   // each wave's segments to take again
   __shared__ int32_t stab[kTablePages];
 
   const int slot = blockIdx.x;
   const int seg_end = a.seg_off[slot + 1];
+  uint64_t again = 0;  // the wave's segments to take again, by their number mod 64
   for (int seg = a.seg_off[slot]; seg < seg_end; seg++) {
   __syncthreads();
   const TileItem it = a.items[seg];
@@ -620,6 +700,7 @@ prefill512_kernel(TileLaunch a) {
     compute_tile(kt + KT, sk1, sv1);
   }
 
+  if (wave_active && any_not_finite(o)) again |= 1ull << ((seg - a.seg_off[slot]) & 63);
   const float l_tot = sum4_lanes(l_run);
   if (!qvalid || !wave_active) continue;
   float *op;
@@ -646,6 +727,17 @@ prefill512_kernel(TileLaunch a) {
     a.part_l[pidx] = l_tot;
   }
   }  // segments
+  // Both halves of a query are taken again if either is not finite: they share its maximum.
+  if ((threadIdx.x & 63) == 0) to_do[threadIdx.x >> 6] = again;
+  __syncthreads();
+  again |= to_do[(threadIdx.x >> 6) ^ 4];
+  for (int seg = a.seg_off[slot]; again && seg < seg_end; seg++) {
+    if (!(again >> ((seg - a.seg_off[slot]) & 63) & 1)) continue;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const TileItem it = a.items[seg];
+    seen_keys_only<D, DH>(a, it, blockIdx.y / (a.hq / a.hkv), blockIdx.y, it.q0 + (wave & 3) * 16,
+                          DH * (wave >> 2));
+  }
 }
 
 namespace {
