@@ -1079,6 +1079,9 @@ Sharing choose_sharing(const nva_ctx *ctx, const PlanKey &key) {
   return s;
 }
 
+// Most keys of a sequence: the kernels count keys in 32 bits and look a few blocks ahead.
+constexpr int kMaxKeys = INT32_MAX - 8192;
+
 // One query row of the row kernel before splitting.
 struct Row {
   int qrow, seq, kbase, kbeg, kend;
@@ -1114,8 +1117,13 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Sharing *sharing, Plan **o
   int covered = 0;
   // Every page a sequence reads must be a real block of the arena: the reference would throw
   // (ArrayIndexOutOfBounds) where a kernel would read out of bounds.
+  auto check_keys = [&](int b, int n) -> nva_status {
+    if (n <= kMaxKeys) return NVA_OK;
+    return fail(ctx, NVA_E_UNSUPPORTED, "sequence %d sees %d keys, more than %d", b, n, kMaxKeys);
+  };
   auto check_pages = [&](int b, int klen) -> nva_status {
     if (klen <= 0) return NVA_OK;
+    if (check_keys(b, klen) != NVA_OK) return NVA_E_UNSUPPORTED;
     const int pages = (int)(((int64_t)klen + key.block_size - 1) / key.block_size);
     if (pages > ctx->bt_stride)
       return fail(ctx, NVA_E_ARG, "sequence %d needs %d pages but its block table has %d", b,
@@ -1151,6 +1159,7 @@ nva_status get_plan(nva_ctx *ctx, const PlanKey &key, Sharing *sharing, Plan **o
       if ((int64_t)start + len > key.kv_rows)
         return fail(ctx, NVA_E_ARG, "sequence %d reads encoder rows [%d, %lld) of %lld", b, start,
                     (long long)start + len, (long long)key.kv_rows);
+      if (check_keys(b, len) != NVA_OK) return NVA_E_UNSUPPORTED;
       covered += n;
       if (n == 0) continue;
       if (!spans.empty()) {

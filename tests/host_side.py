@@ -373,6 +373,39 @@ def plan_time():
     lib.nva_ctx_destroy(ctx)
 
 
+def most_keys():
+    """Key counts from which the kernels' 32-bit key numbers would pass 2^31 are refused, whatever the
+    pages and pools hold; the longest below are planned."""
+    ctx = context()
+    limit = 2 ** 31 - 1 - 8192
+    for keys, want in ((2 ** 31 - 1, N.NVA_E_UNSUPPORTED), (limit + 1, N.NVA_E_UNSUPPORTED),
+                       (limit, N.NVA_OK)):
+        for new in (1, 3):
+            step = Step(2, 64, 0, new, block=1 << 20, heads=(2, 1, 64))
+            step.desc.write_kv = 0
+            step.num_blocks = 1
+            step.table = np.zeros((2, 2048), np.int32)
+            step.context_lens[0] = keys
+            step.cu_k[1:] = [keys, min(keys + 64 + new, 2 ** 31 - 1)]
+            step.groups = (N.PrefixGroup * 1)(N.PrefixGroup(0, 1, keys - new))
+            st, kv = step.arena(ctx)
+            assert st == N.NVA_OK
+            assert step.set(ctx) == N.NVA_OK
+            assert step.attend(ctx, kv) == want, (keys, new)
+            assert step.share(ctx) == N.NVA_OK
+            before = stub.stub_launches()
+            assert step.attend(ctx, kv) == want, (keys, new)
+            step.enc_start, step.enc_len = i32([0, 5]), i32([keys, 60])
+            assert step.encode(ctx) == N.NVA_OK
+            p = step.aligned()
+            got = lib.nva_cross_attention_forward(ctx, ctypes.byref(step.cross), p, p, p, 2 ** 33, 64,
+                                                  step.tokens, p)
+            assert got == want, (keys, new, got)
+            assert want == N.NVA_OK or stub.stub_launches() == before
+            lib.nva_kv_destroy(kv)
+    lib.nva_ctx_destroy(ctx)
+
+
 if __name__ == "__main__":
     globals()[sys.argv[2]]()
     print("ok", flush=True)

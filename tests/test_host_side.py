@@ -38,3 +38,7 @@ def test_shared_plans_that_do_not_fit_the_work_area_are_read_apart(stand_in):
 
 def test_planning_spans_costs_no_more_than_rows(stand_in):
     run(stand_in, "plan_time")
+
+
+def test_key_counts_beyond_the_kernels_are_refused(stand_in):
+    run(stand_in, "most_keys")
