@@ -342,6 +342,7 @@ nva_status no_memory(nva_ctx *ctx) {
 }
 
 nva_status hip_fail(nva_ctx *ctx, hipError_t e, const char *what) {
+  (void)hipGetLastError();  // reported here, it must not surface at a later launch check
   return fail(ctx, e == hipErrorOutOfMemory ? NVA_E_OOM : NVA_E_HIP, "%s: %s", what,
               hipGetErrorString(e));
 }
@@ -2406,7 +2407,6 @@ nva_status nva_kv_create(nva_ctx *ctx, int num_layers, int num_blocks, int block
     if (e == hipSuccess) e = hipMemsetAsync(pk, 0, bytes, ctx->stream);
     if (e == hipSuccess) e = hipMemsetAsync(pv, 0, bytes, ctx->stream);
     if (e != hipSuccess) {
-      (void)hipGetLastError();  // a failed allocation must not surface at a later launch check
       if (pk) (void)hipFree(pk);
       if (pv) (void)hipFree(pv);
       nva_kv_destroy(kv);

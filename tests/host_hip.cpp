@@ -15,7 +15,7 @@ struct Dim3 {
 constexpr int kOk = 0, kOutOfMemory = 2;
 long host_left = -1, device_left = -1;  // allocations until they fail; < 0: never
 long launches = 0;
-int capturing = 0;
+int capturing = 0, last_error = kOk;
 bool spent(long &left) { return left >= 0 && (left == 0 || left-- == 0); }
 struct Config {
   Dim3 grid, block;
@@ -75,11 +75,15 @@ int hipGetDevice(int *d) { return *d = 0, kOk; }
 int hipSetDevice(int) { return kOk; }
 int hipGetDevicePropertiesR0600(void *, int) { return 1; }  // the library's defaults
 const char *hipGetErrorString(int e) { return e == kOutOfMemory ? "out of memory" : "error"; }
-int hipGetLastError() { return kOk; }
+int hipGetLastError() {  // of a call that failed, once
+  const int e = last_error;
+  last_error = kOk;
+  return e;
+}
 
 static int allocate(void **p, size_t n) {
   *p = nullptr;
-  if (spent(device_left)) return kOutOfMemory;
+  if (spent(device_left)) return last_error = kOutOfMemory;
   *p = calloc(1, n ? n : 1);
   return *p ? kOk : kOutOfMemory;
 }
