@@ -2579,6 +2579,8 @@ nva_status nva_step_set(nva_ctx *ctx, int is_prefill, const int32_t *cu_q, const
   if (is_prefill && !cu_k) return fail(ctx, NVA_E_ARG, "prefill step needs cuSeqlensK");
   if (block_tables && bt_stride <= 0 && num_seqs > 0)
     return fail(ctx, NVA_E_ARG, "block tables need bt_stride > 0");
+  if (is_prefill && (cu_q[0] < 0 || cu_k[0] < 0))
+    return fail(ctx, NVA_E_ARG, "cu_seqlens must not start below 0");
   for (Plan *p : ctx->plans) p->valid = false;
   ctx->tile_choices.clear();
   ctx->groups.clear();

@@ -406,6 +406,25 @@ def most_keys():
     lib.nva_ctx_destroy(ctx)
 
 
+def rows_before_the_first():
+    """A prefill step whose first row or key is negative would read in front of q, or of the dense k and
+    v: it is refused, and the step set before stays."""
+    ctx = context()
+    step = Step(3, 128, 10, 4)
+    st, kv = step.arena(ctx)
+    assert st == step.set(ctx) == step.attend(ctx, kv) == N.NVA_OK
+    for cu in ("cu_q", "cu_k"):
+        for first in (-1, -2 ** 31):
+            bad = Step(3, 128, 10, 4)
+            getattr(bad, cu)[0] = first
+            before = stub.stub_launches()
+            assert bad.set(ctx) == N.NVA_E_ARG, (cu, first)
+            assert stub.stub_launches() == before
+            assert step.attend(ctx, kv) == N.NVA_OK
+    lib.nva_kv_destroy(kv)
+    lib.nva_ctx_destroy(ctx)
+
+
 if __name__ == "__main__":
     globals()[sys.argv[2]]()
     print("ok", flush=True)

@@ -42,3 +42,7 @@ def test_planning_spans_costs_no_more_than_rows(stand_in):
 
 def test_key_counts_beyond_the_kernels_are_refused(stand_in):
     run(stand_in, "most_keys")
+
+
+def test_rows_and_keys_before_the_first_are_refused(stand_in):
+    run(stand_in, "rows_before_the_first")
