@@ -16,6 +16,10 @@
  *     q/out [tokens, num_heads, head_dim], k/v [tokens, num_kv_heads, head_dim].
  *     Step metadata (cu_seqlens, slots, tables, positions) are HOST pointers; they are copied
  *     to the device once per nva_step_set() and shared by every layer of that step.
+ *   - Values that are not finite reach what sees them alone: an infinity or NaN in a V row is in the
+ *     results of the queries that see the key, in that dim, as in the sum of the definition.  (A
+ *     weight that is 0, for a score of -infinity or one some 87 below the largest, makes NaN of an
+ *     infinity: 0 * inf.)
  *   - A forward call with num_tokens == 0 (or rows == 0) does nothing and succeeds; its tensor
  *     pointers may then be NULL (the reference returns an empty tensor).
  *   - All work is enqueued on the context's HIP stream and is asynchronous unless stated.
@@ -49,7 +53,7 @@ enum {
   NVA_E_NO_STEP = 6,    /* no step metadata set (Java: NullPointerException on Context) */
   NVA_E_HIP = 7,        /* HIP runtime error or no usable device */
   NVA_E_OOM = 8,        /* device, pinned or host memory ran out */
-  NVA_E_UNSUPPORTED = 9 /* shape this build has no kernel for (e.g. head_dim % 4 != 0) */
+  NVA_E_UNSUPPORTED = 9 /* shape this build has no kernel for (e.g. head_dim % 4 != 0, or 2^31 keys) */
 };
 
 typedef struct nva_ctx nva_ctx;
@@ -244,14 +248,19 @@ typedef struct nva_prefix_group {
 /* Finds them: groups (room for num_seqs / 2) receives the runs of adjacent sequences, in order, that
  * save the most page reads over the tables, *num_groups their number.  Only full pages of cached
  * tokens count: cached_tokens[b] is context_lens[b] - 1 in a decode step, num_cached_tokens in a
- * prefill.  Pure host code. */
+ * prefill.  Runs are of one level: sequences that share a prefix but do not lie side by side are not
+ * joined, and a prompt above several documents is read once per document's run, or each document once
+ * per sequence, whichever costs fewer pages.  Pure host code. */
 nva_status nva_find_shared_prefixes(const int32_t *block_tables, int num_seqs, int bt_stride,
                                     const int32_t *cached_tokens, int block_size,
                                     nva_prefix_group *groups, int *num_groups);
 /* Attention of a batch that shares prefixes: from this call to the next nva_step_set (or call), every
  * attention call over the step's pages reads the tokens of a group once for all rows of its
  * sequences and joins the result with each sequence's own keys; outputs agree with those of the
- * separate reads to fp32 rounding.  Layers with a sliding window, which see too little of a prefix,
+ * separate reads to fp32 rounding.  (Prefixes of many columns, rows times heads of a KV head, run on the
+ * prefill tiles, whose products of split fp16 operands are as exact as fp32 sums, in decode steps too.)
+ * What is shared is chosen by estimated time: a step can take up to 1.12 times as long as without groups,
+ * where there is little to gain.  Layers with a sliding window, which see too little of a prefix,
  * are computed as before, and groups that would not gain are read apart: one row, or prefill chunks
  * that fill their query tiles.  Prefill steps of few tokens run row by row.  Joining takes more
  * partials: in the no-allocation form, groups whose work its array does not hold are read apart.

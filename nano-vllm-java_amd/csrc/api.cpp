@@ -528,8 +528,10 @@ int64_t mixed_tile_cus(int num_cus, double row_bytes, double tile_flops, int hea
 
 // Whether the rows (and items) of a step run beside its span tiles, on a share of the CUs as in a
 // mixed step, or behind them with all CUs for each.  Beside them the longer of the two counts, but
-// 8 us more go to the events; span tiles on all CUs reach 170 / 270 / 170 / 170 TFLOP/s at d = 64 /
-// 128 / 256 / 512, and the rows start 5 us later.
+// 8 us more go to the events; behind them span tiles on all CUs count 170 / 270 / 170 / 170 TFLOP/s at
+// d = 64 / 128 / 256 / 512, and the rows start 5 us later.  (Rates that choose rightly, over pairs without
+// idle columns, not tile_rate()'s: at d = 512 the tiles alone run at 85-160.  With tile_rate()'s 100 there,
+// eleven of 40 drawn steps of 12-260 rows change sides, six to 0.84-0.96 times and five to 1.03-1.13.)
 bool rows_beside_tiles(int num_cus, double row_bytes, double tile_flops, int head_dim) {
   double beside = 0.0;
   mixed_tile_cus(num_cus, row_bytes, tile_flops, head_dim, false, &beside);

@@ -8,8 +8,8 @@
 //
 // Span tiles (SPAN): the queries of a tile are the columns of a span, (row, query head) pairs that all
 // see the segment's keys, so nothing is masked but the keys' end; everything else is alike.  Six prompts of
-// 130-900 tokens over 2000-9000 encoder rows (32 q / 8 KV heads, d = 128) run at 309 TFLOP/s, 48 encoder
-// passages of 9-512 rows (12 heads, d = 64) at 155.
+// 130-900 tokens over 2000-9000 encoder rows (32 q / 8 KV heads, d = 128) run at 303-309 TFLOP/s, 48 encoder
+// passages of 9-512 rows (12 heads, d = 64) at 140-155.
 //
 // Each fp32 operand (q, k, v and the probabilities) is split into two scaled fp16 parts and each
 // product taken as three fp16 ones with fp32 sums (split_f16.h), at 5.3 times the rate of

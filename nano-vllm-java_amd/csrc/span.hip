@@ -14,7 +14,7 @@
 // any value; 155 TFLOP/s) keep up with HBM to 32 columns.  Measured: 128 single tokens over 300-1500
 // encoder rows (16 heads, d = 64, 0.96 GB) 172 us, 5.6 TB/s; 40 x 5 beams over 500-4000 rows (32 q / 8
 // KV heads, d = 128, 0.73 GB) 151 us, 4.9 TB/s.  Short runs of more columns are bound by latency (33 rows
-// of 4 heads under 6144 tokens, d = 256: 26 us, 40% of the matrix unit, 5.5 turns a wave).  One workgroup
+// of 4 heads under 6144 tokens, d = 256: 26 us, 36% of the matrix unit, 5.5 turns a wave).  One workgroup
 // of 4 waves per (item, KV head, head group); each wave takes 16-key blocks of the item in turn, so that
 // 4 waves read 64 consecutive keys at a time, with no barrier and no LDS until the end:
 //   S^T[key][col] = K Q^T    D/4 v_mfma_f32_16x16x4_f32 per block and 16 columns: at step 4v + c
