@@ -59,6 +59,9 @@ enum {
 typedef struct nva_ctx nva_ctx;
 typedef struct nva_kv nva_kv;
 typedef struct nva_rope nva_rope;
+typedef struct nva_tables nva_tables;
+typedef struct nva_kv4 nva_kv4;
+typedef struct nva_linear4 nva_linear4;
 
 /* Constructor arguments of Attention(numHeads, headDim, scale, numKvHeads, slidingWindow,
  * kvLayerIndex, writeKv), Attention.java:108-125.  sliding_window <= 0 means full context. */
@@ -157,6 +160,41 @@ nva_status nva_rope_create(nva_ctx *ctx, const float *cos_sin, int max_pos, int 
 nva_status nva_rope_create_theta(nva_ctx *ctx, int head_size, int rotary_dim, int max_pos,
                                  float base, nva_rope **out);
 nva_status nva_rope_destroy(nva_rope *rope);
+
+/* Rotary positions beyond the reference's: the first rotary_dim dims of a head turn (the others pass
+ * through), paired as halves (i, i + rotary_dim / 2) or, with interleaved, as neighbours (2i, 2i + 1);
+ * pair i turns by position * f_i, where f_i = base^(-2i / rotary_dim), scaled for contexts beyond the
+ * trained one of original_max_pos positions:
+ *   NVA_ROPE_NONE    as it is
+ *   NVA_ROPE_LINEAR  f_i / factor
+ *   NVA_ROPE_NTK     base * factor^(rotary_dim / (rotary_dim - 2)) in place of base
+ *   NVA_ROPE_YARN    f_i of pairs that turn more than `high` times in the trained context, f_i / factor
+ *                    of those that turn fewer than `low` times, and a mix that is linear in the pair's
+ *                    number between; cos and sin are multiplied by 0.1 ln(factor) + 1
+ *   NVA_ROPE_BANDS   the same two ends, mixed by the pair's turns, cos and sin as they are
+ * amplitude, if not 0, is the factor of cos and sin in place of those.  Frequencies and angles are
+ * computed in 64 bits, the table is fp32 (rotary_dim * max_pos * 4 bytes).  Every call that takes an
+ * nva_rope takes these; one whose halves are paired over the whole head runs the same kernels as the
+ * reference's. */
+enum {
+  NVA_ROPE_NONE = 0,
+  NVA_ROPE_LINEAR = 1,
+  NVA_ROPE_NTK = 2,
+  NVA_ROPE_YARN = 3,
+  NVA_ROPE_BANDS = 4
+};
+typedef struct nva_rope_desc {
+  int32_t head_size, rotary_dim;  /* 2 <= rotary_dim <= head_size, both even */
+  int32_t max_pos;
+  int32_t interleaved;
+  float base;                     /* > 1 */
+  int32_t scaling;                /* NVA_ROPE_* */
+  float factor;                   /* >= 1 (not used by NVA_ROPE_NONE) */
+  int32_t original_max_pos;       /* > 0 (YARN and BANDS) */
+  float low, high;                /* 0 < low < high, turns (YARN and BANDS) */
+  float amplitude;                /* 0: the scaling's own */
+} nva_rope_desc;
+nva_status nva_rope_create_scaled(nva_ctx *ctx, const nva_rope_desc *desc, nva_rope **out);
 
 /* ------------------------------------------------------------------ step metadata
  * Context.set(isPrefill, cuSeqlensQ, cuSeqlensK, maxSeqlenQ, maxSeqlenK, slotMapping,
@@ -280,6 +318,48 @@ nva_status nva_step_set_encoder(nva_ctx *ctx, const int32_t *kv_start, const int
  * Norms.java:275, rounded with Math.round as at Norms.java:317).  Valid after nva_step_set; without
  * memory for them the context has no step left. */
 nva_status nva_step_positions(nva_ctx *ctx, const float *positions, int num_tokens);
+/* Steps whose metadata is built on the device.  nva_tables holds, for up to max_seqs sequences (rows,
+ * at most 4000) of up to max_tokens tokens each, the block tables [max_seqs, ceil(max_tokens /
+ * block_size)] (-1 behind a row's blocks), the lengths, and a stack of free blocks: block ids
+ * 0 .. num_blocks - 1, or the num_blocks ids of `pages` (host array, distinct, >= 0), the first of them
+ * handed out first.  A block belongs to one row; sharing stays with the engine's block manager.
+ *
+ * nva_step_extend makes the context's next step: of row b the first keep[b] tokens stay (0 <= keep[b]
+ * <= its length; keep NULL: all) and new_tokens[b] follow, for the rows b < num_seqs (other rows are
+ * left alone).  Blocks behind those that stay go back to the stack, the last row's last one first;
+ * blocks for the tokens that follow are taken in order, so that keeping less and extending again gives
+ * the same blocks.  keep[b] = 0 ends a sequence, with new_tokens[b] > 0 another takes its row.  keep and
+ * new_tokens are DEVICE arrays of num_seqs int32; num_tokens (at most max_step_tokens) is the number of
+ * rows of the step's q, k and v, of which rows behind the new tokens are padding: their slot is -1,
+ * their position 0 and their attention 0.  max_new bounds each new_tokens[b].  The call enqueues work
+ * and does not wait; it may be captured, and replays act on the lengths they find.
+ *
+ * A step that asks for more than there is changes nothing and has no tokens: every row is padding.
+ * nva_tables_status (which waits) tells: status[0] is 0, or 1 for a row (status[1]) whose keep or
+ * new_tokens is out of range, 2 for more than num_tokens new tokens (status[1] of them, at most INT32_MAX), 3 for more
+ * blocks (status[1]) than are free; status[2] is the number of free blocks after the call.
+ *
+ * The step serves nva_rope_forward and the calls over the 4-bit cache; the other attention calls need
+ * nva_step_set (NVA_E_NO_STEP).  Its tables must outlive its use, captured graphs included. */
+nva_status nva_tables_create(nva_ctx *ctx, int max_seqs, int max_tokens, int max_step_tokens,
+                             int num_blocks, int block_size, const int32_t *pages,
+                             nva_tables **out);
+nva_status nva_tables_destroy(nva_tables *tables);
+/* Device arrays (int32): the block tables, lengths [max_seqs], and of the last step the slots and
+ * positions [max_step_tokens] (num_tokens of them set) and row offsets [max_seqs + 1] (num_seqs + 1
+ * set). */
+enum {
+  NVA_TABLES_BLOCKS = 0,
+  NVA_TABLES_LENS = 1,
+  NVA_TABLES_SLOTS = 2,
+  NVA_TABLES_POSITIONS = 3,
+  NVA_TABLES_CU_Q = 4
+};
+nva_status nva_tables_array(nva_tables *tables, int which, void **ptr, int64_t *count);
+nva_status nva_tables_status(nva_tables *tables, int32_t *status);
+nva_status nva_step_extend(nva_ctx *ctx, nva_tables *tables, const int32_t *keep,
+                           const int32_t *new_tokens, int num_seqs, int num_tokens, int max_new);
+
 /* Context.clear(), Context.java:61-74. */
 nva_status nva_step_clear(nva_ctx *ctx);
 
@@ -399,6 +479,75 @@ nva_status nva_qkv_norm_rope_attention_forward(nva_ctx *ctx, nva_kv *kv, const n
                                                const nva_attn_desc *desc, const float *qkv,
                                                int num_tokens, float *q_out, float *k_out,
                                                float *out);
+
+/* ------------------------------------------------------------------ 4 bits
+ * The 4-bit form: 32 values along a row as codes of 4 bits beside one scale byte.  A code is a sign
+ * (bit 3) and one of {0, 0.5, 1, 1.5, 2, 3, 4, 6}; scale byte e + 127 stands for 2^e, the smallest with
+ * -127 <= e <= 125 and every magnitude at most 6 * 2^e, so larger magnitudes than 6 * 2^125 become that.
+ * Each value goes to the nearest code, ties to the even one.  A block that holds an infinity or NaN has
+ * scale byte 255 and is NaN as a whole.  (The e2m1 elements and e8m0 scales of the OCP microscaling
+ * formats, which the matrix cores' converters read.)  Reading uses any scale byte.
+ *
+ * nva_quantize4: x [rows, n] (device, n % 32 == 0, 16-byte aligned) to codes [rows, n / 2] (value 2j in the low bits of
+ * byte j) and scales [rows, n / 32]. */
+nva_status nva_quantize4(nva_ctx *ctx, const float *x, int64_t rows, int n, uint8_t *codes,
+                         uint8_t *scales);
+
+/* A KV arena in the 4-bit form: 34 bytes per 64 values against 256.  Arguments as nva_kv_create;
+ * block_size % 32 == 0, head dims 64, 128, 256 or 512.  Blocks are zero-filled.
+ * nva_kv4_layer gives a layer's buffer (opaque layout) and its bytes. */
+nva_status nva_kv4_create(nva_ctx *ctx, int num_layers, int num_blocks, int block_size,
+                          int num_kv_heads, const int32_t *head_dims, const uint8_t *allocate,
+                          nva_kv4 **out);
+nva_status nva_kv4_destroy(nva_kv4 *kv);
+nva_status nva_kv4_blocks_that_fit(nva_ctx *ctx, int num_layers, int block_size, int num_kv_heads,
+                                   const int32_t *head_dims, const uint8_t *allocate,
+                                   float fraction, int *blocks, int64_t *free_bytes);
+nva_status nva_kv4_layer(nva_kv4 *kv, int layer, void **pages, int64_t *bytes);
+/* Rows of k and v [num_rows, num_kv_heads, head_dim] to the slots (device int32) of a layer, or the
+ * values the slots hold to k and v (either may be NULL when reading).  Slots outside the arena are
+ * skipped, and read as zeros.  Of rows written to one slot in one call any may win, dim by dim. */
+nva_status nva_kv4_write_rows(nva_kv4 *kv, int layer, const int32_t *slots, const float *k,
+                              const float *v, int num_rows);
+nva_status nva_kv4_read_rows(nva_kv4 *kv, int layer, const int32_t *slots, float *k, float *v,
+                             int num_rows);
+
+/* nva_attention_forward over the 4-bit arena: the step's k and v are rounded into their slots, then
+ * every query attends over its sequence's keys as they are held, those of this step included.  A step of
+ * nva_step_set (decode, or prefill with block tables) or of nva_step_extend.  q k^T and p v are fp32
+ * products of the held values (in three exact parts on the matrix cores), sums and softmax are fp32.
+ * num_heads / num_kv_heads may be any number.  Prefix groups are not used: every sequence's keys are
+ * read for it.  A step of nva_step_extend may be captured once a step at least as large has run on the
+ * context (NVA_E_ARG otherwise); replays then serve the lengths of the replayed extends.  The results
+ * do not depend on how a step is cut into workgroups beyond fp32 rounding.  Kernel stats: "store4",
+ * "attention4", "merge4". */
+nva_status nva_attention4_forward(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc *desc,
+                                  const float *q, const float *k, const float *v, int num_tokens,
+                                  float *out);
+/* nva_norm_rope_attention_forward and nva_qkv_norm_rope_attention_forward over the 4-bit arena. */
+nva_status nva_norm_rope_attention4_forward(nva_ctx *ctx, nva_kv4 *kv, const nva_rope *rope,
+                                            const nva_rms_norm *q_norm, const nva_rms_norm *k_norm,
+                                            const nva_rms_norm *v_norm, const nva_attn_desc *desc,
+                                            const float *q, const float *k, const float *v,
+                                            int num_tokens, float *q_out, float *k_out,
+                                            float *out);
+nva_status nva_qkv_norm_rope_attention4_forward(nva_ctx *ctx, nva_kv4 *kv, const nva_rope *rope,
+                                                const nva_rms_norm *q_norm,
+                                                const nva_rms_norm *k_norm,
+                                                const nva_rms_norm *v_norm,
+                                                const nva_attn_desc *desc, const float *qkv,
+                                                int num_tokens, float *q_out, float *k_out,
+                                                float *out);
+
+/* nva_linear_forward with a weight in the 4-bit form: nva_linear4_create lays codes [out, in / 2] and
+ * scales [out, in / 32] (device, as nva_quantize4 writes them; in % 32 == 0) out in memory of its own;
+ * forward computes y [rows, out] = x [rows, in] W^T (+ bias [out]) from it, x 16-byte aligned.  Products
+ * are of x in three exact parts with the held values, sums are fp32. */
+nva_status nva_linear4_create(nva_ctx *ctx, const uint8_t *codes, const uint8_t *scales, int out,
+                              int in, nva_linear4 **linear);
+nva_status nva_linear4_destroy(nva_linear4 *linear);
+nva_status nva_linear4_forward(nva_ctx *ctx, const nva_linear4 *linear, const float *x, int rows,
+                               const float *bias, float *y);
 
 #ifdef __cplusplus
 }

@@ -29,10 +29,7 @@
 #include <string>
 #include <vector>
 
-#include "../../include/nva.h"
-#include "nva_internal.h"
-
-using namespace nva;
+#include "context.h"
 
 // Device scratch of nva_attention_forward_noalloc: the plan lists, split partials and shared-KV
 // gather rows of one call.  One copy per device, held from the library's load on that device
@@ -88,394 +85,9 @@ char *scratch_address(int device, hipError_t *err) {
 
 ScratchTag &scratch_tag(int device, bool cross) { return g_scratch[device].tags[cross ? 1 : 0]; }
 
-size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
-
-
-// Grow-only device buffer.
-struct DevBuf {
-  void *ptr = nullptr;
-  size_t cap = 0;
-  hipError_t reserve(size_t bytes) {
-    if (bytes <= cap) return hipSuccess;
-    if (ptr) {
-      hipError_t e = hipFree(ptr);
-      if (e != hipSuccess) return e;
-      ptr = nullptr;
-      cap = 0;
-    }
-    size_t want = std::max<size_t>(bytes, 4096);
-    hipError_t e = hipMalloc(&ptr, want);
-    if (e == hipSuccess) cap = want;
-    return e;
-  }
-  void release() {
-    if (ptr) (void)hipFree(ptr);
-    ptr = nullptr;
-    cap = 0;
-  }
-};
-
-// Grow-only pinned host buffer whose last upload is tracked by an event, so it is only
-// overwritten once the device has consumed it.
-struct Staging {
-  void *ptr = nullptr;
-  size_t cap = 0;
-  hipEvent_t done = nullptr;
-  bool pending = false;
-  hipError_t wait() {
-    if (pending) {
-      pending = false;
-      return hipEventSynchronize(done);
-    }
-    return hipSuccess;
-  }
-  hipError_t reserve(size_t bytes) {
-    hipError_t e = wait();
-    if (e != hipSuccess) return e;
-    if (!done) {
-      e = hipEventCreateWithFlags(&done, hipEventDisableTiming);
-      if (e != hipSuccess) return e;
-    }
-    if (bytes <= cap) return hipSuccess;
-    if (ptr) (void)hipHostFree(ptr);
-    ptr = nullptr;
-    cap = 0;
-    size_t want = std::max<size_t>(bytes, 4096);
-    e = hipHostMalloc(&ptr, want, hipHostMallocDefault);
-    if (e == hipSuccess) cap = want;
-    return e;
-  }
-  hipError_t upload(DevBuf &dst, size_t bytes, hipStream_t s) {
-    hipError_t e = hipMemcpyAsync(dst.ptr, ptr, bytes, hipMemcpyHostToDevice, s);
-    if (e != hipSuccess) return e;
-    e = hipEventRecord(done, s);
-    if (e == hipSuccess) pending = true;
-    return e;
-  }
-  void release() {
-    if (pending) (void)hipEventSynchronize(done);
-    pending = false;
-    if (ptr) (void)hipHostFree(ptr);
-    if (done) (void)hipEventDestroy(done);
-    ptr = nullptr;
-    done = nullptr;
-    cap = 0;
-  }
-};
-
-// A work plan: the flattened row / merge / tile lists for one attention configuration of the
-// current step, built on the host and uploaded once, then reused by every layer with the same
-// configuration.
-struct PlanKey {
-  int window, mfma, fp32_tiles, tile_q, wg_per_item, blocks_per_cu;
-  int tile_groups;             // prefill grid height: KV heads x query-head groups
-  int tokens;                  // rows of q / out in the forward call
-  int paged;                   // keys through block tables (else dense k/v rows)
-  int block_size, num_blocks;  // arena geometry the tables are checked against
-  int head_dim, num_heads, num_kv_heads;  // size the work of a mixed plan's two kernels
-  int cross = 0;               // over the encoder's rows instead of the sequence's own keys
-  int64_t kv_rows = 0;         // cross: rows of the encoder pool
-  int item_heads = 0;          // query heads of a column group of a span item (0: no span kernel)
-  int split_tile_q = 0;        // queries of a split tile
-  int tile_heads = 0;          // and of a span tile (0: no tile kernel for this head dim)
-  int span_tile_cols = 0;      // columns of a span tile
-  int span_blocks_per_cu = 0;
-  bool operator==(const PlanKey &o) const {
-    return cross == o.cross && kv_rows == o.kv_rows && item_heads == o.item_heads &&
-           split_tile_q == o.split_tile_q && tile_heads == o.tile_heads &&
-           span_tile_cols == o.span_tile_cols &&
-           span_blocks_per_cu == o.span_blocks_per_cu && window == o.window && mfma == o.mfma &&
-           fp32_tiles == o.fp32_tiles && tile_q == o.tile_q &&
-           head_dim == o.head_dim && num_heads == o.num_heads && num_kv_heads == o.num_kv_heads &&
-           wg_per_item == o.wg_per_item && blocks_per_cu == o.blocks_per_cu &&
-           tile_groups == o.tile_groups && tokens == o.tokens && paged == o.paged &&
-           block_size == o.block_size && num_blocks == o.num_blocks;
-  }
-};
-
-struct Plan {
-  PlanKey key{};
-  bool valid = false;
-  int num_rows = 0, num_merge = 0, num_tiles = 0, num_parts = 0;
-  int num_slots = 0;  // prefill stream-K slots (grid x)
-  int num_spans = 0, max_cols = 0;                // span items, and the most columns of one
-  int num_span_tiles = 0, num_span_slots = 0;     // span tiles and their stream-K slots
-  int max_parts = 0;  // most partials any merged row has
-  bool beside = false;     // rows and items run on the side stream, beside the tiles
-  bool covers_all = true;  // every output row is written by some kernel
-  size_t off_rows = 0, off_merge = 0, off_tiles = 0, off_slots = 0;
-  size_t off_spans = 0, off_span_tiles = 0, off_span_slots = 0, off_row_part = 0;
-  std::vector<char> host;  // the packed lists at the offsets above
-  uint64_t id = 0;         // unique per build (identifies the plan held in a scratch array)
-  bool on_device = false;  // host bytes uploaded to dev
-  DevBuf dev;
-  Staging stage;
-};
-
-// Workspace of the no-allocation entry point: the plan, the split partials and the shared-KV
-// gather rows of one call live in fixed regions of a device's static scratch array instead of
-// the context's grow-only buffers.  base is that device's address of the array (from
-// hipGetSymbolAddress), used == bytes already taken (gather rows, at the front).
-struct Scratch {
-  char *base = nullptr;
-  size_t used = 0;
-};
-
-struct PendingTiming {
-  const char *name, *variant;  // variant: null, or the second entry that counts it
-  hipEvent_t start, stop;
-};
-
-// Which tile kernel a layer configuration's prefill runs on in the current step.
-struct TileChoice {
-  int head_dim, num_heads, num_kv_heads, window;
-  int tile_heads;  // of its spans (0: no prefix is shared)
-  bool fp32;
-};
-
-struct KernelStat {
-  int64_t launches = 0;
-  double ms = 0.0;
-};
-
 }  // namespace
 
-struct nva_ctx {
-  int device = 0;
-  int num_cus = 256;
-  hipStream_t own_stream = nullptr;
-  hipStream_t side_stream = nullptr;  // decode rows of a mixed step run here, beside the tiles
-  hipEvent_t fork_ev = nullptr, join_ev = nullptr;
-  hipStream_t stream = nullptr;
-  std::string err;
-
-  // Step metadata (host copies) and its device mirror.
-  bool has_step = false;
-  bool is_prefill = false;
-  int num_seqs = 0;
-  int num_tokens = 0;
-  int max_q = 0, max_k = 0;
-  int bt_stride = 0;
-  int num_slots = 0;
-  int64_t slot_max = -1;  // largest slot of the step (negative slots are skipped)
-  bool has_cu = false, has_slots = false, has_ctx_lens = false, has_tables = false,
-       has_pos = false;
-  std::vector<int32_t> cu_q, cu_k, slots, ctx_lens, tables, seq_ids, pos;
-  // Shared prefixes of the step's sequences, and the page size their tables were compared at (0:
-  // not yet).
-  std::vector<nva_prefix_group> groups;
-  int groups_block_size = 0;
-  // The encoder rows each sequence's cross attention reads.
-  bool has_encoder = false;
-  std::vector<int32_t> enc_start, enc_len;
-  DevBuf d_step;
-  Staging step_stage;
-  size_t off_cu_q = 0, off_cu_k = 0, off_slots = 0, off_ctx = 0, off_tables = 0, off_pos = 0;
-
-  std::vector<Plan *> plans;
-  std::vector<TileChoice> tile_choices;
-  DevBuf d_part;     // split partials
-  DevBuf d_q_rot;    // fused path scratch for rotated q
-  DevBuf d_k_rot;    // fused path scratch for rotated k
-  DevBuf d_v_norm;   // fused path scratch for normalised v (dense prefill with a v norm)
-  DevBuf d_lin;      // split-K partial sums of the linear kernel
-  DevBuf d_gather;   // shared-KV gather [2, T, Hkv, d]
-
-  // One word the store / RoPE kernel writes the XCD of its last workgroup to, read by the decode
-  // launch that follows (null if its allocation failed: no rotation).
-  int32_t *xcd_hint = nullptr;
-
-  // This device's address of the no-allocation scratch array (null if the lookup failed).
-  char *scratch = nullptr;
-  hipError_t scratch_err = hipSuccess;
-
-  // Prefill occupancy (resident workgroups per CU) by (head dim, heads per workgroup), queried
-  // once on this context's device.
-  std::map<int, int> occupancy;
-
-  bool timing = false;
-  std::vector<PendingTiming> pending;
-  std::vector<hipEvent_t> event_pool;
-  std::map<std::string, KernelStat> stats;
-
-  const int32_t *dev_i32(size_t off) const {
-    return reinterpret_cast<const int32_t *>(static_cast<char *>(d_step.ptr) + off);
-  }
-};
-
-struct nva_kv {
-  nva_ctx *ctx = nullptr;
-  int num_layers = 0, num_blocks = 0, block_size = 0, num_kv_heads = 0;
-  std::vector<int32_t> head_dims;
-  std::vector<float *> k, v;
-  std::vector<int64_t> bytes;
-};
-
-struct nva_rope {
-  nva_ctx *ctx = nullptr;
-  int max_pos = 0, head_size = 0;
-  float *table = nullptr;
-};
-
 namespace {
-
-nva_status fail(nva_ctx *ctx, nva_status st, const char *fmt, ...) {
-  if (ctx) {
-    char buf[512];
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(buf, sizeof(buf), fmt, ap);
-    va_end(ap);
-    try {
-      ctx->err = buf;
-    } catch (const std::exception &) {  // no memory for the text
-      ctx->err.clear();
-    }
-  }
-  return st;
-}
-
-// Host memory ran out in an entry point (no exception may leave it).
-nva_status no_memory(nva_ctx *ctx) {
-  ctx->err = "out of memory";  // short: needs no allocation
-  return NVA_E_OOM;
-}
-
-nva_status hip_fail(nva_ctx *ctx, hipError_t e, const char *what) {
-  (void)hipGetLastError();  // reported here, it must not surface at a later launch check
-  return fail(ctx, e == hipErrorOutOfMemory ? NVA_E_OOM : NVA_E_HIP, "%s: %s", what,
-              hipGetErrorString(e));
-}
-
-#define HIP_TRY(ctx, expr, what)                \
-  do {                                          \
-    hipError_t e_ = (expr);                     \
-    if (e_ != hipSuccess) return hip_fail(ctx, e_, what); \
-  } while (0)
-
-bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-// Makes the context's device current for the scope of an entry point (its grow-only buffers
-// are allocated, and its occupancy queried, on that device) and restores the caller's.
-struct DeviceGuard {
-  int prev = -1;
-  explicit DeviceGuard(int device) {
-    if (hipGetDevice(&prev) != hipSuccess) prev = -1;
-    if (prev != device) (void)hipSetDevice(device);
-  }
-  explicit DeviceGuard(const nva_ctx *ctx) : DeviceGuard(ctx->device) {}
-  ~DeviceGuard() {
-    int cur = -1;
-    if (prev >= 0 && hipGetDevice(&cur) == hipSuccess && cur != prev) (void)hipSetDevice(prev);
-  }
-};
-
-int ctx_prefill_blocks_per_cu(nva_ctx *ctx, int head_dim, int hpw, bool fp32) {
-  const int key = (head_dim * 16 + hpw) * 2 + (fp32 ? 1 : 0);
-  auto it = ctx->occupancy.find(key);
-  if (it != ctx->occupancy.end()) return it->second;
-  const int n = fp32 ? prefill_fp32_blocks_per_cu(head_dim, hpw) : prefill_blocks_per_cu(head_dim, hpw);
-  ctx->occupancy[key] = n;
-  return n;
-}
-
-int ctx_span_blocks_per_cu(nva_ctx *ctx, int head_dim) {
-  const int key = -head_dim;  // beside the prefill kernels' keys, which are positive
-  auto it = ctx->occupancy.find(key);
-  if (it == ctx->occupancy.end())
-    it = ctx->occupancy.emplace(key, span_tile_blocks_per_cu(head_dim)).first;
-  return it->second;
-}
-
-// Timings that find no host memory are dropped: the call they time is not to fail for them.
-void give_event(nva_ctx *ctx, hipEvent_t e) {
-  try {
-    ctx->event_pool.push_back(e);
-  } catch (const std::exception &) {
-    (void)hipEventDestroy(e);
-  }
-}
-
-void add_stat(nva_ctx *ctx, const char *name, double ms) {
-  try {
-    KernelStat &s = ctx->stats[name];
-    s.launches++;
-    s.ms += ms;
-  } catch (const std::exception &) {
-  }
-}
-
-hipEvent_t take_event(nva_ctx *ctx) {
-  if (!ctx->event_pool.empty()) {
-    hipEvent_t e = ctx->event_pool.back();
-    ctx->event_pool.pop_back();
-    return e;
-  }
-  hipEvent_t e = nullptr;
-  if (hipEventCreate(&e) != hipSuccess) return nullptr;
-  return e;
-}
-
-// Brackets one kernel launch with timing events when timing is on.  A launch that one of several
-// kernels serves is counted under its own name (variant) too.
-struct Timed {
-  nva_ctx *ctx;
-  const char *name, *variant;
-  hipStream_t stream;
-  hipEvent_t start = nullptr;
-  Timed(nva_ctx *c, const char *n, hipStream_t s = nullptr, const char *v = nullptr)
-      : ctx(c), name(n), variant(v), stream(s ? s : c->stream) {
-    if (ctx->timing) {
-      start = take_event(ctx);
-      if (start) (void)hipEventRecord(start, stream);
-    }
-  }
-  void done() {
-    if (!start) return;
-    hipEvent_t stop = take_event(ctx);
-    if (!stop) return;
-    (void)hipEventRecord(stop, stream);
-    try {
-      ctx->pending.push_back({name, variant, start, stop});
-    } catch (const std::exception &) {
-      give_event(ctx, start);
-      give_event(ctx, stop);
-    }
-    start = nullptr;
-  }
-};
-
-void resolve_timings(nva_ctx *ctx) {
-  for (auto &p : ctx->pending) {
-    float ms = 0.f;
-    if (hipEventSynchronize(p.stop) == hipSuccess &&
-        hipEventElapsedTime(&ms, p.start, p.stop) == hipSuccess) {
-      for (const char *n : {p.name, p.variant})
-        if (n) add_stat(ctx, n, ms);
-    }
-    give_event(ctx, p.start);
-    give_event(ctx, p.stop);
-  }
-  ctx->pending.clear();
-}
-
-// Host time of one plan build (and its upload), kept as the "plan" entry of the kernel stats
-// when timing is on: the per-step planning cost a scheduler step pays at its first layer.
-struct HostTimed {
-  nva_ctx *ctx;
-  const char *name;
-  std::chrono::steady_clock::time_point t0;
-  bool on;
-  HostTimed(nva_ctx *c, const char *n) : ctx(c), name(n), on(c->timing) {
-    if (on) t0 = std::chrono::steady_clock::now();
-  }
-  ~HostTimed() {
-    if (!on) return;
-    const double ms =
-        std::chrono::duration<double, std::milli>(std::chrono::steady_clock::now() - t0).count();
-    add_stat(ctx, name, ms);
-  }
-};
 
 int pow2_shift(int x) {
   if (x <= 0 || (x & (x - 1))) return -1;
@@ -1835,11 +1447,6 @@ void scratch_overwritten(int device, size_t begin, size_t end) {
   }
 }
 
-bool stream_capturing(hipStream_t s) {
-  hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-  return hipStreamIsCapturing(s, &cs) == hipSuccess && cs != hipStreamCaptureStatusNone;
-}
-
 // Whether a plan's call fits the array and, under stream capture, finds its plan there and leaves the
 // other kind's alone (a graph of both would overwrite that plan at every replay).
 nva_status noalloc_fits(nva_ctx *ctx, const Plan &plan, const nva_attn_desc &d, size_t gather) {
@@ -2072,6 +1679,15 @@ nva_status check_slots(nva_ctx *ctx, nva_kv *kv) {
 }
 
 nva_status check_positions(nva_ctx *ctx, int num_tokens, int max_pos) {
+  if (ctx->dev_step) {  // positions the host does not see are below the tables' bound
+    if (ctx->dev_step->max_tokens > max_pos)
+      return fail(ctx, NVA_E_ROPE_POS, "RoPE positions of tables of up to %d tokens out of range [0, %d)",
+                  ctx->dev_step->max_tokens, max_pos);
+    if (num_tokens > ctx->dev_tokens)
+      return fail(ctx, NVA_E_ARG, "%d tokens but the step has %d positions", num_tokens,
+                  ctx->dev_tokens);
+    return NVA_OK;
+  }
   if (!ctx->has_pos) return fail(ctx, NVA_E_ARG, "the step has no positions");
   if (num_tokens > (int)ctx->pos.size())
     return fail(ctx, NVA_E_ARG, "%d tokens but the step has %d positions", num_tokens,
@@ -2084,15 +1700,16 @@ nva_status check_positions(nva_ctx *ctx, int num_tokens, int max_pos) {
   return NVA_OK;
 }
 
-nva_status check_desc(nva_ctx *ctx, const nva_attn_desc *d) {
-  if (!d) return fail(ctx, NVA_E_ARG, "attention descriptor is null");
-  if (d->num_heads <= 0 || d->num_kv_heads <= 0 || d->head_dim <= 0)
-    return fail(ctx, NVA_E_ARG, "numHeads, numKvHeads and headDim must be > 0");
-  if (d->num_heads % d->num_kv_heads)
-    return fail(ctx, NVA_E_ARG, "numHeads %d is not a multiple of numKvHeads %d", d->num_heads,
-                d->num_kv_heads);
-  if (d->head_dim % 4) return fail(ctx, NVA_E_UNSUPPORTED, "headDim must be a multiple of 4");
-  return NVA_OK;
+// The step's positions on the device.
+const int32_t *step_positions(const nva_ctx *ctx) {
+  return ctx->dev_step ? ctx->dev_step->positions : ctx->dev_i32(ctx->off_pos);
+}
+
+// How the launch pairs and turns the dims of a head.
+void set_rotation(RopeStoreLaunch &a, const nva_rope *rope) {
+  a.rotary_dim = rope->rotary_dim;
+  a.part = rope->plain() ? 0 : 1;
+  a.interleaved = rope->interleaved ? 1 : 0;
 }
 
 // The sequences of a prefix group must hold its tokens in the same pages (checked once per step).
@@ -2309,6 +1926,9 @@ nva_status nva_ctx_destroy(nva_ctx *ctx) {
   ctx->d_v_norm.release();
   ctx->d_lin.release();
   ctx->d_gather.release();
+  ctx->d_plan4.release();
+  ctx->d_part4.release();
+  ctx->d_lin4.release();
   if (ctx->xcd_hint) (void)hipFree(ctx->xcd_hint);
   (void)hipEventDestroy(ctx->fork_ev);
   (void)hipEventDestroy(ctx->join_ev);
@@ -2346,7 +1966,8 @@ nva_status nva_ctx_kernel_stats(nva_ctx *ctx, const char *kernel, int64_t *launc
   if (strcmp(kernel, "device_bytes") == 0) {
     // Device memory the context's grow-only buffers hold (not the arenas or RoPE tables).
     size_t b = ctx->d_step.cap + ctx->d_part.cap + ctx->d_q_rot.cap + ctx->d_k_rot.cap +
-               ctx->d_v_norm.cap + ctx->d_lin.cap + ctx->d_gather.cap;
+               ctx->d_v_norm.cap + ctx->d_lin.cap + ctx->d_gather.cap + ctx->d_plan4.cap +
+               ctx->d_part4.cap + ctx->d_lin4.cap;
     for (const Plan *p : ctx->plans) b += p->dev.cap;
     if (launches) *launches = (int64_t)b;
     if (total_ms) *total_ms = 0.0;
@@ -2528,7 +2149,7 @@ nva_status nva_rope_create(nva_ctx *ctx, const float *cos_sin, int max_pos, int 
   }
   r->ctx = ctx;
   r->max_pos = max_pos;
-  r->head_size = head_size;
+  r->head_size = r->rotary_dim = head_size;
   r->table = static_cast<float *>(p);
   *out = r;
   return NVA_OK;
@@ -2588,6 +2209,8 @@ nva_status nva_step_set(nva_ctx *ctx, int is_prefill, const int32_t *cu_q, const
   ctx->groups.clear();
   ctx->has_encoder = false;
   ctx->has_step = false;  // until all of it is set
+  ctx->dev_step = nullptr;
+  ctx->checked_blocks = 0;
   ctx->is_prefill = is_prefill != 0;
   ctx->num_seqs = num_seqs;
   ctx->num_tokens = num_tokens;
@@ -2695,6 +2318,7 @@ nva_status nva_step_positions(nva_ctx *ctx, const float *positions, int num_toke
 nva_status nva_step_clear(nva_ctx *ctx) {
   if (!ctx) return NVA_E_ARG;
   ctx->has_step = false;
+  ctx->dev_step = nullptr;
   for (Plan *p : ctx->plans) p->valid = false;
   ctx->tile_choices.clear();
   ctx->groups.clear();
@@ -2769,7 +2393,8 @@ nva_status nva_rope_forward(nva_ctx *ctx, const nva_rope *rope, const float *q, 
   if (!ctx) return NVA_E_ARG;
   DeviceGuard dg(ctx);
   if (!rope) return fail(ctx, NVA_E_ARG, "RoPE table is null");
-  if (!ctx->has_step) return fail(ctx, NVA_E_NO_STEP, "no step metadata set on the context");
+  if (!ctx->has_step && !ctx->dev_step)
+    return fail(ctx, NVA_E_NO_STEP, "no step metadata set on the context");
   if (num_tokens < 0 || hq < 0 || hk < 0) return fail(ctx, NVA_E_ARG, "negative shape");
   if (num_tokens == 0) return NVA_OK;  // empty batch: empty outputs, no pointers needed
   if (!q || !k || !q_out || !k_out) return fail(ctx, NVA_E_ARG, "q, k, q_out, k_out required");
@@ -2787,12 +2412,13 @@ nva_status nva_rope_forward(nva_ctx *ctx, const nva_rope *rope, const float *q, 
   a.k_cache = nullptr;
   a.v_cache = nullptr;
   a.slots = nullptr;
-  a.positions = ctx->dev_i32(ctx->off_pos);
+  a.positions = step_positions(ctx);
   a.cos_sin = rope->table;
   a.tokens = num_tokens;
   a.hq = hq;
   a.hk = hk;
   a.head_dim = rope->head_size;
+  set_rotation(a, rope);
   Timed tm(ctx, "rope_store");
   HIP_TRY(ctx, launch_rope_store(a, ctx->stream, ctx->num_cus), "rope kernel launch");
   tm.done();
@@ -2941,8 +2567,9 @@ nva_status nva_rope_attention_forward(nva_ctx *ctx, nva_kv *kv, const nva_rope *
 }
 
 // The head norms, RoPE, the store and attention with q, k, v rows read at token strides q_ld,
-// k_ld, v_ld (floats): [T, heads, d] inputs, or the packed qkv_proj output.
-static nva_status norm_rope_attention(nva_ctx *ctx, nva_kv *kv, const nva_rope *rope,
+// k_ld, v_ld (floats): [T, heads, d] inputs, or the packed qkv_proj output;
+// over either arena (kv4 non-null: the 4-bit one, which rounds its rows from k_out and v itself).
+static nva_status norm_rope_attention(nva_ctx *ctx, nva_kv *kv, nva_kv4 *kv4, const nva_rope *rope,
                                       const nva_rms_norm *q_norm, const nva_rms_norm *k_norm,
                                       const nva_rms_norm *v_norm, const nva_attn_desc *desc,
                                       const float *q, const float *k, const float *v, int q_ld,
@@ -2950,7 +2577,8 @@ static nva_status norm_rope_attention(nva_ctx *ctx, nva_kv *kv, const nva_rope *
                                       float *k_out, float *out) try {
   if (!ctx) return NVA_E_ARG;
   DeviceGuard dg(ctx);
-  nva_status st = check_forward(ctx, kv, desc, num_tokens);
+  nva_status st = kv4 ? check_forward4(ctx, kv4, desc, num_tokens)
+                      : check_forward(ctx, kv, desc, num_tokens);
   if (st != NVA_OK) return st;
   if (!rope) return fail(ctx, NVA_E_ARG, "RoPE table is null");
   if (rope->head_size != desc->head_dim)
@@ -2970,11 +2598,20 @@ static nva_status norm_rope_attention(nva_ctx *ctx, nva_kv *kv, const nva_rope *
   const int layer = d.kv_layer_index;
   const size_t qn = (size_t)num_tokens * d.num_heads * d.head_dim;
   const size_t kn = (size_t)num_tokens * d.num_kv_heads * d.head_dim;
+  if (kv4 && stream_capturing(ctx->stream)) {
+    const size_t v4 = v_norm || v_ld != d.num_kv_heads * d.head_dim ? kn * 4 + 16 : 0;
+    if ((!q_out && ctx->d_q_rot.cap < qn * 4 + 16) || (!k_out && ctx->d_k_rot.cap < kn * 4 + 16) ||
+        ctx->d_v_norm.cap < v4)
+      return fail(ctx, NVA_E_ARG, "a captured step must not be larger than every earlier one: run "
+                  "it once before the capture");
+    for (DevBuf *b : {&ctx->d_q_rot, &ctx->d_k_rot, &ctx->d_v_norm}) b->captured = true;
+  }
   if (!q_out) {
     HIP_TRY(ctx, ctx->d_q_rot.reserve(qn * 4 + 16), "rotated q scratch");
     q_out = static_cast<float *>(ctx->d_q_rot.ptr);
   }
-  const bool dense = ctx->is_prefill && !ctx->has_tables;
+  // The 4-bit store reads contiguous rows, as dense prefill does.
+  const bool dense = kv4 || (ctx->is_prefill && !ctx->has_tables);
   if (!k_out && dense) {
     HIP_TRY(ctx, ctx->d_k_rot.reserve(kn * 4 + 16), "rotated k scratch");
     k_out = static_cast<float *>(ctx->d_k_rot.ptr);
@@ -2987,7 +2624,7 @@ static nva_status norm_rope_attention(nva_ctx *ctx, nva_kv *kv, const nva_rope *
     HIP_TRY(ctx, ctx->d_v_norm.reserve(kn * 4 + 16), "normalised v scratch");
     v_out = static_cast<float *>(ctx->d_v_norm.ptr);
   }
-  const bool store = d.write_kv && kv->k[layer] && ctx->has_slots &&
+  const bool store = !kv4 && d.write_kv && kv->k[layer] && ctx->has_slots &&
                      ctx->num_slots == num_tokens;
   if (store) {
     st = check_slots(ctx, kv);
@@ -3007,12 +2644,13 @@ static nva_status norm_rope_attention(nva_ctx *ctx, nva_kv *kv, const nva_rope *
   a.k_cache = store ? kv->k[layer] : nullptr;
   a.v_cache = store ? kv->v[layer] : nullptr;
   a.slots = store ? ctx->dev_i32(ctx->off_slots) : nullptr;
-  a.positions = ctx->dev_i32(ctx->off_pos);
+  a.positions = step_positions(ctx);
   a.cos_sin = rope->table;
   a.tokens = num_tokens;
   a.hq = d.num_heads;
   a.hk = d.num_kv_heads;
   a.head_dim = d.head_dim;
+  set_rotation(a, rope);
   a.qn = head_norm(q_norm);
   a.kn = head_norm(k_norm);
   a.vn = head_norm(v_norm);
@@ -3024,6 +2662,8 @@ static nva_status norm_rope_attention(nva_ctx *ctx, nva_kv *kv, const nva_rope *
     HIP_TRY(ctx, launch_rope_store(a, ctx->stream, ctx->num_cus), "rope_store kernel launch");
     tm.done();
   }
+  if (kv4)
+    return attention4_rows(ctx, kv4, d, q_out, k_out, v_out ? v_out : v, num_tokens, out);
   return attention_after_store(ctx, kv, d, q_out, k_out, v_out ? v_out : v, num_tokens, out);
 } catch (const std::bad_alloc &) {
   return no_memory(ctx);
@@ -3038,19 +2678,18 @@ nva_status nva_norm_rope_attention_forward(nva_ctx *ctx, nva_kv *kv, const nva_r
                                            float *q_out, float *k_out, float *out) {
   if (!ctx) return NVA_E_ARG;
   if (!desc) return fail(ctx, NVA_E_ARG, "attention descriptor is null");
-  return norm_rope_attention(ctx, kv, rope, q_norm, k_norm, v_norm, desc, q, k, v,
+  return norm_rope_attention(ctx, kv, nullptr, rope, q_norm, k_norm, v_norm, desc, q, k, v,
                              desc->num_heads * desc->head_dim,
                              desc->num_kv_heads * desc->head_dim,
                              desc->num_kv_heads * desc->head_dim, num_tokens, q_out, k_out, out);
 }
 
-nva_status nva_qkv_norm_rope_attention_forward(nva_ctx *ctx, nva_kv *kv, const nva_rope *rope,
-                                               const nva_rms_norm *q_norm,
-                                               const nva_rms_norm *k_norm,
-                                               const nva_rms_norm *v_norm,
-                                               const nva_attn_desc *desc, const float *qkv,
-                                               int num_tokens, float *q_out, float *k_out,
-                                               float *out) {
+// The packed rows' three parts to either arena.
+static nva_status packed_attention(nva_ctx *ctx, nva_kv *kv, nva_kv4 *kv4, const nva_rope *rope,
+                                   const nva_rms_norm *q_norm, const nva_rms_norm *k_norm,
+                                   const nva_rms_norm *v_norm, const nva_attn_desc *desc,
+                                   const float *qkv, int num_tokens, float *q_out, float *k_out,
+                                   float *out) {
   if (!ctx) return NVA_E_ARG;
   if (!desc) return fail(ctx, NVA_E_ARG, "attention descriptor is null");
   if (!qkv && num_tokens != 0) return fail(ctx, NVA_E_ARG, "qkv is required");
@@ -3061,10 +2700,49 @@ nva_status nva_qkv_norm_rope_attention_forward(nva_ctx *ctx, nva_kv *kv, const n
                 desc->num_kv_heads, desc->head_dim);
   const int ld = (int)(qs + 2 * ks);
   if (!qkv)  // empty batch: checks only
-    return norm_rope_attention(ctx, kv, rope, q_norm, k_norm, v_norm, desc, nullptr, nullptr,
+    return norm_rope_attention(ctx, kv, kv4, rope, q_norm, k_norm, v_norm, desc, nullptr, nullptr,
                                nullptr, ld, ld, ld, 0, q_out, k_out, out);
-  return norm_rope_attention(ctx, kv, rope, q_norm, k_norm, v_norm, desc, qkv, qkv + qs,
+  return norm_rope_attention(ctx, kv, kv4, rope, q_norm, k_norm, v_norm, desc, qkv, qkv + qs,
                              qkv + qs + ks, ld, ld, ld, num_tokens, q_out, k_out, out);
+}
+
+nva_status nva_qkv_norm_rope_attention_forward(nva_ctx *ctx, nva_kv *kv, const nva_rope *rope,
+                                               const nva_rms_norm *q_norm,
+                                               const nva_rms_norm *k_norm,
+                                               const nva_rms_norm *v_norm,
+                                               const nva_attn_desc *desc, const float *qkv,
+                                               int num_tokens, float *q_out, float *k_out,
+                                               float *out) {
+  return packed_attention(ctx, kv, nullptr, rope, q_norm, k_norm, v_norm, desc, qkv, num_tokens,
+                          q_out, k_out, out);
+}
+
+nva_status nva_norm_rope_attention4_forward(nva_ctx *ctx, nva_kv4 *kv, const nva_rope *rope,
+                                            const nva_rms_norm *q_norm, const nva_rms_norm *k_norm,
+                                            const nva_rms_norm *v_norm, const nva_attn_desc *desc,
+                                            const float *q, const float *k, const float *v,
+                                            int num_tokens, float *q_out, float *k_out,
+                                            float *out) {
+  if (!ctx) return NVA_E_ARG;
+  if (!desc) return fail(ctx, NVA_E_ARG, "attention descriptor is null");
+  if (!kv) return fail(ctx, NVA_E_NO_ARENA, "KV cache arena not bound in Context");
+  return norm_rope_attention(ctx, nullptr, kv, rope, q_norm, k_norm, v_norm, desc, q, k, v,
+                             desc->num_heads * desc->head_dim,
+                             desc->num_kv_heads * desc->head_dim,
+                             desc->num_kv_heads * desc->head_dim, num_tokens, q_out, k_out, out);
+}
+
+nva_status nva_qkv_norm_rope_attention4_forward(nva_ctx *ctx, nva_kv4 *kv, const nva_rope *rope,
+                                                const nva_rms_norm *q_norm,
+                                                const nva_rms_norm *k_norm,
+                                                const nva_rms_norm *v_norm,
+                                                const nva_attn_desc *desc, const float *qkv,
+                                                int num_tokens, float *q_out, float *k_out,
+                                                float *out) {
+  if (!ctx) return NVA_E_ARG;
+  if (!kv) return fail(ctx, NVA_E_NO_ARENA, "KV cache arena not bound in Context");
+  return packed_attention(ctx, nullptr, kv, rope, q_norm, k_norm, v_norm, desc, qkv, num_tokens,
+                          q_out, k_out, out);
 }
 
 nva_status nva_linear_forward(nva_ctx *ctx, const float *x, int rows, int in,

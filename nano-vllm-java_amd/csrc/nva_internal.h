@@ -165,6 +165,8 @@ struct RopeStoreLaunch {
   HeadNorm qn, kn, vn;        // per-head RMSNorm applied to q, k, v before rotation / store
   int32_t iters_per_wg;       // row kernel: row iterations per workgroup (set by the launcher)
   int32_t q_ld, k_ld, v_ld;   // floats per token of the q, k, v inputs (0: hq*d, hk*d, hk*d)
+  int32_t rotary_dim;         // part: dims of a head that turn, the first ones (the rest are copied)
+  int32_t part, interleaved;  // part != 0: any rotary_dim and pairing (cos_sin [max_pos, rotary_dim])
   // When non-null, the launch's last workgroup writes the id of the XCD it ran on here.  The
   // hardware hands consecutive workgroups to the 8 XCDs in turn, continuing across launches, so
   // the next launch's first workgroup lands on the XCD after it; the decode launch that follows
@@ -189,6 +191,92 @@ struct LinearLaunch {
   int32_t splits, k_per_split;
 };
 
+// Device-built step metadata (tables.hip).
+struct TablesLaunch {
+  int32_t *table, *lens, *free_pages, *slots, *positions, *cu_q;
+  int32_t *state;  // status code, its number, free blocks; [3] the stack's height
+  const int32_t *keep, *fresh;  // tokens that stay (null: all) and follow
+  int32_t num_seqs, num_tokens, max_new, max_tokens, block_size, width;
+  int32_t fill_apart;  // set by the launcher
+};
+constexpr int kTablesMaxSeqs = 4000;  // four numbers a row in 64 KB of LDS
+hipError_t launch_tables_clear(const TablesLaunch &a, const int32_t *pages, int num_pages,
+                               int max_seqs, int max_step_tokens, hipStream_t s);
+hipError_t launch_tables_extend(const TablesLaunch &a, hipStream_t s);
+
+// The 4-bit arena and attention over it (kv4.hip).
+struct Kv4View {
+  uint8_t *pages;  // [block][KV head][tile of 32 keys][34 d bytes]
+  int32_t num_blocks, block_size, hkv;
+};
+constexpr int kKv4Cols = 16;      // columns of a column tile
+constexpr int kKv4MinUnits = 8;   // least key tiles of a workgroup
+struct Kv4Tile {
+  int32_t seq, col0, kb, n;  // n 0: no key is seen
+};
+struct Kv4Head {
+  int64_t chunk;  // units of a workgroup
+  int32_t tiles;
+  int32_t first, covered;  // rows of the sequences: [first, covered)
+  int32_t pad;
+};
+// Where the work list goes and what it is made of: row offsets (null: one row a sequence) and the
+// lengths, or the offsets whose differences they are.
+struct Kv4List {
+  Kv4Head *head;  // null: no list
+  Kv4Tile *tiles;
+  int64_t *cum;
+  int32_t *before;  // [num_seqs + 1] column tiles before each sequence
+  const int32_t *cu_q, *cu_k, *lens;
+  int32_t num_seqs, rep, hkv, window, workgroups;
+};
+struct Kv4Store {
+  Kv4View kv;
+  const float *k, *v;  // [tokens, hkv, d]; k null: no rows
+  const int32_t *slots;
+  int32_t tokens;
+  Kv4List list;
+};
+struct Kv4Attention {
+  Kv4View kv;
+  const float *q;
+  float *out;
+  const Kv4Head *head;
+  const Kv4Tile *tiles;
+  const int64_t *cum;
+  const int32_t *cu_q, *cu_k, *lens, *table;
+  int32_t bt_stride, hq, head_dim, window, tokens;
+  int32_t tile_shift;  // log2 of a block's tiles, or -1
+  float scale2;        // scale * log2(e)
+  float *part_m, *part_l, *part_o;
+};
+// Resident workgroups of the attention kernel, a wave of each on every SIMD: by its registers.
+constexpr int kv4_workgroups_per_cu(int head_dim) {
+  return head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1;
+}
+bool kv4_supports(int head_dim);
+hipError_t launch_kv4_store(const Kv4Store &a, int head_dim, hipStream_t s);
+hipError_t launch_kv4_read(const Kv4View &kv, int head_dim, const int32_t *slots, float *k, float *v,
+                           int rows, hipStream_t s);
+hipError_t launch_kv4_attention(const Kv4Attention &a, int workgroups, hipStream_t s);
+hipError_t launch_kv4_merge(const Kv4Attention &a, int max_tiles, hipStream_t s);
+hipError_t launch_quantize4(const float *x, int64_t values, uint8_t *codes, uint8_t *scales,
+                            hipStream_t s);
+
+// y = x W^T with a 4-bit weight (linear4.hip).
+struct Linear4Launch {
+  const float *x, *bias;  // [rows, in]; [out] or null
+  const uint8_t *weight;  // as launch_linear4_layout leaves it
+  float *y;
+  void *work;             // linear4_work_bytes()
+  int32_t rows, in, out;
+};
+size_t linear4_bytes(int out, int in);
+hipError_t launch_linear4_layout(const uint8_t *codes, const uint8_t *scales, int out, int in,
+                                 uint8_t *weight, hipStream_t s);
+size_t linear4_work_bytes(const Linear4Launch &a, int num_cus);
+hipError_t launch_linear4(const Linear4Launch &a, int num_cus, hipStream_t s);
+
 struct GatherLaunch {
   const float *k_cache, *v_cache;
   float *k_out, *v_out;       // [T, hk, d]
@@ -198,6 +286,8 @@ struct GatherLaunch {
 
 // Kernel launchers (each returns the hipGetLastError() of its launch).
 hipError_t launch_rope_store(const RopeStoreLaunch &a, hipStream_t s, int num_cus);
+hipError_t launch_rope_table(const double *freq, float *table, int pairs, int max_pos,
+                             double amplitude, hipStream_t s);
 hipError_t launch_rms_norm(const NormLaunch &a, hipStream_t s);
 // LDS bytes the fused kernel needs for its head norms (0 when no norm is enabled).
 size_t rope_store_norm_lds(const RopeStoreLaunch &a);

@@ -13,6 +13,8 @@
 // with the cos|sin row of the token's position taken from the caller's table.  Java never
 // contracts these into FMAs, so contraction is switched off here: each product and sum is a
 // separately rounded fp32 op and the result is bit-identical to the reference.
+// A launch with `part` set turns the first rotary_dim dims only, of a table [max_pos, rotary_dim],
+// and pairs halves of those or neighbours; the other dims pass through.
 // The store restates Attention.storeKvCache (layers/Attention.java:221-240): the token's
 // Hkv*d floats of rotated k and of v go to cache[slot*Hkv*d ...]; negative slots are skipped.
 //
@@ -122,7 +124,7 @@ __global__ void __launch_bounds__(256) rope_store_kernel(RopeStoreLaunch a) {
     __syncthreads();
   }
   const int pos = a.positions ? a.positions[t] : -1;
-  const float *cs = a.positions ? a.cos_sin + (size_t)pos * d : nullptr;
+  const float *cs = a.positions ? a.cos_sin + (size_t)pos * (a.part ? a.rotary_dim : d) : nullptr;
   const int32_t slot = a.slots ? a.slots[t] : -1;
   const bool store = a.k_cache != nullptr && slot >= 0;
   const size_t krow = (size_t)a.hk * d;
@@ -130,7 +132,36 @@ __global__ void __launch_bounds__(256) rope_store_kernel(RopeStoreLaunch a) {
   float *vc = store ? a.v_cache + (size_t)slot * krow : nullptr;
   const bool vec = (half & 3) == 0;
 
-  if (cs != nullptr) {
+  if (cs != nullptr && a.part) {
+    // Any pairing and any even rotary_dim, one dim an item: its partner is read again.
+    const int turn = a.rotary_dim, th = turn >> 1;
+    const int items = (a.hq + a.hk) * d;
+    for (int it = threadIdx.x; it < items; it += blockDim.x) {
+      const int hh = it / d;
+      const int i = it - hh * d;
+      const bool isq = hh < a.hq;
+      const int h = isq ? hh : hh - a.hq;
+      const float *in = (isq ? a.q + (size_t)t * a.q_ld : a.k + (size_t)t * a.k_ld) + (size_t)h * d;
+      const HeadNorm &nm = isq ? a.qn : a.kn;
+      const float inv = nm.enabled ? inv_lds[hh] : 1.0f;
+      float o = nm.enabled ? norm1(in[i], inv, nm, i) : in[i];
+      if (i < turn) {
+        const int p = a.interleaved ? i >> 1 : (i < th ? i : i - th);
+        const bool first = a.interleaved ? (i & 1) == 0 : i < th;
+        const int j = a.interleaved ? i ^ 1 : (first ? i + th : i - th);
+        const float y = nm.enabled ? norm1(in[j], inv, nm, j) : in[j];
+        const float c = cs[p], sn = cs[th + p];
+        o = first ? o * c - y * sn : o * c + y * sn;
+      }
+      const size_t row = ((size_t)t * (isq ? a.hq : a.hk) + h) * d;
+      if (isq) {
+        a.q_out[row + i] = o;
+      } else {
+        if (a.k_out) a.k_out[row + i] = o;
+        if (store) kc[(size_t)h * d + i] = o;
+      }
+    }
+  } else if (cs != nullptr) {
     // Rotation: items are (head, i) pairs over q heads then k heads.
     const int step = vec ? 4 : 1;
     const int per_head = half / step;
@@ -255,7 +286,9 @@ constexpr int kRopeRowsPerLoad = 4;
 // groups c + LPR * j (j < VPL) of the row.  The norm's group sums are folded in index order with
 // DPP shifts; the rotation partner of a first-half element sits LPR / 2 lanes away (VPL = 1) or
 // in the lane's own column VPL/2 further on (VPL > 1).
-template <int LPR, int VPL>
+// PART (any pairing and rotary_dim % 8 == 0): neighbours are in the lane itself; the other half of
+// the turning dims lies rotary_dim / 8 float4 groups away, fetched across lanes.
+template <int LPR, int VPL, bool PART>
 __global__ void __launch_bounds__(256) rope_rows_kernel(RopeStoreLaunch a) {
   constexpr int D = 4 * LPR * VPL;
   record_last_xcd(a.xcd_hint);
@@ -279,8 +312,28 @@ __global__ void __launch_bounds__(256) rope_rows_kernel(RopeStoreLaunch a) {
   const bool rotate = a.positions != nullptr;
   constexpr int H2 = VPL > 1 ? VPL / 2 : 1;  // cos|sin float4s a lane needs
   static_assert(VPL == 1 || VPL % 2 == 0, "a split row holds both halves in its own lanes");
-  float4 cv[H2], sv[H2];
-  if (rotate) {
+  constexpr int CS = PART ? VPL : H2;
+  float4 cv[CS], sv[CS];
+  const int turn = PART ? a.rotary_dim : D;
+  const int far = turn >> 3;  // groups from a first half's dims to their partners
+  if (PART && rotate) {
+    // Neighbours: the two pairs' cos and sin; halves: those of the group's pairs.
+    const float *cs = a.cos_sin + (size_t)a.positions[t] * turn;
+#pragma unroll
+    for (int j = 0; j < VPL; j++) {
+      const int g = c + LPR * j;
+      cv[j] = sv[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (4 * g >= turn) continue;
+      if (a.interleaved) {
+        cv[j] = make_float4(cs[2 * g], cs[2 * g + 1], 0.f, 0.f);
+        sv[j] = make_float4(cs[(turn >> 1) + 2 * g], cs[(turn >> 1) + 2 * g + 1], 0.f, 0.f);
+      } else {
+        const int p = 4 * (g < far ? g : g - far);
+        cv[j] = ld4(cs + p);
+        sv[j] = ld4(cs + (turn >> 1) + p);
+      }
+    }
+  } else if (rotate) {
     const float *cs = a.cos_sin + (size_t)a.positions[t] * D;
     if constexpr (VPL == 1) {
       // Lane c < LPR/2 rotates x1 = elements 4c.., the others x2 = HALF + 4(c - LPR/2).
@@ -349,8 +402,47 @@ __global__ void __launch_bounds__(256) rope_rows_kernel(RopeStoreLaunch a) {
       }
 
       float4 o[VPL];
-      if (kind[i] != 2 && rotate) {
-        if constexpr (VPL == 1) {
+      if (PART && rotate) {
+#pragma unroll
+        for (int j = 0; j < VPL; j++) {
+          const int g = c + LPR * j;
+          const float4 u = x[i][j];
+          o[j] = u;
+          if (a.interleaved) {  // uniform over the launch
+            if (kind[i] != 2 && 4 * g < turn) {
+              o[j].x = u.x * cv[j].x - u.y * sv[j].x;
+              o[j].y = u.y * cv[j].x + u.x * sv[j].x;
+              o[j].z = u.z * cv[j].y - u.w * sv[j].y;
+              o[j].w = u.w * cv[j].y + u.z * sv[j].y;
+            }
+            continue;
+          }
+          const bool first = g < far;
+          const int pg = 4 * g < turn ? (first ? g + far : g - far) : g;
+          const int src = base + (pg & (LPR - 1));
+          float4 y;
+          if constexpr (VPL == 1) {
+            y = make_float4(__shfl(u.x, src), __shfl(u.y, src), __shfl(u.z, src), __shfl(u.w, src));
+          } else {
+            static_assert(VPL == 2, "a partner is in one of two columns");
+            const float4 p = x[i][0], r = x[i][1];
+            const float4 lo = make_float4(__shfl(p.x, src), __shfl(p.y, src), __shfl(p.z, src),
+                                          __shfl(p.w, src));
+            const float4 hi = make_float4(__shfl(r.x, src), __shfl(r.y, src), __shfl(r.z, src),
+                                          __shfl(r.w, src));
+            y = pg < LPR ? lo : hi;
+          }
+          if (kind[i] != 2 && 4 * g < turn) {
+            o[j].x = first ? u.x * cv[j].x - y.x * sv[j].x : u.x * cv[j].x + y.x * sv[j].x;
+            o[j].y = first ? u.y * cv[j].y - y.y * sv[j].y : u.y * cv[j].y + y.y * sv[j].y;
+            o[j].z = first ? u.z * cv[j].z - y.z * sv[j].z : u.z * cv[j].z + y.z * sv[j].z;
+            o[j].w = first ? u.w * cv[j].w - y.w * sv[j].w : u.w * cv[j].w + y.w * sv[j].w;
+          }
+        }
+      } else if (kind[i] != 2 && rotate) {
+        if constexpr (PART) {
+          // (not reached: PART launches rotate above)
+        } else if constexpr (VPL == 1) {
           // Partner = the other half of the row.
           float4 y;
           y.x = partner<LPR / 2>(x[i][0].x);
@@ -482,7 +574,12 @@ hipError_t launch_rows(const RopeStoreLaunch &a, hipStream_t s, int num_cus) {
   RopeStoreLaunch b = a;
   b.iters_per_wg = (iters + slices - 1) / slices;
   const int grid_y = (iters + b.iters_per_wg - 1) / b.iters_per_wg;
-  hipLaunchKernelGGL((rope_rows_kernel<LPR, VPL>), dim3(a.tokens, grid_y), dim3(256), 0, s, b);
+  if (a.part && a.positions)
+    hipLaunchKernelGGL((rope_rows_kernel<LPR, VPL, true>), dim3(a.tokens, grid_y), dim3(256), 0, s,
+                       b);
+  else
+    hipLaunchKernelGGL((rope_rows_kernel<LPR, VPL, false>), dim3(a.tokens, grid_y), dim3(256), 0, s,
+                       b);
   return hipGetLastError();
 }
 
@@ -494,8 +591,9 @@ hipError_t launch_rope_store(const RopeStoreLaunch &in, hipStream_t s, int num_c
   if (!a.q_ld) a.q_ld = a.hq * a.head_dim;
   if (!a.k_ld) a.k_ld = a.hk * a.head_dim;
   if (!a.v_ld) a.v_ld = a.hk * a.head_dim;
-  // Row kernel for the head dims it is instantiated for; the per-token kernel otherwise.
-  switch (a.head_dim) {
+  // Row kernel for the head dims it is instantiated for; the per-token kernel otherwise, and where the
+  // turning dims' halves do not fall on float4 groups.
+  switch (a.part && a.rotary_dim % 8 ? 0 : a.head_dim) {
     case 8: return launch_rows<2, 1>(a, s, num_cus);
     case 16: return launch_rows<4, 1>(a, s, num_cus);
     case 32: return launch_rows<8, 1>(a, s, num_cus);
@@ -508,6 +606,30 @@ hipError_t launch_rope_store(const RopeStoreLaunch &in, hipStream_t s, int num_c
   const size_t lds = rope_store_norm_lds(a);
   if (lds > kRopeNormMaxLds) return hipErrorInvalidValue;
   hipLaunchKernelGGL(rope_store_kernel, dim3(a.tokens), dim3(128), lds, s, a);
+  return hipGetLastError();
+}
+
+// cos and sin of position x frequency, [max_pos, pairs | pairs]: angles in 64 bits, as a float product
+// would be off by whole turns far out.
+__global__ void __launch_bounds__(256) rope_table_kernel(const double *freq, float *table, int pairs,
+                                                         int64_t entries, double amplitude) {
+  const int64_t stride = (int64_t)gridDim.x * blockDim.x;
+  for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < entries; e += stride) {
+    const int64_t pos = e / pairs;
+    const int i = (int)(e - pos * pairs);
+    double sn, c;
+    sincos((double)pos * freq[i], &sn, &c);
+    table[pos * 2 * pairs + i] = (float)(c * amplitude);
+    table[pos * 2 * pairs + pairs + i] = (float)(sn * amplitude);
+  }
+}
+
+hipError_t launch_rope_table(const double *freq, float *table, int pairs, int max_pos,
+                             double amplitude, hipStream_t s) {
+  const int64_t entries = (int64_t)pairs * max_pos;
+  const unsigned blocks = (unsigned)std::min<int64_t>((entries + 255) / 256, 8192);
+  hipLaunchKernelGGL(rope_table_kernel, dim3(blocks), dim3(256), 0, s, freq, table, pairs, entries,
+                     amplitude);
   return hipGetLastError();
 }
 

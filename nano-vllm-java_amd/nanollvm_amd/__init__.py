@@ -5,15 +5,19 @@ producers; ``workloads`` builds the synthetic workloads of the benchmark and tes
 from . import _native  # noqa: F401
 from .layers import (  # noqa: F401
     Attention,
+    BlockTables,
     Context,
     CrossAttention,
     IllegalArgumentException,
     IllegalStateException,
     KvCacheArena,
+    KvCacheArena4,
     Linear,
+    Linear4,
     NullPointerException,
     NvaError,
     RMSNorm,
     RotaryEmbedding,
     UnsupportedShapeError,
+    quantize4,
 )

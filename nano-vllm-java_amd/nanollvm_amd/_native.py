@@ -106,6 +106,28 @@ class PrefixGroup(ctypes.Structure):
     ]
 
 
+class RopeDesc(ctypes.Structure):
+    """nva_rope_desc: rotary positions of part of a head, of either pairing, scaled."""
+
+    _fields_ = [
+        ("head_size", ctypes.c_int32),
+        ("rotary_dim", ctypes.c_int32),
+        ("max_pos", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("base", ctypes.c_float),
+        ("scaling", ctypes.c_int32),
+        ("factor", ctypes.c_float),
+        ("original_max_pos", ctypes.c_int32),
+        ("low", ctypes.c_float),
+        ("high", ctypes.c_float),
+        ("amplitude", ctypes.c_float),
+    ]
+
+
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
+
+TABLES_BLOCKS, TABLES_LENS, TABLES_SLOTS, TABLES_POSITIONS, TABLES_CU_Q = range(5)
+
 _pgroup = ctypes.POINTER(PrefixGroup)
 _pseq = ctypes.POINTER(Seq)
 _pmeta = ctypes.POINTER(StepMetaOut)
@@ -161,6 +183,30 @@ SIGNATURES = {
     "nva_qkv_norm_rope_attention_forward": ([_vp, _vp, _vp, _pnorm, _pnorm, _pnorm,
                                              ctypes.POINTER(AttnDesc), _vp, _ci, _vp, _vp, _vp],
                                             _st),
+    "nva_rope_create_scaled": ([_vp, ctypes.POINTER(RopeDesc), _pvp], _st),
+    "nva_tables_create": ([_vp, _ci, _ci, _ci, _ci, _ci, _vp, _pvp], _st),
+    "nva_tables_destroy": ([_vp], _st),
+    "nva_tables_array": ([_vp, _ci, _pvp, ctypes.POINTER(_i64)], _st),
+    "nva_tables_status": ([_vp, _vp], _st),
+    "nva_step_extend": ([_vp, _vp, _vp, _vp, _ci, _ci, _ci], _st),
+    "nva_quantize4": ([_vp, _vp, _i64, _ci, _vp, _vp], _st),
+    "nva_kv4_create": ([_vp, _ci, _ci, _ci, _ci, _vp, _vp, _pvp], _st),
+    "nva_kv4_destroy": ([_vp], _st),
+    "nva_kv4_blocks_that_fit": ([_vp, _ci, _ci, _ci, _vp, _vp, _cf, ctypes.POINTER(_ci),
+                                 ctypes.POINTER(_i64)], _st),
+    "nva_kv4_layer": ([_vp, _ci, _pvp, ctypes.POINTER(_i64)], _st),
+    "nva_kv4_write_rows": ([_vp, _ci, _vp, _vp, _vp, _ci], _st),
+    "nva_kv4_read_rows": ([_vp, _ci, _vp, _vp, _vp, _ci], _st),
+    "nva_attention4_forward": ([_vp, _vp, ctypes.POINTER(AttnDesc), _vp, _vp, _vp, _ci, _vp], _st),
+    "nva_norm_rope_attention4_forward": ([_vp, _vp, _vp, _pnorm, _pnorm, _pnorm,
+                                          ctypes.POINTER(AttnDesc), _vp, _vp, _vp, _ci, _vp, _vp,
+                                          _vp], _st),
+    "nva_qkv_norm_rope_attention4_forward": ([_vp, _vp, _vp, _pnorm, _pnorm, _pnorm,
+                                              ctypes.POINTER(AttnDesc), _vp, _ci, _vp, _vp, _vp],
+                                             _st),
+    "nva_linear4_create": ([_vp, _vp, _vp, _ci, _ci, _pvp], _st),
+    "nva_linear4_destroy": ([_vp], _st),
+    "nva_linear4_forward": ([_vp, _vp, _vp, _ci, _vp, _vp], _st),
 }
 
 

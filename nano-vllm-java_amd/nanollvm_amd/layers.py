@@ -14,6 +14,8 @@ the reference's own code:
                         by the model layers before RoPE.
 * ``Linear``         -- layers/Linear.java Linear.Row (``forward``): o_proj on the attention
                         output.
+* ``BlockTables``, ``KvCacheArena4``, ``Linear4`` -- block tables that grow on the device
+                        (``Context.extend``), and the arena and o_proj held in 4 bits.
 
 (Reference paths are relative to nano-vllm-java/src/main/java/com/igormaznitsa/nanollvm/.)
 Tensors are torch CUDA float32 tensors (device memory only; torch does no compute here).  Java
@@ -23,7 +25,7 @@ exceptions map to Python exceptions of the same names.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Sequence
+from typing import Optional, Sequence, Union
 
 import numpy as np
 import torch
@@ -92,6 +94,36 @@ def _dev(t: Optional[torch.Tensor], name: str):
     return t.data_ptr()
 
 
+def _ints(t: Optional[torch.Tensor], name: str, device: int, count: Optional[int] = None):
+    """Pointer of a contiguous int32 device vector."""
+    if t is None:
+        return None
+    if not (t.is_cuda and t.get_device() == device and t.dtype is torch.int32 and t.dim() == 1 and
+            t.is_contiguous()):
+        raise IllegalArgumentException(
+            f"{name} must be a contiguous 1-D int32 tensor on the context's device")
+    if count is not None and t.numel() != count:
+        raise IllegalArgumentException(f"{name} must have {count} entries, got {t.numel()}")
+    return t.data_ptr()
+
+
+def _on(t: Optional[torch.Tensor], name: str, device: int):
+    """_dev of a tensor that has to be on the context's device."""
+    p = _dev(t, name)
+    if t is not None and t.get_device() != device:
+        raise IllegalArgumentException(f"{name} must be on the context's device")
+    return p
+
+
+class _Memory:
+    """Device memory of the library as torch.as_tensor takes it; keeps its owner alive."""
+
+    def __init__(self, ptr: int, shape: tuple, owner):
+        self.owner = owner
+        self.__cuda_array_interface__ = {"shape": shape, "typestr": "<i4", "data": (ptr, False),
+                                         "version": 2, "strides": None}
+
+
 class Context:
     """Context.java plus the native context (device, stream, step buffers).
 
@@ -127,7 +159,7 @@ class Context:
         self._stream = s
 
     # ---- Context.java API
-    def bind_kv_cache(self, arena: "KvCacheArena") -> None:
+    def bind_kv_cache(self, arena: Union["KvCacheArena", "KvCacheArena4"]) -> None:
         self._kv = arena
 
     def kv_cache(self) -> Optional["KvCacheArena"]:
@@ -191,6 +223,22 @@ class Context:
         _check(self._h, N.load().nva_step_prepare_decode(self._h, arr, len(seqs), block_size),
                "Transformer.prepareDecode")
         del keep
+        self._positions_key = None
+
+    def extend(self, tables: "BlockTables", new_tokens: torch.Tensor, num_tokens: int, max_new: int,
+               keep: Optional[torch.Tensor] = None) -> None:
+        """The next step, built on the device: of row b of ``tables`` the first ``keep[b]`` tokens stay
+        (all without ``keep``) and ``new_tokens[b]`` follow, at most ``max_new`` of any and
+        ``num_tokens`` in all, the rows of the step's q, k and v (those behind the new tokens are
+        padding).  ``new_tokens`` and ``keep`` are int32 device tensors, one entry per row from the
+        first.  Nothing is waited for; ``tables.status()`` tells whether the step fitted."""
+        n = new_tokens.numel()
+        fresh = _ints(new_tokens, "new_tokens", self.device)
+        stay = _ints(keep, "keep", self.device, n)
+        _check(self._h, N.load().nva_step_extend(
+            self._h, tables.handle, stay, fresh if n else None, n, int(num_tokens), int(max_new)),
+            "Context.extend")
+        tables._step = (int(num_tokens), n)
         self._positions_key = None
 
     def share_prefixes(self, groups) -> None:
@@ -405,6 +453,31 @@ class RotaryEmbedding:
         self.head_size = head_size
         self.max_position = max_position_embeddings
 
+    @classmethod
+    def scaled(cls, ctx: Context, head_size: int, rotary_dim: int, max_position_embeddings: int,
+               base: float, interleaved: bool = False, scaling: str = "none", factor: float = 1.0,
+               original_max_position: int = 0, low: float = 0.0, high: float = 0.0,
+               amplitude: float = 0.0) -> "RotaryEmbedding":
+        """Rotary positions of the first ``rotary_dim`` dims, halves or neighbours
+        (``interleaved``) paired, whose frequencies are scaled for contexts beyond the trained one:
+        ``"none"``, ``"linear"``, ``"ntk"``, ``"yarn"`` or ``"bands"`` (include/nva.h:
+        nva_rope_create_scaled, which also explains the other arguments)."""
+        if scaling not in N.ROPE_SCALINGS:
+            raise IllegalArgumentException(
+                f"scaling must be one of {sorted(N.ROPE_SCALINGS)}, got {scaling!r}")
+        desc = N.RopeDesc(head_size, rotary_dim, max_position_embeddings, int(bool(interleaved)),
+                          base, N.ROPE_SCALINGS[scaling], factor, original_max_position, low, high,
+                          amplitude)
+        h = ctypes.c_void_p()
+        _check(ctx.handle, N.load().nva_rope_create_scaled(ctx.handle, ctypes.byref(desc),
+                                                           ctypes.byref(h)),
+               "RotaryEmbedding.scaled")
+        rope = cls.__new__(cls)
+        rope._h = h
+        rope.head_size = head_size
+        rope.max_position = max_position_embeddings
+        return rope
+
     @property
     def handle(self):
         return self._h
@@ -526,12 +599,15 @@ class Attention:
     def forward(self, q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Tensor],
                 ctx: Context) -> torch.Tensor:
         """Attention.forward(q, k, v, ctx) (Attention.java:152-171): stores k/v into the bound
-        arena at the step's slots, then attends; returns a new [tokens, numHeads, headDim]."""
+        arena at the step's slots, then attends; returns a new [tokens, numHeads, headDim].  The
+        arena may be a ``KvCacheArena4``, here and in the forms below."""
         self._check_shapes(q, k, v)
         arena = ctx.kv_cache()
         qp = _dev(q, "q")
         out = torch.empty_like(q)
-        _check(ctx.handle, N.load().nva_attention_forward(
+        lib = N.load()
+        _check(ctx.handle, (lib.nva_attention4_forward if isinstance(arena, KvCacheArena4) else
+                            lib.nva_attention_forward)(
             ctx.handle, arena.handle if arena is not None else None, ctypes.byref(self._desc),
             qp, _dev(k, "k"), _dev(v, "v"), q.shape[0], out.data_ptr()), "Attention.forward")
         return out
@@ -547,6 +623,9 @@ class Attention:
         for t, shape in ((q_out, q.shape), (k_out, k.shape)):
             if t is not None and tuple(t.shape) != tuple(shape):
                 raise IllegalArgumentException("q_out/k_out must match q/k")
+        if isinstance(ctx.kv_cache(), KvCacheArena4):
+            return self.forward_with_norm_rope(rope, positions, q, k, v, ctx, q_out=q_out,
+                                               k_out=k_out)
         if positions is not None:
             ctx.set_positions(positions)
         arena = ctx.kv_cache()
@@ -582,7 +661,10 @@ class Attention:
         arena = ctx.kv_cache()
         out = torch.empty((q.shape[0], self.num_heads, self.head_dim), dtype=torch.float32,
                           device=q.device)
-        _check(ctx.handle, N.load().nva_norm_rope_attention_forward(
+        lib = N.load()
+        _check(ctx.handle, (lib.nva_norm_rope_attention4_forward
+                            if isinstance(arena, KvCacheArena4) else
+                            lib.nva_norm_rope_attention_forward)(
             ctx.handle, arena.handle if arena is not None else None, rope.handle,
             None if q_norm is None else q_norm.desc(), None if k_norm is None else k_norm.desc(),
             None if v_norm is None else v_norm.desc(), ctypes.byref(self._desc), _dev(q, "q"),
@@ -616,7 +698,10 @@ class Attention:
         arena = ctx.kv_cache()
         out = torch.empty((T, self.num_heads, self.head_dim), dtype=torch.float32,
                           device=qkv.device)
-        _check(ctx.handle, N.load().nva_qkv_norm_rope_attention_forward(
+        lib = N.load()
+        _check(ctx.handle, (lib.nva_qkv_norm_rope_attention4_forward
+                            if isinstance(arena, KvCacheArena4) else
+                            lib.nva_qkv_norm_rope_attention_forward)(
             ctx.handle, arena.handle if arena is not None else None, rope.handle,
             None if q_norm is None else q_norm.desc(), None if k_norm is None else k_norm.desc(),
             None if v_norm is None else v_norm.desc(), ctypes.byref(self._desc),
@@ -681,3 +766,248 @@ class CrossAttention:
             handle, ctypes.byref(self._desc), qp, kp, vp, rows, stride, shape[0],
             out.data_ptr()), "CrossAttention.forward")
         return out
+
+
+class BlockTables:
+    """Block tables of up to ``max_seqs`` sequences (rows) that ``Context.extend`` grows and shrinks on
+    the device: blocks of ``block_size`` tokens out of ``num_blocks``, numbered from 0 or as ``pages``
+    lists them, in the order in which they are handed out.
+
+    ``block_tables`` and ``lens`` are views of all rows; ``slots``, ``positions`` (one entry per row of
+    the step's q, k and v) and ``cu_q`` (row offsets) are those of the last step.  They are the
+    library's memory, which the next step writes."""
+
+    def __init__(self, ctx: Context, max_seqs: int, max_tokens: int, max_step_tokens: int,
+                 num_blocks: int, block_size: int, pages=None):
+        ids = _i32(pages)
+        if ids is not None and ids.shape != (num_blocks,):
+            raise IllegalArgumentException("pages must list num_blocks block ids")
+        h = ctypes.c_void_p()
+        _check(ctx.handle, N.load().nva_tables_create(
+            ctx.handle, max_seqs, max_tokens, max_step_tokens, num_blocks, block_size, _ptr(ids),
+            ctypes.byref(h)), "BlockTables")
+        self._h = h
+        self._ctx = ctx
+        self.max_seqs, self.block_size = max_seqs, block_size
+        self._step = (0, 0)
+        width = -(-max_tokens // block_size)
+        self._arrays = [self._view(w, s) for w, s in (
+            (N.TABLES_BLOCKS, (max_seqs, width)), (N.TABLES_LENS, (max_seqs,)),
+            (N.TABLES_SLOTS, (max_step_tokens,)), (N.TABLES_POSITIONS, (max_step_tokens,)),
+            (N.TABLES_CU_Q, (max_seqs + 1,)))]
+
+    def _view(self, which: int, shape: tuple) -> torch.Tensor:
+        p, n = ctypes.c_void_p(), ctypes.c_int64()
+        _check(self._ctx.handle, N.load().nva_tables_array(self._h, which, ctypes.byref(p),
+                                                           ctypes.byref(n)), "BlockTables")
+        if n.value == 0:
+            return torch.empty(shape, dtype=torch.int32, device=f"cuda:{self._ctx.device}")
+        return torch.as_tensor(_Memory(p.value, shape, self), device=f"cuda:{self._ctx.device}")
+
+    @property
+    def handle(self):
+        return self._h
+
+    @property
+    def block_tables(self) -> torch.Tensor:
+        return self._arrays[0]
+
+    @property
+    def lens(self) -> torch.Tensor:
+        return self._arrays[1]
+
+    @property
+    def slots(self) -> torch.Tensor:
+        return self._arrays[2][:self._step[0]]
+
+    @property
+    def positions(self) -> torch.Tensor:
+        return self._arrays[3][:self._step[0]]
+
+    @property
+    def cu_q(self) -> torch.Tensor:
+        return self._arrays[4][:self._step[1] + 1]
+
+    def status(self):
+        """(code, its number, free blocks) of the last step, waiting for it: code 0, or why the step
+        changed nothing (include/nva.h: nva_step_extend)."""
+        s = (ctypes.c_int32 * 3)()
+        _check(self._ctx.handle, N.load().nva_tables_status(self._h, s), "BlockTables.status")
+        return tuple(s)
+
+    def close(self) -> None:
+        if self._h:
+            self._arrays = None
+            N.load().nva_tables_destroy(self._h)
+            self._h = None
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+
+class KvCacheArena4:
+    """``KvCacheArena`` in the 4-bit form (include/nva.h: nva_quantize4): head dims 64, 128, 256 and 512,
+    blocks of a multiple of 32 tokens, 34 bytes per 64 values.  Bound with ``Context.bind_kv_cache``,
+    ``Attention`` stores into it and attends over it."""
+
+    def __init__(self, ctx: Context, num_layers: int, num_blocks: int, block_size: int,
+                 num_kv_heads: int, head_dim: int = 0, head_dims: Sequence[int] = None,
+                 allocate: Sequence[bool] = None):
+        hd, al = self._dims(num_layers, head_dim, head_dims, allocate)
+        h = ctypes.c_void_p()
+        _check(ctx.handle, N.load().nva_kv4_create(ctx.handle, len(hd), num_blocks, block_size,
+                                                   num_kv_heads, _ptr(hd), _ptr(al),
+                                                   ctypes.byref(h)), "KvCacheArena4")
+        self._h = h
+        self._ctx = ctx
+        self.num_layers = len(hd)
+        self.num_blocks = num_blocks
+        self.block_size = block_size
+        self.num_kv_heads = num_kv_heads
+        self.head_dims = [int(d) for d in hd]
+
+    @staticmethod
+    def _dims(num_layers, head_dim, head_dims, allocate):
+        if head_dims is None:
+            head_dims = [head_dim] * num_layers
+        if allocate is None:
+            allocate = [True] * len(head_dims)
+        if len(head_dims) != len(allocate):
+            raise IllegalArgumentException("headDims and allocateLayer length mismatch")
+        return np.asarray(head_dims, np.int32), np.asarray([1 if a else 0 for a in allocate],
+                                                           np.uint8)
+
+    @property
+    def handle(self):
+        return self._h
+
+    @staticmethod
+    def blocks_that_fit(ctx: Context, num_layers: int, block_size: int, num_kv_heads: int,
+                        head_dim: int = 0, head_dims: Sequence[int] = None,
+                        allocate: Sequence[bool] = None, fraction: float = 0.9):
+        """``KvCacheArena.blocks_that_fit`` for blocks of this form."""
+        hd, al = KvCacheArena4._dims(num_layers, head_dim, head_dims, allocate)
+        blocks = ctypes.c_int()
+        free = ctypes.c_int64()
+        _check(ctx.handle, N.load().nva_kv4_blocks_that_fit(
+            ctx.handle, len(hd), block_size, num_kv_heads, _ptr(hd), _ptr(al),
+            ctypes.c_float(fraction), ctypes.byref(blocks), ctypes.byref(free)),
+            "KvCacheArena4.blocks_that_fit")
+        return blocks.value, free.value
+
+    def _shape(self, layer: int, rows: int) -> tuple:
+        if not 0 <= layer < self.num_layers:
+            raise IllegalArgumentException(
+                f"layerIndex out of range: {layer} (layers={self.num_layers})")
+        return rows, self.num_kv_heads, self.head_dims[layer]
+
+    def write_rows(self, layer: int, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
+        """Rounds rows of k and v [rows, numKvHeads, headDim] into the slots (an int32 device tensor;
+        slots outside the arena are skipped)."""
+        device = self._ctx.device
+        shape = self._shape(layer, slots.numel())
+        for name, t in (("k", k), ("v", v)):
+            if tuple(t.shape) != shape:
+                raise IllegalArgumentException(f"{name} must be {list(shape)}, got {tuple(t.shape)}")
+        _check(self._ctx.handle, N.load().nva_kv4_write_rows(
+            self._h, layer, _ints(slots, "slots", device), _on(k, "k", device), _on(v, "v", device),
+            shape[0]), "KvCacheArena4.write_rows")
+
+    def read_rows(self, layer: int, slots: torch.Tensor):
+        """(k, v) of the slots, the values they stand for in float32 (zeros outside the arena)."""
+        device = self._ctx.device
+        p = _ints(slots, "slots", device)
+        k, v = (torch.empty(self._shape(layer, slots.numel()), device=slots.device)
+                for _ in range(2))
+        _check(self._ctx.handle, N.load().nva_kv4_read_rows(
+            self._h, layer, p, k.data_ptr(), v.data_ptr(), slots.numel()),
+            "KvCacheArena4.read_rows")
+        return k, v
+
+    def close(self) -> None:
+        if self._h:
+            N.load().nva_kv4_destroy(self._h)
+            self._h = None
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+
+def quantize4(x: torch.Tensor, ctx: Context):
+    """The 4-bit form of x along its last axis (include/nva.h: nva_quantize4): uint8 codes, two a byte,
+    and a scale byte per 32 values."""
+    if x.dim() == 0:
+        raise IllegalArgumentException("x must have at least one dimension")
+    n = x.shape[-1]
+    rows = x.numel() // n if n else 0
+    xp = _on(x, "x", ctx.device)
+    if n % 32:
+        raise UnsupportedShapeError(f"quantize4: 4-bit rows need n % 32 == 0 (got {n})")
+    codes = torch.empty(x.shape[:-1] + (n // 2,), dtype=torch.uint8, device=x.device)
+    scales = torch.empty(x.shape[:-1] + (n // 32,), dtype=torch.uint8, device=x.device)
+    if n:
+        _check(ctx.handle, N.load().nva_quantize4(ctx.handle, xp, rows, n, codes.data_ptr(),
+                                                  scales.data_ptr()), "quantize4")
+    return codes, scales
+
+
+class Linear4:
+    """``Linear`` with its weight in the 4-bit form: ``codes`` [out, in / 2] and ``scales`` [out, in / 32]
+    as ``quantize4`` gives them for [out, in], laid out once for the matrix cores (the tensors are not
+    kept).  ``forward(x, ctx)`` is y = x W^T + b in fp32."""
+
+    def __init__(self, ctx: Context, codes: torch.Tensor, scales: torch.Tensor,
+                 bias: Optional[torch.Tensor] = None):
+        for name, t in (("codes", codes), ("scales", scales)):
+            if not (t.dim() == 2 and t.is_cuda and t.get_device() == ctx.device and
+                    t.dtype is torch.uint8 and t.is_contiguous()):
+                raise IllegalArgumentException(
+                    f"{name} must be a contiguous 2-D uint8 tensor on the context's device")
+        out, inner = codes.shape[0], 2 * codes.shape[1]
+        if tuple(scales.shape) != (out, -(-inner // 32)):
+            raise IllegalArgumentException("scales must be [out, in / 32]")
+        if bias is not None and tuple(bias.shape) != (out,):
+            raise IllegalArgumentException("bias must have out entries")
+        _on(bias, "bias", ctx.device)
+        h = ctypes.c_void_p()
+        _check(ctx.handle, N.load().nva_linear4_create(ctx.handle, codes.data_ptr(),
+                                                       scales.data_ptr(), out, inner,
+                                                       ctypes.byref(h)), "Linear4")
+        self._h = h
+        self.bias = bias
+        self.out_features, self.in_features = out, inner
+
+    @classmethod
+    def from_weight(cls, ctx: Context, weight: torch.Tensor,
+                    bias: Optional[torch.Tensor] = None) -> "Linear4":
+        """Rounds a float32 weight [out, in]."""
+        if weight.dim() != 2:
+            raise IllegalArgumentException("weight must be 2D")
+        return cls(ctx, *quantize4(weight, ctx), bias)
+
+    def forward(self, x: torch.Tensor, ctx: Context) -> torch.Tensor:
+        if x.dim() == 0 or x.shape[-1] != self.in_features:
+            raise IllegalArgumentException("x last dim mismatch")
+        xp = _on(x, "x", ctx.device)
+        y = torch.empty(x.shape[:-1] + (self.out_features,), dtype=torch.float32, device=x.device)
+        _check(ctx.handle, N.load().nva_linear4_forward(
+            ctx.handle, self._h, xp, x.numel() // self.in_features, _on(self.bias, "bias", ctx.device),
+            y.data_ptr()), "Linear4.forward")
+        return y
+
+    def close(self) -> None:
+        if self._h:
+            N.load().nva_linear4_destroy(self._h)
+            self._h = None
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
