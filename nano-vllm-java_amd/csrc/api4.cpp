@@ -131,6 +131,14 @@ nva_status check_tables4(nva_ctx *ctx, const nva_kv4 *kv, int num_tokens) {
   return NVA_OK;
 }
 
+int ctx_kv4_workgroups_per_cu(nva_ctx *ctx, int head_dim, int mode) {
+  const int key = -(head_dim + 1000 * (mode + 1));  // beside the other kernels' keys
+  auto it = ctx->occupancy.find(key);
+  if (it == ctx->occupancy.end())
+    it = ctx->occupancy.emplace(key, kv4_workgroups_per_cu(head_dim, mode)).first;
+  return it->second;
+}
+
 // Growing a buffer of a call that may be captured.
 nva_status reserve_for(nva_ctx *ctx, DevBuf &buf, size_t bytes, bool capturing, const char *what) {
   if (capturing) {
@@ -208,21 +216,52 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
     return fail(ctx, NVA_E_ARG, "slot %lld outside the arena's %lld slots", (long long)ctx->slot_max,
                 (long long)kv->num_blocks * kv->block_size);
 
-  // Work list and partials.
+  // The kernels: sequences of up to 16 columns on the first list, of more on the second.  What the host
+  // knows of their rows bounds them: the lengths themselves, or the most tokens that follow.
   const int seqs = dev ? ctx->dev_seqs : ctx->is_prefill ? ctx->num_seqs : num_tokens;
-  const int64_t cols = (int64_t)num_tokens * rep;
-  const int64_t max_tiles = cols / kKv4Cols + std::min(seqs, num_tokens) + 1;
-  const int workgroups = ctx->num_cus * kv4_workgroups_per_cu(d.head_dim);
-  const size_t off_tiles = 256, off_cum = align256(off_tiles + max_tiles * sizeof(Kv4Tile));
-  const size_t off_before = align256(off_cum + (max_tiles + 1) * 8);
-  const size_t plan_bytes = align256(off_before + ((size_t)seqs + 1) * 4);
-  const size_t parts = (size_t)2 * workgroups * kKv4Cols;
+  int64_t few = 0, many = 0;  // most columns of a sequence on either list
+  const int64_t limit = kv4_has_tiles(d.head_dim) ? 16 : INT32_MAX;
+  auto count = [&](int64_t cols) {
+    if (cols <= limit) few = std::max(few, cols); else many = std::max(many, cols);
+  };
+  if (dev) {
+    const int64_t most = (int64_t)std::min(ctx->dev_max_new, num_tokens) * rep;
+    if (most > limit) many = most;
+    few = std::min(most, limit);
+  } else if (ctx->is_prefill) {
+    for (int b = 0; b < seqs; b++) count((int64_t)(ctx->cu_q[b + 1] - ctx->cu_q[b]) * rep);
+  } else {
+    count(rep);
+  }
+  struct Run {
+    int mode, workgroups;
+    size_t off_head, off_tiles, off_cum, off_before, off_part, parts;
+  } runs[2];
+  int n_runs = 0;
+  size_t plan_bytes = 0, part_floats = 0;
+  auto add = [&](int mode) {
+    Run &r = runs[n_runs++];
+    r.mode = mode;
+    r.workgroups = ctx->num_cus * ctx_kv4_workgroups_per_cu(ctx, d.head_dim, mode);
+    const int cols = kv4_cols(d.head_dim, mode);
+    const int64_t tiles = (int64_t)num_tokens * rep / cols + std::min(seqs, num_tokens) + 1;
+    r.off_head = plan_bytes;
+    r.off_tiles = r.off_head + 256;
+    r.off_cum = align256(r.off_tiles + tiles * sizeof(Kv4Tile));
+    r.off_before = align256(r.off_cum + (tiles + 1) * 8);
+    plan_bytes = align256(r.off_before + ((size_t)seqs + 1) * 4);
+    r.parts = (size_t)2 * r.workgroups * cols;
+    r.off_part = part_floats;
+    part_floats += r.parts * (d.head_dim + 2);
+  };
+  if (many) add(KV4_TILES);
+  // (One list at least: it knows the rows that no sequence covers.)
+  if (few || !many) add(few <= 4 ? KV4_FEW : few <= 8 && kv4_has_tiles(d.head_dim) ? KV4_EIGHT : KV4_ROWS);
   nva_status st = reserve_for(ctx, ctx->d_plan4, plan_bytes, capturing, "attention work list");
   if (st != NVA_OK) return st;
-  st = reserve_for(ctx, ctx->d_part4, parts * (d.head_dim + 2) * 4, capturing, "attention partials");
+  st = reserve_for(ctx, ctx->d_part4, part_floats * 4, capturing, "attention partials");
   if (st != NVA_OK) return st;
   char *plan = static_cast<char *>(ctx->d_plan4.ptr);
-  float *part = static_cast<float *>(ctx->d_part4.ptr);
 
   Kv4Store s{};
   s.kv = view_of(kv, layer);
@@ -230,39 +269,20 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
   s.v = v;
   s.slots = dev ? dev->slots : ctx->dev_i32(ctx->off_slots);
   s.tokens = num_tokens;
-  s.list.head = reinterpret_cast<Kv4Head *>(plan);
-  s.list.tiles = reinterpret_cast<Kv4Tile *>(plan + off_tiles);
-  s.list.cum = reinterpret_cast<int64_t *>(plan + off_cum);
-  s.list.before = reinterpret_cast<int32_t *>(plan + off_before);
-  if (dev) {
-    s.list.cu_q = dev->cu_q;
-    s.list.lens = dev->lens;
-  } else if (ctx->is_prefill) {
-    s.list.cu_q = ctx->dev_i32(ctx->off_cu_q);
-    s.list.cu_k = ctx->dev_i32(ctx->off_cu_k);
-  } else {
-    s.list.lens = ctx->dev_i32(ctx->off_ctx);
-  }
-  s.list.num_seqs = seqs;
-  s.list.rep = rep;
-  s.list.hkv = d.num_kv_heads;
-  s.list.window = d.sliding_window;
-  s.list.workgroups = workgroups;
-  {
-    Timed tm(ctx, "store4");
-    HIP_TRY(ctx, launch_kv4_store(s, d.head_dim, ctx->stream), "4-bit store kernel launch");
-    tm.done();
-  }
+  s.lists = n_runs;
   Kv4Attention a{};
   a.kv = s.kv;
   a.q = q;
   a.out = out;
-  a.head = s.list.head;
-  a.tiles = s.list.tiles;
-  a.cum = s.list.cum;
-  a.cu_q = s.list.cu_q;
-  a.cu_k = s.list.cu_k;
-  a.lens = s.list.lens;
+  if (dev) {
+    a.cu_q = dev->cu_q;
+    a.lens = dev->lens;
+  } else if (ctx->is_prefill) {
+    a.cu_q = ctx->dev_i32(ctx->off_cu_q);
+    a.cu_k = ctx->dev_i32(ctx->off_cu_k);
+  } else {
+    a.lens = ctx->dev_i32(ctx->off_ctx);
+  }
   a.table = dev ? dev->table : ctx->dev_i32(ctx->off_tables);
   a.bt_stride = dev ? dev->width : ctx->bt_stride;
   a.hq = d.num_heads;
@@ -271,18 +291,50 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
   a.tokens = num_tokens;
   a.tile_shift = shift_of(kv->block_size / 32);
   a.scale2 = (float)((double)d.scale * 1.4426950408889634074);
-  a.part_m = part;
-  a.part_l = part + parts;
-  a.part_o = part + 2 * parts;
+  for (int i = 0; i < n_runs; i++) {
+    const Run &r = runs[i];
+    Kv4List &l = s.list[i];
+    l.head = reinterpret_cast<Kv4Head *>(plan + r.off_head);
+    l.tiles = reinterpret_cast<Kv4Tile *>(plan + r.off_tiles);
+    l.cum = reinterpret_cast<int64_t *>(plan + r.off_cum);
+    l.before = reinterpret_cast<int32_t *>(plan + r.off_before);
+    l.cu_q = a.cu_q;
+    l.cu_k = a.cu_k;
+    l.lens = a.lens;
+    l.num_seqs = seqs;
+    l.rep = rep;
+    l.hkv = d.num_kv_heads;
+    l.window = d.sliding_window;
+    l.workgroups = r.workgroups;
+    l.cols = kv4_cols(d.head_dim, r.mode);
+    l.min_cols = r.mode == KV4_TILES ? (int)limit + 1 : 1;
+    l.max_cols = r.mode == KV4_TILES ? INT32_MAX : (int)limit;
+    l.unit = r.mode == KV4_TILES ? 1 : 4;
+    l.min_units = r.mode == KV4_TILES ? 4 : 8;
+  }
   {
-    Timed tm(ctx, "attention4");
-    HIP_TRY(ctx, launch_kv4_attention(a, workgroups, ctx->stream), "4-bit attention kernel launch");
+    Timed tm(ctx, "store4");
+    HIP_TRY(ctx, launch_kv4_store(s, d.head_dim, ctx->stream), "4-bit store kernel launch");
     tm.done();
   }
-  Timed tm(ctx, "merge4");
-  HIP_TRY(ctx, launch_kv4_merge(a, (int)std::min<int64_t>(max_tiles, INT32_MAX), ctx->stream),
-          "4-bit merge kernel launch");
-  tm.done();
+  for (int i = 0; i < n_runs; i++) {
+    const Run &r = runs[i];
+    a.head = s.list[i].head;
+    a.tiles = s.list[i].tiles;
+    a.cum = s.list[i].cum;
+    float *part = static_cast<float *>(ctx->d_part4.ptr) + r.off_part;
+    a.part_m = part;
+    a.part_l = part + r.parts;
+    a.part_o = part + 2 * r.parts;
+    a.zero_rest = i == 0;
+    Timed tm(ctx, "attention4");
+    HIP_TRY(ctx, launch_kv4_attention(a, r.mode, r.workgroups, ctx->stream),
+            "4-bit attention kernel launch");
+    tm.done();
+    Timed tg(ctx, "merge4");
+    HIP_TRY(ctx, launch_kv4_merge(a, r.mode, r.workgroups, ctx->stream), "4-bit merge kernel launch");
+    tg.done();
+  }
   return NVA_OK;
 }
 

@@ -2,22 +2,25 @@
 // attention and the merge of split rows.
 //
 // Layout.  A layer is [block][KV head][tile of 32 keys][34 d bytes], a tile's bytes being
-//   K codes   [key 32][d / 2]            dim 2j in the low bits of byte j
-//   V codes   [quarter 4][row 16][slot 8][d / 32]
-//   K scales  [key % 16][d / 32][key / 16]
-//   V scales  [quarter 4][d / 32][slot 8]
-// where slot s of quarter w is key 16 (s / 4) + 4 w + s % 4, and row r holds dims r d / 16 and on.  Lane
-// l = 16 w + r of a wave thus reads its part of either product in one run of bytes, which neighbouring lanes
-// continue, and a token's codes stay apart from its neighbours' (4-byte words at d = 128), so that tokens
-// are stored independently.
+//   K codes   [key % 2][key / 2][d / 2]       dim 2j in the low bits of byte j
+//   V codes   [key / 8][row 16][key % 8][d / 32]   row r: dims r d / 16 and on
+//   K scales  [key / 2][d / 32][key % 2]
+//   V scales  [key / 8][d / 32][key % 8]
+// Lane l = 16 w + c of a wave thus reads its part of either product in one run of bytes, which neighbouring
+// lanes continue, and a token's codes stay apart from its neighbours' (4-byte words at d = 128), so that
+// tokens are stored independently.
 //
-// Products on the matrix cores (16 x 16 x 32 bf16): S^T = K Q^T with keys as rows and columns (query row,
-// head of the KV head) as columns, then O^T += V^T P^T with dims as rows.  The order of the contraction is
-// free, so that of the dims follows K's bytes (lane quarter w takes dims w d / 4 and on: its scale is its
-// own), and that of the keys the accumulators of S^T: lane 16 w + c holds keys 4 w .. 4 w + 3 of both
-// 16-key halves for column c, which is what the second product wants of P^T, given V's slots above.  No
-// value crosses lanes but the column maxima.  The 4-bit values are exact in bf16; q and p go in as three
-// bf16 parts whose sum they are (split3), so the products are those of fp32.
+// Products on the matrix cores (16 x 16 x 32 bf16; operands hold 8 values of the contraction a lane,
+// results rows 4 w .. 4 w + 3 of column c).  The order of the contraction is free: that of the dims follows
+// K's bytes (lane quarter w takes dims w d / 4 and on, so its scale is its own), that of the keys gives
+// quarter w keys 8 w .. 8 w + 7, and the two halves of a tile are its even and its odd keys.
+//   Few columns (query rows times heads of a KV head): S = Q K^T with a column's three parts as three
+//   rows, 4 h + part, so that lane (w, c) has all parts of column w and keys 2c and 2c + 1: no score is
+//   computed twice.  P goes through 1 KB of LDS to be an operand of O = P V, whose rows again are parts.
+//   Many: S^T = K Q^T, where lane (w, c) has column c and keys 8 w .. 8 w + 7, which is what O^T = V^T P^T
+//   wants of P^T; nothing crosses lanes but the column maxima.
+// The 4-bit values are exact in bf16; q and p go in as three bf16 parts whose sum they are (split3), so the
+// products are those of fp32.
 #include "mx4.h"
 #include "nva_internal.h"
 #include "row_lanes.h"
@@ -27,7 +30,6 @@ namespace nva {
 namespace {
 
 constexpr int kWaves = 4;
-constexpr int kCols = kKv4Cols;
 
 __device__ __forceinline__ size_t tile_at(const Kv4View &kv, int block, int head, int tile, int d) {
   return (((size_t)block * kv.hkv + head) * (kv.block_size >> 5) + tile) * (size_t)(34 * d);
@@ -38,12 +40,12 @@ struct RowPlace {
   int k, v, ks, vs;  // byte offsets in the tile; v for d >= 128
 };
 __device__ __forceinline__ RowPlace row_place(int d, int key, int i) {
-  const int nb = d >> 5, w = (key & 15) >> 2, slot = ((key >> 4) << 2) | (key & 3);
+  const int nb = d >> 5, w = key >> 3, slot = key & 7;
   RowPlace p;
-  p.k = key * (d >> 1) + 4 * i;
+  p.k = ((key & 1) * 16 + (key >> 1)) * (d >> 1) + 4 * i;
   const int per = d >> 4, r = (8 * i) / per, within = (8 * i - r * per) >> 1;
   p.v = 16 * d + ((w * 16 + r) * 8 + slot) * nb + within;
-  p.ks = 32 * d + ((key & 15) * nb + (i >> 2)) * 2 + (key >> 4);
+  p.ks = 32 * d + ((key >> 1) * nb + (i >> 2)) * 2 + (key & 1);
   p.vs = 33 * d + (w * nb + (i >> 2)) * 8 + slot;
   return p;
 }
@@ -78,7 +80,7 @@ __device__ __forceinline__ void store_row(const Kv4View &kv, const float *src, i
 
 // ---------------------------------------------------------------- the work list
 
-// Column tiles: runs of kCols columns of one sequence, column c being query row c / rep and head c % rep
+// Column tiles: runs of a.cols columns of one sequence, column c being query row c / rep and head c % rep
 // of each KV head, over the 32-key tiles [kb, kb + n) that any of their rows sees.  Units are key tiles,
 // numbered by column tile, KV head and tile; workgroup g of the attention takes units [g C, (g + 1) C), so
 // every workgroup does the same work however lengths differ.  cum[t] is the units of one KV head before
@@ -111,8 +113,8 @@ __device__ void build_list(const Kv4List &a) {
     const int b = b0 + tid;
     int64_t mine = 0, all;
     if (b < a.num_seqs) {
-      const int qlen = a.cu_q ? a.cu_q[b + 1] - a.cu_q[b] : 1;
-      mine = ((int64_t)qlen * rep + kCols - 1) / kCols;
+      const int64_t cols = (int64_t)(a.cu_q ? a.cu_q[b + 1] - a.cu_q[b] : 1) * rep;
+      if (cols >= a.min_cols && cols <= a.max_cols) mine = (cols + a.cols - 1) / a.cols;
     }
     const int64_t at = tiles + scan(mine, all);
     if (b < a.num_seqs) a.before[b] = (int32_t)at;
@@ -135,9 +137,9 @@ __device__ void build_list(const Kv4List &a) {
       const int row = a.cu_q ? a.cu_q[lo] : lo;
       const int qlen = a.cu_q ? a.cu_q[lo + 1] - row : 1;
       const int klen = a.lens ? a.lens[lo] : a.cu_k[lo + 1] - a.cu_k[lo];
-      const int64_t col0 = (int64_t)(t - a.before[lo]) * kCols;
+      const int64_t col0 = (int64_t)(t - a.before[lo]) * a.cols;
       const int first = (int)(col0 / rep);
-      const int last = (int)min((int64_t)qlen - 1, (col0 + kCols - 1) / rep);
+      const int last = (int)min((int64_t)qlen - 1, (col0 + a.cols - 1) / rep);
       const int end = min(klen, klen - qlen + last + 1);
       const int64_t beg = a.window > 0 ? (int64_t)klen - qlen + first + 1 - a.window : 0;
       tile.seq = lo;
@@ -156,25 +158,25 @@ __device__ void build_list(const Kv4List &a) {
   if (tid == 0) {
     a.cum[tiles] = units;
     a.head->tiles = (int)tiles;
-    // At least kKv4MinUnits a workgroup: fewer would be spent on joining their results.
+    // A multiple of the waves that share a segment, and not so few units that joining costs more.
     const int64_t all = units * a.hkv;
     const int64_t c = (all + a.workgroups - 1) / a.workgroups;
-    a.head->chunk = max((c + kWaves - 1) / kWaves * kWaves, (int64_t)kKv4MinUnits);
+    a.head->chunk = max((c + a.unit - 1) / a.unit * a.unit, (int64_t)a.min_units);
     a.head->covered = a.cu_q ? a.cu_q[a.num_seqs] : a.num_seqs;
     a.head->first = a.cu_q ? a.cu_q[0] : 0;
   }
 }
 
-// Stores the step's rows and builds its list: workgroup 0 the list, the others 256 / (D / 8) rows of K or
-// V each.
+// Stores the step's rows and builds its lists: the first workgroups a list each, the others
+// 256 / (D / 8) rows of K or V each.
 template <int D>
 __global__ void __launch_bounds__(256) kv4_store_kernel(Kv4Store a) {
-  if (blockIdx.x == 0) {
-    if (a.list.head) build_list(a.list);
+  if ((int)blockIdx.x < a.lists) {
+    build_list(a.list[blockIdx.x]);
     return;
   }
   constexpr int LPR = D / 8, ROWS = 256 / LPR;
-  const int64_t row = (int64_t)(blockIdx.x - 1) * ROWS + threadIdx.x / LPR;
+  const int64_t row = (int64_t)(blockIdx.x - a.lists) * ROWS + threadIdx.x / LPR;
   const int64_t half = (int64_t)a.tokens * a.kv.hkv;
   if (row >= 2 * half) return;  // (whole quads)
   const bool is_v = row >= half;
@@ -229,37 +231,57 @@ template <int D> struct Tile {
   u32x2 vs;
 };
 
-template <int N> __device__ __forceinline__ void load_words(const uint8_t *p, uint32_t *w) {
+// N words from byte `at` of a tile.  NT: keys read once (without the non-temporal bit a decode step's reads
+// push everything else out).
+template <int N, bool NT>
+__device__ __forceinline__ void load_words(__amdgpu_buffer_rsrc_t tile, uint32_t at, uint32_t *w) {
+  constexpr int kPolicy = NT ? 2 : 0;
   if constexpr (N >= 4) {
 #pragma unroll
     for (int i = 0; i < N / 4; i++) {
-      const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p) + i);
+      const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(tile, at + 16 * i, 0, kPolicy);
 #pragma unroll
       for (int j = 0; j < 4; j++) w[4 * i + j] = x[j];
     }
-  } else {
-    static_assert(N == 2, "8 bytes");
-    const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(p));
+  } else if constexpr (N == 2) {
+    const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(tile, at, 0, kPolicy);
     w[0] = x.x, w[1] = x.y;
+  } else {
+    w[0] = __builtin_amdgcn_raw_buffer_load_b32(tile, at, 0, kPolicy);
   }
 }
 
-template <int D>
-__device__ __forceinline__ void load_tile(const uint8_t *tile, int lane, Tile<D> &t) {
+// Where a lane's parts lie in a tile.
+struct TilePlaces {
+  uint32_t k, v, ks, vs;
+};
+template <int D> __device__ __forceinline__ TilePlaces tile_places(int lane) {
   constexpr int NB = D / 32;
   const int c = lane & 15, w = lane >> 4;
-  load_words<D / 32>(tile + c * (D / 2) + w * (D / 8), t.k[0]);
-  load_words<D / 32>(tile + (16 + c) * (D / 2) + w * (D / 8), t.k[1]);
-  load_words<D / 16>(tile + 16 * D + lane * (D / 4), t.v);
-  const uint8_t *ks = tile + 32 * D + (c * NB + (w * D) / 128) * 2;
-  if constexpr (D == 512) {
-    load_words<2>(ks, t.ks);
-  } else if constexpr (D == 256) {
-    t.ks[0] = *reinterpret_cast<const uint32_t *>(ks);
-  } else {
-    t.ks[0] = *reinterpret_cast<const uint16_t *>(ks);
-  }
-  t.vs = *reinterpret_cast<const u32x2 *>(tile + 33 * D + (w * NB + (c * D) / 512) * 8);
+  return {(uint32_t)(c * (D / 2) + w * (D / 8)), (uint32_t)(16 * D + lane * (D / 4)),
+          (uint32_t)(32 * D + (c * NB + (w * D) / 128) * 2),
+          (uint32_t)(33 * D + (w * NB + (c * D) / 512) * 8)};
+}
+
+// As buffer loads: the tile's address stays in scalar registers and the lane's places do not change, so that
+// no address is computed in registers that loads in flight are still to be written to (which would wait for
+// them).
+template <int D, bool NT>
+__device__ __forceinline__ void load_tile(const uint8_t *at, const TilePlaces &p, Tile<D> &t) {
+  const __amdgpu_buffer_rsrc_t tile = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t *>(at), (short)0, 34 * D, kBufferWord3);
+  load_words<D / 32, NT>(tile, p.k, t.k[0]);
+  load_words<D / 32, NT>(tile, p.k + 8 * D, t.k[1]);
+  load_words<D / 16, NT>(tile, p.v, t.v);
+  if constexpr (D == 512)
+    load_words<2, NT>(tile, p.ks, t.ks);
+  else if constexpr (D == 256)
+    load_words<1, NT>(tile, p.ks, t.ks);
+  else
+    t.ks[0] = __builtin_amdgcn_raw_buffer_load_b16(tile, p.ks, 0, NT ? 2 : 0);
+  uint32_t vs[2];
+  load_words<2, NT>(tile, p.vs, vs);
+  t.vs = u32x2{vs[0], vs[1]};
 }
 
 __device__ __forceinline__ uint32_t byte_of(uint32_t word, int i) { return (word >> (8 * i)) & 255u; }
@@ -280,6 +302,10 @@ __device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) {
 __device__ __forceinline__ bf16x8 frag(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   const u32x4 w = {a, b, c, d};
   return __builtin_bit_cast(bf16x8, w);
+}
+
+__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
 // Byte b of every slot: the dims 2 b and 2 b + 1 of the lane's row, over its 8 slots.
@@ -303,19 +329,41 @@ __device__ __forceinline__ void v_frags(const Tile<D> &t, const float *unit, bf1
              high_halves(p[6], p[7]));
 }
 
-template <int D, int B = 0>
-__device__ __forceinline__ void add_values(const Tile<D> &t, const float *unit, const bf16x8 *p,
-                                           f32x4 *o) {
+// O += P V (FEW) or O^T += V^T P^T.
+template <int D, int NG, int NP, bool FEW, int B = 0>
+__device__ __forceinline__ void add_values(const Tile<D> &t, const float *unit, const bf16x8 (*p)[NP],
+                                           f32x4 (*o)[D / 16]) {
   if constexpr (B < D / 32) {
     bf16x8 even, odd;
     v_frags<D, B>(t, unit, even, odd);
 #pragma unroll
-    for (int i = 0; i < 3; i++) {
-      o[2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, p[i], o[2 * B], 0, 0, 0);
-      o[2 * B + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, p[i], o[2 * B + 1], 0, 0, 0);
-    }
-    add_values<D, B + 1>(t, unit, p, o);
+    for (int i = 0; i < NP; i++)
+#pragma unroll
+      for (int g = 0; g < NG; g++) {
+        o[g][2 * B] = FEW ? mfma(p[g][i], even, o[g][2 * B]) : mfma(even, p[g][i], o[g][2 * B]);
+        o[g][2 * B + 1] = FEW ? mfma(p[g][i], odd, o[g][2 * B + 1]) : mfma(odd, p[g][i], o[g][2 * B + 1]);
+      }
+    add_values<D, NG, NP, FEW, B + 1>(t, unit, p, o);
   }
+}
+
+// The maximum or sum over the 16 lanes of a row, in every lane.
+__device__ __forceinline__ float max16(float x) {
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) x = fmaxf(x, __shfl_xor(x, d));
+  return x;
+}
+__device__ __forceinline__ float sum16(float x) {
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) x += __shfl_xor(x, d);
+  return x;
+}
+
+// A wave-uniform load of what earlier launches wrote, through the scalar cache: it waits on a counter of its
+// own, where a vector load would wait for every key in flight.
+template <typename T> __device__ __forceinline__ T uniform(const T *p) {
+  typedef const T __attribute__((address_space(4))) * scalar;
+  return *(scalar)(uintptr_t)p;
 }
 
 // The 64-ary search for the last entry of cum that u reaches (times hkv), by a wave: tile of unit u.
@@ -332,300 +380,517 @@ __device__ __forceinline__ int find_tile(const int64_t *cum, int n, int64_t u, i
   return lo;
 }
 
+// Words between rows of P in LDS.
+constexpr int kPRow = 20;
+
+// How far scores may pass the reference that probabilities are taken relative to before it is raised:
+// they are then below 2^kSlack, which fp32 holds as exactly as those below 1.
+constexpr float kSlack = 40.f;
+
 }  // namespace
 
-// Workgroup g: its units' segments, each of one column tile and KV head.  The four waves take a segment's
-// key tiles in turn, each with the running maximum and sum of a softmax, and join through LDS.  A segment
-// that covers its keys is written out; others leave partials (slot 2 g for the workgroup's first, of keys
-// another one began, 2 g + 1 for its last), which kv4_merge_kernel joins.
-template <int D>
-__global__ void __launch_bounds__(256, kv4_workgroups_per_cu(D)) kv4_attention_kernel(Kv4Attention a) {
-  constexpr bool QLDS = D == 512;  // 192 registers of q's parts would leave none for the loads
-  constexpr int NC = D / 32;       // contraction steps of a score
+// Workgroup g: its units' segments, each of one column tile and KV head, with the running reference and
+// sum of a softmax.  A segment that covers its keys is written out; others leave partials (slot 2 g for
+// the workgroup's first, of keys another one began, 2 g + 1 for its last), which kv4_merge_kernel joins.
+//   KV4_FEW, KV4_EIGHT   NG groups of 4 columns, their parts as rows; the four waves take the key tiles in
+//                        turn and join through LDS
+//   KV4_ROWS             16 columns, three products; the waves as above
+//   KV4_TILES            NG groups of 16 columns a wave, four waves of columns over the same key tiles
+template <int D, int MODE, int NG>
+__global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_kernel(Kv4Attention a) {
+  constexpr bool FEW = MODE == KV4_FEW || MODE == KV4_EIGHT, TILES = MODE == KV4_TILES;
+  constexpr int NP = FEW ? 1 : 3;
+  constexpr bool QLDS = D == 512 && !FEW;  // 192 registers of q's parts would leave none for the loads
+  constexpr bool AHEAD = D < 512;          // the next tile's loads before this one's products
+  constexpr int NC = D / 32;               // contraction steps of a score
+  constexpr int COLS = kv4_cols(D, MODE);
+  constexpr int E = D / 16;                // dims of a row of V
+  static_assert(COLS == (FEW ? 4 : TILES ? 64 : 16) * NG, "the columns of a tile");
   extern __shared__ float4 smem[];
-  float *lds_o = reinterpret_cast<float *>(smem);        // [wave][col][D + 4]
-  float *lds_m = lds_o + kWaves * kCols * (D + 4), *lds_l = lds_m + kWaves * kCols;
-  bf16x8 *lds_q = reinterpret_cast<bf16x8 *>(smem);      // (QLDS) [part][step][lane], before lds_o
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, w = lane >> 4;
-  const int n_tiles = a.head->tiles;
-  const int64_t chunk = a.head->chunk;
-  const int64_t all = a.cum[n_tiles] * a.kv.hkv;
+  float *lds_o = reinterpret_cast<float *>(smem);  // [wave][col][D + 4]
+  float *lds_m = lds_o + kWaves * COLS * (D + 4), *lds_l = lds_m + kWaves * COLS;
+  bf16x8 *lds_q = reinterpret_cast<bf16x8 *>(smem);  // (QLDS) [part][step][lane], before lds_o
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, w = lane >> 4;
+  // (FEW) the wave's P, [group][row 16][key 32] bf16, rows kPRow words apart (no bank conflicts in either
+  // direction); rows of part 3 are zero.
+  uint32_t *lds_p = reinterpret_cast<uint32_t *>(lds_l + kWaves * COLS) + wave * (NG * 16 * kPRow);
+  if constexpr (FEW)
+    for (int i = lane; i < NG * 16 * kPRow; i += 64) lds_p[i] = 0;
+  const int n_tiles = uniform(&a.head->tiles);
+  const int64_t chunk = uniform(&a.head->chunk);
+  const int64_t all = uniform(a.cum + n_tiles) * a.kv.hkv;
   int64_t u = (int64_t)blockIdx.x * chunk;
   const int64_t u_end = min(u + chunk, all);
   if (u >= u_end) return;
   const int rep = a.hq / a.kv.hkv;
   const int per_block = a.kv.block_size >> 5;
-  int ct = find_tile(a.cum, n_tiles, u, a.kv.hkv, lane);
+  const TilePlaces places = tile_places<D>(lane);
+  int ct = __builtin_amdgcn_readfirstlane(find_tile(a.cum, n_tiles, u, a.kv.hkv, lane));
   while (u < u_end) {
-    while (a.tiles[ct].n == 0 || u >= a.cum[ct + 1] * a.kv.hkv) ct++;  // (u is below the last entry's)
-    const Kv4Tile tile = a.tiles[ct];
-    const int64_t in = u - a.cum[ct] * a.kv.hkv;
+    while (uniform(&a.tiles[ct].n) == 0 || u >= uniform(a.cum + ct + 1) * a.kv.hkv) ct++;  // (u is below the last entry's)
+    const Kv4Tile tile{uniform(&a.tiles[ct].seq), uniform(&a.tiles[ct].col0), uniform(&a.tiles[ct].kb),
+                       uniform(&a.tiles[ct].n)};
+    const int64_t in = u - uniform(a.cum + ct) * a.kv.hkv;
     const int head = (int)(in / tile.n);
     const int t0 = (int)(in - (int64_t)head * tile.n);
     const int t1 = (int)min((int64_t)tile.n, t0 + (u_end - u));
-    // The lane's column: its query row and head, and the keys [lo, hi) that it sees.
     const int seq = tile.seq;
-    const int row0 = a.cu_q ? a.cu_q[seq] : seq;
-    const int qlen = a.cu_q ? a.cu_q[seq + 1] - row0 : 1;
-    const int klen = a.lens ? a.lens[seq] : a.cu_k[seq + 1] - a.cu_k[seq];
+    const int row0 = a.cu_q ? uniform(a.cu_q + seq) : seq;
+    const int qlen = a.cu_q ? uniform(a.cu_q + seq + 1) - row0 : 1;
+    const int klen = a.lens ? uniform(a.lens + seq) : uniform(a.cu_k + seq + 1) - uniform(a.cu_k + seq);
     const int64_t cols = (int64_t)qlen * rep;
-    const int64_t col = min((int64_t)tile.col0 + c, cols - 1);  // (columns past the last repeat it)
-    const int qrow = (int)(col / rep);
-    const int hi = klen - qlen + qrow + 1;
-    const int lo = a.window > 0 ? max(0, hi - a.window) : 0;
-    const float *qp = a.q + ((size_t)(row0 + qrow) * a.hq + (size_t)head * rep + (col - (int64_t)qrow * rep)) * D;
-    bf16x8 q[QLDS ? 1 : NC][3];
-    if constexpr (QLDS) {
-      __syncthreads();  // the last segment's results have been read
-      for (int j = wave; j < NC; j += kWaves) {
-        bf16x8 p[3];
-        float x[8];
-        *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(qp + w * (D / 4) + 8 * j);
-        *reinterpret_cast<float4 *>(x + 4) = *reinterpret_cast<const float4 *>(qp + w * (D / 4) + 8 * j + 4);
-        split3<false>(x, p);
-        for (int i = 0; i < 3; i++) lds_q[(i * NC + j) * 64 + lane] = p[i];
-      }
-      __syncthreads();
-    } else {
+    const int64_t first_col = (int64_t)tile.col0 + (TILES ? wave * (16 * NG) : 0);
+    const bool whole = t0 == 0 && t1 == tile.n;
+    const int64_t part0 = (int64_t)(2 * blockIdx.x + (t0 == 0 ? 1 : 0)) * COLS;
+    u += t1 - t0;
+    if (TILES && first_col >= cols) continue;  // (a wave by itself: these waves meet at no barrier)
+    // The columns whose scores the lane has see keys [lo, hi).  (Columns past the last repeat it.)
+    int hi[NG], lo[NG];
+    bf16x8 q[NG][QLDS ? 1 : NC][NP];
+    int all_hi = INT32_MAX, all_lo = 0, any_hi = 0, any_lo = INT32_MAX;
+    if constexpr (QLDS) __syncthreads();  // the last segment's results have been read
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+      const int64_t scol = min(first_col + (FEW ? 4 * g + w : 16 * g + c), cols - 1);
+      hi[g] = klen - qlen + (int)(scol / rep) + 1;
+      lo[g] = a.window > 0 ? max(0, hi[g] - a.window) : 0;
+      all_hi = min(all_hi, hi[g]);
+      any_hi = max(any_hi, hi[g]);
+      all_lo = max(all_lo, lo[g]);
+      any_lo = min(any_lo, lo[g]);
+      // The column of q that the lane loads.
+      const int64_t col = FEW ? min(first_col + 4 * g + (c >> 2), cols - 1) : scol;
+      const int qrow = (int)(col / rep);
+      const float *qp =
+          a.q + ((size_t)(row0 + qrow) * a.hq + (size_t)head * rep + (col - (int64_t)qrow * rep)) * D;
 #pragma unroll
       for (int j = 0; j < NC; j++) {
+        if (QLDS && j % kWaves != wave) continue;
         float x[8];
         *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(qp + w * (D / 4) + 8 * j);
-        *reinterpret_cast<float4 *>(x + 4) = *reinterpret_cast<const float4 *>(qp + w * (D / 4) + 8 * j + 4);
-        split3<false>(x, q[j]);
+        *reinterpret_cast<float4 *>(x + 4) =
+            *reinterpret_cast<const float4 *>(qp + w * (D / 4) + 8 * j + 4);
+        // Scores come out in units of log2 (one rounding of q more).
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] *= a.scale2;
+        bf16x8 p[3];
+        split3<false>(x, p);
+        if constexpr (FEW) {
+          const bf16x8 zero = {};
+          q[g][j][0] = (c & 3) == 0 ? p[0] : (c & 3) == 1 ? p[1] : (c & 3) == 2 ? p[2] : zero;
+        } else if constexpr (QLDS) {
+#pragma unroll
+          for (int i = 0; i < 3; i++) lds_q[(i * NC + j) * 64 + lane] = p[i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 3; i++) q[g][j][i] = p[i];
+        }
       }
     }
-    // Tiles that every column sees whole need no mask.
-    int all_hi = hi, all_lo = lo;
+    if constexpr (QLDS) __syncthreads();
+    // Tiles that every column sees whole need no mask, those that none sees no work.
 #pragma unroll
-    for (int d = 1; d < 16; d <<= 1) {
+    for (int d = FEW ? 16 : 1; d < (FEW ? 64 : 16); d <<= 1) {
       all_hi = min(all_hi, __shfl_xor(all_hi, d));
       all_lo = max(all_lo, __shfl_xor(all_lo, d));
+      any_hi = max(any_hi, __shfl_xor(any_hi, d));
+      any_lo = min(any_lo, __shfl_xor(any_lo, d));
     }
     all_hi = __builtin_amdgcn_readfirstlane(all_hi);
     all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+    // The wave's key tiles of the segment (each is below 2^26).
+    int tb = t0, te = t1;
+    if constexpr (TILES) {
+      any_hi = __builtin_amdgcn_readfirstlane(any_hi);
+      any_lo = __builtin_amdgcn_readfirstlane(any_lo);
+      tb = max(tb, (any_lo >> 5) - tile.kb);
+      te = min(te, (max(any_hi, 0) + 31) / 32 - tile.kb);
+    }
+    constexpr int STRIDE = TILES ? 1 : kWaves;
 
-    f32x4 o[D / 16];
+    f32x4 o[NG][E];
+    float m[NG], l[NG];
+    uint32_t nan[NG];
 #pragma unroll
-    for (int i = 0; i < D / 16; i++) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
+    for (int g = 0; g < NG; g++) {
+      nan[g] = 0;
+      m[g] = -INFINITY;
+      l[g] = 0.f;
+#pragma unroll
+      for (int i = 0; i < E; i++) o[g][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
     const int32_t *table = a.table + (size_t)seq * a.bt_stride;
-    auto address = [&](int t) {  // of key tile t
+    // Key tile t's place among its block's tiles, and its block.
+    auto block_index = [&](int t) {
       const int kt = tile.kb + t;
-      const int bi = a.tile_shift >= 0 ? kt >> a.tile_shift : kt / per_block;
-      const int block = __builtin_amdgcn_readfirstlane(table[bi]);
-      return a.kv.pages + tile_at(a.kv, block, head, kt - bi * per_block, D);
+      return a.tile_shift >= 0 ? kt >> a.tile_shift : kt / per_block;
     };
-    constexpr bool AHEAD = D < 512;  // the next tile's loads before this one's products
-    Tile<D> cur, next;
-    int t = t0 + wave;
-    if (AHEAD && t < t1) load_tile<D>(address(t), lane, cur);
-    for (; t < t1; t += kWaves) {
-      if (!AHEAD) load_tile<D>(address(t), lane, cur);
-      if (AHEAD && t + kWaves < t1) load_tile<D>(address(t + kWaves), lane, next);
-      // Scores of the 32 keys.
-      f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+    auto block_of = [&](int t) { return uniform(table + block_index(t)); };
+    auto load = [&](int t, int block, Tile<D> &into) {
+      const int in_block = tile.kb + t - block_index(t) * per_block;
+      load_tile<D, !TILES>(a.kv.pages + tile_at(a.kv, block, head, in_block, D), places, into);
+      // The loads go out before the products of the tile at hand (the compiler would have them wait for
+      // that tile, whose registers it could then use again).
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto attend = [&](int t, Tile<D> &cur) {
+      // Scores of the 32 keys, of either half of them.
+      f32x4 s[NG][2];
+#pragma unroll
+      for (int g = 0; g < NG; g++) s[g][0] = s[g][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < NC; j++) {
         const bf16x8 k0 = mx4_frag(cur.k[0][j], k_unit<D>(cur, j, 0));
         const bf16x8 k1 = mx4_frag(cur.k[1][j], k_unit<D>(cur, j, 1));
 #pragma unroll
-        for (int i = 0; i < 3; i++) {
-          bf16x8 qv;
-          if constexpr (QLDS) qv = lds_q[(i * NC + j) * 64 + lane]; else qv = q[j][i];
-          s[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, qv, s[0], 0, 0, 0);
-          s[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, qv, s[1], 0, 0, 0);
-        }
+        for (int g = 0; g < NG; g++)
+#pragma unroll
+          for (int i = 0; i < NP; i++) {
+            bf16x8 qv;
+            if constexpr (QLDS) qv = lds_q[(i * NC + j) * 64 + lane]; else qv = q[g][j][i];
+            s[g][0] = FEW ? mfma(qv, k0, s[g][0]) : mfma(k0, qv, s[g][0]);
+            s[g][1] = FEW ? mfma(qv, k1, s[g][1]) : mfma(k1, qv, s[g][1]);
+          }
       }
       const int key0 = (tile.kb + t) * 32;
       const bool edge = key0 + 32 > all_hi || key0 < all_lo;
-      float x[8];
+      constexpr int NX = FEW ? 2 : 8;  // scores of a lane and column: keys NX (lane's) .. + NX - 1
+      const int mine = key0 + NX * (FEW ? c : w);
+      bf16x8 p[NG][NP];
 #pragma unroll
-      for (int i = 0; i < 8; i++) x[i] = s[i >> 2][i & 3] * a.scale2;
-      if (edge) {
+      for (int g = 0; g < NG; g++) {
+        float x[NX];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const int key = key0 + 16 * (i >> 2) + 4 * w + (i & 3);
-          if (key >= hi || key < lo) x[i] = -INFINITY;
+        for (int i = 0; i < NX; i++) {
+          if constexpr (FEW)
+            x[i] = s[g][i][0] + (s[g][i][1] + s[g][i][2]);
+          else
+            x[i] = s[g][i & 1][i >> 1];
+        }
+        if (edge) {
+#pragma unroll
+          for (int i = 0; i < NX; i++)
+            if (mine + i >= hi[g] || mine + i < lo[g]) x[i] = -INFINITY;
+        }
+        float top = fmaxf(x[0], x[1]);
+#pragma unroll
+        for (int i = 2; i < NX; i++) top = fmaxf(top, x[i]);
+        if (__any(top > m[g] + kSlack)) {
+          if constexpr (FEW) top = max16(top); else top = max4_lanes(top);
+          const float grown = top > m[g] + kSlack ? top : m[g];
+          const float f = m[g] == grown ? 1.f : __builtin_amdgcn_exp2f(m[g] - grown);  // 0 from -infinity
+          m[g] = grown;
+          l[g] *= f;
+#pragma unroll
+          for (int i = 0; i < E; i++) o[g][i] *= f;
+        }
+        const float base = m[g] == -INFINITY ? 0.f : m[g];
+#pragma unroll
+        for (int i = 0; i < NX; i++) {
+          x[i] = __builtin_amdgcn_exp2f(x[i] - base);
+          l[g] += x[i];
+        }
+        if constexpr (FEW) {
+          // Both keys' parts, one word each, to row 4 w + part.
+          uint32_t *row = lds_p + (g * 16 + 4 * w) * kPRow + c;
+#pragma unroll
+          for (int i = 0; i < 3; i++) {
+            row[i * kPRow] = high_halves(__float_as_uint(x[0]), __float_as_uint(x[1]));
+            x[0] -= __uint_as_float(__float_as_uint(x[0]) & 0xffff0000u);
+            x[1] -= __uint_as_float(__float_as_uint(x[1]) & 0xffff0000u);
+          }
+        } else {
+          split3<true>(x, p[g]);
         }
       }
-      float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
-                        fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-      top = max4_lanes(top);
-      if (__any(top > m)) {
-        const float grown = fmaxf(m, top);
-        const float f = m == grown ? 1.f : __builtin_amdgcn_exp2f(m - grown);  // 0 from -infinity
-        m = grown;
-        l *= f;
+      if constexpr (FEW) {
+        asm volatile("" ::: "memory");  // (a wave's LDS operations are in order; the compiler's are, too)
 #pragma unroll
-        for (int i = 0; i < D / 16; i++) o[i] *= f;
+        for (int g = 0; g < NG; g++)
+          p[g][0] = __builtin_bit_cast(
+              bf16x8, *reinterpret_cast<const u32x4 *>(lds_p + (g * 16 + c) * kPRow + 4 * w));
+        asm volatile("" ::: "memory");
       }
-      const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        x[i] = __builtin_amdgcn_exp2f(x[i] - base);
-        l += x[i];
-      }
-      bf16x8 p[3];
-      split3<true>(x, p);
       float unit[8];
 #pragma unroll
       for (int i = 0; i < 8; i++) unit[i] = mx4_unit(byte_of(cur.vs[i >> 2], i & 3));
       if (edge) {
         // A block that is NaN reaches only the columns that see its key, though all of a wave's columns are
-        // multiplied with it: its values are taken as 0 here, and NaN added where a column sees one.
+        // multiplied with it: its values are taken as next to nothing here, and the rows of O that a column
+        // sees one of become NaN at the end (bits of nan; a row's dims share one block, d / 16 of 32).
         bool bad = false;
 #pragma unroll
-        for (int i = 0; i < 8; i++) bad |= byte_of(cur.vs[i >> 2], i & 3) == 255u;
+        for (int i = 0; i < 8; i++) bad |= unit[i] == INFINITY;
         if (__any(bad)) {
-          uint32_t mark[8], see[8];
+          uint32_t mark[8];
 #pragma unroll
           for (int i = 0; i < 8; i++) {
-            const bool nan = byte_of(cur.vs[i >> 2], i & 3) == 255u;
-            const int key = key0 + 16 * (i >> 2) + 4 * w + (i & 3);
-            mark[i] = nan ? 0x3f80u : 0u;  // 1 in bf16
-            see[i] = key < hi && key >= lo ? 0x3f80u : 0u;
-            if (nan) {
-              unit[i] = 0.f;
-              constexpr int NB = D / 32;  // the slot's codes to 0
-#pragma unroll
-              for (int b = 0; b < NB; b++) cur.v[(i * NB + b) >> 2] &= ~(255u << (8 * ((i * NB + b) & 3)));
-            }
+            const bool is = unit[i] == INFINITY;
+            mark[i] = is ? 0x3f80u : 0u;  // 1 in bf16
+            unit[i] = is ? 0.f : unit[i];
           }
-          f32x4 n = {0.f, 0.f, 0.f, 0.f};
-          n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-              frag(low_halves(mark[0], mark[1]), low_halves(mark[2], mark[3]),
-                   low_halves(mark[4], mark[5]), low_halves(mark[6], mark[7])),
-              frag(low_halves(see[0], see[1]), low_halves(see[2], see[3]), low_halves(see[4], see[5]),
-                   low_halves(see[6], see[7])),
-              n, 0, 0, 0);
-          // (A row's dims share one block, d / 16 of 32.)
+          const bf16x8 marks = frag(low_halves(mark[0], mark[1]), low_halves(mark[2], mark[3]),
+                                    low_halves(mark[4], mark[5]), low_halves(mark[6], mark[7]));
 #pragma unroll
-          for (int r = 0; r < 4; r++)
-            if (n[r] > 0.f)
+          for (int g = 0; g < NG; g++) {
+            // Which of keys 8 w and on the operand's row or column sees.
+            const int ohi = FEW ? __shfl(hi[g], 16 * (c >> 2)) : hi[g];
+            const int olo = FEW ? __shfl(lo[g], 16 * (c >> 2)) : lo[g];
+            uint32_t see[8];
 #pragma unroll
-              for (int i = 0; i < D / 16; i++) o[i][r] = NAN;
+            for (int i = 0; i < 8; i++) {
+              const int key = key0 + 8 * w + i;
+              see[i] = key < ohi && key >= olo ? 0x3f80u : 0u;
+            }
+            const bf16x8 sees = frag(low_halves(see[0], see[1]), low_halves(see[2], see[3]),
+                                     low_halves(see[4], see[5]), low_halves(see[6], see[7]));
+            const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+            const f32x4 n = FEW ? mfma(sees, marks, zero) : mfma(marks, sees, zero);
+#pragma unroll
+            for (int r = 0; r < 4; r++) nan[g] |= n[r] > 0.f ? 1u << r : 0u;
+          }
         }
       }
-      add_values<D>(cur, unit, p, o);
-      if (AHEAD) cur = next;
+      add_values<D, NG, NP, FEW>(cur, unit, p, o);
+    };
+    int t = tb + (TILES ? 0 : wave);
+    if constexpr (AHEAD) {
+      // (The last turns load the last tile again: loads behind a condition would be waited for as if
+      // they were needed at once.)
+      Tile<D> one, two;
+      if (t < te) {
+        load(t, block_of(t), one);
+        int next = min(t + STRIDE, te - 1), block = block_of(next);
+        while (true) {
+          load(next, block, two);
+          next = min(t + 2 * STRIDE, te - 1);
+          block = block_of(next);
+          attend(t, one);
+          t += STRIDE;
+          if (t >= te) break;
+          load(next, block, one);
+          next = min(t + 2 * STRIDE, te - 1);
+          block = block_of(next);
+          attend(t, two);
+          t += STRIDE;
+          if (t >= te) break;
+        }
+      }
+    } else {
+      Tile<D> one;
+      for (; t < te; t += STRIDE) {
+        load(t, block_of(t), one);
+        attend(t, one);
+      }
+    }
+    // NaN where a column saw one, then the lane's results: FEW has E dims of column 4 g + w (the sum of
+    // its parts, in r = 0), the others E dims of four rows of V for column c.
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+      if constexpr (FEW) {
+        l[g] = sum16(l[g]);
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+          const float sum = o[g][i][0] + (o[g][i][1] + o[g][i][2]);
+          o[g][i][0] = nan[g] & 1 ? NAN : sum;
+        }
+      } else {
+        l[g] = sum4_lanes(l[g]);
+        if (__any(nan[g] != 0))
+#pragma unroll
+          for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int i = 0; i < E; i++) o[g][i][r] = (nan[g] >> r) & 1 ? NAN : o[g][i][r];
+      }
     }
 
-    // Join the waves: column maxima, then sums and rows over the common maximum.
-    l = sum4_lanes(l);
-    if constexpr (QLDS) __syncthreads();  // q's parts have been read
-    if (w == 0) {
-      lds_m[wave * kCols + c] = m;
-      lds_l[wave * kCols + c] = l;
+    if constexpr (TILES) {  // every wave writes its own columns
+#pragma unroll
+      for (int g = 0; g < NG; g++) {
+        const int64_t col = first_col + 16 * g + c;
+        if (col >= cols) continue;
+        const int row = (int)(col / rep);
+        const size_t part = (size_t)part0 + wave * (16 * NG) + 16 * g + c;
+        const float inv = whole ? (l[g] == 0.f ? 0.f : 1.f / l[g]) : 1.f;
+        float *dst = whole ? a.out + ((size_t)(row0 + row) * a.hq + (size_t)head * rep +
+                                      (col - (int64_t)row * rep)) * D
+                           : a.part_o + part * D;
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+          for (int i = 0; i < E; i += 4)
+            *reinterpret_cast<float4 *>(dst + (4 * w + r) * E + i) =
+                make_float4(o[g][i][r] * inv, o[g][i + 1][r] * inv, o[g][i + 2][r] * inv,
+                            o[g][i + 3][r] * inv);
+        if (!whole && w == 0) {
+          a.part_m[part] = m[g];
+          a.part_l[part] = l[g];
+        }
+      }
+      continue;
     }
-    float *mine = lds_o + (wave * kCols + c) * (D + 4);
+
+    // Join the waves: sums and rows over the highest reference.
+    if constexpr (QLDS) __syncthreads();  // q's parts have been read
 #pragma unroll
-    for (int r = 0; r < 4; r++)
+    for (int g = 0; g < NG; g++) {
+      const int at = wave * COLS + (FEW ? 4 * g + w : c);
+      if (FEW ? c == 0 : w == 0) {
+        lds_m[at] = m[g];
+        lds_l[at] = l[g];
+      }
+      float *to = lds_o + at * (D + 4);
 #pragma unroll
-      for (int i = 0; i < D / 16; i += 4)
-        *reinterpret_cast<float4 *>(mine + (4 * w + r) * (D / 16) + i) =
-            make_float4(o[i][r], o[i + 1][r], o[i + 2][r], o[i + 3][r]);
+      for (int r = 0; r < (FEW ? 1 : 4); r++)
+#pragma unroll
+        for (int i = 0; i < E; i += 4)
+          *reinterpret_cast<float4 *>(to + (FEW ? c : 4 * w + r) * E + i) =
+              make_float4(o[g][i][r], o[g][i + 1][r], o[g][i + 2][r], o[g][i + 3][r]);
+    }
     __syncthreads();
-    const int oc = threadIdx.x >> 4, part16 = threadIdx.x & 15;  // column, 16 lanes each
+    constexpr int LANES = 256 / COLS;  // lanes of a column
+    const int oc = threadIdx.x / LANES, ol = threadIdx.x % LANES;
     float ms[kWaves], big = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int i = 0; i < kWaves; i++) {
-      ms[i] = lds_m[i * kCols + oc];
+      ms[i] = lds_m[i * COLS + oc];
       big = fmaxf(big, ms[i]);
     }
 #pragma unroll
     for (int i = 0; i < kWaves; i++) {
-      const float li = lds_l[i * kCols + oc];
-      // (No maximum: no keys, or scores that are NaN, which the sum holds.)
+      const float li = lds_l[i * COLS + oc];
+      // (No reference: no keys, or scores that are NaN, which the sum holds.)
       ms[i] = ms[i] == -INFINITY ? (li == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(ms[i] - big);
       sum += ms[i] * li;
     }
-    const bool whole = t0 == 0 && t1 == tile.n;
     const int64_t ocol = (int64_t)tile.col0 + oc;
     if (ocol < cols) {
       const int orow = (int)(ocol / rep);
       const float inv = whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
-      const size_t part = (size_t)(2 * blockIdx.x + (t0 == 0 ? 1 : 0)) * kCols + oc;
+      const size_t part = (size_t)part0 + oc;
       float *dst = whole ? a.out + ((size_t)(row0 + orow) * a.hq + (size_t)head * rep +
                                     (ocol - (int64_t)orow * rep)) * D
                          : a.part_o + part * D;
 #pragma unroll
-      for (int i = 0; i < D / 64; i++) {
-        const int e = 4 * (part16 + 16 * i);
+      for (int i = 0; i < (D + 4 * LANES - 1) / (4 * LANES); i++) {
+        const int e = 4 * (ol + LANES * i);
+        if (e >= D) break;
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int v = 0; v < kWaves; v++)
           if (ms[v] != 0.f)  // (a wave without keys has nothing)
-            acc += ms[v] * *reinterpret_cast<const f32x4 *>(lds_o + (v * kCols + oc) * (D + 4) + e);
+            acc += ms[v] * *reinterpret_cast<const f32x4 *>(lds_o + (v * COLS + oc) * (D + 4) + e);
         acc *= inv;
         *reinterpret_cast<f32x4 *>(dst + e) = acc;
       }
-      if (!whole && part16 == 0) {
+      if (!whole && ol == 0) {
         a.part_m[part] = big;
         a.part_l[part] = sum;
       }
     }
     if constexpr (!QLDS) __syncthreads();  // lds_o is written again
-    u += t1 - t0;
   }
 }
 
-// Joins the partials of column tiles that several workgroups shared, and zero-fills rows without keys:
-// workgroup (column tile x KV head, four columns) or, behind them, rows that no sequence covers.
-__global__ void __launch_bounds__(256) kv4_merge_kernel(Kv4Attention a) {
-  const int n_tiles = a.head->tiles, D = a.head_dim, rep = a.hq / a.kv.hkv;
-  const int64_t chunk = a.head->chunk;
+// Joins the partials of column tiles that several workgroups shared: workgroup x the one (of a column tile
+// and KV head) whose first border between workgroups is that of x - 1 and x, a wave a column.  Then zeroes
+// for rows without keys and rows that no sequence covers.
+__global__ void __launch_bounds__(256) kv4_merge_kernel(Kv4Attention a, int cols_of_tile) {
+  const int n_tiles = a.head->tiles, D = a.head_dim, rep = a.hq / a.kv.hkv, hkv = a.kv.hkv;
+  const int64_t chunk = a.head->chunk, all = a.cum[n_tiles] * hkv;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (int64_t item = blockIdx.x; item < (int64_t)n_tiles * a.kv.hkv; item += gridDim.x) {
-    const int ct = (int)(item / a.kv.hkv), head = (int)(item - (int64_t)ct * a.kv.hkv);
+  const int64_t border = (int64_t)blockIdx.x * chunk;
+  if (blockIdx.x > 0 && border < all) {
+    int ct = find_tile(a.cum, n_tiles, border, hkv, lane);
+    while (a.tiles[ct].n == 0) ct++;
     const Kv4Tile tile = a.tiles[ct];
-    const int64_t u0 = a.cum[ct] * a.kv.hkv + (int64_t)head * tile.n;
-    const int64_t g0 = u0 / chunk, g1 = tile.n ? (u0 + tile.n - 1) / chunk : g0;
-    if (tile.n && g0 == g1) continue;
-    const int row0 = a.cu_q ? a.cu_q[tile.seq] : tile.seq;
-    const int qlen = a.cu_q ? a.cu_q[tile.seq + 1] - row0 : 1;
-    const int64_t cols = (int64_t)qlen * rep;
-    for (int c = wave + 4 * blockIdx.y; c < kCols; c += 4 * gridDim.y) {
-      const int64_t col = (int64_t)tile.col0 + c;
-      if (col >= cols) continue;
-      const int row = (int)(col / rep);
-      float *dst = a.out + ((size_t)(row0 + row) * a.hq + (size_t)head * rep + (col - (int64_t)row * rep)) * D;
-      if (tile.n == 0) {
-        for (int e = lane; e < D; e += 64) dst[e] = 0.f;
-        continue;
+    const int64_t in = border - a.cum[ct] * hkv;
+    const int head = (int)(in / tile.n);
+    const int64_t u0 = border - (in - (int64_t)head * tile.n), u1 = u0 + tile.n;
+    if (u0 < border && u0 >= border - chunk) {
+      const int64_t g0 = blockIdx.x - 1, g1 = (u1 - 1) / chunk;
+      const int row0 = a.cu_q ? a.cu_q[tile.seq] : tile.seq;
+      const int qlen = a.cu_q ? a.cu_q[tile.seq + 1] - row0 : 1;
+      const int64_t cols = (int64_t)qlen * rep;
+      for (int c = wave + 4 * blockIdx.y; c < cols_of_tile; c += 4 * gridDim.y) {
+        const int64_t col = (int64_t)tile.col0 + c;
+        if (col >= cols) break;
+        const int row = (int)(col / rep);
+        float *dst = a.out + ((size_t)(row0 + row) * a.hq + (size_t)head * rep + (col - (int64_t)row * rep)) * D;
+        // Partial of workgroup g: its last for the first one, its first for the others.
+        auto slot = [&](int64_t g) { return (size_t)(2 * g + (g == g0 ? 1 : 0)) * cols_of_tile + c; };
+        float big = -INFINITY;
+        for (int64_t g = g0 + lane; g <= g1; g += 64) big = fmaxf(big, a.part_m[slot(g)]);
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) big = fmaxf(big, __shfl_xor(big, d));
+        float sum = 0.f;
+        f32x2 acc[4] = {};  // dims 2 lane + 128 i
+        for (int64_t base = g0; base <= g1; base += 64) {
+          // A lane a partial's weight, then all lanes its row.
+          float f = 0.f;
+          if (base + lane <= g1) {
+            const float m = a.part_m[slot(base + lane)], l = a.part_l[slot(base + lane)];
+            // (No reference: no keys, or scores that are NaN, which the sum holds.)
+            f = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - big);
+            sum += f * l;
+          }
+          const int n = (int)min((int64_t)64, g1 - base + 1);
+          for (int i = 0; i < n; i += 4) {  // four rows' loads at once
+            f32x2 row[4][4];
+            float w[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              w[j] = i + j < n ? __shfl(f, i + j) : 0.f;
+              const float *src = a.part_o + slot(base + min(i + j, n - 1)) * D;
+#pragma unroll
+              for (int k = 0; k < 4; k++)
+                if (2 * lane + 128 * k < D)
+                  row[j][k] = *reinterpret_cast<const f32x2 *>(src + 2 * lane + 128 * k);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+              for (int k = 0; k < 4; k++)  // (a row without weight saw nothing)
+                if (2 * lane + 128 * k < D && w[j] != 0.f) acc[k] += w[j] * row[j][k];
+          }
+        }
+        // (In a fixed order: a lane's sums, then lane by lane.)
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+          if (2 * lane + 128 * k < D)
+            *reinterpret_cast<f32x2 *>(dst + 2 * lane + 128 * k) = acc[k] * inv;
       }
-      // Partial of workgroup g: its last for the first one, its first for the others.
-      auto slot = [&](int64_t g) { return (size_t)(2 * g + (g == g0 ? 1 : 0)) * kCols + c; };
-      float big = -INFINITY;
-      for (int64_t g = g0 + lane; g <= g1; g += 64) big = fmaxf(big, a.part_m[slot(g)]);
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) big = fmaxf(big, __shfl_xor(big, d));
-      float sum = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      for (int64_t g = g0; g <= g1; g++) {
-        const float m = a.part_m[slot(g)], l = a.part_l[slot(g)];
-        if (m == -INFINITY && l == 0.f) continue;  // no keys (a sum that is NaN stays)
-        const float f = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - big);
-        sum += f * l;
-        const float *src = a.part_o + slot(g) * D;
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-          if (lane + 64 * i < D) acc[i] += f * src[lane + 64 * i];
-      }
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-      for (int i = 0; i < 8; i++)
-        if (lane + 64 * i < D) dst[lane + 64 * i] = acc[i] * inv;
     }
   }
-  // Rows before the first sequence and behind the last one.
-  if (blockIdx.y == 0) {
-    const int first = a.head->first, covered = a.head->covered;
-    const size_t width = (size_t)a.hq * D;
-    const size_t rows = (size_t)first + (a.tokens - covered), n = rows * width;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-      const size_t r = i / width;
-      a.out[(r < (size_t)first ? r : r - first + covered) * width + (i - r * width)] = 0.f;
+  if (blockIdx.y != 0) return;
+  const int64_t stride = (int64_t)gridDim.x * 256, i0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const size_t width = (size_t)a.hq * D;
+  // Rows whose column tile has no keys, a thread a column tile (there are few, and its rows are few).
+  for (int64_t t = i0; t < n_tiles; t += stride) {
+    const Kv4Tile tile = a.tiles[t];
+    if (tile.n) continue;
+    const int row0 = a.cu_q ? a.cu_q[tile.seq] : tile.seq;
+    const int qlen = a.cu_q ? a.cu_q[tile.seq + 1] - row0 : 1;
+    const int64_t end = min((int64_t)qlen * rep, (int64_t)tile.col0 + cols_of_tile);
+    for (int64_t col = tile.col0; col < end; col++) {
+      const int64_t row = col / rep;
+      for (int h = 0; h < hkv; h++) {
+        float *dst = a.out + (row0 + row) * width + ((size_t)h * rep + (col - row * rep)) * D;
+        for (int e = 0; e < D; e += 4) *reinterpret_cast<float4 *>(dst + e) = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
     }
+  }
+  if (!a.zero_rest) return;
+  // Rows before the first sequence and behind the last one.
+  const int first = a.head->first, covered = a.head->covered;
+  const size_t n = ((size_t)first + (a.tokens - covered)) * width;
+  for (size_t i = i0; i < n; i += stride) {
+    const size_t r = i / width;
+    a.out[(r < (size_t)first ? r : r - first + covered) * width + (i - r * width)] = 0.f;
   }
 }
 
@@ -665,16 +930,24 @@ bool kv4_supports(int head_dim) {
 
 namespace {
 
-template <int D> size_t attention_lds() {
-  const size_t join = (size_t)kWaves * kCols * (D + 4 + 2) * 4;
-  return D == 512 ? std::max<size_t>(join, (size_t)3 * (D / 32) * 64 * 16) : join;
+template <int D, int MODE> size_t attention_lds() {
+  if (MODE == KV4_TILES) return 0;
+  constexpr int cols = kv4_cols(D, MODE);
+  const size_t join = (size_t)kWaves * cols * (D + 4 + 2) * 4;
+  if (MODE == KV4_ROWS) return D == 512 ? std::max<size_t>(join, (size_t)3 * (D / 32) * 64 * 16) : join;
+  return join + (size_t)kWaves * (cols / 4) * 16 * kPRow * 4;
+}
+
+template <int D, int MODE> constexpr int groups() {
+  return kv4_cols(D, MODE) / (MODE == KV4_TILES ? 64 : MODE == KV4_ROWS ? 16 : 4);
 }
 
 template <int D> hipError_t store(const Kv4Store &a, hipStream_t s) {
   constexpr int ROWS = 256 / (D / 8);
   const int64_t rows = a.k ? 2 * (int64_t)a.tokens * a.kv.hkv : 0;
-  const int64_t blocks = (rows + ROWS - 1) / ROWS;
-  hipLaunchKernelGGL(kv4_store_kernel<D>, dim3((unsigned)(blocks + 1)), dim3(256), 0, s, a);
+  const int64_t blocks = (rows + ROWS - 1) / ROWS + a.lists;
+  if (blocks == 0) return hipSuccess;
+  hipLaunchKernelGGL(kv4_store_kernel<D>, dim3((unsigned)blocks), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
@@ -686,15 +959,53 @@ hipError_t read(const Kv4View &kv, const int32_t *slots, float *k, float *v, int
   return hipGetLastError();
 }
 
-template <int D> hipError_t attention(const Kv4Attention &a, int workgroups, hipStream_t s) {
-  const size_t lds = attention_lds<D>();
+template <int D, int MODE> hipError_t attention(const Kv4Attention &a, int workgroups, hipStream_t s) {
+  constexpr int NG = groups<D, MODE>();
+  const auto kernel = &kv4_attention_kernel<D, MODE, NG>;
+  const size_t lds = attention_lds<D, MODE>();
   if (lds > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&kv4_attention_kernel<D>),
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL(kv4_attention_kernel<D>, dim3(workgroups), dim3(256), lds, s, a);
+  hipLaunchKernelGGL((kv4_attention_kernel<D, MODE, NG>), dim3(workgroups), dim3(256), lds, s, a);
   return hipGetLastError();
+}
+
+template <int D> hipError_t attention_of(const Kv4Attention &a, int mode, int workgroups, hipStream_t s) {
+  switch (mode) {
+    case KV4_FEW: return attention<D, KV4_FEW>(a, workgroups, s);
+    case KV4_EIGHT:
+      if constexpr (kv4_has_tiles(D)) return attention<D, KV4_EIGHT>(a, workgroups, s);
+      return hipErrorInvalidValue;
+    case KV4_ROWS: return attention<D, KV4_ROWS>(a, workgroups, s);
+    default:
+      if constexpr (kv4_has_tiles(D)) return attention<D, KV4_TILES>(a, workgroups, s);
+      return hipErrorInvalidValue;
+  }
+}
+
+template <int D, int MODE> int resident() {
+  constexpr int NG = groups<D, MODE>();
+  int n = 0;
+  if (hipOccupancyMaxActiveBlocksPerMultiprocessor(
+          &n, reinterpret_cast<const void *>(&kv4_attention_kernel<D, MODE, NG>), 256,
+          attention_lds<D, MODE>()) != hipSuccess)
+    (void)hipGetLastError();
+  return std::max(1, n);
+}
+
+template <int D> int resident_of(int mode) {
+  switch (mode) {
+    case KV4_FEW: return resident<D, KV4_FEW>();
+    case KV4_EIGHT:
+      if constexpr (kv4_has_tiles(D)) return resident<D, KV4_EIGHT>();
+      return 1;
+    case KV4_ROWS: return resident<D, KV4_ROWS>();
+    default:
+      if constexpr (kv4_has_tiles(D)) return resident<D, KV4_TILES>();
+      return 1;
+  }
 }
 
 }  // namespace
@@ -722,16 +1033,24 @@ hipError_t launch_kv4_read(const Kv4View &kv, int head_dim, const int32_t *slots
 #undef args
 }
 
-hipError_t launch_kv4_attention(const Kv4Attention &a, int workgroups, hipStream_t s) {
-#define args (a, workgroups, s)
-  NVA_BY_DIM(a.head_dim, attention)
+hipError_t launch_kv4_attention(const Kv4Attention &a, int mode, int workgroups, hipStream_t s) {
+#define args (a, mode, workgroups, s)
+  NVA_BY_DIM(a.head_dim, attention_of)
 #undef args
 }
 
-hipError_t launch_kv4_merge(const Kv4Attention &a, int max_tiles, hipStream_t s) {
-  const int64_t items = (int64_t)max_tiles * a.kv.hkv;
-  hipLaunchKernelGGL(kv4_merge_kernel, dim3((unsigned)std::min<int64_t>(std::max<int64_t>(items, 1), 4096), 4),
-                     dim3(256), 0, s, a);
+int kv4_workgroups_per_cu(int head_dim, int mode) {
+  switch (head_dim) {
+    case 64: return resident_of<64>(mode);
+    case 128: return resident_of<128>(mode);
+    case 256: return resident_of<256>(mode);
+    default: return resident_of<512>(mode);
+  }
+}
+
+hipError_t launch_kv4_merge(const Kv4Attention &a, int mode, int workgroups, hipStream_t s) {
+  const int cols = kv4_cols(a.head_dim, mode);
+  hipLaunchKernelGGL(kv4_merge_kernel, dim3(workgroups, (cols + 15) / 16), dim3(256), 0, s, a, cols);
   return hipGetLastError();
 }
 

@@ -209,8 +209,30 @@ struct Kv4View {
   uint8_t *pages;  // [block][KV head][tile of 32 keys][34 d bytes]
   int32_t num_blocks, block_size, hkv;
 };
-constexpr int kKv4Cols = 16;      // columns of a column tile
-constexpr int kKv4MinUnits = 8;   // least key tiles of a workgroup
+// The attention kernels (kv4.hip) by the columns, query rows times heads of a KV head, of their column
+// tiles: a step's sequences of few columns run on one of the first three, the others on the last.  d = 512
+// has the first and third alone (its registers).
+enum { KV4_FEW = 0, KV4_EIGHT = 1, KV4_ROWS = 2, KV4_TILES = 3 };
+constexpr bool kv4_has_tiles(int head_dim) { return head_dim <= 256; }
+constexpr int kv4_cols(int head_dim, int mode) {
+  return mode == KV4_FEW ? 4 : mode == KV4_EIGHT ? 8 : mode == KV4_ROWS ? 16 : head_dim <= 128 ? 128 : 64;
+}
+// Waves a SIMD that the registers are held down to.
+#ifndef KV4_W1
+#define KV4_W1 3
+#endif
+#ifndef KV4_W2
+#define KV4_W2 2
+#endif
+#ifndef KV4_W3
+#define KV4_W3 2
+#endif
+constexpr int kv4_min_waves(int head_dim, int mode) {
+  return mode == KV4_FEW     ? (head_dim <= 128 ? KV4_W1 : head_dim <= 256 ? KV4_W2 : 1)
+         : mode == KV4_EIGHT ? (head_dim <= 128 ? KV4_W3 : 1)
+         : mode == KV4_ROWS  ? (head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1)
+                             : (head_dim <= 64 ? 2 : 1);
+}
 struct Kv4Tile {
   int32_t seq, col0, kb, n;  // n 0: no key is seen
 };
@@ -229,13 +251,17 @@ struct Kv4List {
   int32_t *before;  // [num_seqs + 1] column tiles before each sequence
   const int32_t *cu_q, *cu_k, *lens;
   int32_t num_seqs, rep, hkv, window, workgroups;
+  int32_t cols;                // columns of a column tile
+  int32_t min_cols, max_cols;  // the sequences of the list, by their columns
+  int32_t unit, min_units;     // a workgroup's units: a multiple of unit, at least min_units
 };
 struct Kv4Store {
   Kv4View kv;
   const float *k, *v;  // [tokens, hkv, d]; k null: no rows
   const int32_t *slots;
   int32_t tokens;
-  Kv4List list;
+  int32_t lists;
+  Kv4List list[2];
 };
 struct Kv4Attention {
   Kv4View kv;
@@ -246,20 +272,18 @@ struct Kv4Attention {
   const int64_t *cum;
   const int32_t *cu_q, *cu_k, *lens, *table;
   int32_t bt_stride, hq, head_dim, window, tokens;
+  int32_t zero_rest;   // the merge zeroes the rows that no sequence covers
   int32_t tile_shift;  // log2 of a block's tiles, or -1
   float scale2;        // scale * log2(e)
   float *part_m, *part_l, *part_o;
 };
-// Resident workgroups of the attention kernel, a wave of each on every SIMD: by its registers.
-constexpr int kv4_workgroups_per_cu(int head_dim) {
-  return head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1;
-}
 bool kv4_supports(int head_dim);
 hipError_t launch_kv4_store(const Kv4Store &a, int head_dim, hipStream_t s);
 hipError_t launch_kv4_read(const Kv4View &kv, int head_dim, const int32_t *slots, float *k, float *v,
                            int rows, hipStream_t s);
-hipError_t launch_kv4_attention(const Kv4Attention &a, int workgroups, hipStream_t s);
-hipError_t launch_kv4_merge(const Kv4Attention &a, int max_tiles, hipStream_t s);
+int kv4_workgroups_per_cu(int head_dim, int mode);  // resident on the current device
+hipError_t launch_kv4_attention(const Kv4Attention &a, int mode, int workgroups, hipStream_t s);
+hipError_t launch_kv4_merge(const Kv4Attention &a, int mode, int workgroups, hipStream_t s);
 hipError_t launch_quantize4(const float *x, int64_t values, uint8_t *codes, uint8_t *scales,
                             hipStream_t s);
 

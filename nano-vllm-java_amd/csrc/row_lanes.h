@@ -9,6 +9,7 @@
 namespace nva {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 // A non-temporal load (K/V rows are read once per step) from a wave-uniform base plus a 32-bit lane
 // offset (floats), as a buffer load: the base stays in scalar registers, so no per-lane 64-bit address is formed
