@@ -139,6 +139,8 @@ int ctx_kv4_workgroups_per_cu(nva_ctx *ctx, int head_dim, int mode) {
   return it->second;
 }
 
+constexpr int64_t kJoinUnits = 3500;
+
 // Growing a buffer of a call that may be captured.
 nva_status reserve_for(nva_ctx *ctx, DevBuf &buf, size_t bytes, bool capturing, const char *what) {
   if (capturing) {
@@ -220,7 +222,7 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
   // knows of their rows bounds them: the lengths themselves, or the most tokens that follow.
   const int seqs = dev ? ctx->dev_seqs : ctx->is_prefill ? ctx->num_seqs : num_tokens;
   int64_t few = 0, many = 0;  // most columns of a sequence on either list
-  const int64_t limit = kv4_has_tiles(d.head_dim) ? 16 : INT32_MAX;
+  int64_t limit = kv4_has_tiles(d.head_dim) ? 16 : INT32_MAX;
   auto count = [&](int64_t cols) {
     if (cols <= limit) few = std::max(few, cols); else many = std::max(many, cols);
   };
@@ -229,13 +231,25 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
     if (most > limit) many = most;
     few = std::min(most, limit);
   } else if (ctx->is_prefill) {
-    for (int b = 0; b < seqs; b++) count((int64_t)(ctx->cu_q[b + 1] - ctx->cu_q[b]) * rep);
+    int64_t units = 0;  // key tiles of the sequences of few columns
+    for (int b = 0; b < seqs; b++) {
+      const int64_t cols = (int64_t)(ctx->cu_q[b + 1] - ctx->cu_q[b]) * rep;
+      count(cols);
+      if (cols > 0 && cols <= limit)
+        units += (int64_t)((ctx->cu_k[b + 1] - ctx->cu_k[b] + 31) / 32) * d.num_kv_heads;
+    }
+    // A few of them among others join those: the tile kernel takes some 6.5 ns for a key tile of one column
+    // tile and head, the kernels of few columns 0.9 and the 20 us of two more launches.
+    if (many && units <= kJoinUnits) {
+      limit = 0;
+      few = 0;
+    }
   } else {
     count(rep);
   }
   struct Run {
-    int mode, workgroups;
-    size_t off_head, off_tiles, off_cum, off_before, off_part, parts;
+    int mode, workgroups, tiles;
+    size_t off_head, off_tiles, off_cum, off_before, off_borders, off_part, parts;
   } runs[2];
   int n_runs = 0;
   size_t plan_bytes = 0, part_floats = 0;
@@ -244,12 +258,14 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
     r.mode = mode;
     r.workgroups = ctx->num_cus * ctx_kv4_workgroups_per_cu(ctx, d.head_dim, mode);
     const int cols = kv4_cols(d.head_dim, mode);
-    const int64_t tiles = (int64_t)num_tokens * rep / cols + std::min(seqs, num_tokens) + 1;
+    const int64_t tiles = (int64_t)num_tokens * rep / cols + seqs + 1;
+    r.tiles = (int)tiles;
     r.off_head = plan_bytes;
     r.off_tiles = r.off_head + 256;
     r.off_cum = align256(r.off_tiles + tiles * sizeof(Kv4Tile));
     r.off_before = align256(r.off_cum + (tiles + 1) * 8);
-    plan_bytes = align256(r.off_before + ((size_t)seqs + 1) * 4);
+    r.off_borders = align256(r.off_before + ((size_t)seqs + 1) * 4);
+    plan_bytes = align256(r.off_borders + r.workgroups * sizeof(Kv4Border));
     r.parts = (size_t)2 * r.workgroups * cols;
     r.off_part = part_floats;
     part_floats += r.parts * (d.head_dim + 2);
@@ -274,14 +290,15 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
   a.kv = s.kv;
   a.q = q;
   a.out = out;
+  Kv4List rows{};
   if (dev) {
-    a.cu_q = dev->cu_q;
-    a.lens = dev->lens;
+    rows.cu_q = dev->cu_q;
+    rows.lens = dev->lens;
   } else if (ctx->is_prefill) {
-    a.cu_q = ctx->dev_i32(ctx->off_cu_q);
-    a.cu_k = ctx->dev_i32(ctx->off_cu_k);
+    rows.cu_q = ctx->dev_i32(ctx->off_cu_q);
+    rows.cu_k = ctx->dev_i32(ctx->off_cu_k);
   } else {
-    a.lens = ctx->dev_i32(ctx->off_ctx);
+    rows.lens = ctx->dev_i32(ctx->off_ctx);
   }
   a.table = dev ? dev->table : ctx->dev_i32(ctx->off_tables);
   a.bt_stride = dev ? dev->width : ctx->bt_stride;
@@ -298,9 +315,9 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
     l.tiles = reinterpret_cast<Kv4Tile *>(plan + r.off_tiles);
     l.cum = reinterpret_cast<int64_t *>(plan + r.off_cum);
     l.before = reinterpret_cast<int32_t *>(plan + r.off_before);
-    l.cu_q = a.cu_q;
-    l.cu_k = a.cu_k;
-    l.lens = a.lens;
+    l.cu_q = rows.cu_q;
+    l.cu_k = rows.cu_k;
+    l.lens = rows.lens;
     l.num_seqs = seqs;
     l.rep = rep;
     l.hkv = d.num_kv_heads;
@@ -309,6 +326,7 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
     l.cols = kv4_cols(d.head_dim, r.mode);
     l.min_cols = r.mode == KV4_TILES ? (int)limit + 1 : 1;
     l.max_cols = r.mode == KV4_TILES ? INT32_MAX : (int)limit;
+    l.one_each = n_runs == 1 && std::max(few, many) <= l.cols;
     l.unit = r.mode == KV4_TILES ? 1 : 4;
     l.min_units = r.mode == KV4_TILES ? 4 : 8;
   }
@@ -322,6 +340,8 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
     a.head = s.list[i].head;
     a.tiles = s.list[i].tiles;
     a.cum = s.list[i].cum;
+    a.room = r.tiles;
+    a.borders = reinterpret_cast<Kv4Border *>(plan + r.off_borders);
     float *part = static_cast<float *>(ctx->d_part4.ptr) + r.off_part;
     a.part_m = part;
     a.part_l = part + r.parts;
@@ -332,7 +352,10 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
             "4-bit attention kernel launch");
     tm.done();
     Timed tg(ctx, "merge4");
-    HIP_TRY(ctx, launch_kv4_merge(a, r.mode, r.workgroups, ctx->stream), "4-bit merge kernel launch");
+    const int64_t items = (int64_t)std::min(seqs, num_tokens) * d.num_kv_heads;
+    HIP_TRY(ctx, launch_kv4_merge(a, r.mode, r.workgroups, (int)std::min<int64_t>(items, INT32_MAX),
+                                  ctx->stream),
+            "4-bit merge kernel launch");
     tg.done();
   }
   return NVA_OK;

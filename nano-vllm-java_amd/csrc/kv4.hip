@@ -107,53 +107,76 @@ __device__ void build_list(const Kv4List &a) {
     return before + x - v;
   };
   const int rep = a.rep;
-  // Column tiles before each sequence.
-  int64_t tiles = 0;
-  for (int b0 = 0; b0 < a.num_seqs; b0 += 256) {
-    const int b = b0 + tid;
-    int64_t mine = 0, all;
-    if (b < a.num_seqs) {
-      const int64_t cols = (int64_t)(a.cu_q ? a.cu_q[b + 1] - a.cu_q[b] : 1) * rep;
-      if (cols >= a.min_cols && cols <= a.max_cols) mine = (cols + a.cols - 1) / a.cols;
-    }
-    const int64_t at = tiles + scan(mine, all);
-    if (b < a.num_seqs) a.before[b] = (int32_t)at;
-    tiles += all;
-  }
-  if (tid == 0) a.before[a.num_seqs] = (int32_t)tiles;
-  __threadfence_block();
-  __syncthreads();
-  // Their key tiles.
-  int64_t units = 0;
-  for (int64_t t0 = 0; t0 < tiles; t0 += 256) {
-    const int t = (int)t0 + tid;
-    Kv4Tile tile{0, 0, 0, 0};
-    if (t < tiles) {
-      int lo = 0, hi = a.num_seqs;  // before[lo] <= t < before[hi]
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.before[mid] <= t) lo = mid; else hi = mid;
+  auto rows_of = [&](int b, Kv4Tile &t) {
+    t.seq = b;
+    t.row0 = a.cu_q ? a.cu_q[b] : b;
+    t.qlen = a.cu_q ? a.cu_q[b + 1] - t.row0 : 1;
+    t.klen = a.lens ? a.lens[b] : a.cu_k[b + 1] - a.cu_k[b];
+  };
+  // The key tiles that columns [col0, col0 + a.cols) of a sequence see.
+  auto keys_of = [&](int64_t col0, Kv4Tile &t) {
+    const int first = (int)(col0 / rep);
+    const int last = (int)min((int64_t)t.qlen - 1, (col0 + a.cols - 1) / rep);
+    const int end = min(t.klen, t.klen - t.qlen + last + 1);
+    const int64_t beg = a.window > 0 ? (int64_t)t.klen - t.qlen + first + 1 - a.window : 0;
+    t.col0 = (int)col0;
+    t.kb = beg > 0 ? (int)(beg >> 5) : 0;
+    t.n = t.qlen > 0 && end > max(beg, (int64_t)0) ? ((end + 31) >> 5) - t.kb : 0;
+  };
+  int64_t tiles = 0, units = 0;
+  if (a.one_each) {  // no sequence has more than one column tile: each gets one, of no keys where it has no rows
+    tiles = a.num_seqs;
+    for (int b0 = 0; b0 < a.num_seqs; b0 += 256) {
+      Kv4Tile t{};
+      if (b0 + tid < a.num_seqs) {
+        rows_of(b0 + tid, t);
+        keys_of(0, t);
       }
-      const int row = a.cu_q ? a.cu_q[lo] : lo;
-      const int qlen = a.cu_q ? a.cu_q[lo + 1] - row : 1;
-      const int klen = a.lens ? a.lens[lo] : a.cu_k[lo + 1] - a.cu_k[lo];
-      const int64_t col0 = (int64_t)(t - a.before[lo]) * a.cols;
-      const int first = (int)(col0 / rep);
-      const int last = (int)min((int64_t)qlen - 1, (col0 + a.cols - 1) / rep);
-      const int end = min(klen, klen - qlen + last + 1);
-      const int64_t beg = a.window > 0 ? (int64_t)klen - qlen + first + 1 - a.window : 0;
-      tile.seq = lo;
-      tile.col0 = (int)col0;
-      tile.kb = beg > 0 ? (int)(beg >> 5) : 0;
-      tile.n = end > max(beg, (int64_t)0) ? ((end + 31) >> 5) - tile.kb : 0;
+      int64_t all;
+      const int64_t u = units + scan(t.n, all);
+      if (b0 + tid < a.num_seqs) {
+        a.tiles[b0 + tid] = t;
+        a.cum[b0 + tid] = u;
+      }
+      units += all;
     }
-    int64_t all;
-    const int64_t u = units + scan(tile.n, all);
-    if (t < tiles) {
-      a.tiles[t] = tile;
-      a.cum[t] = u;
+  } else {
+    // Column tiles before each sequence.
+    for (int b0 = 0; b0 < a.num_seqs; b0 += 256) {
+      const int b = b0 + tid;
+      int64_t mine = 0, all;
+      if (b < a.num_seqs) {
+        const int64_t cols = (int64_t)(a.cu_q ? a.cu_q[b + 1] - a.cu_q[b] : 1) * rep;
+        if (cols >= a.min_cols && cols <= a.max_cols) mine = (cols + a.cols - 1) / a.cols;
+      }
+      const int64_t at = tiles + scan(mine, all);
+      if (b < a.num_seqs) a.before[b] = (int32_t)at;
+      tiles += all;
     }
-    units += all;
+    if (tid == 0) a.before[a.num_seqs] = (int32_t)tiles;
+    __threadfence_block();
+    __syncthreads();
+    // Their key tiles.
+    for (int64_t t0 = 0; t0 < tiles; t0 += 256) {
+      const int at = (int)t0 + tid;
+      Kv4Tile t{};
+      if (at < tiles) {
+        int lo = 0, hi = a.num_seqs;  // before[lo] <= at < before[hi]
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (a.before[mid] <= at) lo = mid; else hi = mid;
+        }
+        rows_of(lo, t);
+        keys_of((int64_t)(at - a.before[lo]) * a.cols, t);
+      }
+      int64_t all;
+      const int64_t u = units + scan(t.n, all);
+      if (at < tiles) {
+        a.tiles[at] = t;
+        a.cum[at] = u;
+      }
+      units += all;
+    }
   }
   if (tid == 0) {
     a.cum[tiles] = units;
@@ -267,18 +290,19 @@ template <int D> __device__ __forceinline__ TilePlaces tile_places(int lane) {
 // no address is computed in registers that loads in flight are still to be written to (which would wait for
 // them).
 template <int D, bool NT>
-__device__ __forceinline__ void load_tile(const uint8_t *at, const TilePlaces &p, Tile<D> &t) {
-  const __amdgpu_buffer_rsrc_t tile = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<uint8_t *>(at), (short)0, 34 * D, kBufferWord3);
+__device__ __forceinline__ void load_keys(__amdgpu_buffer_rsrc_t tile, const TilePlaces &p, Tile<D> &t) {
   load_words<D / 32, NT>(tile, p.k, t.k[0]);
   load_words<D / 32, NT>(tile, p.k + 8 * D, t.k[1]);
-  load_words<D / 16, NT>(tile, p.v, t.v);
   if constexpr (D == 512)
     load_words<2, NT>(tile, p.ks, t.ks);
   else if constexpr (D == 256)
     load_words<1, NT>(tile, p.ks, t.ks);
   else
     t.ks[0] = __builtin_amdgcn_raw_buffer_load_b16(tile, p.ks, 0, NT ? 2 : 0);
+}
+template <int D, bool NT>
+__device__ __forceinline__ void load_values(__amdgpu_buffer_rsrc_t tile, const TilePlaces &p, Tile<D> &t) {
+  load_words<D / 16, NT>(tile, p.v, t.v);
   uint32_t vs[2];
   load_words<2, NT>(tile, p.vs, vs);
   t.vs = u32x2{vs[0], vs[1]};
@@ -366,17 +390,26 @@ template <typename T> __device__ __forceinline__ T uniform(const T *p) {
   return *(scalar)(uintptr_t)p;
 }
 
-// The 64-ary search for the last entry of cum that u reaches (times hkv), by a wave: tile of unit u.
-__device__ __forceinline__ int find_tile(const int64_t *cum, int n, int64_t u, int hkv, int lane) {
-  int lo = 0, hi = n;  // cum[lo] * hkv <= u < cum[hi] * hkv
-  while (hi - lo > 1) {
+__device__ __forceinline__ Kv4Tile uniform_tile(const Kv4Tile *p) {
+  typedef int32_t i32x8 __attribute__((ext_vector_type(8)));
+  static_assert(sizeof(Kv4Tile) == sizeof(i32x8), "one scalar load");
+  return __builtin_bit_cast(Kv4Tile, uniform(reinterpret_cast<const i32x8 *>(p)));
+}
+
+// The 64-ary search for the last entry of cum that u reaches (times hkv), by a wave: tile of unit u.  Its first
+// round covers the entries that the list has room for (those behind the n it has count as not reached), so
+// that it need not wait for n.
+__device__ __forceinline__ int find_tile(const int64_t *cum, int room, int n, int64_t u, int hkv, int lane) {
+  int lo = 0, hi = room;
+  do {
     const int step = (hi - lo + 63) >> 6;
     const int at = lo + lane * step;
-    const uint64_t le = __ballot(at < hi && cum[min(at, hi - 1)] * hkv <= u);
-    const int i = 63 - __builtin_clzll(le);  // lane 0 always holds
+    const int64_t before = cum[min(at, hi - 1)];
+    const uint64_t le = __ballot(at < hi && at < n && before * hkv <= u);
+    const int i = 63 - __builtin_clzll(le | 1);  // (lane 0 holds)
     lo += i * step;
     hi = min(hi, lo + step);
-  }
+  } while (hi - lo > 1);
   return lo;
 }
 
@@ -401,7 +434,6 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
   constexpr bool FEW = MODE == KV4_FEW || MODE == KV4_EIGHT, TILES = MODE == KV4_TILES;
   constexpr int NP = FEW ? 1 : 3;
   constexpr bool QLDS = D == 512 && !FEW;  // 192 registers of q's parts would leave none for the loads
-  constexpr bool AHEAD = D < 512;          // the next tile's loads before this one's products
   constexpr int NC = D / 32;               // contraction steps of a score
   constexpr int COLS = kv4_cols(D, MODE);
   constexpr int E = D / 16;                // dims of a row of V
@@ -422,27 +454,33 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
   const int64_t all = uniform(a.cum + n_tiles) * a.kv.hkv;
   int64_t u = (int64_t)blockIdx.x * chunk;
   const int64_t u_end = min(u + chunk, all);
-  if (u >= u_end) return;
+  Kv4Border border{0, -1, 0, 0, 0, 0};
+  if (u >= u_end) {
+    if (threadIdx.x == 0) a.borders[blockIdx.x] = border;
+    return;
+  }
   const int rep = a.hq / a.kv.hkv;
   const int per_block = a.kv.block_size >> 5;
   const TilePlaces places = tile_places<D>(lane);
-  int ct = __builtin_amdgcn_readfirstlane(find_tile(a.cum, n_tiles, u, a.kv.hkv, lane));
+  int ct = __builtin_amdgcn_readfirstlane(find_tile(a.cum, a.room, n_tiles, u, a.kv.hkv, lane));
   while (u < u_end) {
-    while (uniform(&a.tiles[ct].n) == 0 || u >= uniform(a.cum + ct + 1) * a.kv.hkv) ct++;  // (u is below the last entry's)
-    const Kv4Tile tile{uniform(&a.tiles[ct].seq), uniform(&a.tiles[ct].col0), uniform(&a.tiles[ct].kb),
-                       uniform(&a.tiles[ct].n)};
+    while (u >= uniform(a.cum + ct + 1) * a.kv.hkv) ct++;  // (u is below the last entry's)
+    const Kv4Tile tile = uniform_tile(a.tiles + ct);
     const int64_t in = u - uniform(a.cum + ct) * a.kv.hkv;
     const int head = (int)(in / tile.n);
     const int t0 = (int)(in - (int64_t)head * tile.n);
     const int t1 = (int)min((int64_t)tile.n, t0 + (u_end - u));
     const int seq = tile.seq;
-    const int row0 = a.cu_q ? uniform(a.cu_q + seq) : seq;
-    const int qlen = a.cu_q ? uniform(a.cu_q + seq + 1) - row0 : 1;
-    const int klen = a.lens ? uniform(a.lens + seq) : uniform(a.cu_k + seq + 1) - uniform(a.cu_k + seq);
+    const int row0 = tile.row0, qlen = tile.qlen, klen = tile.klen;
     const int64_t cols = (int64_t)qlen * rep;
     const int64_t first_col = (int64_t)tile.col0 + (TILES ? wave * (16 * NG) : 0);
     const bool whole = t0 == 0 && t1 == tile.n;
     const int64_t part0 = (int64_t)(2 * blockIdx.x + (t0 == 0 ? 1 : 0)) * COLS;
+    if (t0 > 0 && t0 <= chunk) {  // (its workgroup's first segment) the workgroup before began it
+      border = Kv4Border{(int32_t)(blockIdx.x - 1),
+                         (int32_t)(blockIdx.x + ((int64_t)tile.n - t0 - 1) / chunk), row0, head * rep,
+                         tile.col0, (int32_t)min((int64_t)COLS, cols - tile.col0)};
+    }
     u += t1 - t0;
     if (TILES && first_col >= cols) continue;  // (a wave by itself: these waves meet at no barrier)
     // The columns whose scores the lane has see keys [lo, hi).  (Columns past the last repeat it.)
@@ -527,16 +565,21 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
       return a.tile_shift >= 0 ? kt >> a.tile_shift : kt / per_block;
     };
     auto block_of = [&](int t) { return uniform(table + block_index(t)); };
-    auto load = [&](int t, int block, Tile<D> &into) {
+    auto buffer = [&](int t, int block) {
       const int in_block = tile.kb + t - block_index(t) * per_block;
-      load_tile<D, !TILES>(a.kv.pages + tile_at(a.kv, block, head, in_block, D), places, into);
+      return __builtin_amdgcn_make_buffer_rsrc(a.kv.pages + tile_at(a.kv, block, head, in_block, D),
+                                               (short)0, 34 * D, kBufferWord3);
+    };
+    auto load = [&](int t, int block, Tile<D> &into) {
+      const __amdgpu_buffer_rsrc_t from = buffer(t, block);
+      load_keys<D, !TILES>(from, places, into);
+      load_values<D, !TILES>(from, places, into);
       // The loads go out before the products of the tile at hand (the compiler would have them wait for
       // that tile, whose registers it could then use again).
       __builtin_amdgcn_sched_barrier(0);
     };
-    auto attend = [&](int t, Tile<D> &cur) {
-      // Scores of the 32 keys, of either half of them.
-      f32x4 s[NG][2];
+    // Scores of the 32 keys, of either half of them.
+    auto scores = [&](const Tile<D> &cur, f32x4 (*s)[2]) {
 #pragma unroll
       for (int g = 0; g < NG; g++) s[g][0] = s[g][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -553,6 +596,9 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
             s[g][1] = FEW ? mfma(qv, k1, s[g][1]) : mfma(k1, qv, s[g][1]);
           }
       }
+    };
+    // Their probabilities, and the values of their V.
+    auto values = [&](int t, Tile<D> &cur, f32x4 (*s)[2]) {
       const int key0 = (tile.kb + t) * 32;
       const bool edge = key0 + 32 > all_hi || key0 < all_lo;
       constexpr int NX = FEW ? 2 : 8;  // scores of a lane and column: keys NX (lane's) .. + NX - 1
@@ -654,27 +700,54 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
       }
       add_values<D, NG, NP, FEW>(cur, unit, p, o);
     };
+    auto attend = [&](int t, Tile<D> &cur) {
+      f32x4 s[NG][2];
+      scores(cur, s);
+      values(t, cur, s);
+    };
     int t = tb + (TILES ? 0 : wave);
-    if constexpr (AHEAD) {
-      // (The last turns load the last tile again: loads behind a condition would be waited for as if
-      // they were needed at once.)
-      Tile<D> one, two;
+    if constexpr (TILES) {
+      // One tile's registers: the next keys are loaded behind the scores, the next values behind the sums.
+      // (The last turns load the last tile again: loads behind a condition would be waited for as if they
+      // were needed at once.)
+      Tile<D> one;
       if (t < te) {
         load(t, block_of(t), one);
         int next = min(t + STRIDE, te - 1), block = block_of(next);
+        for (; t < te; t += STRIDE) {
+          f32x4 s[NG][2];
+          scores(one, s);
+          const __amdgpu_buffer_rsrc_t from = buffer(next, block);
+          __builtin_amdgcn_sched_barrier(0);
+          load_keys<D, !TILES>(from, places, one);
+          next = min(t + 2 * STRIDE, te - 1);
+          block = block_of(next);
+          __builtin_amdgcn_sched_barrier(0);
+          values(t, one, s);
+          __builtin_amdgcn_sched_barrier(0);
+          load_values<D, !TILES>(from, places, one);
+        }
+      }
+    } else if constexpr (D <= 256) {
+      // The next tile loads into the other registers while this one is attended.  (The last turn loads the
+      // last tile again: loads behind a condition would be waited for as if they were needed at once.)  Two
+      // and three tiles ahead were 2 to 20% slower for the registers that they take.
+      Tile<D> even, odd;
+      if (t < te) {
+        int next = t, block = block_of(t);
+        auto ahead = [&](Tile<D> &into) {
+          load(next, block, into);
+          next = min(next + STRIDE, te - 1);
+          block = block_of(next);
+        };
+        ahead(even);
         while (true) {
-          load(next, block, two);
-          next = min(t + 2 * STRIDE, te - 1);
-          block = block_of(next);
-          attend(t, one);
-          t += STRIDE;
-          if (t >= te) break;
-          load(next, block, one);
-          next = min(t + 2 * STRIDE, te - 1);
-          block = block_of(next);
-          attend(t, two);
-          t += STRIDE;
-          if (t >= te) break;
+          ahead(odd);
+          attend(t, even);
+          if ((t += STRIDE) >= te) break;
+          ahead(even);
+          attend(t, odd);
+          if ((t += STRIDE) >= te) break;
         }
       }
     } else {
@@ -791,94 +864,95 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
     }
     if constexpr (!QLDS) __syncthreads();  // lds_o is written again
   }
+  if (threadIdx.x == 0) a.borders[blockIdx.x] = border;
 }
 
-// Joins the partials of column tiles that several workgroups shared: workgroup x the one (of a column tile
-// and KV head) whose first border between workgroups is that of x - 1 and x, a wave a column.  Then zeroes
-// for rows without keys and rows that no sequence covers.
+// Joins the partials of column tiles that several workgroups shared: workgroup x that of the first border
+// between workgroups in it, which workgroup x of the attention left.  W waves a column, 4 / W columns a
+// workgroup.  Then zeroes for rows without keys and rows that no sequence covers.
+template <int W>
 __global__ void __launch_bounds__(256) kv4_merge_kernel(Kv4Attention a, int cols_of_tile) {
-  const int n_tiles = a.head->tiles, D = a.head_dim, rep = a.hq / a.kv.hkv, hkv = a.kv.hkv;
-  const int64_t chunk = a.head->chunk, all = a.cum[n_tiles] * hkv;
+  const int D = a.head_dim, rep = a.hq / a.kv.hkv;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t border = (int64_t)blockIdx.x * chunk;
-  if (blockIdx.x > 0 && border < all) {
-    int ct = find_tile(a.cum, n_tiles, border, hkv, lane);
-    while (a.tiles[ct].n == 0) ct++;
-    const Kv4Tile tile = a.tiles[ct];
-    const int64_t in = border - a.cum[ct] * hkv;
-    const int head = (int)(in / tile.n);
-    const int64_t u0 = border - (in - (int64_t)head * tile.n), u1 = u0 + tile.n;
-    if (u0 < border && u0 >= border - chunk) {
-      const int64_t g0 = blockIdx.x - 1, g1 = (u1 - 1) / chunk;
-      const int row0 = a.cu_q ? a.cu_q[tile.seq] : tile.seq;
-      const int qlen = a.cu_q ? a.cu_q[tile.seq + 1] - row0 : 1;
-      const int64_t cols = (int64_t)qlen * rep;
-      for (int c = wave + 4 * blockIdx.y; c < cols_of_tile; c += 4 * gridDim.y) {
-        const int64_t col = (int64_t)tile.col0 + c;
-        if (col >= cols) break;
-        const int row = (int)(col / rep);
-        float *dst = a.out + ((size_t)(row0 + row) * a.hq + (size_t)head * rep + (col - (int64_t)row * rep)) * D;
-        // Partial of workgroup g: its last for the first one, its first for the others.
-        auto slot = [&](int64_t g) { return (size_t)(2 * g + (g == g0 ? 1 : 0)) * cols_of_tile + c; };
-        float big = -INFINITY;
-        for (int64_t g = g0 + lane; g <= g1; g += 64) big = fmaxf(big, a.part_m[slot(g)]);
+  const Kv4Border b = a.borders[blockIdx.x];
+  const int c = blockIdx.y * (4 / W) + wave / W;
+  if (b.g1 >= 0 && c < b.cols) {  // (uniform over a column's waves)
+    const int col = b.col0 + c, row = col / rep;
+    float *dst = a.out + ((size_t)(b.row0 + row) * a.hq + b.head0 + (col - row * rep)) * D;
+    // Partial of workgroup g: its last for the first one, its first for the others.
+    auto slot = [&](int g) { return (size_t)(2 * g + (g == b.g0 ? 1 : 0)) * cols_of_tile + c; };
+    float big = -INFINITY;
+    for (int g = b.g0 + lane; g <= b.g1; g += 64) big = fmaxf(big, a.part_m[slot(g)]);
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) big = fmaxf(big, __shfl_xor(big, d));
-        float sum = 0.f;
-        f32x2 acc[4] = {};  // dims 2 lane + 128 i
-        for (int64_t base = g0; base <= g1; base += 64) {
-          // A lane a partial's weight, then all lanes its row.
-          float f = 0.f;
-          if (base + lane <= g1) {
-            const float m = a.part_m[slot(base + lane)], l = a.part_l[slot(base + lane)];
-            // (No reference: no keys, or scores that are NaN, which the sum holds.)
-            f = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - big);
-            sum += f * l;
-          }
-          const int n = (int)min((int64_t)64, g1 - base + 1);
-          for (int i = 0; i < n; i += 4) {  // four rows' loads at once
-            f32x2 row[4][4];
-            float w[4];
+    for (int d = 1; d < 64; d <<= 1) big = fmaxf(big, __shfl_xor(big, d));
+    float sum = 0.f;
+    f32x2 acc[4] = {};  // dims 2 lane + 128 i
+    for (int base = b.g0; base <= b.g1; base += 64) {
+      // A lane a partial's weight, then all lanes the wave's rows.
+      float f = 0.f;
+      if (base + lane <= b.g1) {
+        const float m = a.part_m[slot(base + lane)], l = a.part_l[slot(base + lane)];
+        // (No reference: no keys, or scores that are NaN, which the sum holds.)
+        f = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - big);
+        sum += f * l;
+      }
+      const int n = min(64, b.g1 - base + 1);
+      for (int i = W == 1 ? 0 : wave; i < n; i += 4 * W) {  // four rows' loads at once
+        f32x2 row_of[4][4];
+        float w[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-              w[j] = i + j < n ? __shfl(f, i + j) : 0.f;
-              const float *src = a.part_o + slot(base + min(i + j, n - 1)) * D;
+        for (int j = 0; j < 4; j++) {
+          const int at = min(i + j * W, n - 1);
+          w[j] = i + j * W < n ? __shfl(f, at) : 0.f;
+          const float *src = a.part_o + slot(base + at) * D;
 #pragma unroll
-              for (int k = 0; k < 4; k++)
-                if (2 * lane + 128 * k < D)
-                  row[j][k] = *reinterpret_cast<const f32x2 *>(src + 2 * lane + 128 * k);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-#pragma unroll
-              for (int k = 0; k < 4; k++)  // (a row without weight saw nothing)
-                if (2 * lane + 128 * k < D && w[j] != 0.f) acc[k] += w[j] * row[j][k];
-          }
+          for (int k = 0; k < 4; k++)
+            if (2 * lane + 128 * k < D)
+              row_of[j][k] = *reinterpret_cast<const f32x2 *>(src + 2 * lane + 128 * k);
         }
-        // (In a fixed order: a lane's sums, then lane by lane.)
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        for (int j = 0; j < 4; j++)
 #pragma unroll
-        for (int k = 0; k < 4; k++)
-          if (2 * lane + 128 * k < D)
-            *reinterpret_cast<f32x2 *>(dst + 2 * lane + 128 * k) = acc[k] * inv;
+          for (int k = 0; k < 4; k++)  // (a row without weight saw nothing)
+            if (2 * lane + 128 * k < D && w[j] != 0.f) acc[k] += w[j] * row_of[j][k];
+      }
+    }
+    // (In a fixed order: a lane's sums, then lane by lane.)
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if constexpr (W == 1) {
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        if (2 * lane + 128 * k < D)
+          *reinterpret_cast<f32x2 *>(dst + 2 * lane + 128 * k) = acc[k] * inv;
+    } else {
+      __shared__ f32x2 sums[W][256];
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        if (2 * lane + 128 * k < D) sums[wave][lane + 64 * k] = acc[k];
+      __syncthreads();
+      for (int e = threadIdx.x; 2 * e < D; e += 256) {
+        f32x2 all = sums[0][e];
+#pragma unroll
+        for (int i = 1; i < W; i++) all += sums[i][e];
+        *reinterpret_cast<f32x2 *>(dst + 2 * e) = all * inv;
       }
     }
   }
   if (blockIdx.y != 0) return;
+  const int n_tiles = a.head->tiles;
   const int64_t stride = (int64_t)gridDim.x * 256, i0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const size_t width = (size_t)a.hq * D;
   // Rows whose column tile has no keys, a thread a column tile (there are few, and its rows are few).
   for (int64_t t = i0; t < n_tiles; t += stride) {
     const Kv4Tile tile = a.tiles[t];
     if (tile.n) continue;
-    const int row0 = a.cu_q ? a.cu_q[tile.seq] : tile.seq;
-    const int qlen = a.cu_q ? a.cu_q[tile.seq + 1] - row0 : 1;
-    const int64_t end = min((int64_t)qlen * rep, (int64_t)tile.col0 + cols_of_tile);
+    const int row0 = tile.row0;
+    const int64_t end = min((int64_t)tile.qlen * rep, (int64_t)tile.col0 + cols_of_tile);
     for (int64_t col = tile.col0; col < end; col++) {
       const int64_t row = col / rep;
-      for (int h = 0; h < hkv; h++) {
+      for (int h = 0; h < a.kv.hkv; h++) {
         float *dst = a.out + (row0 + row) * width + ((size_t)h * rep + (col - row * rep)) * D;
         for (int e = 0; e < D; e += 4) *reinterpret_cast<float4 *>(dst + e) = make_float4(0.f, 0.f, 0.f, 0.f);
       }
@@ -1048,9 +1122,14 @@ int kv4_workgroups_per_cu(int head_dim, int mode) {
   }
 }
 
-hipError_t launch_kv4_merge(const Kv4Attention &a, int mode, int workgroups, hipStream_t s) {
+hipError_t launch_kv4_merge(const Kv4Attention &a, int mode, int workgroups, int items, hipStream_t s) {
   const int cols = kv4_cols(a.head_dim, mode);
-  hipLaunchKernelGGL(kv4_merge_kernel, dim3(workgroups, (cols + 15) / 16), dim3(256), 0, s, a, cols);
+  // Few column tiles and heads (items) leave many partials each, for which four waves share a column (three
+  // rows of 60-120K tokens, 43 partials: 13.5 -> 7 us; 1024 items: 8.7 us against 6.5 with one wave).
+  if (mode != KV4_TILES && items <= workgroups / 4)
+    hipLaunchKernelGGL(kv4_merge_kernel<4>, dim3(workgroups, cols), dim3(256), 0, s, a, cols);
+  else
+    hipLaunchKernelGGL(kv4_merge_kernel<1>, dim3(workgroups, cols / 4), dim3(256), 0, s, a, cols);
   return hipGetLastError();
 }
 

@@ -218,23 +218,20 @@ constexpr int kv4_cols(int head_dim, int mode) {
   return mode == KV4_FEW ? 4 : mode == KV4_EIGHT ? 8 : mode == KV4_ROWS ? 16 : head_dim <= 128 ? 128 : 64;
 }
 // Waves a SIMD that the registers are held down to.
-#ifndef KV4_W1
-#define KV4_W1 3
-#endif
-#ifndef KV4_W2
-#define KV4_W2 2
-#endif
-#ifndef KV4_W3
-#define KV4_W3 2
-#endif
 constexpr int kv4_min_waves(int head_dim, int mode) {
-  return mode == KV4_FEW     ? (head_dim <= 128 ? KV4_W1 : head_dim <= 256 ? KV4_W2 : 1)
-         : mode == KV4_EIGHT ? (head_dim <= 128 ? KV4_W3 : 1)
+  return mode == KV4_FEW     ? (head_dim <= 128 ? 3 : head_dim <= 256 ? 2 : 1)
+         : mode == KV4_EIGHT ? (head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1)
          : mode == KV4_ROWS  ? (head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1)
-                             : (head_dim <= 64 ? 2 : 1);
+                             : (head_dim <= 64 ? 3 : 2);
 }
 struct Kv4Tile {
-  int32_t seq, col0, kb, n;  // n 0: no key is seen
+  int32_t seq, col0, kb, n;       // n 0: no key is seen
+  int32_t row0, qlen, klen, pad;  // the sequence's rows and keys
+};
+// A column tile that workgroups g0 .. g1 shared (g1 < 0: none): its first row, its KV head's first query head
+// and its columns.
+struct Kv4Border {
+  int32_t g0, g1, row0, head0, col0, cols;
 };
 struct Kv4Head {
   int64_t chunk;  // units of a workgroup
@@ -253,6 +250,7 @@ struct Kv4List {
   int32_t num_seqs, rep, hkv, window, workgroups;
   int32_t cols;                // columns of a column tile
   int32_t min_cols, max_cols;  // the sequences of the list, by their columns
+  int32_t one_each;            // no sequence has more than one column tile
   int32_t unit, min_units;     // a workgroup's units: a multiple of unit, at least min_units
 };
 struct Kv4Store {
@@ -270,11 +268,13 @@ struct Kv4Attention {
   const Kv4Head *head;
   const Kv4Tile *tiles;
   const int64_t *cum;
-  const int32_t *cu_q, *cu_k, *lens, *table;
+  const int32_t *table;
+  int32_t room;  // column tiles that cum has room for
   int32_t bt_stride, hq, head_dim, window, tokens;
   int32_t zero_rest;   // the merge zeroes the rows that no sequence covers
   int32_t tile_shift;  // log2 of a block's tiles, or -1
   float scale2;        // scale * log2(e)
+  Kv4Border *borders;  // [workgroups]
   float *part_m, *part_l, *part_o;
 };
 bool kv4_supports(int head_dim);
@@ -283,7 +283,7 @@ hipError_t launch_kv4_read(const Kv4View &kv, int head_dim, const int32_t *slots
                            int rows, hipStream_t s);
 int kv4_workgroups_per_cu(int head_dim, int mode);  // resident on the current device
 hipError_t launch_kv4_attention(const Kv4Attention &a, int mode, int workgroups, hipStream_t s);
-hipError_t launch_kv4_merge(const Kv4Attention &a, int mode, int workgroups, hipStream_t s);
+hipError_t launch_kv4_merge(const Kv4Attention &a, int mode, int workgroups, int items, hipStream_t s);
 hipError_t launch_quantize4(const float *x, int64_t values, uint8_t *codes, uint8_t *scales,
                             hipStream_t s);
 
