@@ -78,40 +78,77 @@ __device__ __forceinline__ void mx4_values8(uint32_t word, float unit, float *x)
 #undef NVA_PAIR
 }
 
+// The largest magnitude of three (where one is NaN: of the others, or NaN).
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, |%1|, |%2|, |%3|" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+// x less its top half, exactly: the halves of a pair by a dot product with (-1, 0) and (0, -1), one
+// instruction where taking the half apart and subtracting it are two.  (The masks stay in registers: as
+// constants they would be read as fp32 ones.)
+__device__ __forceinline__ float less_half(uint32_t halves, uint32_t minus, float x) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, halves),
+                                         __builtin_bit_cast(bf16x2, minus), x, false);
+}
+
 // fp32 values as three bf16 parts whose sum they are: the top 8 bits of the significand, of what is left
-// and of what is left then (cut off, not rounded, so nothing overflows).  parts[p] holds 8 values.
-// FINITE: the values are finite or quiet NaNs; otherwise an infinity is its first part alone.
-template <bool FINITE> __device__ __forceinline__ void split3(const float *x, bf16x8 *parts) {
-  u32x4 w[3];
-  float v[8];
-#pragma unroll
-  for (int i = 0; i < 8; i++) v[i] = x[i];
+// and of what is left then (cut off, not rounded, so nothing overflows).  w[p] holds the pairs' parts p.
+// FINITE: the values are finite, or the NaNs among them may reach their neighbour too; otherwise an
+// infinity is its first part alone.  (A NaN less its top half is a quiet NaN.)
+template <bool FINITE, int PAIRS>
+__device__ __forceinline__ void split3_pairs(const float *x, uint32_t (*w)[PAIRS]) {
   bool odd = false;
-  if (!FINITE) odd = __any(mx4_top8(x) >= 0x7f800000u);
-  if (odd) {  // NaNs whose payload is below the top half keep being one
+  if (!FINITE) {
+    float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-      if (v[i] != v[i]) v[i] = __uint_as_float(0x7fc00000u);
+    for (int i = 0; i < PAIRS; i++) top = max3_abs(top, x[2 * i], x[2 * i + 1]);
+    odd = __any(!(top < INFINITY));
   }
+  if (odd) {
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    float a = v[2 * i], b = v[2 * i + 1];
+    for (int i = 0; i < PAIRS; i++) {
+      float a = x[2 * i], b = x[2 * i + 1];
+      // NaNs whose payload is below the top half keep being one.
+      if (a != a) a = __uint_as_float(0x7fc00000u);
+      if (b != b) b = __uint_as_float(0x7fc00000u);
 #pragma unroll
-    for (int p = 0; p < 3; p++) {
-      const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
-      w[p][i] = __builtin_amdgcn_perm(ub, ua, 0x07060302u);  // their top halves, a below
-      if (p < 2) {
+      for (int p = 0; p < 3; p++) {
+        const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+        w[p][i] = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
         a -= __uint_as_float(ua & 0xffff0000u);
         b -= __uint_as_float(ub & 0xffff0000u);
-        if (odd && p == 0) {  // (an infinity less itself)
-          if (a != a) a = 0.f;
-          if (b != b) b = 0.f;
-        }
+        if (a != a) a = 0.f;  // (an infinity less itself)
+        if (b != b) b = 0.f;
+      }
+    }
+    return;
+  }
+  uint32_t first = 0x0000bf80u, second = 0xbf800000u;
+  asm("" : "+s"(first));
+  asm("" : "+s"(second));
+#pragma unroll
+  for (int i = 0; i < PAIRS; i++) {
+    float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+    for (int p = 0; p < 3; p++) {
+      w[p][i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);  // a below
+      if (p < 2) {
+        a = less_half(w[p][i], first, a);
+        b = less_half(w[p][i], second, b);
       }
     }
   }
+}
+
+// 8 values; parts[p] holds parts p.
+template <bool FINITE> __device__ __forceinline__ void split3(const float *x, bf16x8 *parts) {
+  uint32_t w[3][4];
+  split3_pairs<FINITE, 4>(x, w);
 #pragma unroll
-  for (int p = 0; p < 3; p++) parts[p] = __builtin_bit_cast(bf16x8, w[p]);
+  for (int p = 0; p < 3; p++)
+    parts[p] = __builtin_bit_cast(bf16x8, u32x4{w[p][0], w[p][1], w[p][2], w[p][3]});
 }
 
 }  // namespace nva
