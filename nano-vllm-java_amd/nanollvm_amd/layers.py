@@ -115,6 +115,13 @@ def _on(t: Optional[torch.Tensor], name: str, device: int):
     return p
 
 
+def _all_on(ctx: "Context", **tensors) -> None:
+    """The 4-bit calls' check that their tensors are on the context's device."""
+    for name, t in tensors.items():
+        if t is not None and t.get_device() != ctx.device:
+            raise IllegalArgumentException(f"{name} must be on the context's device")
+
+
 class _Memory:
     """Device memory of the library as torch.as_tensor takes it; keeps its owner alive."""
 
@@ -604,10 +611,12 @@ class Attention:
         self._check_shapes(q, k, v)
         arena = ctx.kv_cache()
         qp = _dev(q, "q")
+        four = isinstance(arena, KvCacheArena4)
+        if four:
+            _all_on(ctx, q=q, k=k, v=v)
         out = torch.empty_like(q)
         lib = N.load()
-        _check(ctx.handle, (lib.nva_attention4_forward if isinstance(arena, KvCacheArena4) else
-                            lib.nva_attention_forward)(
+        _check(ctx.handle, (lib.nva_attention4_forward if four else lib.nva_attention_forward)(
             ctx.handle, arena.handle if arena is not None else None, ctypes.byref(self._desc),
             qp, _dev(k, "k"), _dev(v, "v"), q.shape[0], out.data_ptr()), "Attention.forward")
         return out
@@ -656,14 +665,16 @@ class Attention:
         for n in (q_norm, k_norm, v_norm):
             if n is not None and n.weight is not None and n.weight.numel() != self.head_dim:
                 raise IllegalArgumentException("head norm weights must have headDim entries")
+        arena = ctx.kv_cache()
+        four = isinstance(arena, KvCacheArena4)
+        if four:
+            _all_on(ctx, q=q, k=k, v=v, q_out=q_out, k_out=k_out)
         if positions is not None:
             ctx.set_positions(positions)
-        arena = ctx.kv_cache()
         out = torch.empty((q.shape[0], self.num_heads, self.head_dim), dtype=torch.float32,
                           device=q.device)
         lib = N.load()
-        _check(ctx.handle, (lib.nva_norm_rope_attention4_forward
-                            if isinstance(arena, KvCacheArena4) else
+        _check(ctx.handle, (lib.nva_norm_rope_attention4_forward if four else
                             lib.nva_norm_rope_attention_forward)(
             ctx.handle, arena.handle if arena is not None else None, rope.handle,
             None if q_norm is None else q_norm.desc(), None if k_norm is None else k_norm.desc(),
@@ -693,14 +704,16 @@ class Attention:
         for n in (q_norm, k_norm, v_norm):
             if n is not None and n.weight is not None and n.weight.numel() != self.head_dim:
                 raise IllegalArgumentException("head norm weights must have headDim entries")
+        arena = ctx.kv_cache()
+        four = isinstance(arena, KvCacheArena4)
+        if four:
+            _all_on(ctx, qkv=qkv, q_out=q_out, k_out=k_out)
         if positions is not None:
             ctx.set_positions(positions)
-        arena = ctx.kv_cache()
         out = torch.empty((T, self.num_heads, self.head_dim), dtype=torch.float32,
                           device=qkv.device)
         lib = N.load()
-        _check(ctx.handle, (lib.nva_qkv_norm_rope_attention4_forward
-                            if isinstance(arena, KvCacheArena4) else
+        _check(ctx.handle, (lib.nva_qkv_norm_rope_attention4_forward if four else
                             lib.nva_qkv_norm_rope_attention_forward)(
             ctx.handle, arena.handle if arena is not None else None, rope.handle,
             None if q_norm is None else q_norm.desc(), None if k_norm is None else k_norm.desc(),
