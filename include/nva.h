@@ -107,6 +107,8 @@ const char *nva_status_string(nva_status status);
  * "attention" spans the attention kernels of one call (decode and prefill kernels that
  * overlap count once).  "prefill_split" and "prefill_fp32" are the part of "prefill" that each of
  * its two tile kernels took, "linear_tiles" the part of "linear" of its 128 x 128-tile kernel.
+ * Steps built on the device: "tables"; what is held in 4 bits: "store4", "read4", "attention4", "merge4",
+ * "quantize4" and "linear4".
  * Host-side entries: "plan" (building a step's work plan on the host, once
  * per step and attention configuration, at its first layer) and "plan_upload" (copying it to
  * the device).  The name "device_bytes" instead returns in *launches the bytes of device memory
@@ -335,7 +337,7 @@ nva_status nva_step_positions(nva_ctx *ctx, const float *positions, int num_toke
  * and does not wait; it may be captured, and replays act on the lengths they find.
  *
  * A step that asks for more than there is changes nothing and has no tokens: every row is padding.
- * nva_tables_status (which waits) tells: status[0] is 0, or 1 for a row (status[1]) whose keep or
+ * nva_tables_status (which waits, and so is not for capture) tells: status[0] is 0, or 1 for a row (status[1]) whose keep or
  * new_tokens is out of range, 2 for more than num_tokens new tokens (status[1] of them, at most INT32_MAX), 3 for more
  * blocks (status[1]) than are free; status[2] is the number of free blocks after the call.
  *
@@ -541,8 +543,10 @@ nva_status nva_qkv_norm_rope_attention4_forward(nva_ctx *ctx, nva_kv4 *kv, const
 
 /* nva_linear_forward with a weight in the 4-bit form: nva_linear4_create lays codes [out, in / 2] and
  * scales [out, in / 32] (device, as nva_quantize4 writes them; in % 32 == 0) out in memory of its own;
- * forward computes y [rows, out] = x [rows, in] W^T (+ bias [out]) from it, x 16-byte aligned.  Products
- * are of x in three exact parts with the held values, sums are fp32. */
+ * forward computes y [rows, out] = x [rows, in] W^T (+ bias [out]) from it, x 16-byte aligned, on any
+ * context of its device.  Products are of x in three exact parts with the held values, sums are fp32.
+ * Under capture a call must not need a larger work area than every earlier one on the context (none is
+ * needed for up to 16 rows).  nva_linear4_destroy waits for the device. */
 nva_status nva_linear4_create(nva_ctx *ctx, const uint8_t *codes, const uint8_t *scales, int out,
                               int in, nva_linear4 **linear);
 nva_status nva_linear4_destroy(nva_linear4 *linear);

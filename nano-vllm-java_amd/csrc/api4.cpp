@@ -524,6 +524,8 @@ nva_status nva_tables_status(nva_tables *t, int32_t *status) {
   if (!t || !status) return NVA_E_ARG;
   nva_ctx *ctx = t->ctx;
   DeviceGuard dg(ctx);
+  if (stream_capturing(ctx->stream))  // (waiting would end the capture)
+    return fail(ctx, NVA_E_ARG, "the status of tables is not for a captured step");
   HIP_TRY(ctx, hipStreamSynchronize(ctx->stream), "stream synchronize");
   HIP_TRY(ctx, hipMemcpy(status, t->state, 12, hipMemcpyDeviceToHost), "tables status");
   return NVA_OK;
@@ -748,7 +750,7 @@ nva_status nva_linear4_create(nva_ctx *ctx, const uint8_t *codes, const uint8_t 
     return fail(ctx, NVA_E_UNSUPPORTED, "linear needs in < 4194304 (got %d)", in);
   if (!codes || !scales) return fail(ctx, NVA_E_ARG, "codes and scales are required");
   std::unique_ptr<nva_linear4> l(new nva_linear4());
-  l->ctx = ctx;
+  l->device = ctx->device;
   l->in = in;
   l->out = out;
   void *p = nullptr;
@@ -768,8 +770,7 @@ nva_status nva_linear4_create(nva_ctx *ctx, const uint8_t *codes, const uint8_t 
 
 nva_status nva_linear4_destroy(nva_linear4 *linear) {
   if (!linear) return NVA_OK;
-  if (linear->ctx) (void)hipStreamSynchronize(linear->ctx->stream);
-  (void)hipFree(linear->weight);
+  (void)hipFree(linear->weight);  // (waits for the device)
   delete linear;
   return NVA_OK;
 }
@@ -779,10 +780,11 @@ nva_status nva_linear4_forward(nva_ctx *ctx, const nva_linear4 *l, const float *
   if (!ctx) return NVA_E_ARG;
   DeviceGuard dg(ctx);
   if (!l) return fail(ctx, NVA_E_ARG, "4-bit linear is null");
-  if (l->ctx->device != ctx->device)
+  if (l->device != ctx->device)
     return fail(ctx, NVA_E_ARG, "4-bit linear belongs to another device");
   if (rows < 0) return fail(ctx, NVA_E_ARG, "rows < 0");
   if (rows == 0) return NVA_OK;
+  if (rows > INT32_MAX - 128) return fail(ctx, NVA_E_UNSUPPORTED, "4-bit linear of %d rows", rows);
   if (!x || !y) return fail(ctx, NVA_E_ARG, "x and y are required");
   if (!aligned16(x)) return fail(ctx, NVA_E_ARG, "x must be a 16-byte aligned device pointer");
   Linear4Launch a{};

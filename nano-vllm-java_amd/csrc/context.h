@@ -285,7 +285,7 @@ struct nva_tables {
 
 // A 4-bit weight, laid out for the matrix cores (linear4.hip).
 struct nva_linear4 {
-  nva_ctx *ctx = nullptr;
+  int device = 0;  // any context of it may use the weight
   int in = 0, out = 0;
   uint8_t *weight = nullptr;
 };
