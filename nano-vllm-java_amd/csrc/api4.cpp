@@ -328,7 +328,8 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
     l.max_cols = r.mode == KV4_TILES ? INT32_MAX : (int)limit;
     l.one_each = n_runs == 1 && std::max(few, many) <= l.cols;
     l.unit = r.mode == KV4_TILES ? 1 : 4;
-    l.min_units = r.mode == KV4_TILES ? 4 : 8;
+    l.min_units = 4;
+    l.slack = r.mode == KV4_TILES ? 0 : 12;
   }
   {
     Timed tm(ctx, "store4");

@@ -85,16 +85,19 @@ __device__ __forceinline__ void store_row(const Kv4View &kv, const float *src, i
 // numbered by column tile, KV head and tile; workgroup g of the attention takes units [g C, (g + 1) C), so
 // every workgroup does the same work however lengths differ.  cum[t] is the units of one KV head before
 // tile t.  The list is built from the lengths on the device, which a captured step's replays find there.
+//
+// A workgroup's segment (its units of one column tile and KV head) costs some 4 us beside its units: q,
+// the first keys and the join of its waves.  So where a few units more, a.slack, let every workgroup have
+// one segment, each column tile's units are rounded up to whole chunks: with 96 rows of 1024 keys of one KV
+// head, d = 256, the attention takes 17.5 us instead of 22.7, with 5 rows of up to 700 keys 7.5 instead of
+// 12.2, with three of 60 to 120 thousand 33.4 instead of 35.6, and the list 1.2 more.
+constexpr int kListThreads = 256, kListRounds = 4;
+
 __device__ void build_list(const Kv4List &a) {
   __shared__ int64_t part[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   auto scan = [&](int64_t v, int64_t &total) {  // exclusive, over the workgroup
-    int64_t x = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int64_t y = __shfl_up((long long)x, d);
-      if (lane >= d) x += y;
-    }
+    const int64_t x = scan_wave(v);
     __syncthreads();
     if (lane == 63) part[wave] = x;
     __syncthreads();
@@ -122,27 +125,12 @@ __device__ void build_list(const Kv4List &a) {
     t.col0 = (int)col0;
     t.kb = beg > 0 ? (int)(beg >> 5) : 0;
     t.n = t.qlen > 0 && end > max(beg, (int64_t)0) ? ((end + 31) >> 5) - t.kb : 0;
+    t.units = t.n;
   };
-  int64_t tiles = 0, units = 0;
-  if (a.one_each) {  // no sequence has more than one column tile: each gets one, of no keys where it has no rows
-    tiles = a.num_seqs;
-    for (int b0 = 0; b0 < a.num_seqs; b0 += 256) {
-      Kv4Tile t{};
-      if (b0 + tid < a.num_seqs) {
-        rows_of(b0 + tid, t);
-        keys_of(0, t);
-      }
-      int64_t all;
-      const int64_t u = units + scan(t.n, all);
-      if (b0 + tid < a.num_seqs) {
-        a.tiles[b0 + tid] = t;
-        a.cum[b0 + tid] = u;
-      }
-      units += all;
-    }
-  } else {
-    // Column tiles before each sequence.
-    for (int b0 = 0; b0 < a.num_seqs; b0 += 256) {
+  int64_t tiles = a.num_seqs;
+  if (!a.one_each) {  // column tiles before each sequence
+    tiles = 0;
+    for (int b0 = 0; b0 < a.num_seqs; b0 += kListThreads) {
       const int b = b0 + tid;
       int64_t mine = 0, all;
       if (b < a.num_seqs) {
@@ -156,19 +144,88 @@ __device__ void build_list(const Kv4List &a) {
     if (tid == 0) a.before[a.num_seqs] = (int32_t)tiles;
     __threadfence_block();
     __syncthreads();
-    // Their key tiles.
-    for (int64_t t0 = 0; t0 < tiles; t0 += 256) {
+  }
+  auto tile_of = [&](int at) {
+    Kv4Tile t{};
+    int64_t col0 = 0;
+    if (a.one_each) {  // no sequence has more than one: each gets one, of no keys where it has no rows
+      rows_of(at, t);
+    } else {
+      int lo = 0, hi = a.num_seqs;  // before[lo] <= at < before[hi]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.before[mid] <= at) lo = mid; else hi = mid;
+      }
+      rows_of(lo, t);
+      col0 = (int64_t)(at - a.before[lo]) * a.cols;
+    }
+    keys_of(col0, t);
+    return t;
+  };
+  int64_t units = 0, chunk = 0;
+  // A multiple of the waves that share a segment, and not so few units that joining costs more.
+  auto chunk_of = [&](int64_t all) {
+    if (all <= (int64_t)a.min_units * a.workgroups) return (int64_t)a.min_units;
+    const int64_t c = (all + a.workgroups - 1) / a.workgroups;
+    return (c + a.unit - 1) / a.unit * a.unit;
+  };
+  if (tiles <= kListRounds * kListThreads) {
+    const int rounds = (int)((tiles + kListThreads - 1) / kListThreads);
+    Kv4Tile mine[kListRounds];
+    int64_t own = 0;
+#pragma unroll
+    for (int i = 0; i < kListRounds; i++) {
+      mine[i] = Kv4Tile{};
+      const int at = i * kListThreads + tid;
+      if (i < rounds && at < tiles) mine[i] = tile_of(at);
+      own += mine[i].n;
+    }
+    int64_t all;
+    scan(own, all);
+    chunk = chunk_of(all * a.hkv);
+    // How many workgroups chunks of 0, 1, 2 and 3 thirds of the slack more would take, two counts a word.
+    if (a.slack > 0 && chunk < (1 << 28)) {
+      int64_t need[2] = {0, 0};
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int c = (int)chunk + k * (a.slack / 3);
+        int64_t n = 0;
+#pragma unroll
+        for (int i = 0; i < kListRounds; i++)
+          if (i < rounds) n += (mine[i].n + c - 1) / c;
+        need[k >> 1] |= min(n, (int64_t)1 << 20) << (32 * (k & 1));
+      }
+      int64_t total[2];
+      scan(need[0], total[0]);
+      scan(need[1], total[1]);
+      for (int k = 0; k < 4; k++)
+        if (((total[k >> 1] >> (32 * (k & 1))) & 0xffffffff) * a.hkv <= a.workgroups) {
+          const int c = (int)chunk + k * (a.slack / 3);
+#pragma unroll
+          for (int i = 0; i < kListRounds; i++)
+            if (i < rounds) mine[i].units = (mine[i].n + c - 1) / c * c;
+          chunk = c;
+          break;
+        }
+    }
+    for (int i = 0; i < rounds; i++) {
+      const int at = i * kListThreads + tid;
+      Kv4Tile t = mine[0];
+#pragma unroll
+      for (int j = 1; j < kListRounds; j++)
+        if (i == j) t = mine[j];
+      const int64_t u = units + scan(t.units, all);
+      if (at < tiles) {
+        a.tiles[at] = t;
+        a.cum[at] = u;
+      }
+      units += all;
+    }
+  } else {
+    for (int64_t t0 = 0; t0 < tiles; t0 += kListThreads) {
       const int at = (int)t0 + tid;
       Kv4Tile t{};
-      if (at < tiles) {
-        int lo = 0, hi = a.num_seqs;  // before[lo] <= at < before[hi]
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) >> 1;
-          if (a.before[mid] <= at) lo = mid; else hi = mid;
-        }
-        rows_of(lo, t);
-        keys_of((int64_t)(at - a.before[lo]) * a.cols, t);
-      }
+      if (at < tiles) t = tile_of(at);
       int64_t all;
       const int64_t u = units + scan(t.n, all);
       if (at < tiles) {
@@ -177,14 +234,12 @@ __device__ void build_list(const Kv4List &a) {
       }
       units += all;
     }
+    chunk = chunk_of(units * a.hkv);
   }
   if (tid == 0) {
     a.cum[tiles] = units;
     a.head->tiles = (int)tiles;
-    // A multiple of the waves that share a segment, and not so few units that joining costs more.
-    const int64_t all = units * a.hkv;
-    const int64_t c = (all + a.workgroups - 1) / a.workgroups;
-    a.head->chunk = max((c + a.unit - 1) / a.unit * a.unit, (int64_t)a.min_units);
+    a.head->chunk = chunk;
     a.head->covered = a.cu_q ? a.cu_q[a.num_seqs] : a.num_seqs;
     a.head->first = a.cu_q ? a.cu_q[0] : 0;
   }
@@ -467,8 +522,8 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
     while (u >= uniform(a.cum + ct + 1) * a.kv.hkv) ct++;  // (u is below the last entry's)
     const Kv4Tile tile = uniform_tile(a.tiles + ct);
     const int64_t in = u - uniform(a.cum + ct) * a.kv.hkv;
-    const int head = (int)(in / tile.n);
-    const int t0 = (int)(in - (int64_t)head * tile.n);
+    const int head = (int)(in / tile.units);
+    const int t0 = (int)(in - (int64_t)head * tile.units);
     const int t1 = (int)min((int64_t)tile.n, t0 + (u_end - u));
     const int seq = tile.seq;
     const int row0 = tile.row0, qlen = tile.qlen, klen = tile.klen;
@@ -481,7 +536,7 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
                          (int32_t)(blockIdx.x + ((int64_t)tile.n - t0 - 1) / chunk), row0, head * rep,
                          tile.col0, (int32_t)min((int64_t)COLS, cols - tile.col0)};
     }
-    u += t1 - t0;
+    u += min((int64_t)tile.units - t0, u_end - u);
     if (TILES && first_col >= cols) continue;  // (a wave by itself: these waves meet at no barrier)
     // The columns whose scores the lane has see keys [lo, hi).  (Columns past the last repeat it.)
     int hi[NG], lo[NG];

@@ -225,8 +225,8 @@ constexpr int kv4_min_waves(int head_dim, int mode) {
                              : (head_dim <= 64 ? 3 : 2);
 }
 struct Kv4Tile {
-  int32_t seq, col0, kb, n;       // n 0: no key is seen
-  int32_t row0, qlen, klen, pad;  // the sequence's rows and keys
+  int32_t seq, col0, kb, n;         // n 0: no key is seen
+  int32_t row0, qlen, klen, units;  // the sequence's rows and keys; n, or n rounded up to whole chunks
 };
 // A column tile that workgroups g0 .. g1 shared (g1 < 0: none): its first row, its KV head's first query head
 // and its columns.
@@ -252,6 +252,7 @@ struct Kv4List {
   int32_t min_cols, max_cols;  // the sequences of the list, by their columns
   int32_t one_each;            // no sequence has more than one column tile
   int32_t unit, min_units;     // a workgroup's units: a multiple of unit, at least min_units
+  int32_t slack;               // how many more units a workgroup may get to have one segment only
 };
 struct Kv4Store {
   Kv4View kv;

@@ -64,4 +64,22 @@ __device__ __forceinline__ float max4_lanes(float x) {
 }
 __device__ __forceinline__ float sum4_lanes(float x) { return add_xor32(add_xor16(x)); }
 
+// The sum over the lanes up to this one of a wave, by moves between neighbouring registers (a scan by
+// shuffles through LDS took four times as long).
+__device__ __forceinline__ int64_t scan_wave(int64_t x) {
+  auto step = [&](auto move) {
+    const uint32_t lo = move((int)(uint32_t)x), hi = move((int)(uint32_t)((uint64_t)x >> 32));
+    x += (int64_t)((uint64_t)hi << 32 | lo);
+  };
+  // Within rows of 16, by 1, 2, 4 and 8 lanes; then a row's last sum to the row behind it, then that of
+  // the first half to the second.
+  step([](int v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false); });
+  step([](int v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false); });
+  step([](int v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false); });
+  step([](int v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false); });
+  step([](int v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false); });
+  step([](int v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false); });
+  return x;
+}
+
 }  // namespace nva

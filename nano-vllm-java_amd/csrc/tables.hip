@@ -12,6 +12,7 @@
 // small step, as a second launch would cost more than the work; steps of more than kFillApart tokens
 // write their slots and positions from a launch of many workgroups.
 #include "nva_internal.h"
+#include "row_lanes.h"
 
 namespace nva {
 
@@ -70,14 +71,7 @@ __global__ void __launch_bounds__(kThreads) tables_extend_kernel(TablesLaunch a)
       }
       kept[b] = (int32_t)keep;
     }
-    int64_t x[3] = {v[0], v[1], v[2]};
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1)
-#pragma unroll
-      for (int i = 0; i < 3; i++) {
-        const int64_t y = __shfl_up((long long)x[i], d);
-        if (lane >= d) x[i] += y;
-      }
+    const int64_t x[3] = {scan_wave(v[0]), scan_wave(v[1]), scan_wave(v[2])};
     if (lane == 63)
       for (int i = 0; i < 3; i++) wave_sum[i][wave] = x[i];
     __syncthreads();
