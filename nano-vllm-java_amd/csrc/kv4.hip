@@ -2,13 +2,15 @@
 // attention and the merge of split rows.
 //
 // Layout.  A layer is [block][KV head][tile of 32 keys][34 d bytes], a tile's bytes being
-//   K codes   [key % 2][key / 2][d / 2]       dim 2j in the low bits of byte j
-//   V codes   [key / 8][row 16][key % 8][d / 32]   row r: dims r d / 16 and on
+//   K codes   [key % 2][run 64][d / 8]   run 16 w + c: of keys 2c and 2c + 1 the dims w d / 4 and on
+//   V codes   [run 64][key % 8][d / 32]  run 16 w + c: of keys 8w .. 8w + 7 the dims c d / 16 and on
 //   K scales  [key / 2][d / 32][key % 2]
 //   V scales  [key / 8][d / 32][key % 8]
-// Lane l = 16 w + c of a wave thus reads its part of either product in one run of bytes, which neighbouring
-// lanes continue, and a token's codes stay apart from its neighbours' (4-byte words at d = 128), so that
-// tokens are stored independently.
+// a pair of dims a byte, the even one in its low bits.  Run l is what lane l of a wave needs for either
+// product; runs of more than 16 bytes are cut into pieces of 16, [piece][run][16], so that each load of a
+// wave is 1 KB in a row (with whole runs in a row a load touched every line of the tile, and 128 rows
+// of up to 16K keys, d = 256, took 83 us instead of 53, and 8 columns of d = 512 141 instead of 97).  A token's codes stay
+// apart from its neighbours' (4-byte words at d = 128), so that tokens are stored independently.
 //
 // Products on the matrix cores (16 x 16 x 32 bf16; operands hold 8 values of the contraction a lane,
 // results rows 4 w .. 4 w + 3 of column c).  The order of the contraction is free: that of the dims follows
@@ -35,6 +37,11 @@ __device__ __forceinline__ size_t tile_at(const Kv4View &kv, int block, int head
   return (((size_t)block * kv.hkv + head) * (kv.block_size >> 5) + tile) * (size_t)(34 * d);
 }
 
+// Where a byte of a lane's run lies among the wave's runs of `run` bytes.
+__host__ __device__ constexpr int run_at(int lane, int byte, int run) {
+  return run <= 16 ? lane * run + byte : (byte >> 4) * 1024 + lane * 16 + (byte & 15);
+}
+
 // Where 8 dims (the i-th 8) of key `key` of a tile lie.
 struct RowPlace {
   int k, v, ks, vs;  // byte offsets in the tile; v for d >= 128
@@ -42,9 +49,10 @@ struct RowPlace {
 __device__ __forceinline__ RowPlace row_place(int d, int key, int i) {
   const int nb = d >> 5, w = key >> 3, slot = key & 7;
   RowPlace p;
-  p.k = ((key & 1) * 16 + (key >> 1)) * (d >> 1) + 4 * i;
+  const int krun = d >> 3, kw = 4 * i / krun;
+  p.k = (key & 1) * 8 * d + run_at(16 * kw + (key >> 1), 4 * i - kw * krun, krun);
   const int per = d >> 4, r = (8 * i) / per, within = (8 * i - r * per) >> 1;
-  p.v = 16 * d + ((w * 16 + r) * 8 + slot) * nb + within;
+  p.v = 16 * d + run_at(w * 16 + r, slot * nb + within, d >> 2);
   p.ks = 32 * d + ((key >> 1) * nb + (i >> 2)) * 2 + (key & 1);
   p.vs = 33 * d + (w * nb + (i >> 2)) * 8 + slot;
   return p;
@@ -309,7 +317,7 @@ template <int D> struct Tile {
   u32x2 vs;
 };
 
-// N words from byte `at` of a tile.  NT: keys read once (without the non-temporal bit a decode step's reads
+// N words from byte `at` of a tile, 4 from each KB.  NT: keys read once (without the non-temporal bit a decode step's reads
 // push everything else out).
 template <int N, bool NT>
 __device__ __forceinline__ void load_words(__amdgpu_buffer_rsrc_t tile, uint32_t at, uint32_t *w) {
@@ -317,7 +325,7 @@ __device__ __forceinline__ void load_words(__amdgpu_buffer_rsrc_t tile, uint32_t
   if constexpr (N >= 4) {
 #pragma unroll
     for (int i = 0; i < N / 4; i++) {
-      const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(tile, at + 16 * i, 0, kPolicy);
+      const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(tile, at + 1024 * i, 0, kPolicy);
 #pragma unroll
       for (int j = 0; j < 4; j++) w[4 * i + j] = x[j];
     }
@@ -336,7 +344,7 @@ struct TilePlaces {
 template <int D> __device__ __forceinline__ TilePlaces tile_places(int lane) {
   constexpr int NB = D / 32;
   const int c = lane & 15, w = lane >> 4;
-  return {(uint32_t)(c * (D / 2) + w * (D / 8)), (uint32_t)(16 * D + lane * (D / 4)),
+  return {(uint32_t)run_at(lane, 0, D / 8), (uint32_t)(16 * D + run_at(lane, 0, D / 4)),
           (uint32_t)(32 * D + (c * NB + (w * D) / 128) * 2),
           (uint32_t)(33 * D + (w * NB + (c * D) / 512) * 8)};
 }
@@ -761,7 +769,7 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
       values(t, cur, s);
     };
     int t = tb + (TILES ? 0 : wave);
-    if constexpr (TILES) {
+    if constexpr (TILES || D == 512) {
       // One tile's registers: the next keys are loaded behind the scores, the next values behind the sums.
       // (The last turns load the last tile again: loads behind a condition would be waited for as if they
       // were needed at once.)
@@ -783,7 +791,7 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
           load_values<D, !TILES>(from, places, one);
         }
       }
-    } else if constexpr (D <= 256) {
+    } else {
       // The next tile loads into the other registers while this one is attended.  (The last turn loads the
       // last tile again: loads behind a condition would be waited for as if they were needed at once.)  Two
       // and three tiles ahead were 2 to 20% slower for the registers that they take.
@@ -804,12 +812,6 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
           attend(t, odd);
           if ((t += STRIDE) >= te) break;
         }
-      }
-    } else {
-      Tile<D> one;
-      for (; t < te; t += STRIDE) {
-        load(t, block_of(t), one);
-        attend(t, one);
       }
     }
     // NaN where a column saw one, then the lane's results: FEW has E dims of column 4 g + w (the sum of

@@ -109,8 +109,10 @@ def _ints(t: Optional[torch.Tensor], name: str, device: int, count: Optional[int
 
 def _on(t: Optional[torch.Tensor], name: str, device: int):
     """_dev of a tensor that has to be on the context's device."""
+    if t is None:
+        return None
     p = _dev(t, name)
-    if t is not None and t.get_device() != device:
+    if t.get_device() != device:
         raise IllegalArgumentException(f"{name} must be on the context's device")
     return p
 
@@ -610,15 +612,18 @@ class Attention:
         arena may be a ``KvCacheArena4``, here and in the forms below."""
         self._check_shapes(q, k, v)
         arena = ctx.kv_cache()
-        qp = _dev(q, "q")
-        four = isinstance(arena, KvCacheArena4)
-        if four:
-            _all_on(ctx, q=q, k=k, v=v)
-        out = torch.empty_like(q)
         lib = N.load()
-        _check(ctx.handle, (lib.nva_attention4_forward if four else lib.nva_attention_forward)(
+        if isinstance(arena, KvCacheArena4):
+            device = ctx.device
+            qp, kp, vp = _on(q, "q", device), _on(k, "k", device), _on(v, "v", device)
+            call = lib.nva_attention4_forward
+        else:
+            qp, kp, vp = _dev(q, "q"), _dev(k, "k"), _dev(v, "v")
+            call = lib.nva_attention_forward
+        out = torch.empty_like(q)
+        _check(ctx.handle, call(
             ctx.handle, arena.handle if arena is not None else None, ctypes.byref(self._desc),
-            qp, _dev(k, "k"), _dev(v, "v"), q.shape[0], out.data_ptr()), "Attention.forward")
+            qp, kp, vp, q.shape[0], out.data_ptr()), "Attention.forward")
         return out
 
     def forward_with_rope(self, rope: RotaryEmbedding, positions, q: torch.Tensor,
@@ -933,11 +938,10 @@ class KvCacheArena4:
         """(k, v) of the slots, the values they stand for in float32 (zeros outside the arena)."""
         device = self._ctx.device
         p = _ints(slots, "slots", device)
-        k, v = (torch.empty(self._shape(layer, slots.numel()), device=slots.device)
-                for _ in range(2))
+        k = torch.empty(self._shape(layer, slots.numel()), dtype=torch.float32, device=slots.device)
+        v = torch.empty_like(k)
         _check(self._ctx.handle, N.load().nva_kv4_read_rows(
-            self._h, layer, p, k.data_ptr(), v.data_ptr(), slots.numel()),
-            "KvCacheArena4.read_rows")
+            self._h, layer, p, k.data_ptr(), v.data_ptr(), k.shape[0]), "KvCacheArena4.read_rows")
         return k, v
 
     def close(self) -> None:
