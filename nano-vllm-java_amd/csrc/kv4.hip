@@ -98,7 +98,9 @@ __device__ __forceinline__ void store_row(const Kv4View &kv, const float *src, i
 // the first keys and the join of its waves.  So where a few units more, a.slack, let every workgroup have
 // one segment, each column tile's units are rounded up to whole chunks: with 96 rows of 1024 keys of one KV
 // head, d = 256, the attention takes 17.5 us instead of 22.7, with 5 rows of up to 700 keys 7.5 instead of
-// 12.2, with three of 60 to 120 thousand 33.4 instead of 35.6, and the list 1.2 more.
+// 12.2, with three of 60 to 120 thousand 33.4 instead of 35.6, and the list 1.2 more.  Elsewhere a segment
+// counts a.over units more, so that a workgroup of many short ones gets fewer keys (20 more: 128 rows of up
+// to 16K keys, four columns of d = 128, 208 -> 194 us, 64 of up to 8K, eight columns, 99 -> 67).
 constexpr int kListThreads = 256, kListRounds = 4;
 
 __device__ void build_list(const Kv4List &a) {
@@ -133,7 +135,7 @@ __device__ void build_list(const Kv4List &a) {
     t.col0 = (int)col0;
     t.kb = beg > 0 ? (int)(beg >> 5) : 0;
     t.n = t.qlen > 0 && end > max(beg, (int64_t)0) ? ((end + 31) >> 5) - t.kb : 0;
-    t.units = t.n;
+    t.units = t.n ? t.n + a.over : 0;
   };
   int64_t tiles = a.num_seqs;
   if (!a.one_each) {  // column tiles before each sequence
@@ -171,6 +173,7 @@ __device__ void build_list(const Kv4List &a) {
     return t;
   };
   int64_t units = 0, chunk = 0;
+  int over = a.over;
   // A multiple of the waves that share a segment, and not so few units that joining costs more.
   auto chunk_of = [&](int64_t all) {
     if (all <= (int64_t)a.min_units * a.workgroups) return (int64_t)a.min_units;
@@ -180,17 +183,20 @@ __device__ void build_list(const Kv4List &a) {
   if (tiles <= kListRounds * kListThreads) {
     const int rounds = (int)((tiles + kListThreads - 1) / kListThreads);
     Kv4Tile mine[kListRounds];
-    int64_t own = 0;
+    int64_t own = 0, begun = 0;
 #pragma unroll
     for (int i = 0; i < kListRounds; i++) {
       mine[i] = Kv4Tile{};
       const int at = i * kListThreads + tid;
       if (i < rounds && at < tiles) mine[i] = tile_of(at);
       own += mine[i].n;
+      begun += mine[i].units;
     }
-    int64_t all;
+    int64_t all, all_begun;
     scan(own, all);
+    scan(begun, all_begun);
     chunk = chunk_of(all * a.hkv);
+    bool single = false;  // every workgroup has one segment
     // How many workgroups chunks of 0, 1, 2 and 3 thirds of the slack more would take, two counts a word.
     if (a.slack > 0 && chunk < (1 << 28)) {
       int64_t need[2] = {0, 0};
@@ -213,9 +219,12 @@ __device__ void build_list(const Kv4List &a) {
           for (int i = 0; i < kListRounds; i++)
             if (i < rounds) mine[i].units = (mine[i].n + c - 1) / c * c;
           chunk = c;
+          over = 0;
+          single = true;
           break;
         }
     }
+    if (!single) chunk = chunk_of(all_begun * a.hkv);
     for (int i = 0; i < rounds; i++) {
       const int at = i * kListThreads + tid;
       Kv4Tile t = mine[0];
@@ -235,7 +244,7 @@ __device__ void build_list(const Kv4List &a) {
       Kv4Tile t{};
       if (at < tiles) t = tile_of(at);
       int64_t all;
-      const int64_t u = units + scan(t.n, all);
+      const int64_t u = units + scan(t.units, all);
       if (at < tiles) {
         a.tiles[at] = t;
         a.cum[at] = u;
@@ -248,6 +257,7 @@ __device__ void build_list(const Kv4List &a) {
     a.cum[tiles] = units;
     a.head->tiles = (int)tiles;
     a.head->chunk = chunk;
+    a.head->over = over;
     a.head->covered = a.cu_q ? a.cu_q[a.num_seqs] : a.num_seqs;
     a.head->first = a.cu_q ? a.cu_q[0] : 0;
   }
@@ -514,6 +524,7 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
     for (int i = lane; i < NG * 16 * kPRow; i += 64) lds_p[i] = 0;
   const int n_tiles = uniform(&a.head->tiles);
   const int64_t chunk = uniform(&a.head->chunk);
+  const int over = uniform(&a.head->over);
   const int64_t all = uniform(a.cum + n_tiles) * a.kv.hkv;
   int64_t u = (int64_t)blockIdx.x * chunk;
   const int64_t u_end = min(u + chunk, all);
@@ -531,8 +542,12 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
     const Kv4Tile tile = uniform_tile(a.tiles + ct);
     const int64_t in = u - uniform(a.cum + ct) * a.kv.hkv;
     const int head = (int)(in / tile.units);
-    const int t0 = (int)(in - (int64_t)head * tile.units);
-    const int t1 = (int)min((int64_t)tile.n, t0 + (u_end - u));
+    // Units [v0, v1) of the KV head's, of which the first `over` are no keys.
+    const int v0 = (int)(in - (int64_t)head * tile.units);
+    const int v1 = (int)min((int64_t)tile.units, v0 + (u_end - u));
+    const int t0 = max(v0 - over, 0), t1 = min(tile.n, v1 - over);
+    u += v1 - v0;
+    if (t1 <= t0) continue;
     const int seq = tile.seq;
     const int row0 = tile.row0, qlen = tile.qlen, klen = tile.klen;
     const int64_t cols = (int64_t)qlen * rep;
@@ -544,7 +559,6 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
                          (int32_t)(blockIdx.x + ((int64_t)tile.n - t0 - 1) / chunk), row0, head * rep,
                          tile.col0, (int32_t)min((int64_t)COLS, cols - tile.col0)};
     }
-    u += min((int64_t)tile.units - t0, u_end - u);
     if (TILES && first_col >= cols) continue;  // (a wave by itself: these waves meet at no barrier)
     // The columns whose scores the lane has see keys [lo, hi).  (Columns past the last repeat it.)
     int hi[NG], lo[NG];

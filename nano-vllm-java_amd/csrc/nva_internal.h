@@ -226,7 +226,7 @@ constexpr int kv4_min_waves(int head_dim, int mode) {
 }
 struct Kv4Tile {
   int32_t seq, col0, kb, n;         // n 0: no key is seen
-  int32_t row0, qlen, klen, units;  // the sequence's rows and keys; n, or n rounded up to whole chunks
+  int32_t row0, qlen, klen, units;  // the sequence's rows and keys; units of a KV head
 };
 // A column tile that workgroups g0 .. g1 shared (g1 < 0: none): its first row, its KV head's first query head
 // and its columns.
@@ -237,7 +237,7 @@ struct Kv4Head {
   int64_t chunk;  // units of a workgroup
   int32_t tiles;
   int32_t first, covered;  // rows of the sequences: [first, covered)
-  int32_t pad;
+  int32_t over;            // units that stand for the beginning of a segment
 };
 // Where the work list goes and what it is made of: row offsets (null: one row a sequence) and the
 // lengths, or the offsets whose differences they are.
@@ -253,6 +253,7 @@ struct Kv4List {
   int32_t one_each;            // no sequence has more than one column tile
   int32_t unit, min_units;     // a workgroup's units: a multiple of unit, at least min_units
   int32_t slack;               // how many more units a workgroup may get to have one segment only
+  int32_t over;                // what beginning a segment costs, in units
 };
 struct Kv4Store {
   Kv4View kv;
