@@ -493,6 +493,12 @@ constexpr int kPRow = 20;
 // they are then below 2^kSlack, which fp32 holds as exactly as those below 1.
 constexpr float kSlack = 40.f;
 
+// The weight of a partial beside those of the highest reference.  (No reference: no keys, or scores that are
+// NaN, which the sum holds.)
+__device__ __forceinline__ float weight_of(float m, float l, float big) {
+  return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - big);
+}
+
 }  // namespace
 
 // Workgroup g: its units' segments, each of one column tile and KV head, with the running reference and
@@ -904,8 +910,7 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
 #pragma unroll
     for (int i = 0; i < kWaves; i++) {
       const float li = lds_l[i * COLS + oc];
-      // (No reference: no keys, or scores that are NaN, which the sum holds.)
-      ms[i] = ms[i] == -INFINITY ? (li == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(ms[i] - big);
+      ms[i] = weight_of(ms[i], li, big);
       sum += ms[i] * li;
     }
     const int64_t ocol = (int64_t)tile.col0 + oc;
@@ -952,62 +957,90 @@ __global__ void __launch_bounds__(256) kv4_merge_kernel(Kv4Attention a, int cols
     float *dst = a.out + ((size_t)(b.row0 + row) * a.hq + b.head0 + (col - row * rep)) * D;
     // Partial of workgroup g: its last for the first one, its first for the others.
     auto slot = [&](int g) { return (size_t)(2 * g + (g == b.g0 ? 1 : 0)) * cols_of_tile + c; };
-    float big = -INFINITY;
-    for (int g = b.g0 + lane; g <= b.g1; g += 64) big = fmaxf(big, a.part_m[slot(g)]);
+    if (W == 1 && b.g1 - b.g0 < 4) {  // few partials: all of their loads at once
+      float m[4], l[4], big = -INFINITY, sum = 0.f;
+      f32x2 row_of[4][4], acc[4] = {};
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) big = fmaxf(big, __shfl_xor(big, d));
-    float sum = 0.f;
-    f32x2 acc[4] = {};  // dims 2 lane + 128 i
-    for (int base = b.g0; base <= b.g1; base += 64) {
-      // A lane a partial's weight, then all lanes the wave's rows.
-      float f = 0.f;
-      if (base + lane <= b.g1) {
-        const float m = a.part_m[slot(base + lane)], l = a.part_l[slot(base + lane)];
-        // (No reference: no keys, or scores that are NaN, which the sum holds.)
-        f = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - big);
-        sum += f * l;
+      for (int j = 0; j < 4; j++) {
+        const size_t at = slot(min(b.g0 + j, b.g1));
+        m[j] = a.part_m[at];
+        l[j] = a.part_l[at];
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+          if (2 * lane + 128 * k < D)
+            row_of[j][k] = *reinterpret_cast<const f32x2 *>(a.part_o + at * D + 2 * lane + 128 * k);
       }
-      const int n = min(64, b.g1 - base + 1);
-      for (int i = W == 1 ? 0 : wave; i < n; i += 4 * W) {  // four rows' loads at once
-        f32x2 row_of[4][4];
-        float w[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const int at = min(i + j * W, n - 1);
-          w[j] = i + j * W < n ? __shfl(f, at) : 0.f;
-          const float *src = a.part_o + slot(base + at) * D;
+      for (int j = 0; j < 4; j++) big = fmaxf(big, m[j]);
 #pragma unroll
-          for (int k = 0; k < 4; k++)
-            if (2 * lane + 128 * k < D)
-              row_of[j][k] = *reinterpret_cast<const f32x2 *>(src + 2 * lane + 128 * k);
-        }
+      for (int j = 0; j < 4; j++) {
+        const float f = b.g0 + j > b.g1 ? 0.f : weight_of(m[j], l[j], big);
+        sum += f * l[j];
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-#pragma unroll
-          for (int k = 0; k < 4; k++)  // (a row without weight saw nothing)
-            if (2 * lane + 128 * k < D && w[j] != 0.f) acc[k] += w[j] * row_of[j][k];
+        for (int k = 0; k < 4; k++)
+          if (2 * lane + 128 * k < D && f != 0.f) acc[k] += f * row_of[j][k];
       }
-    }
-    // (In a fixed order: a lane's sums, then lane by lane.)
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    if constexpr (W == 1) {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
       for (int k = 0; k < 4; k++)
-        if (2 * lane + 128 * k < D)
-          *reinterpret_cast<f32x2 *>(dst + 2 * lane + 128 * k) = acc[k] * inv;
+        if (2 * lane + 128 * k < D) *reinterpret_cast<f32x2 *>(dst + 2 * lane + 128 * k) = acc[k] * inv;
     } else {
-      __shared__ f32x2 sums[W][256];
+      float big = -INFINITY;
+      for (int g = b.g0 + lane; g <= b.g1; g += 64) big = fmaxf(big, a.part_m[slot(g)]);
 #pragma unroll
-      for (int k = 0; k < 4; k++)
-        if (2 * lane + 128 * k < D) sums[wave][lane + 64 * k] = acc[k];
-      __syncthreads();
-      for (int e = threadIdx.x; 2 * e < D; e += 256) {
-        f32x2 all = sums[0][e];
+      for (int d = 1; d < 64; d <<= 1) big = fmaxf(big, __shfl_xor(big, d));
+      float sum = 0.f;
+      f32x2 acc[4] = {};  // dims 2 lane + 128 i
+      for (int base = b.g0; base <= b.g1; base += 64) {
+        // A lane a partial's weight, then all lanes the wave's rows.
+        float f = 0.f;
+        if (base + lane <= b.g1) {
+          const float m = a.part_m[slot(base + lane)], l = a.part_l[slot(base + lane)];
+          f = weight_of(m, l, big);
+          sum += f * l;
+        }
+        const int n = min(64, b.g1 - base + 1);
+        for (int i = W == 1 ? 0 : wave; i < n; i += 4 * W) {  // four rows' loads at once
+          f32x2 row_of[4][4];
+          float w[4];
 #pragma unroll
-        for (int i = 1; i < W; i++) all += sums[i][e];
-        *reinterpret_cast<f32x2 *>(dst + 2 * e) = all * inv;
+          for (int j = 0; j < 4; j++) {
+            const int at = min(i + j * W, n - 1);
+            w[j] = i + j * W < n ? __shfl(f, at) : 0.f;
+            const float *src = a.part_o + slot(base + at) * D;
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+              if (2 * lane + 128 * k < D)
+                row_of[j][k] = *reinterpret_cast<const f32x2 *>(src + 2 * lane + 128 * k);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int k = 0; k < 4; k++)  // (a row without weight saw nothing)
+              if (2 * lane + 128 * k < D && w[j] != 0.f) acc[k] += w[j] * row_of[j][k];
+        }
+      }
+      // (In a fixed order: a lane's sums, then lane by lane.)
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      if constexpr (W == 1) {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+          if (2 * lane + 128 * k < D)
+            *reinterpret_cast<f32x2 *>(dst + 2 * lane + 128 * k) = acc[k] * inv;
+      } else {
+        __shared__ f32x2 sums[W][256];
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+          if (2 * lane + 128 * k < D) sums[wave][lane + 64 * k] = acc[k];
+        __syncthreads();
+        for (int e = threadIdx.x; 2 * e < D; e += 256) {
+          f32x2 all = sums[0][e];
+#pragma unroll
+          for (int i = 1; i < W; i++) all += sums[i][e];
+          *reinterpret_cast<f32x2 *>(dst + 2 * e) = all * inv;
+        }
       }
     }
   }
