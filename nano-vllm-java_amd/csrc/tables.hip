@@ -8,9 +8,10 @@
 // from entry top + returned - 1 - e of the stack as it is then.  So the order of threads decides
 // nothing, and taking is the inverse of returning.
 //
-// What bounds it is latency: a decode step of 256 rows moves some 10 KB.  One workgroup does all of a
-// small step, as a second launch would cost more than the work; steps of more than kFillApart tokens
-// write their slots and positions from a launch of many workgroups.
+// What bounds it is latency: a decode step of 256 rows moves some 10 KB and takes 6.2 us (an empty launch
+// 2.2).  One workgroup does all of a small step, as a second launch would cost more than the work; steps of
+// more than kFillApart tokens write their slots and positions from a launch of many workgroups (61 prompts
+// of 25 thousand tokens: 6.9 and 3.2 us).
 #include "nva_internal.h"
 #include "row_lanes.h"
 
