@@ -222,7 +222,7 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
   // knows of their rows bounds them: the lengths themselves, or the most tokens that follow.
   const int seqs = dev ? ctx->dev_seqs : ctx->is_prefill ? ctx->num_seqs : num_tokens;
   int64_t few = 0, many = 0;  // most columns of a sequence on either list
-  int64_t limit = kv4_has_tiles(d.head_dim) ? 16 : INT32_MAX;
+  int64_t limit = kv4_by_dims(d.head_dim) ? INT32_MAX : 16;
   auto count = [&](int64_t cols) {
     if (cols <= limit) few = std::max(few, cols); else many = std::max(many, cols);
   };
@@ -272,7 +272,8 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
   };
   if (many) add(KV4_TILES);
   // (One list at least: it knows the rows that no sequence covers.)
-  if (few || !many) add(few <= 4 ? KV4_FEW : few <= 8 && kv4_has_tiles(d.head_dim) ? KV4_EIGHT : KV4_ROWS);
+  if (few || !many)
+    add(kv4_by_dims(d.head_dim) ? KV4_DIMS : few <= 4 ? KV4_FEW : few <= 8 ? KV4_EIGHT : KV4_ROWS);
   nva_status st = reserve_for(ctx, ctx->d_plan4, plan_bytes, capturing, "attention work list");
   if (st != NVA_OK) return st;
   st = reserve_for(ctx, ctx->d_part4, part_floats * 4, capturing, "attention partials");
@@ -327,7 +328,7 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
     l.min_cols = r.mode == KV4_TILES ? (int)limit + 1 : 1;
     l.max_cols = r.mode == KV4_TILES ? INT32_MAX : (int)limit;
     l.one_each = n_runs == 1 && std::max(few, many) <= l.cols;
-    l.unit = r.mode == KV4_TILES ? 1 : 4;
+    l.unit = r.mode == KV4_TILES || r.mode == KV4_DIMS ? 1 : 4;
     l.min_units = 4;
     l.slack = r.mode == KV4_TILES ? 0 : 12;
     l.over = r.mode == KV4_TILES ? 2 : 20;

@@ -53,7 +53,9 @@ __device__ __forceinline__ RowPlace row_place(int d, int key, int i) {
   const int krun = d >> 3, kw = 4 * i / krun;
   p.k = (key & 1) * 8 * d + run_at(16 * kw + (key >> 1), 4 * i - kw * krun, krun);
   const int per = d >> 4, r = (8 * i) / per, within = (8 * i - r * per) >> 1;
-  p.v = 16 * d + run_at(w * 16 + r, slot * nb + within, d >> 2);
+  // (The quarters of the dims apart where waves share them.)
+  const int byte = kv4_by_dims(d) ? (within >> 2) * 32 + slot * 4 + (within & 3) : slot * nb + within;
+  p.v = 16 * d + run_at(w * 16 + r, byte, d >> 2);
   p.ks = 32 * d + ((key >> 1) * nb + (i >> 2)) * 2 + (key & 1);
   p.vs = 33 * d + (w * nb + (i >> 2)) * 8 + slot;
   return p;
@@ -329,11 +331,11 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(Kv4View kv, const int32_t
 
 namespace {
 
-// One lane's part of a tile.
+// One lane's part of a tile (of a quarter of the dims where waves share them).
 template <int D> struct Tile {
   uint32_t k[2][D / 32];
   uint32_t v[D / 16];
-  uint32_t ks[D == 512 ? 2 : 1];
+  uint32_t ks;
   u32x2 vs;
 };
 
@@ -357,31 +359,29 @@ __device__ __forceinline__ void load_words(__amdgpu_buffer_rsrc_t tile, uint32_t
   }
 }
 
-// Where a lane's parts lie in a tile.
+// Where a lane's parts lie in a tile: of all dims, or (DIMS) of wave's quarter.
 struct TilePlaces {
   uint32_t k, v, ks, vs;
 };
-template <int D> __device__ __forceinline__ TilePlaces tile_places(int lane) {
+template <int D, bool DIMS> __device__ __forceinline__ TilePlaces tile_places(int lane, int wave) {
   constexpr int NB = D / 32;
-  const int c = lane & 15, w = lane >> 4;
-  return {(uint32_t)run_at(lane, 0, D / 8), (uint32_t)(16 * D + run_at(lane, 0, D / 4)),
-          (uint32_t)(32 * D + (c * NB + (w * D) / 128) * 2),
+  const int c = lane & 15, w = lane >> 4, quarter = DIMS ? wave : 0;
+  return {(uint32_t)run_at(lane, 16 * quarter, D / 8), (uint32_t)(16 * D + run_at(lane, 32 * quarter, D / 4)),
+          (uint32_t)(32 * D + (c * NB + (w * D) / 128 + quarter) * 2),
           (uint32_t)(33 * D + (w * NB + (c * D) / 512) * 8)};
 }
 
 // As buffer loads: the tile's address stays in scalar registers and the lane's places do not change, so that
 // no address is computed in registers that loads in flight are still to be written to (which would wait for
-// them).
-template <int D, bool NT>
+// them).  D: the dims that are loaded, of FULL.
+template <int D, int FULL, bool NT>
 __device__ __forceinline__ void load_keys(__amdgpu_buffer_rsrc_t tile, const TilePlaces &p, Tile<D> &t) {
   load_words<D / 32, NT>(tile, p.k, t.k[0]);
-  load_words<D / 32, NT>(tile, p.k + 8 * D, t.k[1]);
-  if constexpr (D == 512)
-    load_words<2, NT>(tile, p.ks, t.ks);
-  else if constexpr (D == 256)
-    load_words<1, NT>(tile, p.ks, t.ks);
+  load_words<D / 32, NT>(tile, p.k + 8 * FULL, t.k[1]);
+  if constexpr (D == 256)
+    load_words<1, NT>(tile, p.ks, &t.ks);
   else
-    t.ks[0] = __builtin_amdgcn_raw_buffer_load_b16(tile, p.ks, 0, NT ? 2 : 0);
+    t.ks = __builtin_amdgcn_raw_buffer_load_b16(tile, p.ks, 0, NT ? 2 : 0);
 }
 template <int D, bool NT>
 __device__ __forceinline__ void load_values(__amdgpu_buffer_rsrc_t tile, const TilePlaces &p, Tile<D> &t) {
@@ -394,8 +394,7 @@ __device__ __forceinline__ void load_values(__amdgpu_buffer_rsrc_t tile, const T
 __device__ __forceinline__ uint32_t byte_of(uint32_t word, int i) { return (word >> (8 * i)) & 255u; }
 
 template <int D> __device__ __forceinline__ float k_unit(const Tile<D> &t, int j, int half) {
-  const int i = (j / 4) * 2 + half;
-  return mx4_unit(byte_of(t.ks[i / 4], i % 4));
+  return mx4_unit(byte_of(t.ks, (j / 4) * 2 + half));
 }
 
 // Low halves, and high halves, of two words: neighbouring slots of one dim out of two dims of each slot.
@@ -518,11 +517,15 @@ __device__ __forceinline__ float weight_of(float m, float l, float big) {
 //                        turn and join through LDS
 //   KV4_ROWS             16 columns, three products; the waves as above
 //   KV4_TILES            NG groups of 16 columns a wave, four waves of columns over the same key tiles
+//   KV4_DIMS             16 columns, the four waves a quarter of the dims each over the same key tiles: their
+//                        parts of the scores are added through LDS, and nothing joins at the end.  (d = 512 as
+//                        KV4_ROWS has 128 registers of results a wave and q in LDS: one wave a SIMD, and
+//                        prompts of 121 rows take 322 us instead of 196.)
 //
 // Decode is bound by reading the keys once: d = 128, 4 columns, 128 rows of up to 16K tokens (1.18 GB) take
 // 194 us, 6.1 TB/s (the loads alone 186); 128 rows of d = 256 (295 MB) 53, 5.5 TB/s; 64 rows of eight
-// columns (306 MB) 70, with both groups' softmax to do; 8 columns of d = 512 (307 MB) 85, with q in LDS and
-// one wave a SIMD.  Few or short rows are bound by the chain of launch, list, q, keys and join: 5 rows of up
+// columns (306 MB) 70, with both groups' softmax to do; 8 columns of d = 512 (307 MB) 83, half of its products
+// on columns that are not there.  Few or short rows are bound by the chain of launch, list, q, keys and join: 5 rows of up
 // to 700 tokens take 7.5 us (an empty launch 2.2).  Prompts are bound by the matrix cores: 3 x 181 GFLOP
 // of products (d = 128, chunks of up to 700 behind up to 4000 tokens) take 510 us, 1.07 PFLOP/s (a library
 // product of 8192 cubed makes 1.22 here).  Few columns as rows of three parts do no score twice: 16-column
@@ -530,16 +533,18 @@ __device__ __forceinline__ float weight_of(float m, float l, float big) {
 template <int D, int MODE, int NG>
 __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_kernel(Kv4Attention a) {
   constexpr bool FEW = MODE == KV4_FEW || MODE == KV4_EIGHT, TILES = MODE == KV4_TILES;
+  constexpr bool DIMS = MODE == KV4_DIMS;
+  constexpr int DW = DIMS ? D / kWaves : D;  // dims of a wave
   constexpr int NP = FEW ? 1 : 3;
-  constexpr bool QLDS = D == 512 && !FEW;  // 192 registers of q's parts would leave none for the loads
-  constexpr int NC = D / 32;               // contraction steps of a score
+  constexpr int NC = DW / 32;  // contraction steps of a score
   constexpr int COLS = kv4_cols(D, MODE);
-  constexpr int E = D / 16;                // dims of a row of V
+  constexpr int E = DW / 16;   // the wave's dims of a row of V
   static_assert(COLS == (FEW ? 4 : TILES ? 64 : 16) * NG, "the columns of a tile");
   extern __shared__ float4 smem[];
   float *lds_o = reinterpret_cast<float *>(smem);  // [wave][col][D + 4]
   float *lds_m = lds_o + kWaves * COLS * (D + 4), *lds_l = lds_m + kWaves * COLS;
-  bf16x8 *lds_q = reinterpret_cast<bf16x8 *>(smem);  // (QLDS) [part][step][lane], before lds_o
+  f32x4 *lds_s = reinterpret_cast<f32x4 *>(smem);  // (DIMS) [turn][wave][group][half][lane]
+  int turn = 0;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, w = lane >> 4;
   // (FEW) the wave's P, [group][row 16][key 32] bf16, rows kPRow words apart (no bank conflicts in either
@@ -560,7 +565,7 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
   }
   const int rep = a.hq / a.kv.hkv;
   const int per_block = a.kv.block_size >> 5;
-  const TilePlaces places = tile_places<D>(lane);
+  const TilePlaces places = tile_places<D, DIMS>(lane, wave);
   int ct = __builtin_amdgcn_readfirstlane(find_tile(a.cum, a.room, n_tiles, u, a.kv.hkv, lane));
   while (u < u_end) {
     while (u >= uniform(a.cum + ct + 1) * a.kv.hkv) ct++;  // (u is below the last entry's)
@@ -597,25 +602,20 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
       return __builtin_amdgcn_make_buffer_rsrc(a.kv.pages + tile_at(a.kv, block, head, in_block, D),
                                                (short)0, 34 * D, kBufferWord3);
     };
-    auto load = [&](int t, int block, Tile<D> &into) {
+    auto load = [&](int t, int block, Tile<DW> &into) {
       const __amdgpu_buffer_rsrc_t from = buffer(t, block);
-      load_keys<D, !TILES>(from, places, into);
-      load_values<D, !TILES>(from, places, into);
+      load_keys<DW, D, !TILES>(from, places, into);
+      load_values<DW, !TILES>(from, places, into);
       // The loads go out before the products of the tile at hand (the compiler would have them wait for
       // that tile, whose registers it could then use again).
       __builtin_amdgcn_sched_barrier(0);
     };
-    constexpr int STRIDE = TILES ? 1 : kWaves;
-    int t = t0 + (TILES ? 0 : wave);
-    // With d = 512 the first tile is under way while q is loaded and split (with fewer dims there are more
-    // waves, and no registers to hold it: 5% slower).
-    Tile<D> one;
-    if (D == 512 && t < t1) load(t, block_of(t), one);
+    constexpr int STRIDE = TILES || DIMS ? 1 : kWaves;
+    int t = t0 + (TILES || DIMS ? 0 : wave);
     // The columns whose scores the lane has see keys [lo, hi).  (Columns past the last repeat it.)
     int hi[NG], lo[NG];
-    bf16x8 q[NG][QLDS ? 1 : NC][NP];
+    bf16x8 q[NG][NC][NP];
     int all_hi = INT32_MAX, all_lo = 0, any_hi = 0, any_lo = INT32_MAX;
-    if constexpr (QLDS) __syncthreads();  // the last segment's results have been read
 #pragma unroll
     for (int g = 0; g < NG; g++) {
       const int64_t scol = min(first_col + (FEW ? 4 * g + w : 16 * g + c), cols - 1);
@@ -629,14 +629,13 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
       const int64_t col = FEW ? min(first_col + 4 * g + (c >> 2), cols - 1) : scol;
       const int qrow = (int)(col / rep);
       const float *qp =
-          a.q + ((size_t)(row0 + qrow) * a.hq + (size_t)head * rep + (col - (int64_t)qrow * rep)) * D;
+          a.q + ((size_t)(row0 + qrow) * a.hq + (size_t)head * rep + (col - (int64_t)qrow * rep)) * D +
+          w * (D / 4) + (DIMS ? wave * 32 : 0);
 #pragma unroll
       for (int j = 0; j < NC; j++) {
-        if (QLDS && j % kWaves != wave) continue;
         float x[8];
-        *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(qp + w * (D / 4) + 8 * j);
-        *reinterpret_cast<float4 *>(x + 4) =
-            *reinterpret_cast<const float4 *>(qp + w * (D / 4) + 8 * j + 4);
+        *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(qp + 8 * j);
+        *reinterpret_cast<float4 *>(x + 4) = *reinterpret_cast<const float4 *>(qp + 8 * j + 4);
         // Scores come out in units of log2 (one rounding of q more).
 #pragma unroll
         for (int i = 0; i < 8; i++) x[i] *= a.scale2;
@@ -645,16 +644,12 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
         if constexpr (FEW) {
           const bf16x8 zero = {};
           q[g][j][0] = (c & 3) == 0 ? p[0] : (c & 3) == 1 ? p[1] : (c & 3) == 2 ? p[2] : zero;
-        } else if constexpr (QLDS) {
-#pragma unroll
-          for (int i = 0; i < 3; i++) lds_q[(i * NC + j) * 64 + lane] = p[i];
         } else {
 #pragma unroll
           for (int i = 0; i < 3; i++) q[g][j][i] = p[i];
         }
       }
     }
-    if constexpr (QLDS) __syncthreads();
     // Tiles that every column sees whole need no mask, those that none sees no work.
 #pragma unroll
     for (int d = FEW ? 16 : 1; d < (FEW ? 64 : 16); d <<= 1) {
@@ -685,26 +680,46 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
       for (int i = 0; i < E; i++) o[g][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     // Scores of the 32 keys, of either half of them.
-    auto scores = [&](const Tile<D> &cur, f32x4 (*s)[2]) {
+    auto scores = [&](const Tile<DW> &cur, f32x4 (*s)[2]) {
 #pragma unroll
       for (int g = 0; g < NG; g++) s[g][0] = s[g][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < NC; j++) {
-        const bf16x8 k0 = mx4_frag(cur.k[0][j], k_unit<D>(cur, j, 0));
-        const bf16x8 k1 = mx4_frag(cur.k[1][j], k_unit<D>(cur, j, 1));
+        const bf16x8 k0 = mx4_frag(cur.k[0][j], k_unit<DW>(cur, j, 0));
+        const bf16x8 k1 = mx4_frag(cur.k[1][j], k_unit<DW>(cur, j, 1));
 #pragma unroll
         for (int g = 0; g < NG; g++)
 #pragma unroll
           for (int i = 0; i < NP; i++) {
-            bf16x8 qv;
-            if constexpr (QLDS) qv = lds_q[(i * NC + j) * 64 + lane]; else qv = q[g][j][i];
+            const bf16x8 qv = q[g][j][i];
             s[g][0] = FEW ? mfma(qv, k0, s[g][0]) : mfma(k0, qv, s[g][0]);
             s[g][1] = FEW ? mfma(qv, k1, s[g][1]) : mfma(k1, qv, s[g][1]);
           }
       }
+      if constexpr (DIMS) {
+        // The sum of the waves' parts, the same bits in each.  (The other half of the buffer was read before
+        // the last barrier; loads in flight stay so.)
+        f32x4 *buf = lds_s + (turn & 1) * (kWaves * NG * 2 * 64);
+        turn++;
+#pragma unroll
+        for (int g = 0; g < NG; g++)
+#pragma unroll
+          for (int h = 0; h < 2; h++) buf[((wave * NG + g) * 2 + h) * 64 + lane] = s[g][h];
+        wait_lds_reads();
+        lds_barrier();
+#pragma unroll
+        for (int g = 0; g < NG; g++)
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            f32x4 sum = buf[(g * 2 + h) * 64 + lane];
+#pragma unroll
+            for (int v = 1; v < kWaves; v++) sum += buf[((v * NG + g) * 2 + h) * 64 + lane];
+            s[g][h] = sum;
+          }
+      }
     };
     // Their probabilities, and the values of their V.
-    auto values = [&](int t, Tile<D> &cur, f32x4 (*s)[2]) {
+    auto values = [&](int t, Tile<DW> &cur, f32x4 (*s)[2]) {
       const int key0 = (tile.kb + t) * 32;
       const bool edge = key0 + 32 > all_hi || key0 < all_lo;
       constexpr int NX = FEW ? 2 : 8;  // scores of a lane and column: keys NX (lane's) .. + NX - 1
@@ -804,42 +819,43 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
           }
         }
       }
-      add_values<D, NG, NP, FEW>(cur, unit, p, o);
+      add_values<DW, NG, NP, FEW>(cur, unit, p, o);
     };
-    auto attend = [&](int t, Tile<D> &cur) {
+    auto attend = [&](int t, Tile<DW> &cur) {
       f32x4 s[NG][2];
       scores(cur, s);
       values(t, cur, s);
     };
-    if constexpr (TILES || D == 512) {
+    if constexpr (TILES) {
       // One tile's registers: the next keys are loaded behind the scores, the next values behind the sums.
       // (The last turns load the last tile again: loads behind a condition would be waited for as if they
       // were needed at once.)
+      Tile<DW> one;
       if (t < te) {
-        if (TILES) load(t, block_of(t), one);
+        load(t, block_of(t), one);
         int next = min(t + STRIDE, te - 1), block = block_of(next);
         for (; t < te; t += STRIDE) {
           f32x4 s[NG][2];
           scores(one, s);
           const __amdgpu_buffer_rsrc_t from = buffer(next, block);
           __builtin_amdgcn_sched_barrier(0);
-          load_keys<D, !TILES>(from, places, one);
+          load_keys<DW, D, !TILES>(from, places, one);
           next = min(t + 2 * STRIDE, te - 1);
           block = block_of(next);
           __builtin_amdgcn_sched_barrier(0);
           values(t, one, s);
           __builtin_amdgcn_sched_barrier(0);
-          load_values<D, !TILES>(from, places, one);
+          load_values<DW, !TILES>(from, places, one);
         }
       }
     } else {
       // The next tile loads into the other registers while this one is attended.  (The last turn loads the
       // last tile again: loads behind a condition would be waited for as if they were needed at once.)  Two
       // and three tiles ahead were 2 to 20% slower for the registers that they take.
-      Tile<D> even, odd;
+      Tile<DW> even, odd;
       if (t < te) {
         int next = t, block = block_of(t);
-        auto ahead = [&](Tile<D> &into) {
+        auto ahead = [&](Tile<DW> &into) {
           load(next, block, into);
           next = min(next + STRIDE, te - 1);
           block = block_of(next);
@@ -876,13 +892,13 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
       }
     }
 
-    if constexpr (TILES) {  // every wave writes its own columns
+    if constexpr (TILES || DIMS) {  // every wave writes its own columns, or its own dims
 #pragma unroll
       for (int g = 0; g < NG; g++) {
         const int64_t col = first_col + 16 * g + c;
         if (col >= cols) continue;
         const int row = (int)(col / rep);
-        const size_t part = (size_t)part0 + wave * (16 * NG) + 16 * g + c;
+        const size_t part = (size_t)part0 + (TILES ? wave * (16 * NG) : 0) + 16 * g + c;
         const float inv = whole ? (l[g] == 0.f ? 0.f : 1.f / l[g]) : 1.f;
         float *dst = whole ? a.out + ((size_t)(row0 + row) * a.hq + (size_t)head * rep +
                                       (col - (int64_t)row * rep)) * D
@@ -891,10 +907,10 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
         for (int r = 0; r < 4; r++)
 #pragma unroll
           for (int i = 0; i < E; i += 4)
-            *reinterpret_cast<float4 *>(dst + (4 * w + r) * E + i) =
+            *reinterpret_cast<float4 *>(dst + (4 * w + r) * (D / 16) + (DIMS ? wave * E : 0) + i) =
                 make_float4(o[g][i][r] * inv, o[g][i + 1][r] * inv, o[g][i + 2][r] * inv,
                             o[g][i + 3][r] * inv);
-        if (!whole && w == 0) {
+        if (!whole && w == 0 && (TILES || wave == 0)) {
           a.part_m[part] = m[g];
           a.part_l[part] = l[g];
         }
@@ -903,7 +919,6 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
     }
 
     // Join the waves: sums and rows over the highest reference.
-    if constexpr (QLDS) __syncthreads();  // q's parts have been read
 #pragma unroll
     for (int g = 0; g < NG; g++) {
       const int at = wave * COLS + (FEW ? 4 * g + w : c);
@@ -959,7 +974,7 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
         a.part_l[part] = sum;
       }
     }
-    if constexpr (!QLDS) __syncthreads();  // lds_o is written again
+    __syncthreads();  // lds_o is written again
   }
   if (threadIdx.x == 0) a.borders[blockIdx.x] = border;
 }
@@ -1136,12 +1151,13 @@ template <int D, int MODE> size_t attention_lds() {
   if (MODE == KV4_TILES) return 0;
   constexpr int cols = kv4_cols(D, MODE);
   const size_t join = (size_t)kWaves * cols * (D + 4 + 2) * 4;
-  if (MODE == KV4_ROWS) return D == 512 ? std::max<size_t>(join, (size_t)3 * (D / 32) * 64 * 16) : join;
+  if (MODE == KV4_ROWS) return join;
+  if (MODE == KV4_DIMS) return (size_t)2 * kWaves * (cols / 16) * 2 * 64 * 16;
   return join + (size_t)kWaves * (cols / 4) * 16 * kPRow * 4;
 }
 
 template <int D, int MODE> constexpr int groups() {
-  return kv4_cols(D, MODE) / (MODE == KV4_TILES ? 64 : MODE == KV4_ROWS ? 16 : 4);
+  return kv4_cols(D, MODE) / (MODE == KV4_TILES ? 64 : MODE == KV4_ROWS || MODE == KV4_DIMS ? 16 : 4);
 }
 
 template <int D> hipError_t store(const Kv4Store &a, hipStream_t s) {
@@ -1175,15 +1191,15 @@ template <int D, int MODE> hipError_t attention(const Kv4Attention &a, int workg
 }
 
 template <int D> hipError_t attention_of(const Kv4Attention &a, int mode, int workgroups, hipStream_t s) {
-  switch (mode) {
-    case KV4_FEW: return attention<D, KV4_FEW>(a, workgroups, s);
-    case KV4_EIGHT:
-      if constexpr (kv4_has_tiles(D)) return attention<D, KV4_EIGHT>(a, workgroups, s);
-      return hipErrorInvalidValue;
-    case KV4_ROWS: return attention<D, KV4_ROWS>(a, workgroups, s);
-    default:
-      if constexpr (kv4_has_tiles(D)) return attention<D, KV4_TILES>(a, workgroups, s);
-      return hipErrorInvalidValue;
+  if constexpr (kv4_by_dims(D)) {
+    return attention<D, KV4_DIMS>(a, workgroups, s);
+  } else {
+    switch (mode) {
+      case KV4_FEW: return attention<D, KV4_FEW>(a, workgroups, s);
+      case KV4_EIGHT: return attention<D, KV4_EIGHT>(a, workgroups, s);
+      case KV4_ROWS: return attention<D, KV4_ROWS>(a, workgroups, s);
+      default: return attention<D, KV4_TILES>(a, workgroups, s);
+    }
   }
 }
 
@@ -1198,15 +1214,15 @@ template <int D, int MODE> int resident() {
 }
 
 template <int D> int resident_of(int mode) {
-  switch (mode) {
-    case KV4_FEW: return resident<D, KV4_FEW>();
-    case KV4_EIGHT:
-      if constexpr (kv4_has_tiles(D)) return resident<D, KV4_EIGHT>();
-      return 1;
-    case KV4_ROWS: return resident<D, KV4_ROWS>();
-    default:
-      if constexpr (kv4_has_tiles(D)) return resident<D, KV4_TILES>();
-      return 1;
+  if constexpr (kv4_by_dims(D)) {
+    return resident<D, KV4_DIMS>();
+  } else {
+    switch (mode) {
+      case KV4_FEW: return resident<D, KV4_FEW>();
+      case KV4_EIGHT: return resident<D, KV4_EIGHT>();
+      case KV4_ROWS: return resident<D, KV4_ROWS>();
+      default: return resident<D, KV4_TILES>();
+    }
   }
 }
 

@@ -210,18 +210,22 @@ struct Kv4View {
   int32_t num_blocks, block_size, hkv;
 };
 // The attention kernels (kv4.hip) by the columns, query rows times heads of a KV head, of their column
-// tiles: a step's sequences of few columns run on one of the first three, the others on the last.  d = 512
-// has the first and third alone (its registers).
-enum { KV4_FEW = 0, KV4_EIGHT = 1, KV4_ROWS = 2, KV4_TILES = 3 };
-constexpr bool kv4_has_tiles(int head_dim) { return head_dim <= 256; }
+// tiles: a step's sequences of few columns run on one of the first three, the others on the fourth.  d = 512
+// has the last alone, whose waves share the dims.
+enum { KV4_FEW = 0, KV4_EIGHT = 1, KV4_ROWS = 2, KV4_TILES = 3, KV4_DIMS = 4 };
+constexpr bool kv4_by_dims(int head_dim) { return head_dim > 256; }
 constexpr int kv4_cols(int head_dim, int mode) {
-  return mode == KV4_FEW ? 4 : mode == KV4_EIGHT ? 8 : mode == KV4_ROWS ? 16 : head_dim <= 128 ? 128 : 64;
+  return mode == KV4_FEW     ? 4
+         : mode == KV4_EIGHT ? 8
+         : mode == KV4_TILES ? (head_dim <= 128 ? 128 : 64)
+                             : 16;
 }
 // Waves a SIMD that the registers are held down to.
 constexpr int kv4_min_waves(int head_dim, int mode) {
-  return mode == KV4_FEW     ? (head_dim <= 128 ? 3 : head_dim <= 256 ? 2 : 1)
+  return mode == KV4_FEW     ? (head_dim <= 128 ? 3 : 2)
          : mode == KV4_EIGHT ? (head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1)
          : mode == KV4_ROWS  ? (head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1)
+         : mode == KV4_DIMS  ? 2
                              : (head_dim <= 64 ? 3 : 2);
 }
 struct Kv4Tile {
