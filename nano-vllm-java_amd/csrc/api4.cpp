@@ -331,7 +331,7 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
     l.unit = r.mode == KV4_TILES || r.mode == KV4_DIMS ? 1 : 4;
     l.min_units = 4;
     l.slack = r.mode == KV4_TILES ? 0 : 12;
-    l.over = r.mode == KV4_TILES ? 2 : 20;
+    l.over = r.mode == KV4_TILES ? 4 : r.mode == KV4_DIMS ? 6 : 20;
   }
   {
     Timed tm(ctx, "store4");

@@ -103,7 +103,8 @@ __device__ __forceinline__ void store_row(const Kv4View &kv, const float *src, i
 // head, d = 256, the attention takes 17.5 us instead of 22.7, with 5 rows of up to 700 keys 7.5 instead of
 // 12.2, with three of 60 to 120 thousand 33.4 instead of 35.6, and the list 1.2 more.  Elsewhere a segment
 // counts a.over units more, so that a workgroup of many short ones gets fewer keys (20 more: 128 rows of up
-// to 16K keys, four columns of d = 128, 208 -> 194 us, 64 of up to 8K, eight columns, 99 -> 67).
+// to 16K keys, four columns of d = 128, 208 -> 194 us, 64 of up to 8K, eight columns, 99 -> 67; 4 for tiles,
+// where a unit is more work: 91 prompts of 147 rows of 40 heads 281 -> 260).
 constexpr int kListThreads = 256, kListRounds = 4, kListNear = 1025;
 
 __device__ void build_list(const Kv4List &a) {

@@ -595,10 +595,11 @@ class Attention:
                                 self.sliding_window, kv_layer_index, int(self.write_kv))
 
     def _check_shapes(self, q, k, v) -> None:
-        if q.dim() != 3 or q.shape[1:] != (self.num_heads, self.head_dim):
+        shape = q.shape
+        if len(shape) != 3 or shape[1] != self.num_heads or shape[2] != self.head_dim:
             raise IllegalArgumentException(
-                f"q must be [tokens, {self.num_heads}, {self.head_dim}], got {tuple(q.shape)}")
-        want = (q.shape[0], self.num_kv_heads, self.head_dim)
+                f"q must be [tokens, {self.num_heads}, {self.head_dim}], got {tuple(shape)}")
+        want = (shape[0], self.num_kv_heads, self.head_dim)
         for name, t in (("k", k), ("v", v)):
             if t is not None and t.shape != want:
                 raise IllegalArgumentException(
@@ -1012,7 +1013,7 @@ class Linear4:
         if x.dim() == 0 or x.shape[-1] != self.in_features:
             raise IllegalArgumentException("x last dim mismatch")
         xp = _on(x, "x", ctx.device)
-        y = torch.empty(x.shape[:-1] + (self.out_features,), dtype=torch.float32, device=x.device)
+        y = x.new_empty(x.shape[:-1] + (self.out_features,))
         _check(ctx.handle, N.load().nva_linear4_forward(
             ctx.handle, self._h, xp, x.numel() // self.in_features, _on(self.bias, "bias", ctx.device),
             y.data_ptr()), "Linear4.forward")
