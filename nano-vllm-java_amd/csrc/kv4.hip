@@ -572,7 +572,8 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
     while (u >= uniform(a.cum + ct + 1) * a.kv.hkv) ct++;  // (u is below the last entry's)
     const Kv4Tile tile = uniform_tile(a.tiles + ct);
     const int64_t in = u - uniform(a.cum + ct) * a.kv.hkv;
-    const int head = (int)(in / tile.units);
+    // (64-bit divisions cost hundreds of instructions: columns are below 2^30, chunks as good as never larger.)
+    const int head = in <= UINT32_MAX ? (int)((uint32_t)in / (uint32_t)tile.units) : (int)(in / tile.units);
     // Units [v0, v1) of the KV head's, of which the first `over` are no keys.
     const int v0 = (int)(in - (int64_t)head * tile.units);
     const int v1 = (int)min((int64_t)tile.units, v0 + (u_end - u));
@@ -581,14 +582,14 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
     if (t1 <= t0) continue;
     const int seq = tile.seq;
     const int row0 = tile.row0, qlen = tile.qlen, klen = tile.klen;
-    const int64_t cols = (int64_t)qlen * rep;
-    const int64_t first_col = (int64_t)tile.col0 + (TILES ? wave * (16 * NG) : 0);
+    const int cols = qlen * rep;
+    const int first_col = tile.col0 + (TILES ? wave * (16 * NG) : 0);
     const bool whole = t0 == 0 && t1 == tile.n;
     const int64_t part0 = (int64_t)(2 * blockIdx.x + (t0 == 0 ? 1 : 0)) * COLS;
     if (t0 > 0 && t0 <= chunk) {  // (its workgroup's first segment) the workgroup before began it
       border = Kv4Border{(int32_t)(blockIdx.x - 1),
-                         (int32_t)(blockIdx.x + ((int64_t)tile.n - t0 - 1) / chunk), row0, head * rep,
-                         tile.col0, (int32_t)min((int64_t)COLS, cols - tile.col0)};
+                         (int32_t)blockIdx.x + (chunk < tile.n ? (tile.n - t0 - 1) / (int)chunk : 0), row0,
+                         head * rep, tile.col0, min(COLS, cols - tile.col0)};
     }
     if (TILES && first_col >= cols) continue;  // (a wave by itself: these waves meet at no barrier)
     const int32_t *table = a.table + (size_t)seq * a.bt_stride;
@@ -614,42 +615,15 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
     constexpr int STRIDE = TILES || DIMS ? 1 : kWaves;
     int t = t0 + (TILES || DIMS ? 0 : wave);
     // The columns whose scores the lane has see keys [lo, hi).  (Columns past the last repeat it.)
-    int hi[NG], lo[NG];
-    bf16x8 q[NG][NC][NP];
-    int all_hi = INT32_MAX, all_lo = 0, any_hi = 0, any_lo = INT32_MAX;
+    int hi[NG], lo[NG], all_hi = INT32_MAX, all_lo = 0, any_hi = 0, any_lo = INT32_MAX;
 #pragma unroll
     for (int g = 0; g < NG; g++) {
-      const int64_t scol = min(first_col + (FEW ? 4 * g + w : 16 * g + c), cols - 1);
-      hi[g] = klen - qlen + (int)(scol / rep) + 1;
+      hi[g] = klen - qlen + min(first_col + (FEW ? 4 * g + w : 16 * g + c), cols - 1) / rep + 1;
       lo[g] = a.window > 0 ? max(0, hi[g] - a.window) : 0;
       all_hi = min(all_hi, hi[g]);
       any_hi = max(any_hi, hi[g]);
       all_lo = max(all_lo, lo[g]);
       any_lo = min(any_lo, lo[g]);
-      // The column of q that the lane loads.
-      const int64_t col = FEW ? min(first_col + 4 * g + (c >> 2), cols - 1) : scol;
-      const int qrow = (int)(col / rep);
-      const float *qp =
-          a.q + ((size_t)(row0 + qrow) * a.hq + (size_t)head * rep + (col - (int64_t)qrow * rep)) * D +
-          w * (D / 4) + (DIMS ? wave * 32 : 0);
-#pragma unroll
-      for (int j = 0; j < NC; j++) {
-        float x[8];
-        *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(qp + 8 * j);
-        *reinterpret_cast<float4 *>(x + 4) = *reinterpret_cast<const float4 *>(qp + 8 * j + 4);
-        // Scores come out in units of log2 (one rounding of q more).
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] *= a.scale2;
-        bf16x8 p[3];
-        split3<false>(x, p);
-        if constexpr (FEW) {
-          const bf16x8 zero = {};
-          q[g][j][0] = (c & 3) == 0 ? p[0] : (c & 3) == 1 ? p[1] : (c & 3) == 2 ? p[2] : zero;
-        } else {
-#pragma unroll
-          for (int i = 0; i < 3; i++) q[g][j][i] = p[i];
-        }
-      }
     }
     // Tiles that every column sees whole need no mask, those that none sees no work.
 #pragma unroll
@@ -668,6 +642,37 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
       any_lo = __builtin_amdgcn_readfirstlane(any_lo);
       t = max(t, (any_lo >> 5) - tile.kb);
       te = min(te, (max(any_hi, 0) + 31) / 32 - tile.kb);
+    }
+    // (TILES) the first tile is on its way while q is loaded and split.  (Where the registers that hold it are
+    // not there anyway, in the kernels of few columns, it cost 5%.)
+    Tile<DW> one;
+    if (TILES && t < te) load(t, block_of(t), one);
+    bf16x8 q[NG][NC][NP];
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+      // The column of q that the lane loads.
+      const int col = min(first_col + (FEW ? 4 * g + (c >> 2) : 16 * g + c), cols - 1);
+      const int qrow = col / rep;
+      const float *qp = a.q + ((size_t)(row0 + qrow) * a.hq + head * rep + (col - qrow * rep)) * D +
+                        w * (D / 4) + (DIMS ? wave * 32 : 0);
+#pragma unroll
+      for (int j = 0; j < NC; j++) {
+        float x[8];
+        *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(qp + 8 * j);
+        *reinterpret_cast<float4 *>(x + 4) = *reinterpret_cast<const float4 *>(qp + 8 * j + 4);
+        // Scores come out in units of log2 (one rounding of q more).
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] *= a.scale2;
+        bf16x8 p[3];
+        split3<false>(x, p);
+        if constexpr (FEW) {
+          const bf16x8 zero = {};
+          q[g][j][0] = (c & 3) == 0 ? p[0] : (c & 3) == 1 ? p[1] : (c & 3) == 2 ? p[2] : zero;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 3; i++) q[g][j][i] = p[i];
+        }
+      }
     }
     f32x4 o[NG][E];
     float m[NG], l[NG];
@@ -831,9 +836,7 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
       // One tile's registers: the next keys are loaded behind the scores, the next values behind the sums.
       // (The last turns load the last tile again: loads behind a condition would be waited for as if they
       // were needed at once.)
-      Tile<DW> one;
       if (t < te) {
-        load(t, block_of(t), one);
         int next = min(t + STRIDE, te - 1), block = block_of(next);
         for (; t < te; t += STRIDE) {
           f32x4 s[NG][2];
@@ -896,13 +899,12 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
     if constexpr (TILES || DIMS) {  // every wave writes its own columns, or its own dims
 #pragma unroll
       for (int g = 0; g < NG; g++) {
-        const int64_t col = first_col + 16 * g + c;
+        const int col = first_col + 16 * g + c;
         if (col >= cols) continue;
-        const int row = (int)(col / rep);
+        const int row = col / rep;
         const size_t part = (size_t)part0 + (TILES ? wave * (16 * NG) : 0) + 16 * g + c;
         const float inv = whole ? (l[g] == 0.f ? 0.f : 1.f / l[g]) : 1.f;
-        float *dst = whole ? a.out + ((size_t)(row0 + row) * a.hq + (size_t)head * rep +
-                                      (col - (int64_t)row * rep)) * D
+        float *dst = whole ? a.out + ((size_t)(row0 + row) * a.hq + head * rep + (col - row * rep)) * D
                            : a.part_o + part * D;
 #pragma unroll
         for (int r = 0; r < 4; r++)
@@ -950,13 +952,12 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
       ms[i] = weight_of(ms[i], li, big);
       sum += ms[i] * li;
     }
-    const int64_t ocol = (int64_t)tile.col0 + oc;
+    const int ocol = tile.col0 + oc;
     if (ocol < cols) {
-      const int orow = (int)(ocol / rep);
+      const int orow = ocol / rep;
       const float inv = whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
       const size_t part = (size_t)part0 + oc;
-      float *dst = whole ? a.out + ((size_t)(row0 + orow) * a.hq + (size_t)head * rep +
-                                    (ocol - (int64_t)orow * rep)) * D
+      float *dst = whole ? a.out + ((size_t)(row0 + orow) * a.hq + head * rep + (ocol - orow * rep)) * D
                          : a.part_o + part * D;
 #pragma unroll
       for (int i = 0; i < (D + 4 * LANES - 1) / (4 * LANES); i++) {
