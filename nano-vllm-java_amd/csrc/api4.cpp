@@ -791,14 +791,18 @@ nva_status nva_linear4_forward(nva_ctx *ctx, const nva_linear4 *l, const float *
   if (!x || !y) return fail(ctx, NVA_E_ARG, "x and y are required");
   if (!aligned16(x)) return fail(ctx, NVA_E_ARG, "x must be a 16-byte aligned device pointer");
   Linear4Launch a{};
-  a.x = x;
   a.weight = l->weight;
   a.bias = bias;
-  a.y = y;
-  a.rows = rows;
   a.in = l->in;
   a.out = l->out;
-  const size_t work = linear4_work_bytes(a, ctx->num_cus);
+  // Rows at a time: the parts of x, half as large again as x, stay within bounds.
+  constexpr int kRows = 16384;
+  a.rows = std::min(rows, kRows);
+  // (The last rows may be few, whose work area is another.)
+  Linear4Launch rest = a;
+  rest.rows = rows % kRows;
+  size_t work = linear4_work_bytes(a, ctx->num_cus);
+  if (rest.rows) work = std::max(work, linear4_work_bytes(rest, ctx->num_cus));
   if (work) {
     nva_status st = reserve_for(ctx, ctx->d_lin4, work, stream_capturing(ctx->stream),
                                 "4-bit linear work area");
@@ -806,7 +810,12 @@ nva_status nva_linear4_forward(nva_ctx *ctx, const nva_linear4 *l, const float *
     a.work = ctx->d_lin4.ptr;
   }
   Timed tm(ctx, "linear4");
-  HIP_TRY(ctx, launch_linear4(a, ctx->num_cus, ctx->stream), "4-bit linear kernel launch");
+  for (int r = 0; r < rows; r += a.rows) {
+    a.rows = std::min(rows - r, kRows);
+    a.x = x + (size_t)r * l->in;
+    a.y = y + (size_t)r * l->out;
+    HIP_TRY(ctx, launch_linear4(a, ctx->num_cus, ctx->stream), "4-bit linear kernel launch");
+  }
   tm.done();
   return NVA_OK;
 } catch (const std::exception &) {
