@@ -140,6 +140,12 @@ int ctx_kv4_workgroups_per_cu(nva_ctx *ctx, int head_dim, int mode) {
 }
 
 constexpr int64_t kJoinUnits = 3500;
+// The key tiles up to which the rows of a decode step are not split where there are workgroups for all, so
+// that nothing is to be merged (which takes 4 to 5 us, and a launch of the host's 4): 5 rows of 32 / 8 heads of
+// 128 take 8.8 us with 40 tiles split and 12.1 whole, 11.4 and 15.6 with 64; 5 rows of 4 / 1 heads of 256 8.6
+// and 13.4 with 32 (96 rows with 33, 14.6 and 16); 5 rows of 8 / 1 heads of 512, where four waves share a tile,
+// 10.4 and 14.4 with 8.
+constexpr int whole_tiles(int head_dim) { return head_dim <= 128 ? 48 : head_dim <= 256 ? 36 : 8; }
 
 // Growing a buffer of a call that may be captured.
 nva_status reserve_for(nva_ctx *ctx, DevBuf &buf, size_t bytes, bool capturing, const char *what) {
@@ -222,6 +228,7 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
   // knows of their rows bounds them: the lengths themselves, or the most tokens that follow.
   const int seqs = dev ? ctx->dev_seqs : ctx->is_prefill ? ctx->num_seqs : num_tokens;
   int64_t few = 0, many = 0;  // most columns of a sequence on either list
+  int whole = 0;              // decode rows that are all this short take one workgroup a KV head
   int64_t limit = kv4_by_dims(d.head_dim) ? INT32_MAX : 16;
   auto count = [&](int64_t cols) {
     if (cols <= limit) few = std::max(few, cols); else many = std::max(many, cols);
@@ -246,6 +253,14 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
     }
   } else {
     count(rep);
+    int most = 0, least = INT32_MAX;
+    for (int b = 0; b < seqs; b++) {
+      most = std::max(most, ctx->ctx_lens[b]);
+      least = std::min(least, ctx->ctx_lens[b]);
+    }
+    if (d.sliding_window > 0) most = std::min(most, d.sliding_window + 31);
+    const int tiles = (int)(((int64_t)most + 31) / 32);
+    if (least > 0 && !many && tiles <= whole_tiles(d.head_dim)) whole = tiles;
   }
   struct Run {
     int mode, workgroups, tiles;
@@ -274,6 +289,11 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
   // (One list at least: it knows the rows that no sequence covers.)
   if (few || !many)
     add(kv4_by_dims(d.head_dim) ? KV4_DIMS : few <= 4 ? KV4_FEW : few <= 8 ? KV4_EIGHT : KV4_ROWS);
+  if (whole) {  // a workgroup for every column tile and KV head, by a list that gives them one each
+    const int cols = kv4_cols(d.head_dim, runs[0].mode);
+    const int64_t tiles = (int64_t)seqs * ((rep + cols - 1) / cols);
+    if (tiles > kKv4ListTiles || tiles * d.num_kv_heads > runs[0].workgroups) whole = 0;
+  }
   nva_status st = reserve_for(ctx, ctx->d_plan4, plan_bytes, capturing, "attention work list");
   if (st != NVA_OK) return st;
   st = reserve_for(ctx, ctx->d_part4, part_floats * 4, capturing, "attention partials");
@@ -329,7 +349,7 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
     l.max_cols = r.mode == KV4_TILES ? INT32_MAX : (int)limit;
     l.one_each = n_runs == 1 && std::max(few, many) <= l.cols;
     l.unit = r.mode == KV4_TILES || r.mode == KV4_DIMS ? 1 : 4;
-    l.min_units = 4;
+    l.min_units = std::max(4, (whole + 3) / 4 * 4);
     l.slack = r.mode == KV4_TILES ? 0 : 12;
     l.over = r.mode == KV4_TILES ? 4 : r.mode == KV4_DIMS ? 6 : 20;
   }
@@ -354,6 +374,7 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
     HIP_TRY(ctx, launch_kv4_attention(a, r.mode, r.workgroups, ctx->stream),
             "4-bit attention kernel launch");
     tm.done();
+    if (whole) continue;  // every row has keys and one segment: nothing to join, none to zero
     Timed tg(ctx, "merge4");
     const int64_t items = (int64_t)std::min(seqs, num_tokens) * d.num_kv_heads;
     HIP_TRY(ctx, launch_kv4_merge(a, r.mode, r.workgroups, (int)std::min<int64_t>(items, INT32_MAX),

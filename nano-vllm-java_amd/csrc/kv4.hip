@@ -106,6 +106,7 @@ __device__ __forceinline__ void store_row(const Kv4View &kv, const float *src, i
 // to 16K keys, four columns of d = 128, 208 -> 194 us, 64 of up to 8K, eight columns, 99 -> 67; 4 for tiles,
 // where a unit is more work: 91 prompts of 147 rows of 40 heads 281 -> 260).
 constexpr int kListThreads = 256, kListRounds = 4, kListNear = 1025;
+static_assert(kListRounds * kListThreads == kKv4ListTiles);
 
 __device__ void build_list(const Kv4List &a) {
   __shared__ int64_t part[4];
@@ -527,7 +528,7 @@ __device__ __forceinline__ float weight_of(float m, float l, float big) {
 // 194 us, 6.1 TB/s (the loads alone 186); 128 rows of d = 256 (295 MB) 53, 5.5 TB/s; 64 rows of eight
 // columns (306 MB) 70, with both groups' softmax to do; 8 columns of d = 512 (307 MB) 83, half of its products
 // on columns that are not there.  Few or short rows are bound by the chain of launch, list, q, keys and join: 5 rows of up
-// to 700 tokens take 7.5 us (an empty launch 2.2).  Prompts are bound by the matrix cores: 3 x 181 GFLOP
+// to 700 tokens take 9.3 us whole and 7.5 split (an empty launch 2.2).  Prompts are bound by the matrix cores: 3 x 181 GFLOP
 // of products (d = 128, chunks of up to 700 behind up to 4000 tokens) take 510 us, 1.07 PFLOP/s (a library
 // product of 8192 cubed makes 1.22 here).  Few columns as rows of three parts do no score twice: 16-column
 // products for 4 columns were compute-bound at 242 us for the 128 rows.

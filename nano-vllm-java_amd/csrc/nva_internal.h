@@ -243,6 +243,8 @@ struct Kv4Head {
   int32_t first, covered;  // rows of the sequences: [first, covered)
   int32_t over;            // units that stand for the beginning of a segment
 };
+// The column tiles up to which a list gives every workgroup one segment where it can.
+constexpr int kKv4ListTiles = 1024;
 // Where the work list goes and what it is made of: row offsets (null: one row a sequence) and the
 // lengths, or the offsets whose differences they are.
 struct Kv4List {

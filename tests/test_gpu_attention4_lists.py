@@ -67,3 +67,36 @@ def test_division_does_not_change_results(ctx):
     got, one = case.run(ctx), alone.run(ctx)
     close(got[:1], one.double().cpu().numpy())
     assert torch.equal(case.run(ctx), got) and torch.equal(alone.run(ctx), one)
+
+
+@pytest.mark.parametrize("d,limit", [(64, 48), (128, 48), (256, 36), (512, 8)])
+@pytest.mark.parametrize("hq,hkv", [(4, 1), (8, 8), (12, 2), (16, 1), (17, 1), (40, 2)])
+def test_short_decode_rows_whole_and_split(ctx, d, limit, hq, hkv):
+    """Rows up to the length that is not split, one key longer, and as short in a window."""
+    for seqs, tiles, extra, window in ((3, limit, 0, 0), (3, limit, 1, 0), (150, 2, 0, 0), (2, 70, 0, 200),
+                                       (1, 1, -31, 0)):
+        n = 32 * tiles + extra
+        lens = [n, max(1, n - 33), max(1, n // 2)] * (seqs // 3 + 1)
+        case = Case([(m - 1, 1) for m in lens[:seqs]], hq, hkv, d, block=64, window=window, seed=tiles + hq)
+        close(case.run(ctx), case.want(), f"{seqs} rows of {n}, window {window}")
+
+
+def test_short_decode_rows_among_empty_and_padded_ones(ctx):
+    """What a row of no keys is, and rows of the step that a call leaves out."""
+    case = Case([(40, 1), (5, 1), (90, 1)], 4, 2, 64, block=32, seed=2)
+    with case.arena(ctx) as a:
+        step = case.step()
+        step["context_lens"] = [41, 0, 91]
+        ctx.set(**step)
+        ctx.bind_kv_cache(a)
+        q, k, v = dev(case.q), dev(case.k_new), dev(case.v_new)
+        out = case.layer().forward(q, k, v, ctx)
+        want = case.want()
+        assert not out[1].any()
+        close(out[[0, 2]], want[[0, 2]])
+        step["context_lens"] = [41, 6, 91]
+        step["slot_mapping"] = step["slot_mapping"][:2]
+        ctx.set(**step)
+        ctx.bind_kv_cache(a)
+        close(case.layer().forward(q[:2], k[:2], v[:2], ctx), want[:2])
+        ctx.clear()
