@@ -337,9 +337,10 @@ nva_status nva_step_positions(nva_ctx *ctx, const float *positions, int num_toke
  * and does not wait; it may be captured, and replays act on the lengths they find.
  *
  * A step that asks for more than there is changes nothing and has no tokens: every row is padding.
- * nva_tables_status (which waits, and so is not for capture) tells: status[0] is 0, or 1 for a row (status[1]) whose keep or
- * new_tokens is out of range, 2 for more than num_tokens new tokens (status[1] of them, at most INT32_MAX), 3 for more
- * blocks (status[1]) than are free; status[2] is the number of free blocks after the call.
+ * nva_tables_status (which waits, and so is not for capture) tells: status[0] is 0, or 1 for a row
+ * (status[1]) whose keep or new_tokens is out of range, 2 for more than num_tokens new tokens (status[1] of
+ * them, at most INT32_MAX), 3 for more blocks (status[1]) than are free; status[2] is the number of free
+ * blocks after the call.
  *
  * The step serves nva_rope_forward and the calls over the 4-bit cache; the other attention calls need
  * nva_step_set (NVA_E_NO_STEP).  Its tables must outlive its use, captured graphs included. */
@@ -490,8 +491,8 @@ nva_status nva_qkv_norm_rope_attention_forward(nva_ctx *ctx, nva_kv *kv, const n
  * scale byte 255 and is NaN as a whole.  (The e2m1 elements and e8m0 scales of the OCP microscaling
  * formats, which the matrix cores' converters read.)  Reading uses any scale byte.
  *
- * nva_quantize4: x [rows, n] (device, n % 32 == 0, 16-byte aligned) to codes [rows, n / 2] (value 2j in the low bits of
- * byte j) and scales [rows, n / 32]. */
+ * nva_quantize4: x [rows, n] (device, n % 32 == 0, 16-byte aligned) to codes [rows, n / 2] (value 2j in the
+ * low bits of byte j, 4-byte aligned) and scales [rows, n / 32]. */
 nva_status nva_quantize4(nva_ctx *ctx, const float *x, int64_t rows, int n, uint8_t *codes,
                          uint8_t *scales);
 

@@ -526,12 +526,13 @@ __device__ __forceinline__ float weight_of(float m, float l, float big) {
 //
 // Decode is bound by reading the keys once: d = 128, 4 columns, 128 rows of up to 16K tokens (1.18 GB) take
 // 194 us, 6.1 TB/s (the loads alone 186); 128 rows of d = 256 (295 MB) 53, 5.5 TB/s; 64 rows of eight
-// columns (306 MB) 70, with both groups' softmax to do; 8 columns of d = 512 (307 MB) 83, half of its products
-// on columns that are not there.  Few or short rows are bound by the chain of launch, list, q, keys and join: 5 rows of up
-// to 700 tokens take 9.3 us whole and 7.5 split (an empty launch 2.2).  Prompts are bound by the matrix cores: 3 x 181 GFLOP
-// of products (d = 128, chunks of up to 700 behind up to 4000 tokens) take 510 us, 1.07 PFLOP/s (a library
-// product of 8192 cubed makes 1.22 here).  Few columns as rows of three parts do no score twice: 16-column
-// products for 4 columns were compute-bound at 242 us for the 128 rows.
+// columns (306 MB) 65 to 70, with both groups' softmax to do; 8 columns of d = 512 (307 MB) 82, half of its
+// products on columns that are not there.  Few or short rows are bound by the chain of launch, list, q, keys
+// and join: 5 rows of up to 700 tokens take 9.3 us whole and 7.5 split (an empty launch 2.2).  Prompts are
+// bound by the matrix cores: 3 x 181 GFLOP of products (d = 128, chunks of up to 700 behind up to 4000
+// tokens) take 500 us, 1.09 PFLOP/s (a library product of 8192 cubed makes 1.22 here).  Few columns as rows
+// of three parts do no score twice: 16-column products for 4 columns were compute-bound at 242 us for the
+// 128 rows.
 template <int D, int MODE, int NG>
 __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_kernel(Kv4Attention a) {
   constexpr bool FEW = MODE == KV4_FEW || MODE == KV4_EIGHT, TILES = MODE == KV4_TILES;
