@@ -253,14 +253,15 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
     }
   } else {
     count(rep);
-    int most = 0, least = INT32_MAX;
+    int64_t most = 0;  // keys that a row sees, and those before them in its first tile
+    int least = INT32_MAX;
     for (int b = 0; b < seqs; b++) {
-      most = std::max(most, ctx->ctx_lens[b]);
+      most = std::max<int64_t>(most, ctx->ctx_lens[b]);
       least = std::min(least, ctx->ctx_lens[b]);
     }
-    if (d.sliding_window > 0) most = std::min(most, d.sliding_window + 31);
-    const int tiles = (int)(((int64_t)most + 31) / 32);
-    if (least > 0 && !many && tiles <= whole_tiles(d.head_dim)) whole = tiles;
+    if (d.sliding_window > 0) most = std::min(most, (int64_t)d.sliding_window + 31);
+    const int64_t tiles = (most + 31) / 32;
+    if (least > 0 && !many && tiles <= whole_tiles(d.head_dim)) whole = (int)tiles;
   }
   struct Run {
     int mode, workgroups, tiles;

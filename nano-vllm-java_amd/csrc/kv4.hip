@@ -621,7 +621,7 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
 #pragma unroll
     for (int g = 0; g < NG; g++) {
       hi[g] = klen - qlen + min(first_col + (FEW ? 4 * g + w : 16 * g + c), cols - 1) / rep + 1;
-      lo[g] = a.window > 0 ? max(0, hi[g] - a.window) : 0;
+      lo[g] = a.window > 0 ? max(0, max(hi[g], 0) - a.window) : 0;
       all_hi = min(all_hi, hi[g]);
       any_hi = max(any_hi, hi[g]);
       all_lo = max(all_lo, lo[g]);
