@@ -501,8 +501,13 @@ __device__ __forceinline__ int find_tile(const int64_t *cum, int room, int n, in
 constexpr int kPRow = 20;
 
 // How far scores may pass the reference that probabilities are taken relative to before it is raised:
-// they are then below 2^kSlack, which fp32 holds as exactly as those below 1.
-constexpr float kSlack = 40.f;
+// they are then at most 2^kSlack, which fp32 holds as exactly as those below 1.  Sums of probabilities times
+// values stay finite where the values are below 2^67 (scale bytes below 192): 2^31 keys make less than 2^122.
+// A tile with larger values, up to 6 * 2^125, raises the reference to kGuard above its highest score, so
+// that its probabilities are at most 2^-31 and 2^31 of its keys sum to no more than the largest value.
+// (Always taking probabilities that low would lose the small values instead.  Looking at the scales costs
+// prompts of d = 64 3% and others less than 1%.)
+constexpr float kSlack = 24.f, kGuard = 31.f;
 
 // The weight of a partial beside those of the highest reference.  (No reference: no keys, or scores that are
 // NaN, which the sum holds.)
@@ -637,11 +642,11 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
     }
     all_hi = __builtin_amdgcn_readfirstlane(all_hi);
     all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+    any_hi = __builtin_amdgcn_readfirstlane(any_hi);
+    any_lo = __builtin_amdgcn_readfirstlane(any_lo);
     // The wave's key tiles of the segment (each is below 2^26).
     int te = t1;
     if constexpr (TILES) {
-      any_hi = __builtin_amdgcn_readfirstlane(any_hi);
-      any_lo = __builtin_amdgcn_readfirstlane(any_lo);
       t = max(t, (any_lo >> 5) - tile.kb);
       te = min(te, (max(any_hi, 0) + 31) / 32 - tile.kb);
     }
@@ -730,6 +735,21 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
     auto values = [&](int t, Tile<DW> &cur, f32x4 (*s)[2]) {
       const int key0 = (tile.kb + t) * 32;
       const bool edge = key0 + 32 > all_hi || key0 < all_lo;
+      // Does any of its values pass 2^67: a scale byte with both upper bits, of a key that some column sees?
+      // (All of the waves that share the dims hold the same scales.)
+      const u32x2 both = cur.vs & (cur.vs << 1);
+      bool large = __any(((both.x | both.y) & 0x80808080u) != 0);
+      if (large) {
+        const u32x2 upper = both & 0x80808080u;
+        bool seen = false;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const int key = key0 + 8 * w + i;
+          seen |= (byte_of(upper[i >> 2], i & 3) != 0) & (key < any_hi) & (key >= any_lo);
+        }
+        large = __any(seen);
+      }
+      const float slack = large ? -kGuard : kSlack, guard = large ? kGuard : 0.f;
       constexpr int NX = FEW ? 2 : 8;  // scores of a lane and column: keys NX (lane's) .. + NX - 1
       const int mine = key0 + NX * (FEW ? c : w);
       bf16x8 p[NG][NP];
@@ -751,9 +771,9 @@ __global__ void __launch_bounds__(256, kv4_min_waves(D, MODE)) kv4_attention_ker
         float top = fmaxf(x[0], x[1]);
 #pragma unroll
         for (int i = 2; i < NX; i++) top = fmaxf(top, x[i]);
-        if (__any(top > m[g] + kSlack)) {
+        if (__any(top > m[g] + slack)) {
           if constexpr (FEW) top = max16(top); else top = max4_lanes(top);
-          const float grown = top > m[g] + kSlack ? top : m[g];
+          const float grown = top > m[g] + slack ? top + guard : m[g];
           const float f = m[g] == grown ? 1.f : __builtin_amdgcn_exp2f(m[g] - grown);  // 0 from -infinity
           m[g] = grown;
           l[g] *= f;
