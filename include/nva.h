@@ -368,7 +368,7 @@ nva_status nva_step_clear(nva_ctx *ctx);
 
 /* ------------------------------------------------------------------ compute
  * RotaryEmbedding.forward(positions, q, k, ctx), Norms.java:275-346: q_out/k_out receive the
- * rotated q [tokens, hq, d] and k [tokens, hk, d].  Positions come from nva_step_set().
+ * rotated q [tokens, hq, d] and k [tokens, hk, d], and may be q and k themselves.  Positions come from nva_step_set().
  * NVA_E_ROPE_POS if a rounded position is outside [0, max_pos) (no work is enqueued then). */
 nva_status nva_rope_forward(nva_ctx *ctx, const nva_rope *rope, const float *q, const float *k,
                             int num_tokens, int hq, int hk, float *q_out, float *k_out);
