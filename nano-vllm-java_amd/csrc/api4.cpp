@@ -141,11 +141,18 @@ int ctx_kv4_workgroups_per_cu(nva_ctx *ctx, int head_dim, int mode) {
 
 constexpr int64_t kJoinUnits = 3500;
 // The key tiles up to which the rows of a decode step are not split where there are workgroups for all, so
-// that nothing is to be merged (which takes 4 to 5 us, and a launch of the host's 4): 5 rows of 32 / 8 heads of
-// 128 take 8.8 us with 40 tiles split and 12.1 whole, 11.4 and 15.6 with 64; 5 rows of 4 / 1 heads of 256 8.6
-// and 13.4 with 32 (96 rows with 33, 14.6 and 16); 5 rows of 8 / 1 heads of 512, where four waves share a tile,
-// 10.4 and 14.4 with 8.
-constexpr int whole_tiles(int head_dim) { return head_dim <= 128 ? 48 : head_dim <= 256 ? 36 : 8; }
+// that nothing is to be merged (4 to 5 us, and a launch).  Items are rows times KV heads (and column tiles).
+// Few of them split over idle CUs; where the pieces of eight would share CUs, splitting gains less.  A step's
+// kernels, split and whole, us:
+//   few    1 row of 32 / 8 heads of 128: 18.1, 17.9 with 32 tiles, 18.4, 19.7 with 40; 5 rows of 4 / 1 heads
+//          of 256: 19.8, 20.3 with 28, 19.7, 21.8 with 36; 5 of 8 / 1 heads of 512: 22, 20.7 with 8, 23, 24.3
+//          with 10
+//   many   5 rows of 32 / 8 heads of 128: 20.4, 20.6 with 48, 21.5, 21.8 with 56 (32 rows 25, 21.9 and 26,
+//          23); 96 of 4 / 1 heads of 256: 28.8, 26 with 48; 100 of 8 / 1 heads of 512: 30.4, 27.9 with 12
+int whole_tiles(int head_dim, int64_t items, int num_cus) {
+  const bool few = items * 8 < num_cus;
+  return head_dim <= 128 ? (few ? 32 : 48) : head_dim <= 256 ? (few ? 28 : 48) : few ? 8 : 12;
+}
 
 // Growing a buffer of a call that may be captured.
 nva_status reserve_for(nva_ctx *ctx, DevBuf &buf, size_t bytes, bool capturing, const char *what) {
@@ -228,7 +235,7 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
   // knows of their rows bounds them: the lengths themselves, or the most tokens that follow.
   const int seqs = dev ? ctx->dev_seqs : ctx->is_prefill ? ctx->num_seqs : num_tokens;
   int64_t few = 0, many = 0;  // most columns of a sequence on either list
-  int whole = 0;              // decode rows that are all this short take one workgroup a KV head
+  int64_t whole = 0;          // key tiles of decode rows that are short enough for one workgroup a KV head
   int64_t limit = kv4_by_dims(d.head_dim) ? INT32_MAX : 16;
   auto count = [&](int64_t cols) {
     if (cols <= limit) few = std::max(few, cols); else many = std::max(many, cols);
@@ -260,8 +267,7 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
       least = std::min(least, ctx->ctx_lens[b]);
     }
     if (d.sliding_window > 0) most = std::min(most, (int64_t)d.sliding_window + 31);
-    const int64_t tiles = (most + 31) / 32;
-    if (least > 0 && !many && tiles <= whole_tiles(d.head_dim)) whole = (int)tiles;
+    if (least > 0 && !many) whole = (most + 31) / 32;
   }
   struct Run {
     int mode, workgroups, tiles;
@@ -292,8 +298,10 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
     add(kv4_by_dims(d.head_dim) ? KV4_DIMS : few <= 4 ? KV4_FEW : few <= 8 ? KV4_EIGHT : KV4_ROWS);
   if (whole) {  // a workgroup for every column tile and KV head, by a list that gives them one each
     const int cols = kv4_cols(d.head_dim, runs[0].mode);
-    const int64_t tiles = (int64_t)seqs * ((rep + cols - 1) / cols);
-    if (tiles > kKv4ListTiles || tiles * d.num_kv_heads > runs[0].workgroups) whole = 0;
+    const int64_t tiles = (int64_t)seqs * ((rep + cols - 1) / cols), items = tiles * d.num_kv_heads;
+    if (tiles > kKv4ListTiles || items > runs[0].workgroups ||
+        whole > whole_tiles(d.head_dim, items, ctx->num_cus))
+      whole = 0;
   }
   nva_status st = reserve_for(ctx, ctx->d_plan4, plan_bytes, capturing, "attention work list");
   if (st != NVA_OK) return st;
@@ -350,7 +358,7 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
     l.max_cols = r.mode == KV4_TILES ? INT32_MAX : (int)limit;
     l.one_each = n_runs == 1 && std::max(few, many) <= l.cols;
     l.unit = r.mode == KV4_TILES || r.mode == KV4_DIMS ? 1 : 4;
-    l.min_units = std::max(4, (whole + 3) / 4 * 4);
+    l.min_units = std::max(4, (int)(whole + 3) / 4 * 4);
     l.slack = r.mode == KV4_TILES ? 0 : 12;
     l.over = r.mode == KV4_TILES ? 4 : r.mode == KV4_DIMS ? 6 : 20;
   }

@@ -136,8 +136,7 @@ __global__ void __launch_bounds__(256) rope_store_kernel(RopeStoreLaunch a) {
     // Any pairing and any even rotary_dim: items are pairs of a head, first those that turn, then neighbours
     // that pass through.  Both dims are read before either is written, so that outputs may be the inputs.
     // 8192 tokens of 40 heads of 96 dims (252 MB) take 59 us as neighbours, 4.3 TB/s, and 47 as halves; with one
-    // dim an item, its partner read again, 85 and 47.  Of 128 dims, 20 of them turned, 120 (163): rows of few
-    // pairs and many neighbours two dims apart, which the row kernel does where rotary_dim % 8 is 0.
+    // dim an item, its partner read again, 85 and 47.  Of 128 dims, 20 of them turned, it is 120 (163).
     const int turn = a.rotary_dim, th = turn >> 1;
     const int items = (a.hq + a.hk) * half;
     for (int it = threadIdx.x; it < items; it += blockDim.x) {

@@ -35,6 +35,30 @@ def largest_windows():
         lib.nva_ctx_destroy(ctx)
 
 
+def short_rows():
+    """Rows of a decode step up to a length are not split, by how many of them there are."""
+    for rows, heads, limit in ((1, (32, 8, 128), 32), (1, (4, 1, 64), 32), (3, (32, 8, 128), 32),
+                               (5, (32, 8, 128), 48), (32, (4, 1, 64), 48), (60, (40, 8, 128), 48),
+                               (5, (4, 1, 256), 28), (31, (4, 1, 256), 28), (32, (4, 1, 256), 48),
+                               (96, (4, 1, 256), 48), (512, (4, 1, 256), 48), (513, (4, 1, 256), 0),
+                               (5, (8, 1, 512), 8), (100, (8, 1, 512), 12),
+                               (16, (20, 1, 512), 12), (15, (20, 1, 512), 8)):  # two column tiles a row
+        ctx = context()
+        for tiles, extra in ((1, 0), (limit - 1, 1), (limit, 0), (limit, 1), (limit + 1, 0)):
+            keys = 32 * tiles + extra
+            if keys < 1:
+                continue
+            step = Step(rows, keys - 1, 0, 1, heads=heads)
+            kv = ctypes.c_void_p()
+            assert lib.nva_kv4_create(ctx, 1, step.num_blocks, step.block, step.hkv, ptr(i32([step.d])),
+                                      None, ctypes.byref(kv)) == N.NVA_OK
+            assert step.set(ctx) == N.NVA_OK
+            want = STORE + ATTENTION + (0 if keys <= 32 * limit else MERGE)
+            assert launches(ctx, kv, step, 0) == want, (rows, heads, keys)
+            lib.nva_kv4_destroy(kv)
+        lib.nva_ctx_destroy(ctx)
+
+
 if __name__ == "__main__":
     globals()[sys.argv[2]]()
     print("ok", flush=True)
