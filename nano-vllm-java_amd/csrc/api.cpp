@@ -2210,7 +2210,7 @@ nva_status nva_step_set(nva_ctx *ctx, int is_prefill, const int32_t *cu_q, const
   ctx->has_encoder = false;
   ctx->has_step = false;  // until all of it is set
   ctx->dev_step = nullptr;
-  ctx->checked_blocks = 0;
+  ctx->checked_blocks = ctx->checked_seqs = 0;
   ctx->is_prefill = is_prefill != 0;
   ctx->num_seqs = num_seqs;
   ctx->num_tokens = num_tokens;

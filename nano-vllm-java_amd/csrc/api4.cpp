@@ -103,13 +103,13 @@ nva_status check_layer(nva_kv4 *kv, int layer) {
   return NVA_OK;
 }
 
-// The host step's block tables against the arena, once per step: every block that a sequence's keys lie
-// in exists.
+// The host step's block tables against the arena, once per step and sequence: every block that a sequence's
+// keys lie in exists.
 nva_status check_tables4(nva_ctx *ctx, const nva_kv4 *kv, int num_tokens) {
-  if (ctx->checked_blocks == kv->num_blocks && ctx->checked_block_size == kv->block_size)
-    return NVA_OK;
+  if (ctx->checked_blocks != kv->num_blocks || ctx->checked_block_size != kv->block_size)
+    ctx->checked_seqs = 0;
   const int seqs = ctx->is_prefill ? ctx->num_seqs : std::min(ctx->num_seqs, num_tokens);
-  for (int b = 0; b < seqs; b++) {
+  for (int b = ctx->checked_seqs; b < seqs; b++) {
     const int klen = ctx->is_prefill ? ctx->cu_k[b + 1] - ctx->cu_k[b] : ctx->ctx_lens[b];
     const int64_t pages = ((int64_t)klen + kv->block_size - 1) / kv->block_size;
     if (klen <= 0 || (ctx->is_prefill && ctx->cu_q[b + 1] == ctx->cu_q[b])) continue;
@@ -124,10 +124,9 @@ nva_status check_tables4(nva_ctx *ctx, const nva_kv4 *kv, int num_tokens) {
         return fail(ctx, NVA_E_ARG, "sequence %d: block %d outside the arena's %d", b, t[i],
                     kv->num_blocks);
   }
-  if (seqs == ctx->num_seqs) {  // (a call of fewer rows has looked at fewer)
-    ctx->checked_blocks = kv->num_blocks;
-    ctx->checked_block_size = kv->block_size;
-  }
+  ctx->checked_blocks = kv->num_blocks;
+  ctx->checked_block_size = kv->block_size;
+  ctx->checked_seqs = std::max(ctx->checked_seqs, seqs);  // (a call of fewer rows has looked at fewer)
   return NVA_OK;
 }
 

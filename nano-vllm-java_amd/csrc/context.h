@@ -218,8 +218,9 @@ struct nva_ctx {
   // arrays are those of the tables.
   const nva_tables *dev_step = nullptr;
   int dev_seqs = 0, dev_tokens = 0, dev_max_new = 0;
-  // The arena geometry that the host step's tables were checked against for the 4-bit cache.
-  int checked_blocks = 0, checked_block_size = 0;
+  // The arena geometry that the host step's tables were checked against for the 4-bit cache, and of how many
+  // of its sequences.
+  int checked_blocks = 0, checked_block_size = 0, checked_seqs = 0;
 
   std::vector<Plan *> plans;
   std::vector<TileChoice> tile_choices;

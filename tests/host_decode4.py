@@ -1,5 +1,5 @@
-"""Which launches a decode step over the 4-bit arena makes, by its window, over the stand-in HIP runtime of
-host_hip4.cpp: ``python host_windows4.py <stand-in> <scenario>``."""
+"""Which launches a decode step over the 4-bit arena makes and which steps it refuses, over the stand-in HIP runtime of
+host_hip4.cpp: ``python host_decode4.py <stand-in> <scenario>``."""
 
 import ctypes
 import sys
@@ -57,6 +57,43 @@ def short_rows():
             assert launches(ctx, kv, step, 0) == want, (rows, heads, keys)
             lib.nva_kv4_destroy(kv)
         lib.nva_ctx_destroy(ctx)
+
+
+def fewer_rows():
+    """Calls of fewer rows than the step's are checked for their rows, and each row for every arena."""
+    def arena(blocks, block):
+        kv = ctypes.c_void_p()
+        assert lib.nva_kv4_create(ctx, 1, blocks, block, step.hkv, ptr(i32([step.d])), None,
+                                  ctypes.byref(kv)) == N.NVA_OK
+        return kv
+
+    def attend(kv, rows):
+        p = step.aligned()
+        before = stub.stub_launches()
+        got = lib.nva_attention4_forward(ctx, kv, ctypes.byref(desc), p, p, p, rows, p)
+        assert (got == N.NVA_OK) == (stub.stub_launches() > before)
+        return got
+
+    ctx = context()
+    step = Step(9, 512, 30, 1)
+    desc = N.AttnDesc(step.hq, step.d, 0.1, step.hkv, 0, 0, 0)
+    kv, wide, small = (arena(*a) for a in ((step.num_blocks, 64), (step.num_blocks, 128), (8, 64)))
+    step.table[6, 3] = step.num_blocks
+    assert step.set(ctx) == N.NVA_OK
+    for _ in range(2):
+        for rows, want in ((5, N.NVA_OK), (9, N.NVA_E_ARG), (6, N.NVA_OK), (7, N.NVA_E_ARG), (1, N.NVA_OK)):
+            assert attend(kv, rows) == want, rows
+        assert attend(wide, 6) == N.NVA_OK and attend(small, 1) == N.NVA_E_ARG
+        assert attend(wide, 7) == N.NVA_E_ARG
+    step.table[6, 3] = 3  # another step
+    step.table[0, 0] = -1
+    assert step.set(ctx) == N.NVA_OK
+    assert attend(kv, 1) == N.NVA_E_ARG
+    step.table[0, 0] = 0
+    assert step.set(ctx) == attend(kv, 1) == attend(kv, 9) == attend(kv, 4) == N.NVA_OK
+    for h in (kv, wide, small):
+        lib.nva_kv4_destroy(h)
+    lib.nva_ctx_destroy(ctx)
 
 
 if __name__ == "__main__":
