@@ -1184,21 +1184,48 @@ template <int D, int MODE> constexpr int groups() {
   return kv4_cols(D, MODE) / (MODE == KV4_TILES ? 64 : MODE == KV4_ROWS || MODE == KV4_DIMS ? 16 : 4);
 }
 
+// Rows of K and V that a launch takes: its threads are counted in 32 bits, and those of a larger grid would be
+// left out without an error.
+template <int D> int rows_at_once(int hkv) {
+  return (int)std::max<int64_t>(1, ((int64_t)1 << 31) / (2 * (int64_t)hkv * (D / 8)));
+}
+
 template <int D> hipError_t store(const Kv4Store &a, hipStream_t s) {
   constexpr int ROWS = 256 / (D / 8);
-  const int64_t rows = a.k ? 2 * (int64_t)a.tokens * a.kv.hkv : 0;
-  const int64_t blocks = (rows + ROWS - 1) / ROWS + a.lists;
-  if (blocks == 0) return hipSuccess;
-  hipLaunchKernelGGL(kv4_store_kernel<D>, dim3((unsigned)blocks), dim3(256), 0, s, a);
-  return hipGetLastError();
+  Kv4Store piece = a;
+  int t = 0;
+  do {
+    piece.tokens = a.k ? std::min(a.tokens - t, rows_at_once<D>(a.kv.hkv)) : 0;
+    const int64_t blocks = (2 * (int64_t)piece.tokens * a.kv.hkv + ROWS - 1) / ROWS + piece.lists;
+    if (blocks == 0) break;
+    hipLaunchKernelGGL(kv4_store_kernel<D>, dim3((unsigned)blocks), dim3(256), 0, s, piece);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    t += piece.tokens;
+    piece.lists = 0;
+    if (a.k) {
+      piece.k = a.k + (size_t)t * a.kv.hkv * D;
+      piece.v = a.v + (size_t)t * a.kv.hkv * D;
+      piece.slots = a.slots + t;
+    }
+  } while (a.k && t < a.tokens);
+  return hipSuccess;
 }
 
 template <int D>
 hipError_t read(const Kv4View &kv, const int32_t *slots, float *k, float *v, int rows, hipStream_t s) {
   constexpr int ROWS = 256 / (D / 8);
-  const int64_t blocks = (2 * (int64_t)rows * kv.hkv + ROWS - 1) / ROWS;
-  hipLaunchKernelGGL(kv4_read_kernel<D>, dim3((unsigned)blocks), dim3(256), 0, s, kv, slots, k, v, rows);
-  return hipGetLastError();
+  for (int t = 0; t < rows;) {
+    const int n = std::min(rows - t, rows_at_once<D>(kv.hkv));
+    const int64_t blocks = (2 * (int64_t)n * kv.hkv + ROWS - 1) / ROWS;
+    const size_t at = (size_t)t * kv.hkv * D;
+    hipLaunchKernelGGL(kv4_read_kernel<D>, dim3((unsigned)blocks), dim3(256), 0, s, kv, slots + t,
+                       k ? k + at : nullptr, v ? v + at : nullptr, n);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    t += n;
+  }
+  return hipSuccess;
 }
 
 template <int D, int MODE> hipError_t attention(const Kv4Attention &a, int workgroups, hipStream_t s) {
