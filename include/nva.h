@@ -543,7 +543,8 @@ nva_status nva_qkv_norm_rope_attention4_forward(nva_ctx *ctx, nva_kv4 *kv, const
                                                 float *out);
 
 /* nva_linear_forward with a weight in the 4-bit form: nva_linear4_create lays codes [out, in / 2] and
- * scales [out, in / 32] (device, as nva_quantize4 writes them; in % 32 == 0) out in memory of its own;
+ * scales [out, in / 32] (device, as nva_quantize4 writes them; in % 32 == 0, out <= 2^26 - 16, and
+ * out * in, rounded up to multiples of 16 and 128, < 2^37) out in memory of its own;
  * forward computes y [rows, out] = x [rows, in] W^T (+ bias [out]) from it, x 16-byte aligned, on any
  * context of its device.  Products are of x in three exact parts with the held values, sums are fp32.
  * Under capture a call must not need a larger work area than every earlier one on the context (none is

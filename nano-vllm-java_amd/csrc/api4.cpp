@@ -780,6 +780,11 @@ nva_status nva_linear4_create(nva_ctx *ctx, const uint8_t *codes, const uint8_t 
   if (in % 32) return fail(ctx, NVA_E_UNSUPPORTED, "4-bit linear needs in %% 32 == 0 (got %d)", in);
   if (in >= (1 << 22))
     return fail(ctx, NVA_E_UNSUPPORTED, "linear needs in < 4194304 (got %d)", in);
+  // A launch's threads are counted in 32 bits: a thread a lane of 16 x 128 tiles lays out, and up to 1024 a tile
+  // of outs multiply.
+  const int64_t out_tiles = ((int64_t)out + 15) / 16, in_tiles = ((int64_t)in + 127) / 128;
+  if (out_tiles >= 1 << 22 || out_tiles * in_tiles >= 1 << 26)
+    return fail(ctx, NVA_E_UNSUPPORTED, "4-bit linear of in=%d out=%d", in, out);
   if (!codes || !scales) return fail(ctx, NVA_E_ARG, "codes and scales are required");
   std::unique_ptr<nva_linear4> l(new nva_linear4());
   l->device = ctx->device;

@@ -96,6 +96,26 @@ def fewer_rows():
     lib.nva_ctx_destroy(ctx)
 
 
+def largest_weights():
+    """Projections whose launches would pass 2^32 threads are refused before anything is allocated."""
+    ctx = context()
+    p = Step(1, 64, 0, 1).aligned()
+    for out, inner in ((2 ** 26 - 15, 32), (2 ** 31 - 1, 32), (2 ** 31 - 1, 2 ** 22 - 32), (2 ** 25, 4096),
+                       (2 ** 18 * 16, 128 * 256), (2 ** 18 * 16 - 15, 128 * 255 + 32)):
+        h = ctypes.c_void_p()
+        before = stub.stub_launches()
+        stub.stub_fail_device_after(0)  # (an allocation would be NVA_E_OOM)
+        got = lib.nva_linear4_create(ctx, p, p, out, inner, ctypes.byref(h))
+        stub.stub_fail_device_after(-1)
+        assert got == N.NVA_E_UNSUPPORTED and not h and stub.stub_launches() == before, (out, inner)
+    for out, inner in ((2 ** 26 - 16, 32), (2 ** 22 * 16 - 16, 128 * 15), (2 ** 18 * 16, 128 * 255)):
+        h = ctypes.c_void_p()
+        stub.stub_fail_device_after(0)
+        assert lib.nva_linear4_create(ctx, p, p, out, inner, ctypes.byref(h)) == N.NVA_E_OOM, (out, inner)
+        stub.stub_fail_device_after(-1)
+    lib.nva_ctx_destroy(ctx)
+
+
 if __name__ == "__main__":
     globals()[sys.argv[2]]()
     print("ok", flush=True)

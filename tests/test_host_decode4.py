@@ -1,5 +1,5 @@
-"""The launches of decode steps over the 4-bit arena under windows up to the largest, of short rows and
-of fewer rows than a step's, without a device: in processes of their own over a stand-in HIP runtime."""
+"""Decode steps over the 4-bit arena (windows up to the largest, short rows, fewer rows than a step's) and
+the largest projections, without a device: in processes of their own over a stand-in HIP runtime."""
 
 import os
 import subprocess
@@ -10,7 +10,7 @@ import pytest
 HERE = os.path.dirname(os.path.abspath(__file__))
 
 
-@pytest.mark.parametrize("scenario", ["largest_windows", "short_rows", "fewer_rows"])
+@pytest.mark.parametrize("scenario", ["largest_windows", "short_rows", "fewer_rows", "largest_weights"])
 def test_scenario(tmp_path, scenario):
     so = str(tmp_path / "host_hip4.so")
     subprocess.run(["g++", "-shared", "-fPIC", "-O1", "-std=c++17",
