@@ -598,14 +598,11 @@ hipError_t launch_rows(const RopeStoreLaunch &a, hipStream_t s, int num_cus) {
   return hipGetLastError();
 }
 
-}  // namespace
+// A launch's threads are counted in 32 bits, and those of a larger grid are left out without an error: rows
+// (or tokens) of a workgroup each go in runs of this many.
+constexpr int kRowsAtOnce = 1 << 23;
 
-hipError_t launch_rope_store(const RopeStoreLaunch &in, hipStream_t s, int num_cus) {
-  if (in.tokens <= 0) return hipSuccess;
-  RopeStoreLaunch a = in;  // inputs with no stride given are contiguous [T, heads, d]
-  if (!a.q_ld) a.q_ld = a.hq * a.head_dim;
-  if (!a.k_ld) a.k_ld = a.hk * a.head_dim;
-  if (!a.v_ld) a.v_ld = a.hk * a.head_dim;
+hipError_t launch_tokens(const RopeStoreLaunch &a, hipStream_t s, int num_cus) {
   // Row kernel for the head dims it is instantiated for; the per-token kernel otherwise, and where the
   // turning dims' halves do not fall on float4 groups.
   switch (a.part && a.rotary_dim % 8 ? 0 : a.head_dim) {
@@ -622,6 +619,30 @@ hipError_t launch_rope_store(const RopeStoreLaunch &in, hipStream_t s, int num_c
   if (lds > kRopeNormMaxLds) return hipErrorInvalidValue;
   hipLaunchKernelGGL(rope_store_kernel, dim3(a.tokens), dim3(128), lds, s, a);
   return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_rope_store(const RopeStoreLaunch &in, hipStream_t s, int num_cus) {
+  RopeStoreLaunch a = in;  // inputs with no stride given are contiguous [T, heads, d]
+  if (!a.q_ld) a.q_ld = a.hq * a.head_dim;
+  if (!a.k_ld) a.k_ld = a.hk * a.head_dim;
+  if (!a.v_ld) a.v_ld = a.hk * a.head_dim;
+  for (int left = in.tokens; left > 0; left -= a.tokens) {
+    a.tokens = std::min(left, kRowsAtOnce);
+    const hipError_t e = launch_tokens(a, s, num_cus);
+    if (e != hipSuccess) return e;
+    const size_t n = a.tokens, q_row = (size_t)a.hq * a.head_dim, k_row = (size_t)a.hk * a.head_dim;
+    if (a.q) a.q += n * a.q_ld;
+    if (a.k) a.k += n * a.k_ld;
+    if (a.v) a.v += n * a.v_ld;
+    if (a.q_out) a.q_out += n * q_row;
+    if (a.k_out) a.k_out += n * k_row;
+    if (a.v_out) a.v_out += n * k_row;
+    if (a.slots) a.slots += n;
+    if (a.positions) a.positions += n;
+  }
+  return hipSuccess;
 }
 
 // cos and sin of position x frequency, [max_pos, pairs | pairs]: angles in 64 bits, as a float product
@@ -650,8 +671,16 @@ hipError_t launch_rope_table(const double *freq, float *table, int pairs, int ma
 
 hipError_t launch_rms_norm(const NormLaunch &a, hipStream_t s) {
   if (a.rows <= 0 || a.width <= 0) return hipSuccess;
-  hipLaunchKernelGGL(rms_norm_kernel, dim3(a.rows), dim3(256), 0, s, a);
-  return hipGetLastError();
+  NormLaunch run = a;
+  for (int at = 0; at < a.rows; at += run.rows) {
+    run.rows = std::min(a.rows - at, kRowsAtOnce);
+    run.x = a.x + (size_t)at * a.width;
+    run.out = a.out + (size_t)at * a.width;
+    hipLaunchKernelGGL(rms_norm_kernel, dim3(run.rows), dim3(256), 0, s, run);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 hipError_t launch_zero(float *out, size_t n, hipStream_t s) {
