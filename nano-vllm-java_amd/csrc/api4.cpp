@@ -130,6 +130,11 @@ nva_status check_tables4(nva_ctx *ctx, const nva_kv4 *kv, int num_tokens) {
   return NVA_OK;
 }
 
+// Whether a call's rows go to the step's slots.
+bool stores(const nva_ctx *ctx, const nva_attn_desc &d, int num_tokens) {
+  return d.write_kv && (ctx->dev_step || (ctx->has_slots && ctx->num_slots == num_tokens));
+}
+
 int ctx_kv4_workgroups_per_cu(nva_ctx *ctx, int head_dim, int mode) {
   const int key = -(head_dim + 1000 * (mode + 1));  // beside the other kernels' keys
   auto it = ctx->occupancy.find(key);
@@ -171,6 +176,7 @@ nva_status reserve_for(nva_ctx *ctx, DevBuf &buf, size_t bytes, bool capturing, 
 
 namespace nva {
 
+// What attention4_rows could not serve (but for work areas under capture), before a fused call rotates.
 nva_status check_forward4(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc *desc, int num_tokens) {
   nva_status st = check_desc(ctx, desc);
   if (st != NVA_OK) return st;
@@ -213,6 +219,12 @@ nva_status check_forward4(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc *desc, 
                   num_tokens);
   }
   if (num_tokens == 0) return NVA_OK;
+  if (stream_capturing(ctx->stream))
+    return fail(ctx, NVA_E_ARG,
+                "only steps of nva_step_extend may be captured over the 4-bit arena");
+  if (stores(ctx, *desc, num_tokens) && ctx->slot_max >= (int64_t)kv->num_blocks * kv->block_size)
+    return fail(ctx, NVA_E_ARG, "slot %lld outside the arena's %lld slots", (long long)ctx->slot_max,
+                (long long)kv->num_blocks * kv->block_size);
   return check_tables4(ctx, kv, num_tokens);
 }
 
@@ -221,14 +233,8 @@ nva_status attention4_rows(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc &d, co
   const nva_tables *dev = ctx->dev_step;
   const int layer = d.kv_layer_index, rep = d.num_heads / d.num_kv_heads;
   const bool capturing = stream_capturing(ctx->stream);
-  if (capturing && !dev)
-    return fail(ctx, NVA_E_ARG,
-                "only steps of nva_step_extend may be captured over the 4-bit arena");
-  const bool store = d.write_kv && (dev || (ctx->has_slots && ctx->num_slots == num_tokens));
+  const bool store = stores(ctx, d, num_tokens);
   if (store && (!k || !v)) return fail(ctx, NVA_E_ARG, "k and v are required to store");
-  if (store && !dev && ctx->slot_max >= (int64_t)kv->num_blocks * kv->block_size)
-    return fail(ctx, NVA_E_ARG, "slot %lld outside the arena's %lld slots", (long long)ctx->slot_max,
-                (long long)kv->num_blocks * kv->block_size);
 
   // The kernels: sequences of up to 16 columns on the first list, of more on the second.  What the host
   // knows of their rows bounds them: the lengths themselves, or the most tokens that follow.

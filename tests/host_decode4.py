@@ -6,6 +6,7 @@ import sys
 
 from host_side import N, Step, context, lib, ptr, i32, stub
 
+stub.stub_set_capturing.argtypes = [ctypes.c_int]
 STORE, ATTENTION, MERGE = 1, 1, 1
 
 
@@ -93,6 +94,50 @@ def fewer_rows():
     assert step.set(ctx) == attend(kv, 1) == attend(kv, 9) == attend(kv, 4) == N.NVA_OK
     for h in (kv, wide, small):
         lib.nva_kv4_destroy(h)
+    lib.nva_ctx_destroy(ctx)
+
+
+def refused_before_anything():
+    """The fused calls refuse what the attention behind them would, before they rotate (whose outputs may be
+    their inputs)."""
+    ctx = context()
+    for new in (1, 5):
+        step = Step(9, 512, 30, new)
+        p = step.aligned()
+        kv, rope = ctypes.c_void_p(), ctypes.c_void_p()
+        assert lib.nva_kv4_create(ctx, 1, step.num_blocks, step.block, step.hkv, ptr(i32([step.d])), None,
+                                  ctypes.byref(kv)) == N.NVA_OK
+        assert lib.nva_rope_create_theta(ctx, step.d, step.d, 4096, ctypes.c_float(1e4),
+                                         ctypes.byref(rope)) == N.NVA_OK
+        desc = ctypes.byref(step.desc)
+        calls = (lambda: lib.nva_norm_rope_attention4_forward(ctx, kv, rope, None, None, None, desc, p, p, p,
+                                                              step.tokens, p, p, p),
+                 lambda: lib.nva_qkv_norm_rope_attention4_forward(ctx, kv, rope, None, None, None, desc, p,
+                                                                  step.tokens, None, None, p),
+                 lambda: lib.nva_attention4_forward(ctx, kv, desc, p, p, p, step.tokens, p))
+
+        def refused():
+            for call in calls:
+                before = stub.stub_launches()
+                assert call() == N.NVA_E_ARG and stub.stub_launches() == before
+
+        assert step.set(ctx) == N.NVA_OK
+        for call in calls:
+            assert call() == N.NVA_OK
+        stub.stub_set_capturing(1)  # a step of the host is not for capture
+        refused()
+        stub.stub_set_capturing(0)
+        step.slots[3] = step.num_blocks * step.block  # a slot outside the arena
+        assert step.set(ctx) == N.NVA_OK
+        refused()
+        step.desc.write_kv = 0  # (which a call that does not store does not look at)
+        for call in calls:
+            assert call() == N.NVA_OK
+        step.slots[3] = step.table[3, 0] = step.num_blocks
+        assert step.set(ctx) == N.NVA_OK
+        refused()
+        lib.nva_kv4_destroy(kv)
+        lib.nva_rope_destroy(rope)
     lib.nva_ctx_destroy(ctx)
 
 

@@ -1,4 +1,4 @@
-"""Decode steps over the 4-bit arena (windows up to the largest, short rows, fewer rows than a step's) and
+"""Decode steps over the 4-bit arena (windows up to the largest, short rows, fewer rows than a step's, refusals) and
 the largest projections, without a device: in processes of their own over a stand-in HIP runtime."""
 
 import os
@@ -10,7 +10,8 @@ import pytest
 HERE = os.path.dirname(os.path.abspath(__file__))
 
 
-@pytest.mark.parametrize("scenario", ["largest_windows", "short_rows", "fewer_rows", "largest_weights"])
+@pytest.mark.parametrize("scenario", ["largest_windows", "short_rows", "fewer_rows", "refused_before_anything",
+                                      "largest_weights"])
 def test_scenario(tmp_path, scenario):
     so = str(tmp_path / "host_hip4.so")
     subprocess.run(["g++", "-shared", "-fPIC", "-O1", "-std=c++17",
