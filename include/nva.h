@@ -343,7 +343,8 @@ nva_status nva_step_positions(nva_ctx *ctx, const float *positions, int num_toke
  * blocks after the call.
  *
  * The step serves nva_rope_forward and the calls over the 4-bit cache; the other attention calls need
- * nva_step_set (NVA_E_NO_STEP).  Its tables must outlive its use, captured graphs included. */
+ * nva_step_set (NVA_E_NO_STEP).  The host does not see its positions, so a table of angles has to hold
+ * max_tokens of them (NVA_E_ROPE_POS).  Its tables must outlive its use, captured graphs included. */
 nva_status nva_tables_create(nva_ctx *ctx, int max_seqs, int max_tokens, int max_step_tokens,
                              int num_blocks, int block_size, const int32_t *pages,
                              nva_tables **out);
@@ -509,7 +510,8 @@ nva_status nva_kv4_blocks_that_fit(nva_ctx *ctx, int num_layers, int block_size,
 nva_status nva_kv4_layer(nva_kv4 *kv, int layer, void **pages, int64_t *bytes);
 /* Rows of k and v [num_rows, num_kv_heads, head_dim] to the slots (device int32) of a layer, or the
  * values the slots hold to k and v (either may be NULL when reading).  Slots outside the arena are
- * skipped, and read as zeros.  Of rows written to one slot in one call any may win, dim by dim. */
+ * skipped, and read as zeros.  The rows of a call go to slots of their own, here and where a step's k and v
+ * are stored: what a slot named twice holds is unspecified (codes of one row may meet the scales of another). */
 nva_status nva_kv4_write_rows(nva_kv4 *kv, int layer, const int32_t *slots, const float *k,
                               const float *v, int num_rows);
 nva_status nva_kv4_read_rows(nva_kv4 *kv, int layer, const int32_t *slots, float *k, float *v,
@@ -522,7 +524,8 @@ nva_status nva_kv4_read_rows(nva_kv4 *kv, int layer, const int32_t *slots, float
  * num_heads / num_kv_heads may be any number.  Prefix groups are not used: every sequence's keys are
  * read for it.  A step of nva_step_extend may be captured once a step at least as large has run on the
  * context (NVA_E_ARG otherwise); replays then serve the lengths of the replayed extends.  The results
- * do not depend on how a step is cut into workgroups beyond fp32 rounding.  Kernel stats: "store4",
+ * do not depend on how a step is cut into workgroups beyond fp32 rounding, and are finite for all values that
+ * the cache holds where the scores are.  Kernel stats: "store4",
  * "attention4", "merge4". */
 nva_status nva_attention4_forward(nva_ctx *ctx, nva_kv4 *kv, const nva_attn_desc *desc,
                                   const float *q, const float *k, const float *v, int num_tokens,

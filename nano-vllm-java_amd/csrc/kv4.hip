@@ -530,8 +530,8 @@ __device__ __forceinline__ float weight_of(float m, float l, float big) {
 //                        prompts of 121 rows take 322 us instead of 196.)
 //
 // Decode is bound by reading the keys once: d = 128, 4 columns, 128 rows of up to 16K tokens (1.18 GB) take
-// 194 us, 6.1 TB/s (the loads alone 186); 128 rows of d = 256 (295 MB) 53, 5.5 TB/s; 64 rows of eight
-// columns (306 MB) 65 to 70, with both groups' softmax to do; 8 columns of d = 512 (307 MB) 82, half of its
+// 194 us, 6.1 TB/s (the loads alone 186); 128 rows of d = 256 (295 MB) 52, 5.7 TB/s; 64 rows of eight
+// columns (306 MB) 67 to 75, with both groups' softmax to do; 8 columns of d = 512 (307 MB) 81, half of its
 // products on columns that are not there.  Few or short rows are bound by the chain of launch, list, q, keys
 // and join: 5 rows of up to 700 tokens take 9.3 us whole and 7.5 split (an empty launch 2.2).  Prompts are
 // bound by the matrix cores: 3 x 181 GFLOP of products (d = 128, chunks of up to 700 behind up to 4000

@@ -925,7 +925,7 @@ class KvCacheArena4:
 
     def write_rows(self, layer: int, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
         """Rounds rows of k and v [rows, numKvHeads, headDim] into the slots (an int32 device tensor;
-        slots outside the arena are skipped)."""
+        slots outside the arena are skipped, and no two are the same)."""
         device = self._ctx.device
         shape = self._shape(layer, slots.numel())
         for name, t in (("k", k), ("v", v)):
